@@ -15,7 +15,7 @@ import torch
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libdspine_verify.so")
 
 DSV_OK, DSV_ERR_INVALID, DSV_ERR_UNSUPPORTED, DSV_ERR_LAUNCH, DSV_ERR_WORKSPACE = range(5)
-DSV_F32, DSV_BF16, DSV_F16 = 0, 1, 2
+DSV_F32, DSV_BF16, DSV_F16, DSV_E4M3, DSV_I8 = range(5)
 DSV_BACKEND_PYTORCH, DSV_BACKEND_FLASHINFER = 0, 1
 LIST_K = 64
 
@@ -29,6 +29,8 @@ EXPORTS = (
     "dsv_greedy_verify_noalloc", "dsv_commit_accept", "dsv_rs_table", "dsv_rs_table_workspace_bytes",
     "dsv_factor_table", "dsv_factor_direct", "dsv_factor_workspace_doubles", "dsv_factor_widen",
     "dsv_factor_gemm", "dsv_filter_probs", "dsv_filter_workspace_bytes",
+    "dsv_kv_write", "dsv_kv_read", "dsv_tree_attention", "dsv_tree_attention_workspace_bytes",
+    "dsv_tree_masks", "dsv_tree_verify", "dsv_tree_verify_workspace_bytes", "dsv_commit_tree",
 )
 DSV_ADJ_ADD, DSV_ADJ_SCALE = 0, 1
 
@@ -89,6 +91,32 @@ class FactorArgs(ctypes.Structure):
         ("eps", _c.c_double), ("out", vp), ("base_out", vp), ("x", vp), ("scale", vp), ("first", vp),
         ("message", vp), ("tg", vp), ("safe", vp), ("d", vp), ("magnitude", vp), ("y", vp),
         ("gemm_ws", vp), ("gemm_ws_doubles", i64),
+    ]
+
+
+class KvCache(ctypes.Structure):
+    """Mirror of ``dsv_kv_cache``."""
+
+    _fields_ = [
+        ("k", vp), ("v", vp), ("dtype", i32), ("heads", i32), ("dim", i32), ("pad0", i32),
+        ("num_slots", i64),
+        ("k_slot_stride", i64), ("k_head_stride", i64), ("v_slot_stride", i64), ("v_head_stride", i64),
+        ("k_scale", vp), ("v_scale", vp),
+        ("ks_slot_stride", i64), ("ks_head_stride", i64), ("vs_slot_stride", i64), ("vs_head_stride", i64),
+    ]
+
+
+class TreeAttentionArgs(ctypes.Structure):
+    """Mirror of ``dsv_tree_attention_args``."""
+
+    _fields_ = [
+        ("cache", KvCache),
+        ("q", vp), ("out", vp), ("lse", vp), ("dtype", i32), ("q_heads", i32), ("rows", i64),
+        ("q_row_stride", i64), ("q_head_stride", i64), ("out_row_stride", i64), ("out_head_stride", i64),
+        ("bs", i32), ("T", i32), ("prefix_lens", vp), ("verify_lens", vp),
+        ("row_offsets", vp), ("row_offsets_i64", i32), ("scale", _c.c_float), ("masks", vp),
+        ("page_table", vp), ("page_stride", i64), ("page_cols", i64),
+        ("workspace", vp), ("workspace_bytes", i64),
     ]
 
 
@@ -165,6 +193,24 @@ def load():
         lib.dsv_commit_accept.restype = i32
         lib.dsv_commit_accept.argtypes = [i32, i32, vp, vp, vp, i32, vp, i32, vp, i64, i64, vp, vp, vp, i32, vp, vp,
                                           vp]
+        lib.dsv_kv_write.restype = i32
+        lib.dsv_kv_write.argtypes = [ctypes.POINTER(KvCache), vp, vp, i32, i64, i64, i64, i64, i64, vp, i32, vp]
+        lib.dsv_kv_read.restype = i32
+        lib.dsv_kv_read.argtypes = [ctypes.POINTER(KvCache), vp, vp, i32, i64, vp, i32, vp]
+        lib.dsv_tree_attention_workspace_bytes.restype = i64
+        lib.dsv_tree_attention_workspace_bytes.argtypes = [i32, i32, i32, i32, i32]
+        lib.dsv_tree_attention.restype = i32
+        lib.dsv_tree_attention.argtypes = [ctypes.POINTER(TreeAttentionArgs), vp]
+        lib.dsv_tree_masks.restype = i32
+        lib.dsv_tree_masks.argtypes = [vp, i32, i32, vp, vp, vp]
+        lib.dsv_tree_verify_workspace_bytes.restype = i64
+        lib.dsv_tree_verify_workspace_bytes.argtypes = [i64, i64]
+        lib.dsv_tree_verify.restype = i32
+        lib.dsv_tree_verify.argtypes = [vp, i32, i64, i64, i64, i32, i32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp,
+                                        i64, vp]
+        lib.dsv_commit_tree.restype = i32
+        lib.dsv_commit_tree.argtypes = [i32, i32, vp, vp, vp, vp, i32, vp, i32, vp, i64, i64, vp, vp, vp, i32, vp, vp,
+                                        vp]
         lib.dsv_factor_workspace_doubles.restype = i64
         lib.dsv_factor_workspace_doubles.argtypes = [i64, i32, i32, i32]
         lib.dsv_factor_table.restype = i32

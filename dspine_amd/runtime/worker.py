@@ -279,7 +279,7 @@ def accept_dspine_sampled_round(*, candidates, next_token_logits, sampling_info,
 
 
 def commit_accept(outputs, *, prefix_lens, req_pool_indices, req_to_token, out_cache_loc=None,
-                  verify_lens=None, slot_offsets=None, seq_lens=None, free_slots=None, free_count=None):
+                  verify_lens=None, slot_offsets=None, seq_lens=None, free_slots=None, free_count=None, path=None):
     """Commit one verified round (``dsv_commit_accept``): what SGLang's speculative worker does
     with the accept / bonus buffers after verification (its ``_commit_accept``, which the
     reference's tests/test_tp_accept.py:106-180 drive; SGLang itself is not part of the
@@ -293,11 +293,17 @@ def commit_accept(outputs, *, prefix_lens, req_pool_indices, req_to_token, out_c
     req_pool_indices[b], prefix + i]``; without it the slots are already in the table.
     ``seq_lens[req_pool_indices[b]]`` becomes ``prefix + accept + 1``; the slots of the rejected
     positions are compacted into ``free_slots`` (int64, (b, i) order) and counted in
-    ``free_count[0]``.  Returns ``(free_slots, free_count)``."""
+    ``free_count[0]``.  Returns ``(free_slots, free_count)``.
+
+    ``path`` (int32 [bs, T], T <= 64; ``accept_greedy_tree``'s) commits a drafted tree: the accepted
+    positions are the nodes ``path[b, :accept[b] + 1]`` of the window, in that order, and the slots of
+    its other nodes are freed (``dsv_commit_tree``)."""
     accept, output = outputs[0], outputs[3]
     bs, T = output.shape
     dev = _lib.require_cuda(accept, prefix_lens, req_pool_indices, req_to_token, out_cache_loc, verify_lens,
-                            slot_offsets, seq_lens, free_slots, free_count)
+                            slot_offsets, seq_lens, free_slots, free_count, path)
+    if path is not None and (path.shape != (bs, T) or path.dtype != torch.int32 or not path.is_contiguous() or T > 64):
+        raise ValueError("path must be contiguous int32 [bs, T], T at most 64")
     if accept.shape != (bs,) or accept.dtype != torch.int32 or not accept.is_contiguous():
         raise ValueError("accept must be contiguous int32 [bs]")
     for name, t in (("prefix_lens", prefix_lens), ("req_pool_indices", req_pool_indices)):
@@ -325,6 +331,16 @@ def commit_accept(outputs, *, prefix_lens, req_pool_indices, req_to_token, out_c
         free_count = torch.empty(1, device=dev, dtype=torch.int32)
     elif free_count.dtype != torch.int32 or free_count.numel() < 1:
         raise ValueError("free_count must be int32 [1]")
+    if path is not None:
+        with torch.cuda.device(dev):
+            _lib.check(_lib.load().dsv_commit_tree(
+                bs, T, accept.data_ptr(), path.data_ptr(), _lib.ptr(verify_lens), prefix_lens.data_ptr(),
+                int(prefix_lens.dtype == torch.int64), req_pool_indices.data_ptr(),
+                int(req_pool_indices.dtype == torch.int64), req_to_token.data_ptr(), req_to_token.stride(0),
+                req_to_token.shape[1], _lib.ptr(out_cache_loc), _lib.ptr(slot_offsets), _lib.ptr(seq_lens),
+                int(seq_lens is not None and seq_lens.dtype == torch.int64), free_slots.data_ptr(),
+                free_count.data_ptr(), _lib.stream_of(dev)), "dsv_commit_tree")
+        return free_slots, free_count
     _lib.check(_lib.load().dsv_commit_accept(
         bs, T, accept.data_ptr(), _lib.ptr(verify_lens), prefix_lens.data_ptr(),
         int(prefix_lens.dtype == torch.int64), req_pool_indices.data_ptr(), int(req_pool_indices.dtype == torch.int64),

@@ -43,6 +43,15 @@
  *   dsv_commit_accept     the commit after the accept buffers (SGLang's _commit_accept, not in
  *                         the reference; its accept-buffer discipline tests/test_tp_accept.py
  *                         :106-180)
+ *
+ * Operators around the target forward of a drafted tree (no counterpart in the reference, which
+ * verifies chains and leaves the cache and its attention to SGLang):
+ *   dsv_kv_write          new keys and values into cache slots, quantised where the cache is
+ *   dsv_kv_read           cache slots gathered and brought back to activations
+ *   dsv_tree_attention    attention of drafted nodes over a request's cached positions
+ *   dsv_tree_masks        a drafted tree's ancestor masks and depths from its parents
+ *   dsv_tree_verify       greedy acceptance of a drafted tree
+ *   dsv_commit_tree       dsv_commit_accept for an accepted path of a tree
  */
 #ifndef DSPINE_VERIFY_H
 #define DSPINE_VERIFY_H
@@ -63,7 +72,7 @@ enum {
   DSV_ERR_WORKSPACE = 4    /* workspace too small */
 };
 
-enum { DSV_F32 = 0, DSV_BF16 = 1, DSV_F16 = 2 };
+enum { DSV_F32 = 0, DSV_BF16 = 1, DSV_F16 = 2, DSV_E4M3 = 3, DSV_I8 = 4 };
 
 /* Sampling-backend semantics of the target filter (runtime/worker.py:482-505). */
 enum {
@@ -409,6 +418,101 @@ int dsv_commit_accept(int32_t bs, int32_t T, const int32_t* accept, const int32_
                       int32_t req_pool_i64, int32_t* req_to_token, int64_t rt_stride, int64_t rt_cols,
                       const int64_t* out_cache_loc, const int64_t* slot_offsets, void* seq_lens,
                       int32_t seq_lens_i64, int64_t* free_slots, int32_t* free_count, dsv_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------- */
+/* The KV cache and a drafted tree's round over it.                                          */
+/* ---------------------------------------------------------------------------------------- */
+/* One layer's cache: k and v [num_slots, heads, dim] with strides in elements (the last      */
+/* dimension contiguous, every row on a 16-byte boundary, dim a multiple of 16 up to 256).    */
+/* DSV_BF16 / DSV_F16 hold the values; DSV_E4M3 (OCP) / DSV_I8 hold codes, value = code *      */
+/* scale, with a float32 scale for each (slot, head).                                          */
+typedef struct dsv_kv_cache {
+  void* k;
+  void* v;
+  int32_t dtype;               /* DSV_BF16 / DSV_F16 / DSV_E4M3 / DSV_I8 */
+  int32_t heads, dim, pad0;
+  int64_t num_slots;
+  int64_t k_slot_stride, k_head_stride, v_slot_stride, v_head_stride;
+  float* k_scale;              /* quantised caches only, else NULL */
+  float* v_scale;
+  int64_t ks_slot_stride, ks_head_stride, vs_slot_stride, vs_head_stride;
+} dsv_kv_cache;
+
+/* k, v [n, heads, dim] (DSV_BF16 / DSV_F16, 16-byte-aligned rows, strides in elements) into the */
+/* cache's slots[i] (int32 / int64; a slot outside [0, num_slots) is skipped; the others must be */
+/* distinct).  A quantised cache takes, for each (token, head), a = max |x| in float32, the scale */
+/* a * (1 / top) and the codes rne(x * ((1 / a) * top)), top = 448 (E4M3) or 127 (I8); a < 2^-100: */
+/* scale and codes 0; a NaN or an infinity in the row: scale NaN, codes 0.  Other caches hold the */
+/* values of x's own type.                                                                        */
+int dsv_kv_write(const dsv_kv_cache* cache, const void* k, const void* v, int32_t dtype, int64_t n,
+                 int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride, int64_t v_head_stride,
+                 const void* slots, int32_t slots_i64, dsv_stream_t stream);
+/* The slots' values into k, v [n, heads, dim] (DSV_F32 / DSV_BF16 / DSV_F16, contiguous), rounded */
+/* once; zeros for a slot outside [0, num_slots).  A slot may be named any number of times.        */
+int dsv_kv_read(const dsv_kv_cache* cache, void* k, void* v, int32_t dtype, int64_t n, const void* slots,
+                int32_t slots_i64, dsv_stream_t stream);
+
+/* Attention of drafted nodes over the cache.  Request b's node i (i < n_b, n_b = verify_lens[b] */
+/* clamped into [0, T], NULL: T; T <= 64) has the query rows q[row(b, i)] of q_heads heads (a      */
+/* multiple of the cache's heads: query head h reads cache head h / (q_heads / heads)),           */
+/* row = row_offsets[b] + i, else b * T + i.  It sees the positions p < prefix_lens[b] and, of the */
+/* window p = prefix_lens[b] + j, j < n_b, those whose bit j is set in masks[b, i] (int64          */
+/* [bs, T]; NULL: j <= i).  Position p lies in slot page_table[b, p]; positions past page_cols and */
+/* slots outside [0, num_slots) hold nothing.  s = scale * q.k, out = sum softmax(s) v             */
+/* [rows, q_heads, dim] of q's type, lse = log sum e^s (float32 [rows, q_heads], may be NULL); a   */
+/* node that sees nothing: 0 and -inf.  Rows of no node are left as they were.                     */
+typedef struct dsv_tree_attention_args {
+  dsv_kv_cache cache;
+  const void* q;               /* [rows, q_heads, dim], 16-byte-aligned rows */
+  void* out;
+  float* lse;
+  int32_t dtype;               /* DSV_BF16 / DSV_F16; an unquantised cache's own */
+  int32_t q_heads;
+  int64_t rows;
+  int64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride;
+  int32_t bs, T;
+  const int32_t* prefix_lens;  /* [bs] */
+  const int32_t* verify_lens;  /* [bs] or NULL */
+  const void* row_offsets;     /* [bs] int32 / int64, or NULL (then rows == bs * T) */
+  int32_t row_offsets_i64;
+  float scale;
+  const int64_t* masks;        /* [bs, T] or NULL */
+  const int32_t* page_table;   /* [bs, page_cols] */
+  int64_t page_stride, page_cols;
+  void* workspace;             /* dsv_tree_attention_workspace_bytes */
+  int64_t workspace_bytes;
+} dsv_tree_attention_args;
+int64_t dsv_tree_attention_workspace_bytes(int32_t bs, int32_t T, int32_t heads, int32_t q_heads, int32_t dim);
+int dsv_tree_attention(const dsv_tree_attention_args* args, dsv_stream_t stream);
+
+/* parents [bs, T] int32 (T <= 64; parents[b, 0] = -1, a node's parent is an earlier node) to      */
+/* masks [bs, T] int64 (bit j: node j is node i or one of its ancestors) and depths [bs, T] int32 */
+/* (may be NULL).  A node i > 0 whose parent is not in [0, i) is a root of its own.               */
+int dsv_tree_masks(const int32_t* parents, int32_t bs, int32_t T, int64_t* masks, int32_t* depths,
+                   dsv_stream_t stream);
+
+/* Greedy acceptance of drafted trees.  candidates [bs, T] int64: node tokens (node 0 the last      */
+/* accepted token); logits row b * T + i follows node i, top1 = its first argmax.  From node 0 the */
+/* path moves to the child that carries top1 of the node it is at (of several the first; children  */
+/* at or past verify_lens[b], clamped into [1, T], do not count) until none does.  accept = moves, */
+/* commit = accept + 1, bonus = top1 of the last node, output = the accepted tokens, the bonus,    */
+/* then zeros, new_seq = prefix + commit, path [bs, T] int32 = the nodes of the path, then -1.     */
+int dsv_tree_verify(const void* logits, int32_t logits_dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                    int32_t bs, int32_t T, const int64_t* candidates, const int32_t* parents,
+                    const int32_t* verify_lens, const int32_t* prefix_lens, int32_t* accept, int32_t* commit,
+                    int64_t* bonus, int64_t* output, int32_t* new_seq, int32_t* path, void* workspace,
+                    int64_t workspace_bytes, dsv_stream_t stream);
+int64_t dsv_tree_verify_workspace_bytes(int64_t rows, int64_t vocab);
+
+/* dsv_commit_accept where the accepted positions are the nodes path[b, i] (int32 [bs, T], T <= 64) */
+/* of the window: table position prefix + i takes the slot of node path[b, i], the slots of the    */
+/* window's other nodes go to free_slots in node order.  A path entry outside the window is left   */
+/* out.                                                                                            */
+int dsv_commit_tree(int32_t bs, int32_t T, const int32_t* accept, const int32_t* path, const int32_t* verify_lens,
+                    const void* prefix_lens, int32_t prefix_i64, const void* req_pool_indices,
+                    int32_t req_pool_i64, int32_t* req_to_token, int64_t rt_stride, int64_t rt_cols,
+                    const int64_t* out_cache_loc, const int64_t* slot_offsets, void* seq_lens,
+                    int32_t seq_lens_i64, int64_t* free_slots, int32_t* free_count, dsv_stream_t stream);
 
 #ifdef __cplusplus
 }
