@@ -29,14 +29,17 @@ __device__ __forceinline__ float act_to_f32(uint32_t bits) {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)bits);
 }
 
-// Two float32 as activations, rounded to nearest even, the first in the low half.
+// Two float32 as activations, rounded to nearest even, the first in the low half (one instruction).
 template <int XT>
 __device__ __forceinline__ uint32_t pack_act(float lo, float hi) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2 v = {lo, hi};
   if constexpr (XT == DSV_BF16) {
-    return f32_to_bf16_bits(lo) | (f32_to_bf16_bits(hi) << 16);
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
   } else {
-    const uint32_t a = __builtin_bit_cast(uint16_t, (_Float16)lo), b = __builtin_bit_cast(uint16_t, (_Float16)hi);
-    return a | (b << 16);
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
   }
 }
 
