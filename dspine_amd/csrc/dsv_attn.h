@@ -1,0 +1,671 @@
+// Attention of drafted nodes over a request's cached positions for gfx950.
+//
+// For request b, cache head h and the query rows r = (node, query head of h's group), with s = scale * q.k:
+// out = sum_p e^(s_p - m) v_p / sum_p e^(s_p - m), in one pass over the positions with a reference m of the softmax
+// that moves up where a score exceeds it by more than a few powers of two (the weights are then at most 2^LIM, and the
+// partial sums are rescaled; most steps only compare).
+//
+// The matrix cores take keys as they lie in memory: S^T = K Q^T with the positions on the rows of the tile, so that a
+// lane holds, for one query row, the weights of the four (twice: eight) positions that the second product
+// O^T = V^T P^T wants from it: no weight moves between lanes.  Keys go from memory to the operand registers; values
+// too, as 16-byte pieces of whole rows whose 16-bit elements a v_perm each puts in the positions' order.  Nothing is
+// staged in LDS, the waves run free of each other, and each holds all its rows' sums in registers.
+//
+// The positions of a batch are cut into about `target` equal pieces (a rule on the lengths, which only the device
+// knows: every workgroup computes the same plan from them); pieces of a request are joined by k_attn_join.
+#pragma once
+#include "dsv_cache.h"
+#include "dsv_common.h"
+
+namespace dsv {
+
+constexpr int AT_THREADS = 256;
+constexpr int AT_WAVES = AT_THREADS / WAVE;
+constexpr int AT_NODES = 64;
+constexpr int AT_TILE = 32;  // positions of a step
+constexpr float AT_LOW = -3e38f;
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2v __attribute__((ext_vector_type(2)));
+typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+struct AttnParams {
+  dsv_tree_attention_args a;
+  int G, WR, RB;       // query heads a cache head; waves over the rows, row blocks of a request
+  int target;          // pieces aimed at
+  int least;           // tiles of a piece at least
+  int joined;          // whether a request may have several pieces
+  uint32_t num_slots, k_step, v_step;  // slots; bytes from slot to slot
+  float* part_o;       // [item][head][row][dim]
+  float2* part_ml;     // [item][head][row]: reference, sum
+};
+
+// The request's nodes, its context and its positions (context and window) that the page table has.
+struct Request {
+  int nodes;
+  int prefix, total;  // within the table
+};
+__device__ __forceinline__ Request request_of(const dsv_tree_attention_args& a, int64_t b) {
+  Request r;
+  int n = a.verify_lens ? a.verify_lens[b] : a.T;
+  r.nodes = n < 0 ? 0 : (n > a.T ? a.T : n);
+  const int pre = a.prefix_lens[b];
+  const int64_t from = pre < 0 ? 0 : pre, to = from + r.nodes;
+  r.prefix = (int)(from < a.page_cols ? from : a.page_cols);
+  r.total = (int)(to < a.page_cols ? to : a.page_cols);
+  return r;
+}
+__device__ __forceinline__ int tiles_of(const Request& r) {
+  const int t = (r.total + AT_TILE - 1) / AT_TILE;
+  return r.nodes == 0 ? 0 : (t < 1 ? 1 : t);
+}
+
+// The plan, computed by every wave from the batch's lengths: tiles of a piece.
+__device__ __forceinline__ int plan_chunk(const AttnParams& P, int lane) {
+  int64_t sum = 0;
+  for (int b = lane; b < P.a.bs; b += WAVE) sum += tiles_of(request_of(P.a, b));
+  sum = wave_sum(sum);
+  const int64_t c = (sum + P.target - 1) / P.target;
+  return (int)(c < P.least ? P.least : c);
+}
+__device__ __forceinline__ int pieces_of(int tiles, int chunk) { return (tiles + chunk - 1) / chunk; }
+
+// Pieces of the requests before b.
+__device__ __forceinline__ int items_before(const AttnParams& P, int chunk, int b, int lane) {
+  int sum = 0;
+  for (int i = lane; i < b; i += WAVE) sum += pieces_of(tiles_of(request_of(P.a, i)), chunk);
+  return wave_sum(sum);
+}
+// The request and the piece of a work item; false past the last.
+__device__ __forceinline__ bool item_at(const AttnParams& P, int chunk, int item, int lane, int& b, int& piece) {
+  int before = 0;
+  for (int b0 = 0; b0 < P.a.bs; b0 += WAVE) {
+    const int i = b0 + lane;
+    const int n = i < P.a.bs ? pieces_of(tiles_of(request_of(P.a, i)), chunk) : 0;
+    const int end = before + wave_incl_scan(n);
+    const uint64_t past = __ballot(end > item);
+    if (past) {
+      const int l = __ffsll((unsigned long long)past) - 1;
+      b = b0 + l;
+      piece = item - (readlane_at(end, l) - readlane_at(n, l));
+      return true;
+    }
+    before = readlane<WAVE - 1>(end);
+  }
+  return false;
+}
+
+template <int XT>
+__device__ __forceinline__ f32x4 mfma(const uint32_t (&x)[4], const uint32_t (&y)[4], f32x4 c) {
+  const uint4 a = make_uint4(x[0], x[1], x[2], x[3]), b = make_uint4(y[0], y[1], y[2], y[3]);
+  if constexpr (XT == DSV_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bhalf8, a), __builtin_bit_cast(bhalf8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+
+// N 32-bit words from memory (16-byte loads where there are that many).
+template <int N>
+__device__ __forceinline__ void load_words(const void* p, uint32_t (&w)[N]) {
+  if constexpr (N >= 4) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+}
+
+// int8 codes as float16: a byte of code + 128 is the float16 (code + 128) * 2^-24; times 2^15 less 1/4 that is
+// code / 512, exact.  (Two instructions for two codes.)
+constexpr float I8_UNIT = 512.f;
+__device__ __forceinline__ uint32_t i8_pair(uint32_t bytes) {
+  const half2v up = {(_Float16)32768.f, (_Float16)32768.f}, off = {(_Float16)-0.25f, (_Float16)-0.25f};
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2v, bytes), up, off));
+}
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t w, bool hi, bool bf) {
+  if (bf)
+    return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true)
+                                           : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
+  return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true)
+                                         : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false));
+}
+
+// Eight keys' elements of the products' type (8-bit codes: two words) -- exact in either type.
+template <int XT, int CT>
+__device__ __forceinline__ void key_operand(const uint32_t* w, uint32_t (&o)[4]) {
+  if constexpr (CT == DSV_E4M3) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = e4m3_pair(w[i / 2], i & 1, XT == DSV_BF16);
+  } else if constexpr (CT == DSV_I8 && XT == DSV_F16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      o[i] = i8_pair(__builtin_amdgcn_perm(0u, w[i / 2] ^ 0x80808080u, i & 1 ? 0x0c030c02u : 0x0c010c00u));
+  } else if constexpr (CT == DSV_I8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t x = w[i / 2] >> (16 * (i & 1));
+      const float lo = (float)(int8_t)x, hi = (float)(int8_t)(x >> 8);
+      o[i] = __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = w[i];
+  }
+}
+
+// Element e of eight positions' value words (wv[j]: position j's elements) in the positions' order.
+template <int CT, int W>
+__device__ __forceinline__ void value_operand(const uint32_t (&wv)[8][W], int e, uint32_t (&o)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (CT == DSV_I8) {
+      const uint32_t sel = 0x0c040c00u + (uint32_t)(e & 3) * 0x00010001u;
+      o[i] = i8_pair(__builtin_amdgcn_perm(wv[2 * i + 1][e / 4] ^ 0x80808080u, wv[2 * i][e / 4] ^ 0x80808080u, sel));
+    } else if constexpr (CT == DSV_E4M3) {
+      const uint32_t lo = e4m3_pair(wv[2 * i][e / 4], (e & 2) != 0, false);
+      const uint32_t hi = e4m3_pair(wv[2 * i + 1][e / 4], (e & 2) != 0, false);
+      o[i] = __builtin_amdgcn_perm(hi, lo, e & 1 ? 0x07060302u : 0x05040100u);
+    } else {
+      o[i] = __builtin_amdgcn_perm(wv[2 * i + 1][e / 2], wv[2 * i][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
+    }
+  }
+}
+
+__device__ __forceinline__ float across_groups_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, WAVE));
+  return fmaxf(v, __shfl_xor(v, 32, WAVE));
+}
+__device__ __forceinline__ float across_groups_sum(float v) {
+  v += __shfl_xor(v, 16, WAVE);
+  return v + __shfl_xor(v, 32, WAVE);
+}
+
+// The row of q of a request's node, or -1 where it lies outside.
+__device__ __forceinline__ int64_t row_of(const dsv_tree_attention_args& a, int64_t b, int node) {
+  const int64_t r = (a.row_offsets ? load_index(a.row_offsets, a.row_offsets_i64, b) : b * a.T) + node;
+  return r >= 0 && r < a.rows ? r : -1;
+}
+__device__ __forceinline__ uint64_t mask_of(const dsv_tree_attention_args& a, int64_t b, int node) {
+  if (a.masks) return (uint64_t)a.masks[b * a.T + node];
+  return node >= 63 ? ~0ull : (2ull << node) - 1ull;
+}
+
+template <int XT, int CT, int DP, bool FULL, int R, int OCC>
+__global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
+  const dsv_tree_attention_args& a = P.a;
+  const dsv_kv_cache& c = a.cache;
+  const int dim = FULL ? DP : c.dim;  // (a constant for the common sizes: no test of it in the loop)
+  constexpr bool QUANT = CT == DSV_E4M3 || CT == DSV_I8;
+  constexpr int PT = CT == DSV_BF16 ? DSV_BF16 : DSV_F16;  // the weights' type
+  // float16 weights are held 2^11 higher, so that what their range loses lies below 2^-35 of the row's largest
+  constexpr float SHIFT = PT == DSV_F16 ? 11.f : 0.f, LIM = PT == DSV_F16 ? 4.f : 8.f;
+  constexpr int ESZ = QUANT ? 1 : 2;
+  constexpr int EPL = DP / 16;            // value elements a lane loads of a position
+  constexpr int VW = EPL * ESZ / 4;       // words of them
+  constexpr int NK = DP / 32;             // key products of a tile
+  constexpr int KL = DP * ESZ / 64;       // 16-byte key loads a lane of a position
+  constexpr int OS = DP + 4;              // row stride of the sums in LDS
+  __shared__ float s_o[AT_WAVES][16][OS];
+  __shared__ float s_m[AT_WAVES][16 * R], s_l[AT_WAVES][16 * R];
+
+  const int tid = threadIdx.x, lane = tid & (WAVE - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);  // (and all that follows from it: scalar)
+  const int m = lane & 15, g = lane >> 4;
+  // Items round the XCDs, a request's heads and row blocks on one: they share its page table rows, scales and keys in
+  // that XCD's L2.
+  const int HB = c.heads * P.RB;
+  const int inner = (int)((blockIdx.x / 8) % HB), item = (int)((blockIdx.x / 8) / HB) * 8 + (int)(blockIdx.x % 8);
+  const int h = inner / P.RB, rb = inner - h * P.RB;
+  const int chunk = plan_chunk(P, lane);
+  int b, piece;
+  if (!item_at(P, chunk, item, lane, b, piece)) return;
+  b = __builtin_amdgcn_readfirstlane(b);
+  piece = __builtin_amdgcn_readfirstlane(piece);
+  const Request req = request_of(a, b);
+  const int n_rows = req.nodes * P.G, tiles = tiles_of(req), pieces = pieces_of(tiles, chunk);
+  const int WR = P.WR, WK = AT_WAVES / WR, wr = wave / WK, wk = wave - wr * WK;
+  const int block0 = rb * 16 * R * WR;
+  if (block0 >= n_rows) return;
+  const int row0 = block0 + wr * 16 * R;
+
+  // queries, in the order of the keys' elements
+  uint32_t qf[R][NK][4];
+#pragma unroll
+  for (int rt = 0; rt < R; ++rt) {
+    const int r = row0 + rt * 16 + m;
+    const int64_t row = r < n_rows ? row_of(a, b, r / P.G) : -1;
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (row < 0 ? 0 : row) * a.q_row_stride +
+                        (int64_t)(h * P.G + r % P.G) * a.q_head_stride;
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) {
+      const int d = QUANT ? (kk / 2) * 64 + g * 16 + (kk & 1) * 8 : kk * 32 + g * 8;
+      uint32_t w[4] = {0, 0, 0, 0};
+      if (row >= 0 && d < dim) load_words<4>(q + d, w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qf[rt][kk][i] = w[i];
+    }
+  }
+
+  const int32_t* table = a.page_table + (int64_t)b * a.page_stride;
+  const uint8_t* kbase = reinterpret_cast<const uint8_t*>(c.k) + (int64_t)h * c.k_head_stride * ESZ + g * 16;
+  const bool v_in = m * EPL < dim;  // (else the lane repeats the row's first piece: its sums are not stored)
+  const uint8_t* vbase = reinterpret_cast<const uint8_t*>(c.v) + (int64_t)h * c.v_head_stride * ESZ + (v_in ? m * EPL * ESZ : 0);
+  const float* ksc = QUANT ? c.k_scale + (int64_t)h * c.ks_head_stride : nullptr;
+  const float* vsc = QUANT ? c.v_scale + (int64_t)h * c.vs_head_stride : nullptr;
+  const float c0 = a.scale * 1.44269504088896340736f * (CT == DSV_I8 && XT == DSV_F16 ? I8_UNIT : 1.f);
+  const int clear = req.prefix;  // positions before it are seen by every row
+
+  f32x4 o[R][EPL];
+  float mref[R], l[R];
+  float vref = 0.f, vinv = 0.f;
+  bool fresh = true;  // some row has no reference yet
+#pragma unroll
+  for (int rt = 0; rt < R; ++rt) {
+    mref[rt] = AT_LOW;
+    l[rt] = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) o[rt][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  const int t0 = (int)((int64_t)tiles * piece / pieces), t1 = (int)((int64_t)tiles * (piece + 1) / pieces);
+  const int last = req.total - 1;
+  // a tile's slots: of the key rows m and 16 + m, and of this lane's eight positions g * 4 + j, 16 + g * 4 + j
+  auto load_slots = [&](int t, uint32_t (&ks)[2], uint32_t (&vs)[8]) {
+    const int32_t* from = table + t * AT_TILE;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ks[i] = (uint32_t)from[i * 16 + m];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint4 v;
+      __builtin_memcpy(&v, from + i * 16 + g * 4, 16);
+      vs[4 * i] = v.x, vs[4 * i + 1] = v.y, vs[4 * i + 2] = v.z, vs[4 * i + 3] = v.w;
+    }
+  };
+  auto load_some_slots = [&](int t, uint32_t (&ks)[2], uint32_t (&vs)[8]) {
+    const int base = t * AT_TILE;
+    auto at = [&](int p) { return p <= last ? (uint32_t)table[p] : ~0u; };
+#pragma unroll
+    for (int i = 0; i < 2; ++i) ks[i] = at(base + i * 16 + m);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) vs[j] = at(base + (j / 4) * 16 + g * 4 + (j & 3));
+  };
+  auto load_keys = [&](const uint32_t (&ks)[2], uint32_t (&kw)[2][KL][4]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t s = ks[i] < P.num_slots ? ks[i] : 0u;
+      const uint8_t* p = kbase + (uint64_t)s * P.k_step;
+#pragma unroll
+      for (int u = 0; u < KL; ++u)
+        if (u * 64 < dim * ESZ) {
+          // (past the row's end: its first piece, replaced by zeros before it is used)
+          load_words<4>(p + (u * 64 + g * 16 < dim * ESZ ? u * 64 : -(g * 16)), kw[i][u]);
+        }
+    }
+  };
+  auto load_scales = [&](const uint32_t (&vs)[8], float (&kf)[8], float (&vf)[8]) {
+    if constexpr (QUANT) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t s = vs[j] < P.num_slots ? vs[j] : 0u;
+        kf[j] = ksc[(int64_t)s * c.ks_slot_stride];
+        vf[j] = vsc[(int64_t)s * c.vs_slot_stride];
+      }
+    }
+  };
+
+  // The positions' factors of a score (base 2) and of a weight.  Value scales are taken relative to a power of two at or
+  // above the largest so far.
+  auto factors = [&](const float (&kf)[8], const float (&vf)[8], float (&cs)[8], float (&vn)[8]) {
+    if constexpr (QUANT) {
+      float top = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        cs[j] = kf[j] * c0;
+        const float v = fabsf(vf[j]);
+        top = fmaxf(top, v < INFINITY ? v : 0.f);
+      }
+      if (__any(top > vref)) {
+        top = wave_max_f32(top);
+        int ex;
+        (void)frexpf(top, &ex);
+        ex = ex > 120 ? 120 : (ex < -120 ? -120 : ex);
+        const float up = ldexpf(1.f, ex);
+        if (up > vref) {
+          const float keep = vref / up;
+#pragma unroll
+          for (int rt = 0; rt < R; ++rt)
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) o[rt][e] *= keep;
+          vref = up;
+          vinv = 1.f / up;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) vn[j] = vf[j] * vinv;
+    }
+  };
+  // A step: scores of a tile's keys, weights, weighted values.  WHOLE: every row sees every position.  `next` runs when
+  // the keys' registers are free.
+  auto step = [&](auto whole_, int base, const uint32_t (&kw)[2][KL][4], const uint32_t (&wv)[8][VW],
+                  const float (&cs)[8], const float (&vn)[8], uint32_t here, auto next) {
+    constexpr bool WHOLE = decltype(whole_)::value;
+    f32x4 s[R][2];
+#pragma unroll
+    for (int rt = 0; rt < R; ++rt)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) s[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) {
+      const int from = QUANT ? (kk / 2) * 64 : kk * 32, width = QUANT ? 64 : 32;  // elements of the loads behind it
+      if (from < dim) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t ko[4];
+          key_operand<XT, CT>(&kw[i][QUANT ? kk / 2 : kk][QUANT ? (kk & 1) * 2 : 0], ko);
+          if (from + width > dim)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) ko[u] = from + g * (width / 4) < dim ? ko[u] : 0u;
+#pragma unroll
+          for (int rt = 0; rt < R; ++rt) s[rt][i] = mfma<XT>(ko, qf[rt][kk], s[rt][i]);
+        }
+      }
+    }
+    next();
+    uint32_t seen[R];  // bit j: the row sees this lane's position j
+    if constexpr (!WHOLE) {
+#pragma unroll
+      for (int rt = 0; rt < R; ++rt) {
+        const int r = row0 + rt * 16 + m;
+        const uint64_t mask = r < n_rows ? mask_of(a, b, r / P.G) : 0ull;
+        uint32_t bits = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int p = base + (j / 4) * 16 + g * 4 + (j & 3) - req.prefix;
+          const bool sees = p < 0 || (p < 64 && ((mask >> (p & 63)) & 1));
+          bits |= (sees ? 1u : 0u) << j;
+        }
+        seen[rt] = bits & here;
+      }
+    }
+    // scores against the rows' references
+    float over = AT_LOW;
+#pragma unroll
+    for (int rt = 0; rt < R; ++rt) {
+      const float ref = mref[rt] == AT_LOW ? 0.f : mref[rt];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float x = fmaf(s[rt][j / 4][j & 3], QUANT ? cs[j] : c0, -ref);
+        if (!WHOLE && !((seen[rt] >> j) & 1)) x = -INFINITY;
+        s[rt][j / 4][j & 3] = x;
+        over = fmaxf(over, x);
+      }
+    }
+    if (fresh || __any(over > SHIFT + LIM)) {
+      bool none = false;
+#pragma unroll
+      for (int rt = 0; rt < R; ++rt) {
+        float top = AT_LOW;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, s[rt][j / 4][j & 3]);
+        top = across_groups_max(top);
+        const bool unset = mref[rt] == AT_LOW;
+        float move = top - SHIFT;  // of the reference: up, or anywhere from none
+        if (top == AT_LOW || (!unset && move < 0.f)) move = 0.f;
+        if (top != AT_LOW || !unset) mref[rt] = (unset ? 0.f : mref[rt]) + move;
+        none |= mref[rt] == AT_LOW;
+        const float keep = unset ? 0.f : __builtin_amdgcn_exp2f(-move);
+        l[rt] *= keep;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) o[rt][e] *= keep;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[rt][j / 4][j & 3] -= move;
+      }
+      fresh = __any(none);
+    }
+    uint32_t pf[R][4];
+#pragma unroll
+    for (int rt = 0; rt < R; ++rt) {
+      float w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        w[j] = __builtin_amdgcn_exp2f(s[rt][j / 4][j & 3]);
+        l[rt] += w[j];
+        if constexpr (QUANT) {
+          w[j] *= vn[j];
+          if (!WHOLE && !((seen[rt] >> j) & 1)) w[j] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) pf[rt][i] = pack_act<PT>(w[2 * i], w[2 * i + 1]);
+    }
+    // sums
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) {
+      uint32_t vo[4];
+      value_operand<CT, VW>(wv, e, vo);
+#pragma unroll
+      for (int rt = 0; rt < R; ++rt) o[rt][e] = mfma<PT>(vo, pf[rt], o[rt][e]);
+    }
+  };
+  auto load_values = [&](const uint32_t (&vs)[8], uint32_t (&wv)[8][VW]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t s = vs[j] < P.num_slots ? vs[j] : 0u;
+      load_words<VW>(vbase + (uint64_t)s * P.v_step, wv[j]);
+    }
+  };
+  // A value that is not finite reaches only the rows that see it (0 * NaN is NaN in the product, so it leaves the
+  // product): kinds of such values are noted for (row, element) in this wave's part of s_o, which is free until the end.
+  bool marked = false;
+  uint32_t* const marks = reinterpret_cast<uint32_t*>(&s_o[wave][0][0]);
+  static_assert(16 * R * DP <= 16 * OS * 4, "a byte for each row and element");
+  auto set_aside = [&](int base, uint32_t here, uint32_t (&wv)[8][VW]) {
+    if constexpr (CT != DSV_I8) {
+      constexpr uint32_t INF = CT == DSV_BF16 ? 0x7f80u : 0x7c00u;
+      // (16 bits: the halves' largest magnitude; codes: a carry into a byte's top bit where the others are ones)
+      uint32_t acc = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int u = 0; u < VW; ++u) {
+          if (!((here >> j) & 1)) wv[j][u] = 0u;  // (a position that holds nothing)
+          if constexpr (CT == DSV_E4M3) {
+            acc |= (wv[j][u] & 0x7f7f7f7fu) + 0x01010101u;
+          } else {
+            typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+            acc = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, acc),
+                                                                         __builtin_bit_cast(us2, wv[j][u] & 0x7fff7fffu)));
+          }
+        }
+      const bool odd = CT == DSV_E4M3 ? (acc & 0x80808080u) != 0 : (acc & 0xffffu) >= INF || (acc >> 16) >= INF;
+      if (!__any(odd)) return;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int u = 0; u < VW; ++u) {
+          const uint32_t w = wv[j][u];
+          if constexpr (CT == DSV_E4M3)
+            wv[j][u] = w & ~(((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu);
+          else
+            wv[j][u] = w & (((w & 0x7fffu) >= INF ? 0u : 0xffffu) | (((w >> 16) & 0x7fffu) >= INF ? 0u : 0xffff0000u));
+        }
+      if (!marked)
+        for (int i = lane; i < 16 * R * DP / 4; i += WAVE) marks[i] = 0u;
+      marked = true;
+      __builtin_amdgcn_wave_barrier();
+      const uint8_t* rows = reinterpret_cast<const uint8_t*>(c.v) + (int64_t)h * c.v_head_stride * ESZ;
+      for (int i = 0; i < AT_TILE && base + i <= last; ++i) {
+        const uint32_t slot = (uint32_t)table[base + i];
+        if (slot >= P.num_slots) continue;
+        const int p = base + i - req.prefix;
+        for (int d = lane; d < dim; d += WAVE) {
+          const uint8_t* at = rows + (uint64_t)slot * P.v_step + d * ESZ;
+          uint32_t kind = 0;
+          if constexpr (CT == DSV_E4M3) {
+            kind = (*at & 0x7fu) == 0x7fu ? 4u : 0u;
+          } else {
+            const uint32_t v = *reinterpret_cast<const uint16_t*>(at);
+            if ((v & 0x7fffu) >= INF) kind = (v & 0x7fffu) != INF ? 4u : 1u << (v >> 15);
+          }
+          if (!kind) continue;
+          for (int r = 0; r < 16 * R && row0 + r < n_rows; ++r)
+            if (p < 0 || (p < 64 && ((mask_of(a, b, (row0 + r) / P.G) >> (p & 63)) & 1)))
+              atomicOr(&marks[(r * DP + d) / 4], kind << (8 * (d & 3)));
+        }
+      }
+    }
+  };
+
+  int t = t0 + wk;
+  if (row0 >= n_rows) t = t1;
+  // The tiles of the context, while their slots are good: a tile's values are loaded at its beginning, the next one's
+  // keys and scales when its scores are done, the slots two tiles ahead.
+  const int whole = clear / AT_TILE < t1 ? clear / AT_TILE : t1;  // tiles before it lie in the context
+  if (t < whole) {
+    uint32_t ks0[2], vs0[8], ks1[2], vs1[8], kw[2][KL][4], wv[8][VW];
+    float kf[8], vf[8];
+    load_slots(t, ks0, vs0);
+    load_keys(ks0, kw);
+    load_scales(vs0, kf, vf);
+    load_slots(t + WK < whole ? t + WK : t, ks1, vs1);
+    for (; t < whole; t += WK) {
+      if (__any(ks0[0] >= P.num_slots || ks0[1] >= P.num_slots)) break;
+      load_values(vs0, wv);
+      float cs[8], vn[8];
+      factors(kf, vf, cs, vn);
+      step(Int<1>{}, t * AT_TILE, kw, wv, cs, vn, 0xffu, [&]() {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) ks0[i] = ks1[i];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) vs0[j] = vs1[j];
+        load_keys(ks0, kw);
+        load_scales(vs0, kf, vf);
+        load_slots(t + 2 * WK < whole ? t + 2 * WK : t, ks1, vs1);
+      });
+    }
+  }
+  // The window's tiles, and what follows a bad slot.
+  for (; t < t1; t += WK) {
+    uint32_t ks0[2], vs0[8], kw[2][KL][4], wv[8][VW];
+    float kf[8], vf[8];
+    load_some_slots(t, ks0, vs0);
+    load_keys(ks0, kw);
+    load_scales(vs0, kf, vf);
+    load_values(vs0, wv);
+    uint32_t here = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) here |= (vs0[j] < P.num_slots ? 1u : 0u) << j;
+    float cs[8], vn[8];
+    factors(kf, vf, cs, vn);
+    set_aside(t * AT_TILE, here, wv);
+    step(Int<0>{}, t * AT_TILE, kw, wv, cs, vn, here, [] {});
+  }
+
+  if (marked) {
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int rt = 0; rt < R; ++rt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) {
+          const int at = (rt * 16 + m) * DP + (g * 4 + r) * EPL + e;
+          const uint32_t kind = (marks[at / 4] >> (8 * (at & 3))) & 7u;
+          if (kind & 1) o[rt][e][r] += INFINITY;
+          if (kind & 2) o[rt][e][r] -= INFINITY;
+          if (kind & 4) o[rt][e][r] = NAN;
+        }
+  }
+  // The waves of the same rows join: their references, then the sums of one row tile after another through LDS.
+#pragma unroll
+  for (int rt = 0; rt < R; ++rt) {
+    l[rt] = across_groups_sum(l[rt]);
+    if (g == 0) {
+      s_m[wave][rt * 16 + m] = mref[rt];
+      s_l[wave][rt * 16 + m] = l[rt];
+    }
+  }
+  __syncthreads();
+  const float unit = QUANT ? vref * (CT == DSV_I8 ? I8_UNIT : 1.f) : 1.f;
+#pragma unroll
+  for (int rt = 0; rt < R; ++rt) {
+    float top = AT_LOW;
+    for (int k = 0; k < WK; ++k) top = fmaxf(top, s_m[wr * WK + k][rt * 16 + m]);
+    const float f = __builtin_amdgcn_exp2f(mref[rt] - top) * unit;
+    if (rt) __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int e = 0; e < EPL; e += 4)
+        *reinterpret_cast<float4*>(&s_o[wave][m][(g * 4 + r) * EPL + e]) =
+            make_float4(o[rt][e][r] * f, o[rt][e + 1][r] * f, o[rt][e + 2][r] * f, o[rt][e + 3][r] * f);
+    __syncthreads();
+    for (int i = tid - wr * WK * WAVE; i < 16 * DP / 8; i += WK * WAVE) {
+      const int rr = i / (DP / 8), d = i % (DP / 8) * 8, r = row0 + rt * 16 + rr;
+      if (r >= n_rows || d >= dim) continue;
+      float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      float mt = AT_LOW, lt = 0.f;
+      for (int k = 0; k < WK; ++k) mt = fmaxf(mt, s_m[wr * WK + k][rt * 16 + rr]);
+      for (int k = 0; k < WK; ++k) {
+        lt += s_l[wr * WK + k][rt * 16 + rr] * __builtin_amdgcn_exp2f(s_m[wr * WK + k][rt * 16 + rr] - mt);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) sum[u] += s_o[wr * WK + k][rr][d + u];
+      }
+      if (pieces > 1) {
+        const int64_t at = ((int64_t)item * c.heads + h) * (a.T * P.G) + r;
+        float* po = P.part_o + at * dim + d;
+        *reinterpret_cast<float4*>(po) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+        *reinterpret_cast<float4*>(po + 4) = make_float4(sum[4], sum[5], sum[6], sum[7]);
+        if (d == 0) P.part_ml[at] = make_float2(mt, lt);
+      } else {
+        const int node = r / P.G, qh = h * P.G + r - node * P.G;
+        const int64_t row = row_of(a, b, node);
+        if (row < 0) continue;
+        const float inv = lt == 0.f ? 0.f : 1.f / lt;
+        uint4 v;
+        v.x = pack_act<XT>(sum[0] * inv, sum[1] * inv);
+        v.y = pack_act<XT>(sum[2] * inv, sum[3] * inv);
+        v.z = pack_act<XT>(sum[4] * inv, sum[5] * inv);
+        v.w = pack_act<XT>(sum[6] * inv, sum[7] * inv);
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + row * a.out_row_stride + qh * a.out_head_stride + d) = v;
+        if (d == 0 && a.lse) a.lse[row * a.q_heads + qh] = lt == 0.f ? -INFINITY : (mt + log2f(lt)) * 0.693147180559945309f;
+      }
+    }
+  }
+}
+
+// Row tiles a wave, waves over the rows and row blocks of T nodes with G query heads each.
+struct AttnShape {
+  int R, WR, RB;
+};
+
+template <int XT, int CT>
+void launch_attn(const AttnParams& P, const AttnShape& s, unsigned blocks, hipStream_t stream) {
+  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(blocks), dim3(AT_THREADS), 0, stream, P); };
+  const int D = P.a.cache.dim;
+  auto width = [&](auto dp, auto full) {
+    constexpr int DP = decltype(dp)::value;
+    constexpr bool FULL = decltype(full)::value;
+    if constexpr (DP > 128)
+      s.R == 1 ? go(k_attn<XT, CT, DP, FULL, 1, 1>) : go(k_attn<XT, CT, DP, FULL, 2, 1>);
+    else
+      s.R == 1   ? go(k_attn<XT, CT, DP, FULL, 1, 2>)
+      : s.R == 2 ? go(k_attn<XT, CT, DP, FULL, 2, 2>)
+                 : go(k_attn<XT, CT, DP, FULL, 4, 1>);
+  };
+  if (D <= 64)
+    D == 64 ? width(Int<64>{}, Int<1>{}) : width(Int<64>{}, Int<0>{});
+  else if (D <= 128)
+    D == 128 ? width(Int<128>{}, Int<1>{}) : width(Int<128>{}, Int<0>{});
+  else
+    D == 256 ? width(Int<256>{}, Int<1>{}) : width(Int<256>{}, Int<0>{});
+}
+
+}  // namespace dsv
