@@ -7,9 +7,13 @@
 //
 // The matrix cores take keys as they lie in memory: S^T = K Q^T with the positions on the rows of the tile, so that a
 // lane holds, for one query row, the weights of the four (twice: eight) positions that the second product
-// O^T = V^T P^T wants from it: no weight moves between lanes.  Keys go from memory to the operand registers; values
-// too, as 16-byte pieces of whole rows whose 16-bit elements a v_perm each puts in the positions' order.  Nothing is
-// staged in LDS, the waves run free of each other, and each holds all its rows' sums in registers.
+// O^T = V^T P^T wants from it: no weight moves between lanes.  Values come as 16-byte pieces of whole rows, whose
+// elements a v_perm each puts in the positions' order.  Two forms of one kernel:
+//   direct   (few rows) every wave loads the operands of its own positions from memory to registers; the waves run free
+//            of each other and join at the end
+//   staged   the workgroup's waves share their positions and split the rows: each wave brings a quarter of a tile
+//            of 64 positions from memory, converts it to the operands' 16-bit layout once and puts it into LDS (two
+//            buffers), from where every wave reads whole operands without bank conflicts
 //
 // The positions of a batch are cut into about `target` equal pieces (a rule on the lengths, which only the device
 // knows: every workgroup computes the same plan from them); pieces of a request are joined by k_attn_join.
@@ -22,7 +26,8 @@ namespace dsv {
 constexpr int AT_THREADS = 256;
 constexpr int AT_WAVES = AT_THREADS / WAVE;
 constexpr int AT_NODES = 64;
-constexpr int AT_TILE = 32;  // positions of a step
+constexpr int AT_STEP = 32;  // positions of a step: two tiles of the first product, one of the second
+constexpr int AT_TILE = 64;  // positions of a plan's unit, and of a staged tile
 constexpr float AT_LOW = -3e38f;
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -32,7 +37,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct AttnParams {
   dsv_tree_attention_args a;
-  int G, WR, RB;       // query heads a cache head; waves over the rows, row blocks of a request
+  int G, WR, RB;       // query heads a cache head; waves over the rows; row blocks of a request
   int target;          // pieces aimed at
   int least;           // tiles of a piece at least
   int joined;          // whether a request may have several pieces
@@ -160,11 +165,11 @@ __device__ __forceinline__ void key_operand(const uint32_t* w, uint32_t (&o)[4])
   }
 }
 
-// Element e of eight positions' value words (wv[j]: position j's elements) in the positions' order.
-template <int CT, int W>
-__device__ __forceinline__ void value_operand(const uint32_t (&wv)[8][W], int e, uint32_t (&o)[4]) {
+// Element e of N positions' value words (wv[j]: position j's elements) in the positions' order.
+template <int CT, int N, int W>
+__device__ __forceinline__ void value_operand(const uint32_t (&wv)[N][W], int e, uint32_t (&o)[N / 2]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < N / 2; ++i) {
     if constexpr (CT == DSV_I8) {
       const uint32_t sel = 0x0c040c00u + (uint32_t)(e & 3) * 0x00010001u;
       o[i] = i8_pair(__builtin_amdgcn_perm(wv[2 * i + 1][e / 4] ^ 0x80808080u, wv[2 * i][e / 4] ^ 0x80808080u, sel));
@@ -187,6 +192,20 @@ __device__ __forceinline__ float across_groups_sum(float v) {
   return v + __shfl_xor(v, 32, WAVE);
 }
 
+// An element of the cache's rows.
+template <int CT>
+__device__ __forceinline__ float cache_value(const void* row, int i) {
+  if constexpr (CT == DSV_E4M3) {
+    float f[4];
+    unpack_codes<CT>(reinterpret_cast<const uint8_t*>(row)[i], f);
+    return f[0];
+  } else if constexpr (CT == DSV_I8) {
+    return (float)reinterpret_cast<const int8_t*>(row)[i];
+  } else {
+    return act_to_f32<CT>(reinterpret_cast<const uint16_t*>(row)[i]);
+  }
+}
+
 // The row of q of a request's node, or -1 where it lies outside.
 __device__ __forceinline__ int64_t row_of(const dsv_tree_attention_args& a, int64_t b, int node) {
   const int64_t r = (a.row_offsets ? load_index(a.row_offsets, a.row_offsets_i64, b) : b * a.T) + node;
@@ -197,7 +216,7 @@ __device__ __forceinline__ uint64_t mask_of(const dsv_tree_attention_args& a, in
   return node >= 63 ? ~0ull : (2ull << node) - 1ull;
 }
 
-template <int XT, int CT, int DP, bool FULL, int R, int OCC>
+template <int XT, int CT, int DP, bool FULL, int R, bool STAGED, int OCC>
 __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
   const dsv_tree_attention_args& a = P.a;
   const dsv_kv_cache& c = a.cache;
@@ -209,11 +228,17 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
   constexpr int ESZ = QUANT ? 1 : 2;
   constexpr int EPL = DP / 16;            // value elements a lane loads of a position
   constexpr int VW = EPL * ESZ / 4;       // words of them
-  constexpr int NK = DP / 32;             // key products of a tile
+  constexpr int NK = DP / 32;             // key products of a step
   constexpr int KL = DP * ESZ / 64;       // 16-byte key loads a lane of a position
   constexpr int OS = DP + 4;              // row stride of the sums in LDS
-  __shared__ float s_o[AT_WAVES][16][OS];
+  constexpr int SET_ASIDE = STAGED ? AT_TILE : AT_STEP;
+  constexpr int FRAGS = 4 * NK + 2 * EPL;  // operands of a staged tile: keys, then values, 16 bytes a lane each (values as
+                                           // two halves of 8, so that their writes find all banks)
+  constexpr size_t SUMS = sizeof(float) * AT_WAVES * 16 * OS, TILES = STAGED ? sizeof(uint4) * 2 * FRAGS * WAVE : 0;
+  __shared__ __attribute__((aligned(16))) unsigned char s_mem[SUMS > TILES ? SUMS : TILES];
   __shared__ float s_m[AT_WAVES][16 * R], s_l[AT_WAVES][16 * R];
+  __shared__ int s_odd;
+  float(*const s_o)[16][OS] = reinterpret_cast<float(*)[16][OS]>(s_mem);
 
   const int tid = threadIdx.x, lane = tid & (WAVE - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);  // (and all that follows from it: scalar)
@@ -234,6 +259,7 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
   const int block0 = rb * 16 * R * WR;
   if (block0 >= n_rows) return;
   const int row0 = block0 + wr * 16 * R;
+  if (tid == 0) s_odd = 0;
 
   // queries, in the order of the keys' elements
   uint32_t qf[R][NK][4];
@@ -256,7 +282,8 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
   const int32_t* table = a.page_table + (int64_t)b * a.page_stride;
   const uint8_t* kbase = reinterpret_cast<const uint8_t*>(c.k) + (int64_t)h * c.k_head_stride * ESZ + g * 16;
   const bool v_in = m * EPL < dim;  // (else the lane repeats the row's first piece: its sums are not stored)
-  const uint8_t* vbase = reinterpret_cast<const uint8_t*>(c.v) + (int64_t)h * c.v_head_stride * ESZ + (v_in ? m * EPL * ESZ : 0);
+  const uint8_t* vhead = reinterpret_cast<const uint8_t*>(c.v) + (int64_t)h * c.v_head_stride * ESZ;
+  const uint8_t* vbase = vhead + (v_in ? m * EPL * ESZ : 0);
   const float* ksc = QUANT ? c.k_scale + (int64_t)h * c.ks_head_stride : nullptr;
   const float* vsc = QUANT ? c.v_scale + (int64_t)h * c.vs_head_stride : nullptr;
   const float c0 = a.scale * 1.44269504088896340736f * (CT == DSV_I8 && XT == DSV_F16 ? I8_UNIT : 1.f);
@@ -276,50 +303,83 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
 
   const int t0 = (int)((int64_t)tiles * piece / pieces), t1 = (int)((int64_t)tiles * (piece + 1) / pieces);
   const int last = req.total - 1;
-  // a tile's slots: of the key rows m and 16 + m, and of this lane's eight positions g * 4 + j, 16 + g * 4 + j
-  auto load_slots = [&](int t, uint32_t (&ks)[2], uint32_t (&vs)[8]) {
-    const int32_t* from = table + t * AT_TILE;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) ks[i] = (uint32_t)from[i * 16 + m];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint4 v;
-      __builtin_memcpy(&v, from + i * 16 + g * 4, 16);
-      vs[4 * i] = v.x, vs[4 * i + 1] = v.y, vs[4 * i + 2] = v.z, vs[4 * i + 3] = v.w;
+  auto good = [&](uint32_t slot) { return slot < P.num_slots; };
+  // the slots of 32 positions from `base`: of the key rows m and 16 + m, and of this lane's eight positions
+  // g * 4 + j, 16 + g * 4 + j (j < 4); the others' entries are not touched
+  auto key_slots = [&](int base, uint32_t& k0, uint32_t& k1) {
+    if (base + AT_STEP <= req.total) {
+      k0 = (uint32_t)table[base + m];
+      k1 = (uint32_t)table[base + 16 + m];
+    } else {
+      k0 = base + m <= last ? (uint32_t)table[base + m] : ~0u;
+      k1 = base + 16 + m <= last ? (uint32_t)table[base + 16 + m] : ~0u;
     }
   };
-  auto load_some_slots = [&](int t, uint32_t (&ks)[2], uint32_t (&vs)[8]) {
-    const int base = t * AT_TILE;
-    auto at = [&](int p) { return p <= last ? (uint32_t)table[p] : ~0u; };
+  auto value_slots = [&](auto whole_, int base, uint32_t (&vs)[8]) {
+    if (decltype(whole_)::value || base + AT_STEP <= req.total) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) ks[i] = at(base + i * 16 + m);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) vs[j] = at(base + (j / 4) * 16 + g * 4 + (j & 3));
-  };
-  auto load_keys = [&](const uint32_t (&ks)[2], uint32_t (&kw)[2][KL][4]) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint32_t s = ks[i] < P.num_slots ? ks[i] : 0u;
-      const uint8_t* p = kbase + (uint64_t)s * P.k_step;
-#pragma unroll
-      for (int u = 0; u < KL; ++u)
-        if (u * 64 < dim * ESZ) {
-          // (past the row's end: its first piece, replaced by zeros before it is used)
-          load_words<4>(p + (u * 64 + g * 16 < dim * ESZ ? u * 64 : -(g * 16)), kw[i][u]);
-        }
-    }
-  };
-  auto load_scales = [&](const uint32_t (&vs)[8], float (&kf)[8], float (&vf)[8]) {
-    if constexpr (QUANT) {
+      for (int i = 0; i < 2; ++i) {
+        uint4 v;
+        __builtin_memcpy(&v, table + base + i * 16 + g * 4, 16);
+        vs[4 * i] = v.x, vs[4 * i + 1] = v.y, vs[4 * i + 2] = v.z, vs[4 * i + 3] = v.w;
+      }
+    } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t s = vs[j] < P.num_slots ? vs[j] : 0u;
-        kf[j] = ksc[(int64_t)s * c.ks_slot_stride];
-        vf[j] = vsc[(int64_t)s * c.vs_slot_stride];
+        const int p = base + (j / 4) * 16 + g * 4 + (j & 3);
+        vs[j] = p <= last ? (uint32_t)table[p] : ~0u;
       }
     }
   };
-
+  auto load_key = [&](uint32_t slot, uint32_t (&kw)[KL][4]) {
+    const uint8_t* p = kbase + (uint64_t)(good(slot) ? slot : 0u) * P.k_step;
+#pragma unroll
+    for (int u = 0; u < KL; ++u)
+      if (u * 64 < dim * ESZ)  // (past the row's end: its first piece, replaced by zeros before it is used)
+        load_words<4>(p + (u * 64 + g * 16 < dim * ESZ ? u * 64 : -(g * 16)), kw[u]);
+  };
+  auto load_value = [&](uint32_t slot, uint32_t (&wv)[VW]) {
+    load_words<VW>(vbase + (uint64_t)(good(slot) ? slot : 0u) * P.v_step, wv);
+  };
+  // the operand of key product kk
+  auto key_frag = [&](const uint32_t (&kw)[KL][4], int kk, uint32_t (&ko)[4]) {
+    const int from = QUANT ? (kk / 2) * 64 : kk * 32, width = QUANT ? 64 : 32;  // elements of the loads behind it
+    if (from >= dim) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) ko[u] = 0u;
+      return;
+    }
+    key_operand<XT, CT>(&kw[QUANT ? kk / 2 : kk][QUANT ? (kk & 1) * 2 : 0], ko);
+    if (from + width > dim)
+#pragma unroll
+      for (int u = 0; u < 4; ++u) ko[u] = from + g * (width / 4) < dim ? ko[u] : 0u;
+  };
+  // Values of positions that hold nothing (bits of `here` unset) become zeros, and so do values that are not finite
+  // where not every row sees them (0 * NaN is NaN in the product): the rows that do get them at the end.
+  auto clear_values = [&](uint32_t here, bool aside, auto& wv) {
+    constexpr int N = sizeof(wv) / sizeof(wv[0]);
+    constexpr uint32_t INF = CT == DSV_BF16 ? 0x7f80u : 0x7c00u;
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int u = 0; u < VW; ++u) {
+        uint32_t w = (here >> j) & 1 ? wv[j][u] : 0u;
+        if constexpr (CT != DSV_I8) {
+          if (aside) {
+            uint32_t bad;
+            if constexpr (CT == DSV_E4M3)
+              bad = ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu;
+            else
+              bad = ((w & 0x7fffu) >= INF ? 0xffffu : 0u) | (((w >> 16) & 0x7fffu) >= INF ? 0xffff0000u : 0u);
+            odd |= bad != 0;
+            w &= ~bad;
+          }
+        }
+        wv[j][u] = w;
+      }
+    if (odd) s_odd = 1;
+  };
   // The positions' factors of a score (base 2) and of a weight.  Value scales are taken relative to a power of two at or
   // above the largest so far.
   auto factors = [&](const float (&kf)[8], const float (&vf)[8], float (&cs)[8], float (&vn)[8]) {
@@ -351,10 +411,10 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
       for (int j = 0; j < 8; ++j) vn[j] = vf[j] * vinv;
     }
   };
-  // A step: scores of a tile's keys, weights, weighted values.  WHOLE: every row sees every position.  `next` runs when
-  // the keys' registers are free.
-  auto step = [&](auto whole_, int base, const uint32_t (&kw)[2][KL][4], const uint32_t (&wv)[8][VW],
-                  const float (&cs)[8], const float (&vn)[8], uint32_t here, auto next) {
+  // A step: scores of 32 positions' keys, weights, weighted values.  WHOLE: every row sees every position that holds
+  // anything (bit j of `here`: this lane's position j does).  `next` runs when the keys have been used.
+  auto step = [&](auto whole_, int base, uint32_t here, const float (&cs)[8], const float (&vn)[8], auto key, auto value,
+                  auto next) {
     constexpr bool WHOLE = decltype(whole_)::value;
     f32x4 s[R][2];
 #pragma unroll
@@ -362,21 +422,14 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) s[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int kk = 0; kk < NK; ++kk) {
-      const int from = QUANT ? (kk / 2) * 64 : kk * 32, width = QUANT ? 64 : 32;  // elements of the loads behind it
-      if (from < dim) {
+    for (int kk = 0; kk < NK; ++kk)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t ko[4];
-          key_operand<XT, CT>(&kw[i][QUANT ? kk / 2 : kk][QUANT ? (kk & 1) * 2 : 0], ko);
-          if (from + width > dim)
+      for (int i = 0; i < 2; ++i) {
+        uint32_t ko[4];
+        key(i, kk, ko);
 #pragma unroll
-            for (int u = 0; u < 4; ++u) ko[u] = from + g * (width / 4) < dim ? ko[u] : 0u;
-#pragma unroll
-          for (int rt = 0; rt < R; ++rt) s[rt][i] = mfma<XT>(ko, qf[rt][kk], s[rt][i]);
-        }
+        for (int rt = 0; rt < R; ++rt) s[rt][i] = mfma<XT>(ko, qf[rt][kk], s[rt][i]);
       }
-    }
     next();
     uint32_t seen[R];  // bit j: the row sees this lane's position j
     if constexpr (!WHOLE) {
@@ -406,6 +459,16 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
         s[rt][j / 4][j & 3] = x;
         over = fmaxf(over, x);
       }
+    }
+    if (WHOLE && __any(here != 0xffu)) {
+      over = AT_LOW;
+#pragma unroll
+      for (int rt = 0; rt < R; ++rt)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (!((here >> j) & 1)) s[rt][j / 4][j & 3] = -INFINITY;
+          over = fmaxf(over, s[rt][j / 4][j & 3]);
+        }
     }
     if (fresh || __any(over > SHIFT + LIM)) {
       bool none = false;
@@ -445,144 +508,201 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) pf[rt][i] = pack_act<PT>(w[2 * i], w[2 * i + 1]);
     }
-    // sums
 #pragma unroll
     for (int e = 0; e < EPL; ++e) {
       uint32_t vo[4];
-      value_operand<CT, VW>(wv, e, vo);
+      value(e, vo);
 #pragma unroll
       for (int rt = 0; rt < R; ++rt) o[rt][e] = mfma<PT>(vo, pf[rt], o[rt][e]);
     }
   };
-  auto load_values = [&](const uint32_t (&vs)[8], uint32_t (&wv)[8][VW]) {
+
+  if constexpr (!STAGED) {
+    // (scales of positions that hold nothing are zeros)
+    auto load_scales = [&](const uint32_t (&vs)[8], float (&kf)[8], float (&vf)[8]) {
+      if constexpr (QUANT) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t s = vs[j] < P.num_slots ? vs[j] : 0u;
-      load_words<VW>(vbase + (uint64_t)s * P.v_step, wv[j]);
-    }
-  };
-  // A value that is not finite reaches only the rows that see it (0 * NaN is NaN in the product, so it leaves the
-  // product): kinds of such values are noted for (row, element) in this wave's part of s_o, which is free until the end.
-  bool marked = false;
-  uint32_t* const marks = reinterpret_cast<uint32_t*>(&s_o[wave][0][0]);
-  static_assert(16 * R * DP <= 16 * OS * 4, "a byte for each row and element");
-  auto set_aside = [&](int base, uint32_t here, uint32_t (&wv)[8][VW]) {
-    if constexpr (CT != DSV_I8) {
-      constexpr uint32_t INF = CT == DSV_BF16 ? 0x7f80u : 0x7c00u;
-      // (16 bits: the halves' largest magnitude; codes: a carry into a byte's top bit where the others are ones)
-      uint32_t acc = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int u = 0; u < VW; ++u) {
-          if (!((here >> j) & 1)) wv[j][u] = 0u;  // (a position that holds nothing)
-          if constexpr (CT == DSV_E4M3) {
-            acc |= (wv[j][u] & 0x7f7f7f7fu) + 0x01010101u;
-          } else {
-            typedef unsigned short us2 __attribute__((ext_vector_type(2)));
-            acc = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(us2, acc),
-                                                                         __builtin_bit_cast(us2, wv[j][u] & 0x7fff7fffu)));
-          }
-        }
-      const bool odd = CT == DSV_E4M3 ? (acc & 0x80808080u) != 0 : (acc & 0xffffu) >= INF || (acc >> 16) >= INF;
-      if (!__any(odd)) return;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int u = 0; u < VW; ++u) {
-          const uint32_t w = wv[j][u];
-          if constexpr (CT == DSV_E4M3)
-            wv[j][u] = w & ~(((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 0xffu);
-          else
-            wv[j][u] = w & (((w & 0x7fffu) >= INF ? 0u : 0xffffu) | (((w >> 16) & 0x7fffu) >= INF ? 0u : 0xffff0000u));
-        }
-      if (!marked)
-        for (int i = lane; i < 16 * R * DP / 4; i += WAVE) marks[i] = 0u;
-      marked = true;
-      __builtin_amdgcn_wave_barrier();
-      const uint8_t* rows = reinterpret_cast<const uint8_t*>(c.v) + (int64_t)h * c.v_head_stride * ESZ;
-      for (int i = 0; i < AT_TILE && base + i <= last; ++i) {
-        const uint32_t slot = (uint32_t)table[base + i];
-        if (slot >= P.num_slots) continue;
-        const int p = base + i - req.prefix;
-        for (int d = lane; d < dim; d += WAVE) {
-          const uint8_t* at = rows + (uint64_t)slot * P.v_step + d * ESZ;
-          uint32_t kind = 0;
-          if constexpr (CT == DSV_E4M3) {
-            kind = (*at & 0x7fu) == 0x7fu ? 4u : 0u;
-          } else {
-            const uint32_t v = *reinterpret_cast<const uint16_t*>(at);
-            if ((v & 0x7fffu) >= INF) kind = (v & 0x7fffu) != INF ? 4u : 1u << (v >> 15);
-          }
-          if (!kind) continue;
-          for (int r = 0; r < 16 * R && row0 + r < n_rows; ++r)
-            if (p < 0 || (p < 64 && ((mask_of(a, b, (row0 + r) / P.G) >> (p & 63)) & 1)))
-              atomicOr(&marks[(r * DP + d) / 4], kind << (8 * (d & 3)));
+        for (int j = 0; j < 8; ++j) {
+          const bool ok = good(vs[j]);
+          const uint32_t s = ok ? vs[j] : 0u;
+          kf[j] = ksc[(int64_t)s * c.ks_slot_stride];
+          vf[j] = vsc[(int64_t)s * c.vs_slot_stride];
+          if (!ok) kf[j] = vf[j] = 0.f;
         }
       }
+    };
+    auto holds = [&](const uint32_t (&vs)[8]) {
+      uint32_t here = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) here |= (good(vs[j]) ? 1u : 0u) << j;
+      return here;
+    };
+    // steps of this wave: every WK-th
+    int t = t0 * (AT_TILE / AT_STEP) + wk;
+    int end = t1 * (AT_TILE / AT_STEP);
+    const int some = (req.total + AT_STEP - 1) / AT_STEP;
+    end = end < some ? end : some;
+    if (row0 >= n_rows) t = end;
+    // Those in the context: a step's values are loaded at its beginning, the next one's keys and scales when its scores
+    // are done, the slots two steps ahead.
+    const int whole = clear / AT_STEP < end ? clear / AT_STEP : end;
+    if (t < whole) {
+      uint32_t ks[2], vs0[8], vs1[8], kw[2][KL][4], wv[8][VW];
+      float kf[8], vf[8], cs[8], vn[8];
+      key_slots(t * AT_STEP, ks[0], ks[1]);
+      value_slots(Int<1>{}, t * AT_STEP, vs0);
+      load_key(ks[0], kw[0]);
+      load_key(ks[1], kw[1]);
+      load_scales(vs0, kf, vf);
+      key_slots((t + WK < whole ? t + WK : t) * AT_STEP, ks[0], ks[1]);
+      value_slots(Int<1>{}, (t + WK < whole ? t + WK : t) * AT_STEP, vs1);
+      for (; t < whole; t += WK) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) load_value(vs0[j], wv[j]);
+        const uint32_t here = holds(vs0);
+        if (__any(here != 0xffu)) clear_values(here, false, wv);
+        factors(kf, vf, cs, vn);
+        step(Int<1>{}, t * AT_STEP, here, cs, vn, [&](int i, int kk, uint32_t (&ko)[4]) { key_frag(kw[i], kk, ko); },
+             [&](int e, uint32_t (&vo)[4]) { value_operand<CT>(wv, e, vo); },
+             [&]() {
+               load_key(ks[0], kw[0]);
+               load_key(ks[1], kw[1]);
+#pragma unroll
+               for (int j = 0; j < 8; ++j) vs0[j] = vs1[j];
+               load_scales(vs0, kf, vf);
+               const int ahead = t + 2 * WK < whole ? t + 2 * WK : t;
+               ks[0] = (uint32_t)table[ahead * AT_STEP + m];
+               ks[1] = (uint32_t)table[ahead * AT_STEP + 16 + m];
+               value_slots(Int<1>{}, ahead * AT_STEP, vs1);
+             });
+      }
     }
-  };
-
-  int t = t0 + wk;
-  if (row0 >= n_rows) t = t1;
-  // The tiles of the context, while their slots are good: a tile's values are loaded at its beginning, the next one's
-  // keys and scales when its scores are done, the slots two tiles ahead.
-  const int whole = clear / AT_TILE < t1 ? clear / AT_TILE : t1;  // tiles before it lie in the context
-  if (t < whole) {
-    uint32_t ks0[2], vs0[8], ks1[2], vs1[8], kw[2][KL][4], wv[8][VW];
-    float kf[8], vf[8];
-    load_slots(t, ks0, vs0);
-    load_keys(ks0, kw);
-    load_scales(vs0, kf, vf);
-    load_slots(t + WK < whole ? t + WK : t, ks1, vs1);
-    for (; t < whole; t += WK) {
-      if (__any(ks0[0] >= P.num_slots || ks0[1] >= P.num_slots)) break;
-      load_values(vs0, wv);
-      float cs[8], vn[8];
+    // The window's.
+    for (; t < end; t += WK) {
+      uint32_t ks[2], vs[8], kw[2][KL][4], wv[8][VW];
+      float kf[8], vf[8], cs[8], vn[8];
+      const int base = t * AT_STEP;
+      key_slots(base, ks[0], ks[1]);
+      value_slots(Int<0>{}, base, vs);
+      load_key(ks[0], kw[0]);
+      load_key(ks[1], kw[1]);
+      load_scales(vs, kf, vf);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) load_value(vs[j], wv[j]);
+      const uint32_t here = holds(vs);
+      clear_values(here, true, wv);
       factors(kf, vf, cs, vn);
-      step(Int<1>{}, t * AT_TILE, kw, wv, cs, vn, 0xffu, [&]() {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) ks0[i] = ks1[i];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) vs0[j] = vs1[j];
-        load_keys(ks0, kw);
-        load_scales(vs0, kf, vf);
-        load_slots(t + 2 * WK < whole ? t + 2 * WK : t, ks1, vs1);
-      });
+      step(Int<0>{}, base, here, cs, vn, [&](int i, int kk, uint32_t (&ko)[4]) { key_frag(kw[i], kk, ko); },
+           [&](int e, uint32_t (&vo)[4]) { value_operand<CT>(wv, e, vo); }, [] {});
     }
-  }
-  // The window's tiles, and what follows a bad slot.
-  for (; t < t1; t += WK) {
-    uint32_t ks0[2], vs0[8], kw[2][KL][4], wv[8][VW];
-    float kf[8], vf[8];
-    load_some_slots(t, ks0, vs0);
-    load_keys(ks0, kw);
-    load_scales(vs0, kf, vf);
-    load_values(vs0, wv);
-    uint32_t here = 0;
+  } else {
+    uint4(*const s_frag)[FRAGS][WAVE] = reinterpret_cast<uint4(*)[FRAGS][WAVE]>(s_mem);
+    __shared__ float s_scale[2][2][AT_TILE];
+    __shared__ uint32_t s_here[2][AT_WAVES];
+    // A wave brings 16 positions: lane (m, g) pieces of the key of position m, and of the values of g * 4 .. g * 4 + 3.
+    uint32_t kw[KL][4], wv[4][VW], kslot = ~0u, vslot[4];
+    uint32_t have = 0;  // bits of the 16 positions
+    float scale = 0.f;
+    auto fetch_slots = [&](int t) {
+      const int base = t * AT_TILE + wave * 16;
+      if (base + 16 <= req.total) {
+        kslot = (uint32_t)table[base + m];
+        uint4 v;
+        __builtin_memcpy(&v, table + base + g * 4, 16);
+        vslot[0] = v.x, vslot[1] = v.y, vslot[2] = v.z, vslot[3] = v.w;
+      } else {
+        kslot = base + m <= last ? (uint32_t)table[base + m] : ~0u;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) here |= (vs0[j] < P.num_slots ? 1u : 0u) << j;
-    float cs[8], vn[8];
-    factors(kf, vf, cs, vn);
-    set_aside(t * AT_TILE, here, wv);
-    step(Int<0>{}, t * AT_TILE, kw, wv, cs, vn, here, [] {});
+        for (int j = 0; j < 4; ++j) vslot[j] = base + g * 4 + j <= last ? (uint32_t)table[base + g * 4 + j] : ~0u;
+      }
+    };
+    auto fetch = [&]() {
+      load_key(kslot, kw);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) load_value(vslot[j], wv[j]);
+      have = (uint32_t)__ballot(good(kslot)) & 0xffffu;
+      if constexpr (QUANT) {
+        const int64_t s = good(kslot) ? kslot : 0u;
+        if (g < 2) scale = g == 0 ? ksc[s * c.ks_slot_stride] : vsc[s * c.vs_slot_stride];
+        if (!good(kslot)) scale = 0.f;
+      }
+    };
+    auto put = [&](int t, int buf) {
+      uint4(*const f)[WAVE] = s_frag[buf];
+      const bool aside = t * AT_TILE + SET_ASIDE > clear;
+      if (aside || have != 0xffffu) clear_values(have >> (g * 4), aside, wv);
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) {
+        uint32_t ko[4];
+        key_frag(kw, kk, ko);
+        f[wave * NK + kk][lane] = make_uint4(ko[0], ko[1], ko[2], ko[3]);
+      }
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) {
+        uint32_t vo[2];
+        value_operand<CT>(wv, e, vo);
+        reinterpret_cast<uint2*>(f[4 * NK + (wave / 2) * EPL + e])[(wave & 1) * WAVE + lane] = make_uint2(vo[0], vo[1]);
+      }
+      if constexpr (QUANT)
+        if (g < 2) s_scale[buf][g][wave * 16 + m] = scale;
+      if (lane == 0) s_here[buf][wave] = have;
+    };
+    int buf = 0;
+    fetch_slots(t0);
+    fetch();
+    if (t0 + 1 < t1) fetch_slots(t0 + 1);
+    __syncthreads();  // (s_odd)
+    put(t0, 0);
+    if (t0 + 1 < t1) {
+      fetch();
+      if (t0 + 2 < t1) fetch_slots(t0 + 2);
+    }
+    // A turn: the next tile into the other buffer, the loads of the one after it, the products of this one.
+    auto turn = [&](auto whole_, int t) {
+      __syncthreads();
+      if (t + 1 < t1) {
+        put(t + 1, buf ^ 1);
+        if (t + 2 < t1) {
+          fetch();
+          if (t + 3 < t1) fetch_slots(t + 3);
+        }
+      }
+      if (row0 < n_rows) {
+        for (int blk = wk; blk < 2; blk += WK) {
+          const uint32_t all = __builtin_amdgcn_readfirstlane(s_here[buf][2 * blk] | s_here[buf][2 * blk + 1] << 16);
+          float cs[8], vn[8];
+          if constexpr (QUANT) {
+            float kf[8], vf[8];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float4 k4 = *reinterpret_cast<const float4*>(&s_scale[buf][0][blk * AT_STEP + i * 16 + g * 4]);
+              const float4 v4 = *reinterpret_cast<const float4*>(&s_scale[buf][1][blk * AT_STEP + i * 16 + g * 4]);
+              kf[4 * i] = k4.x, kf[4 * i + 1] = k4.y, kf[4 * i + 2] = k4.z, kf[4 * i + 3] = k4.w;
+              vf[4 * i] = v4.x, vf[4 * i + 1] = v4.y, vf[4 * i + 2] = v4.z, vf[4 * i + 3] = v4.w;
+            }
+            factors(kf, vf, cs, vn);
+          }
+          const uint32_t here = ((all >> (g * 4)) & 0xfu) | (((all >> (16 + g * 4)) & 0xfu) << 4);
+          step(whole_, t * AT_TILE + blk * AT_STEP, here, cs, vn,
+               [&](int i, int kk, uint32_t (&ko)[4]) {
+                 const uint4 v = s_frag[buf][(blk * 2 + i) * NK + kk][lane];
+                 ko[0] = v.x, ko[1] = v.y, ko[2] = v.z, ko[3] = v.w;
+               },
+               [&](int e, uint32_t (&vo)[4]) {
+                 const uint2* v = reinterpret_cast<const uint2*>(s_frag[buf][4 * NK + blk * EPL + e]);
+                 vo[0] = v[lane].x, vo[1] = v[lane].y, vo[2] = v[WAVE + lane].x, vo[3] = v[WAVE + lane].y;
+               },
+               [] {});
+        }
+      }
+      buf ^= 1;
+    };
+    const int whole = clear / AT_TILE < t1 ? clear / AT_TILE : t1;
+    int t = t0;
+    for (; t < whole; ++t) turn(Int<1>{}, t);
+    for (; t < t1; ++t) turn(Int<0>{}, t);
   }
 
-  if (marked) {
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int rt = 0; rt < R; ++rt)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) {
-          const int at = (rt * 16 + m) * DP + (g * 4 + r) * EPL + e;
-          const uint32_t kind = (marks[at / 4] >> (8 * (at & 3))) & 7u;
-          if (kind & 1) o[rt][e][r] += INFINITY;
-          if (kind & 2) o[rt][e][r] -= INFINITY;
-          if (kind & 4) o[rt][e][r] = NAN;
-        }
-  }
   // The waves of the same rows join: their references, then the sums of one row tile after another through LDS.
 #pragma unroll
   for (int rt = 0; rt < R; ++rt) {
@@ -594,6 +714,9 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
   }
   __syncthreads();
   const float unit = QUANT ? vref * (CT == DSV_I8 ? I8_UNIT : 1.f) : 1.f;
+  // the positions whose values were set aside where they are not finite
+  const int aside0 = clear / SET_ASIDE * SET_ASIDE > t0 * AT_TILE ? clear / SET_ASIDE * SET_ASIDE : t0 * AT_TILE;
+  const int aside1 = t1 * AT_TILE < req.total ? t1 * AT_TILE : req.total;
 #pragma unroll
   for (int rt = 0; rt < R; ++rt) {
     float top = AT_LOW;
@@ -618,6 +741,20 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
 #pragma unroll
         for (int u = 0; u < 8; ++u) sum[u] += s_o[wr * WK + k][rr][d + u];
       }
+      const int node = r / P.G, qh = h * P.G + r - node * P.G;
+      if (CT != DSV_I8 && s_odd) {
+        const uint64_t mask = mask_of(a, b, node);
+        for (int p = aside0; p < aside1; ++p) {
+          const uint32_t slot = (uint32_t)table[p];
+          const int j = p - req.prefix;
+          if (!good(slot) || !(j < 0 || (j < 64 && ((mask >> (j & 63)) & 1)))) continue;
+          const uint8_t* v = vhead + (uint64_t)slot * P.v_step + d * ESZ;
+          for (int u = 0; u < 8; ++u) {
+            const float x = cache_value<CT>(v, u);
+            if (!(fabsf(x) < INFINITY)) sum[u] += x;
+          }
+        }
+      }
       if (pieces > 1) {
         const int64_t at = ((int64_t)item * c.heads + h) * (a.T * P.G) + r;
         float* po = P.part_o + at * dim + d;
@@ -625,7 +762,6 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
         *reinterpret_cast<float4*>(po + 4) = make_float4(sum[4], sum[5], sum[6], sum[7]);
         if (d == 0) P.part_ml[at] = make_float2(mt, lt);
       } else {
-        const int node = r / P.G, qh = h * P.G + r - node * P.G;
         const int64_t row = row_of(a, b, node);
         if (row < 0) continue;
         const float inv = lt == 0.f ? 0.f : 1.f / lt;
@@ -644,6 +780,7 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
 // Row tiles a wave, waves over the rows and row blocks of T nodes with G query heads each.
 struct AttnShape {
   int R, WR, RB;
+  bool staged;
 };
 
 template <int XT, int CT>
@@ -653,12 +790,13 @@ void launch_attn(const AttnParams& P, const AttnShape& s, unsigned blocks, hipSt
   auto width = [&](auto dp, auto full) {
     constexpr int DP = decltype(dp)::value;
     constexpr bool FULL = decltype(full)::value;
-    if constexpr (DP > 128)
-      s.R == 1 ? go(k_attn<XT, CT, DP, FULL, 1, 1>) : go(k_attn<XT, CT, DP, FULL, 2, 1>);
+    constexpr int OCC = DP > 128 ? 1 : 2;
+    if (!s.staged)
+      go(k_attn<XT, CT, DP, FULL, 1, false, OCC>);
+    else if (s.R == 1)
+      go(k_attn<XT, CT, DP, FULL, 1, true, OCC>);
     else
-      s.R == 1   ? go(k_attn<XT, CT, DP, FULL, 1, 2>)
-      : s.R == 2 ? go(k_attn<XT, CT, DP, FULL, 2, 2>)
-                 : go(k_attn<XT, CT, DP, FULL, 4, 1>);
+      go(k_attn<XT, CT, DP, FULL, 2, true, OCC>);
   };
   if (D <= 64)
     D == 64 ? width(Int<64>{}, Int<1>{}) : width(Int<64>{}, Int<0>{});

@@ -59,17 +59,17 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_join(AttnParams P) {
 }
 
 static int attn_target(int heads, int RB) {
-  const int t = (2048 + heads * RB - 1) / (heads * RB);
+  const int t = (1024 + heads * RB - 1) / (heads * RB);
   return t < 1 ? 1 : t;
 }
 
-static AttnShape attn_shape(int T, int G, int dim) {
-  const int rows = T * G, tiles = (rows + 15) / 16;
+static AttnShape attn_shape(int T, int G) {
+  const int tiles = (T * G + 15) / 16;
   AttnShape s;
-  const int most = dim > 128 ? 2 : 4;
-  s.R = tiles <= 1 ? 1 : (tiles <= 2 ? 2 : most);
+  s.staged = tiles > 1;
+  s.R = tiles > 4 ? 2 : 1;
   const int groups = (tiles + s.R - 1) / s.R;
-  s.WR = groups >= 3 ? 4 : groups;
+  s.WR = !s.staged ? 1 : (groups > 2 ? 4 : 2);  // (a staged tile has two steps for waves of the same rows)
   s.RB = (groups + s.WR - 1) / s.WR;
   return s;
 }
@@ -81,7 +81,7 @@ using namespace dsv;
 extern "C" int64_t dsv_tree_attention_workspace_bytes(int32_t bs, int32_t T, int32_t heads, int32_t q_heads,
                                                       int32_t dim) {
   if (bs < 1 || T < 1 || heads < 1 || q_heads < heads || dim < 1) return 0;
-  const AttnShape s = attn_shape(T, q_heads / heads, dim);
+  const AttnShape s = attn_shape(T, q_heads / heads);
   const int64_t rows = ((int64_t)attn_target(heads, s.RB) + bs) * q_heads * T;
   return rows * (dim * (int64_t)sizeof(float) + (int64_t)sizeof(float2));
 }
@@ -114,11 +114,11 @@ extern "C" int dsv_tree_attention(const dsv_tree_attention_args* args, dsv_strea
   AttnParams P;
   P.a = a;
   P.G = a.q_heads / a.cache.heads;
-  const AttnShape s = attn_shape(a.T, P.G, a.cache.dim);
+  const AttnShape s = attn_shape(a.T, P.G);
   P.WR = s.WR;
   P.RB = s.RB;
   P.target = attn_target(a.cache.heads, s.RB);
-  P.least = 4;
+  P.least = 2;
   P.joined = a.page_cols > (int64_t)P.least * AT_TILE;
   const int64_t items = (int64_t)P.target + a.bs, blocks = (items + 7) / 8 * 8 * a.cache.heads * s.RB;
   const int64_t rows = (int64_t)a.bs * a.T * a.q_heads;
