@@ -15,8 +15,10 @@
 //            of 64 positions from memory, converts it to the operands' 16-bit layout once and puts it into LDS (two
 //            buffers), from where every wave reads whole operands without bank conflicts
 //
-// The positions of a batch are cut into about `target` equal pieces (a rule on the lengths, which only the device
-// knows: every workgroup computes the same plan from them); pieces of a request are joined by k_attn_join.
+// The tiles of all requests, one request after the other, are cut into `ranges` equal ranges, as many as workgroups run
+// at once, so that all end together; a range may hold the end of a request, whole requests and the beginning of one.
+// Only the device knows the lengths: every wave computes the same plan from them.  A request within one range is
+// finished there; the parts of the others are left as sums and joined by k_attn_join.
 #pragma once
 #include "dsv_cache.h"
 #include "dsv_common.h"
@@ -38,12 +40,11 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 struct AttnParams {
   dsv_tree_attention_args a;
   int G, WR, RB;       // query heads a cache head; waves over the rows; row blocks of a request
-  int target;          // pieces aimed at
-  int least;           // tiles of a piece at least
-  int joined;          // whether a request may have several pieces
+  int most;            // ranges at most
+  int least;           // tiles of a range at least (the last part of the batch may be less)
   uint32_t num_slots, k_step, v_step;  // slots; bytes from slot to slot
-  float* part_o;       // [item][head][row][dim]
-  float2* part_ml;     // [item][head][row]: reference, sum
+  float* part_o;       // [2 * range + (the range's last request, not its first)][head][row][dim]
+  float2* part_ml;     // the same of [row]: reference, sum
 };
 
 // The request's nodes, its context and its positions (context and window) that the page table has.
@@ -66,39 +67,45 @@ __device__ __forceinline__ int tiles_of(const Request& r) {
   return r.nodes == 0 ? 0 : (t < 1 ? 1 : t);
 }
 
-// The plan, computed by every wave from the batch's lengths: tiles of a piece.
-__device__ __forceinline__ int plan_chunk(const AttnParams& P, int lane) {
+// The plan, computed by every wave from the batch's lengths: range i is the tiles [total * i / ranges,
+// total * (i + 1) / ranges) of the batch.
+struct Plan {
+  int64_t total;
+  int ranges;
+  __device__ __forceinline__ int64_t start(int i) const { return total * i / ranges; }
+  // the range that holds a tile
+  __device__ __forceinline__ int range_of(int64_t tile) const { return (int)(((tile + 1) * ranges + total - 1) / total) - 1; }
+};
+__device__ __forceinline__ Plan plan_of(const AttnParams& P, int lane) {
   int64_t sum = 0;
   for (int b = lane; b < P.a.bs; b += WAVE) sum += tiles_of(request_of(P.a, b));
-  sum = wave_sum(sum);
-  const int64_t c = (sum + P.target - 1) / P.target;
-  return (int)(c < P.least ? P.least : c);
+  Plan p;
+  p.total = wave_sum(sum);
+  const int64_t r = (p.total + P.least - 1) / P.least;
+  p.ranges = (int)(r < 1 ? 1 : (r > P.most ? P.most : r));
+  return p;
 }
-__device__ __forceinline__ int pieces_of(int tiles, int chunk) { return (tiles + chunk - 1) / chunk; }
-
-// Pieces of the requests before b.
-__device__ __forceinline__ int items_before(const AttnParams& P, int chunk, int b, int lane) {
-  int sum = 0;
-  for (int i = lane; i < b; i += WAVE) sum += pieces_of(tiles_of(request_of(P.a, i)), chunk);
+// Tiles of the requests before b.
+__device__ __forceinline__ int64_t tiles_before(const AttnParams& P, int b, int lane) {
+  int64_t sum = 0;
+  for (int i = lane; i < b; i += WAVE) sum += tiles_of(request_of(P.a, i));
   return wave_sum(sum);
 }
-// The request and the piece of a work item; false past the last.
-__device__ __forceinline__ bool item_at(const AttnParams& P, int chunk, int item, int lane, int& b, int& piece) {
-  int before = 0;
-  for (int b0 = 0; b0 < P.a.bs; b0 += WAVE) {
+// The request of a tile (tile < total) and the tiles before it.
+__device__ __forceinline__ int request_at(const AttnParams& P, int64_t tile, int lane, int64_t& before) {
+  before = 0;
+  for (int b0 = 0;; b0 += WAVE) {
     const int i = b0 + lane;
-    const int n = i < P.a.bs ? pieces_of(tiles_of(request_of(P.a, i)), chunk) : 0;
-    const int end = before + wave_incl_scan(n);
-    const uint64_t past = __ballot(end > item);
+    const int n = i < P.a.bs ? tiles_of(request_of(P.a, i)) : 0;
+    const int64_t end = before + wave_incl_scan((int64_t)n);
+    const uint64_t past = __ballot(end > tile);
     if (past) {
       const int l = __ffsll((unsigned long long)past) - 1;
-      b = b0 + l;
-      piece = item - (readlane_at(end, l) - readlane_at(n, l));
-      return true;
+      before = readlane_at(end, l) - readlane_at(n, l);
+      return b0 + l;
     }
     before = readlane<WAVE - 1>(end);
   }
-  return false;
 }
 
 template <int XT>
@@ -243,30 +250,38 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
   const int tid = threadIdx.x, lane = tid & (WAVE - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);  // (and all that follows from it: scalar)
   const int m = lane & 15, g = lane >> 4;
-  // Items round the XCDs, a request's heads and row blocks on one: they share its page table rows, scales and keys in
+  // Ranges round the XCDs, a range's heads and row blocks on one: they share its page table rows, scales and keys in
   // that XCD's L2.
   const int HB = c.heads * P.RB;
-  const int inner = (int)((blockIdx.x / 8) % HB), item = (int)((blockIdx.x / 8) / HB) * 8 + (int)(blockIdx.x % 8);
+  const int inner = (int)((blockIdx.x / 8) % HB), range = (int)((blockIdx.x / 8) / HB) * 8 + (int)(blockIdx.x % 8);
   const int h = inner / P.RB, rb = inner - h * P.RB;
-  const int chunk = plan_chunk(P, lane);
-  int b, piece;
-  if (!item_at(P, chunk, item, lane, b, piece)) return;
-  b = __builtin_amdgcn_readfirstlane(b);
-  piece = __builtin_amdgcn_readfirstlane(piece);
-  const Request req = request_of(a, b);
-  const int n_rows = req.nodes * P.G, tiles = tiles_of(req), pieces = pieces_of(tiles, chunk);
+  const Plan plan = plan_of(P, lane);
+  if (range >= plan.ranges || plan.total == 0) return;
   const int WR = P.WR, WK = AT_WAVES / WR, wr = wave / WK, wk = wave - wr * WK;
-  const int block0 = rb * 16 * R * WR;
-  if (block0 >= n_rows) return;
-  const int row0 = block0 + wr * 16 * R;
+  const int block0 = rb * 16 * R * WR, row0 = block0 + wr * 16 * R;
+  int64_t tile = plan.start(range), before;
+  const int64_t stop = plan.start(range + 1);
+  int b = __builtin_amdgcn_readfirstlane(request_at(P, tile, lane, before));
+  // the range's requests, one after the other
+  for (bool first = true; tile < stop; first = false) {
+  const Request req = request_of(a, b);
+  const int n_rows = req.nodes * P.G, tiles = tiles_of(req);
+  const int t0 = (int)(tile - before), t1 = (int)(stop - before < tiles ? stop - before : tiles);
+  const int request = b;
+  before += tiles;
+  tile += t1 - t0;
+  ++b;
+  if (block0 >= n_rows || t0 == t1) continue;
+  __syncthreads();  // (the sums of the request before have been read)
   if (tid == 0) s_odd = 0;
+  __syncthreads();
 
   // queries, in the order of the keys' elements
   uint32_t qf[R][NK][4];
 #pragma unroll
   for (int rt = 0; rt < R; ++rt) {
     const int r = row0 + rt * 16 + m;
-    const int64_t row = r < n_rows ? row_of(a, b, r / P.G) : -1;
+    const int64_t row = r < n_rows ? row_of(a, request, r / P.G) : -1;
     const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (row < 0 ? 0 : row) * a.q_row_stride +
                         (int64_t)(h * P.G + r % P.G) * a.q_head_stride;
 #pragma unroll
@@ -279,7 +294,7 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
     }
   }
 
-  const int32_t* table = a.page_table + (int64_t)b * a.page_stride;
+  const int32_t* table = a.page_table + (int64_t)request * a.page_stride;
   const uint8_t* kbase = reinterpret_cast<const uint8_t*>(c.k) + (int64_t)h * c.k_head_stride * ESZ + g * 16;
   const bool v_in = m * EPL < dim;  // (else the lane repeats the row's first piece: its sums are not stored)
   const uint8_t* vhead = reinterpret_cast<const uint8_t*>(c.v) + (int64_t)h * c.v_head_stride * ESZ;
@@ -301,7 +316,6 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
     for (int e = 0; e < EPL; ++e) o[rt][e] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  const int t0 = (int)((int64_t)tiles * piece / pieces), t1 = (int)((int64_t)tiles * (piece + 1) / pieces);
   const int last = req.total - 1;
   auto good = [&](uint32_t slot) { return slot < P.num_slots; };
   // the slots of 32 positions from `base`: of the key rows m and 16 + m, and of this lane's eight positions
@@ -436,7 +450,7 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
 #pragma unroll
       for (int rt = 0; rt < R; ++rt) {
         const int r = row0 + rt * 16 + m;
-        const uint64_t mask = r < n_rows ? mask_of(a, b, r / P.G) : 0ull;
+        const uint64_t mask = r < n_rows ? mask_of(a, request, r / P.G) : 0ull;
         uint32_t bits = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -651,7 +665,6 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
     fetch_slots(t0);
     fetch();
     if (t0 + 1 < t1) fetch_slots(t0 + 1);
-    __syncthreads();  // (s_odd)
     put(t0, 0);
     if (t0 + 1 < t1) {
       fetch();
@@ -743,7 +756,7 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
       }
       const int node = r / P.G, qh = h * P.G + r - node * P.G;
       if (CT != DSV_I8 && s_odd) {
-        const uint64_t mask = mask_of(a, b, node);
+        const uint64_t mask = mask_of(a, request, node);
         for (int p = aside0; p < aside1; ++p) {
           const uint32_t slot = (uint32_t)table[p];
           const int j = p - req.prefix;
@@ -755,14 +768,15 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
           }
         }
       }
-      if (pieces > 1) {
-        const int64_t at = ((int64_t)item * c.heads + h) * (a.T * P.G) + r;
+      if (t1 - t0 < tiles) {
+        // (its first part is its range's last request's, unless it begins the range; the others begin theirs)
+        const int64_t at = ((int64_t)(2 * range + (first ? 0 : 1)) * c.heads + h) * (a.T * P.G) + r;
         float* po = P.part_o + at * dim + d;
         *reinterpret_cast<float4*>(po) = make_float4(sum[0], sum[1], sum[2], sum[3]);
         *reinterpret_cast<float4*>(po + 4) = make_float4(sum[4], sum[5], sum[6], sum[7]);
         if (d == 0) P.part_ml[at] = make_float2(mt, lt);
       } else {
-        const int64_t row = row_of(a, b, node);
+        const int64_t row = row_of(a, request, node);
         if (row < 0) continue;
         const float inv = lt == 0.f ? 0.f : 1.f / lt;
         uint4 v;
@@ -774,6 +788,7 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
         if (d == 0 && a.lse) a.lse[row * a.q_heads + qh] = lt == 0.f ? -INFINITY : (mt + log2f(lt)) * 0.693147180559945309f;
       }
     }
+  }
   }
 }
 

@@ -11,56 +11,69 @@ extern template void launch_attn<DSV_F16, DSV_E4M3>(const AttnParams&, const Att
 extern template void launch_attn<DSV_BF16, DSV_I8>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
 extern template void launch_attn<DSV_F16, DSV_I8>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
 
-// The pieces of a request's row joined, a wave a row: references, then sums in the pieces' order.
+// The parts of a request joined: 8 elements of a row a thread, the parts in their order.  Bound by latency (the plan's
+// lengths, the references, the sums) and by the sums' bytes.
 template <int XT, int DP>
 __global__ __launch_bounds__(AT_THREADS) void k_attn_join(AttnParams P) {
   const dsv_tree_attention_args& a = P.a;
   const dsv_kv_cache& c = a.cache;
-  constexpr int PER = DP / WAVE;
+  constexpr int PER = DP / 8, ROWS = AT_THREADS / PER;
   const int lane = threadIdx.x & (WAVE - 1);
-  const int per = c.heads * a.T * P.G;
-  const int64_t i = (int64_t)blockIdx.x * AT_WAVES + threadIdx.x / WAVE;
-  const int b = (int)(i / per);
-  if (b >= a.bs) return;
-  const int in = (int)(i - (int64_t)b * per), h = in / (a.T * P.G), r = in - h * (a.T * P.G);
+  const int rows = a.T * P.G, blocks = (rows + ROWS - 1) / ROWS;
+  const int b = (int)(blockIdx.x / (c.heads * blocks)), in = (int)(blockIdx.x - (int64_t)b * c.heads * blocks);
+  const int h = in / blocks, r = (in - h * blocks) * ROWS + (int)threadIdx.x / PER, d = (int)threadIdx.x % PER * 8;
   const Request req = request_of(a, b);
-  if (r >= req.nodes * P.G) return;
-  const int chunk = plan_chunk(P, lane), pieces = pieces_of(tiles_of(req), chunk);
-  if (pieces < 2) return;
-  const int first = items_before(P, chunk, b, lane);
-  const int64_t rows = (int64_t)a.T * P.G, step = c.heads * rows;
-  const int64_t at = ((int64_t)first * c.heads + h) * rows + r;
-  float top = AT_LOW;
-  for (int k = lane; k < pieces; k += WAVE) top = fmaxf(top, P.part_ml[at + k * step].x);
-  top = wave_max_f32(top);
-  float sum[PER], lt = 0.f;
-#pragma unroll
-  for (int u = 0; u < PER; ++u) sum[u] = 0.f;
-  const int d = lane * PER;
-#pragma unroll 4
-  for (int k = 0; k < pieces; ++k) {
-    const float2 ml = P.part_ml[at + k * step];
-    const float f = __builtin_amdgcn_exp2f(ml.x - top);
-    lt = fmaf(ml.y, f, lt);
-    const float* po = P.part_o + (at + k * step) * c.dim + (d < c.dim ? d : 0);
-#pragma unroll
-    for (int u = 0; u < PER; ++u) sum[u] = fmaf(po[u], f, sum[u]);
-  }
+  const int tiles = tiles_of(req);
+  if ((in - h * blocks) * ROWS >= req.nodes * P.G) return;
+  const Plan plan = plan_of(P, lane);
+  const int64_t before = tiles_before(P, b, lane);
+  const int i0 = plan.range_of(before), i1 = plan.range_of(before + tiles - 1);
+  if (i0 == i1 || r >= req.nodes * P.G || d >= c.dim) return;
   const int node = r / P.G, qh = h * P.G + r - node * P.G;
   const int64_t row = row_of(a, b, node);
   if (row < 0) return;
-  const float inv = lt == 0.f ? 0.f : 1.f / lt;
-  if (d < c.dim) {
-    uint16_t* out = reinterpret_cast<uint16_t*>(a.out) + row * a.out_row_stride + qh * a.out_head_stride + d;
+  // the request's part of range i: the last of its range where that begins before it
+  auto part = [&](int i) {
+    return ((int64_t)(2 * i + (i == i0 && plan.start(i) < before ? 1 : 0)) * c.heads + h) * rows + r;
+  };
+  float top = AT_LOW;
+#pragma unroll 4
+  for (int i = i0; i <= i1; ++i) top = fmaxf(top, P.part_ml[part(i)].x);
+  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, lt = 0.f;
+#pragma unroll 4
+  for (int i = i0; i <= i1; ++i) {
+    const int64_t at = part(i);
+    const float2 ml = P.part_ml[at];
+    const float4 x = *reinterpret_cast<const float4*>(P.part_o + at * c.dim + d);
+    const float4 y = *reinterpret_cast<const float4*>(P.part_o + at * c.dim + d + 4);
+    const float f = __builtin_amdgcn_exp2f(ml.x - top);
+    lt = fmaf(ml.y, f, lt);
+    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
 #pragma unroll
-    for (int u = 0; u < PER; ++u) out[u] = (uint16_t)pack_act<XT>(sum[u] * inv, 0.f);
+    for (int u = 0; u < 8; ++u) sum[u] = fmaf(v[u], f, sum[u]);
   }
-  if (lane == 0 && a.lse) a.lse[row * a.q_heads + qh] = lt == 0.f ? -INFINITY : (top + log2f(lt)) * 0.693147180559945309f;
+  const float inv = lt == 0.f ? 0.f : 1.f / lt;
+  uint4 v;
+  v.x = pack_act<XT>(sum[0] * inv, sum[1] * inv);
+  v.y = pack_act<XT>(sum[2] * inv, sum[3] * inv);
+  v.z = pack_act<XT>(sum[4] * inv, sum[5] * inv);
+  v.w = pack_act<XT>(sum[6] * inv, sum[7] * inv);
+  *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + row * a.out_row_stride + qh * a.out_head_stride + d) = v;
+  if (d == 0 && a.lse) a.lse[row * a.q_heads + qh] = lt == 0.f ? -INFINITY : (top + log2f(lt)) * 0.693147180559945309f;
 }
 
-static int attn_target(int heads, int RB) {
-  const int t = (1024 + heads * RB - 1) / (heads * RB);
-  return t < 1 ? 1 : t;
+// Ranges at most: as many as workgroups run at once (or a few times as many where the heads and row blocks leave too
+// many of those idle otherwise).
+static int attn_ranges(int heads, int RB, bool wide) {
+  const int64_t slots = wide ? 256 : 512, hb = (int64_t)heads * RB;
+  int64_t best = 1;
+  double use = 0.0;
+  for (int k = 1; k <= 4; ++k) {
+    const int64_t n = k * slots / hb;
+    const double u = (double)(n * hb) / (double)(k * slots);
+    if (n > 0 && u > use + 0.05) use = u, best = n;
+  }
+  return (int)best;
 }
 
 static AttnShape attn_shape(int T, int G) {
@@ -82,7 +95,7 @@ extern "C" int64_t dsv_tree_attention_workspace_bytes(int32_t bs, int32_t T, int
                                                       int32_t dim) {
   if (bs < 1 || T < 1 || heads < 1 || q_heads < heads || dim < 1) return 0;
   const AttnShape s = attn_shape(T, q_heads / heads);
-  const int64_t rows = ((int64_t)attn_target(heads, s.RB) + bs) * q_heads * T;
+  const int64_t rows = 2 * (int64_t)attn_ranges(heads, s.RB, dim > 128) * q_heads * T;
   return rows * (dim * (int64_t)sizeof(float) + (int64_t)sizeof(float2));
 }
 
@@ -117,12 +130,12 @@ extern "C" int dsv_tree_attention(const dsv_tree_attention_args* args, dsv_strea
   const AttnShape s = attn_shape(a.T, P.G);
   P.WR = s.WR;
   P.RB = s.RB;
-  P.target = attn_target(a.cache.heads, s.RB);
+  P.most = attn_ranges(a.cache.heads, s.RB, a.cache.dim > 128);
   P.least = 2;
-  P.joined = a.page_cols > (int64_t)P.least * AT_TILE;
-  const int64_t items = (int64_t)P.target + a.bs, blocks = (items + 7) / 8 * 8 * a.cache.heads * s.RB;
-  const int64_t rows = (int64_t)a.bs * a.T * a.q_heads;
-  if (blocks > 0x7fffffffll || rows / AT_WAVES >= 0x7fffffffll)
+  const int64_t blocks = (P.most + 7) / 8 * 8 * (int64_t)a.cache.heads * s.RB;
+  const int64_t wide = a.cache.dim <= 64 ? 64 : (a.cache.dim <= 128 ? 128 : 256), per = AT_THREADS / (wide / 8);
+  const int64_t joins = (a.T * (int64_t)P.G + per - 1) / per * a.cache.heads * a.bs;
+  if (blocks > 0x7fffffffll || joins > 0x7fffffffll)
     DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: too many nodes for one call");
   const int64_t need = dsv_tree_attention_workspace_bytes(a.bs, a.T, a.cache.heads, a.q_heads, a.cache.dim);
   if (!a.workspace || (uintptr_t)a.workspace % 16)
@@ -133,7 +146,7 @@ extern "C" int dsv_tree_attention(const dsv_tree_attention_args* args, dsv_strea
   P.k_step = (uint32_t)(a.cache.k_slot_stride * esize);
   P.v_step = (uint32_t)(a.cache.v_slot_stride * esize);
   P.part_o = reinterpret_cast<float*>(a.workspace);
-  P.part_ml = reinterpret_cast<float2*>(P.part_o + items * a.q_heads * a.T * a.cache.dim);
+  P.part_ml = reinterpret_cast<float2*>(P.part_o + 2 * (int64_t)P.most * a.q_heads * a.T * a.cache.dim);
   const bool bf = a.dtype == DSV_BF16;
   if (a.cache.dtype == DSV_E4M3)
     bf ? launch_attn<DSV_BF16, DSV_E4M3>(P, s, (unsigned)blocks, stream) : launch_attn<DSV_F16, DSV_E4M3>(P, s, (unsigned)blocks, stream);
@@ -142,12 +155,11 @@ extern "C" int dsv_tree_attention(const dsv_tree_attention_args* args, dsv_strea
   else
     bf ? launch_attn<DSV_BF16, DSV_BF16>(P, s, (unsigned)blocks, stream) : launch_attn<DSV_F16, DSV_F16>(P, s, (unsigned)blocks, stream);
   DSV_CHECK_LAUNCH("k_attn");
-  if (P.joined) {
-    const dim3 grid((unsigned)((rows + AT_WAVES - 1) / AT_WAVES));
-    auto join = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(AT_THREADS), 0, stream, P); };
-    if (a.cache.dim <= 64)
+  if (P.most > 1) {
+    auto join = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)joins), dim3(AT_THREADS), 0, stream, P); };
+    if (wide == 64)
       bf ? join(k_attn_join<DSV_BF16, 64>) : join(k_attn_join<DSV_F16, 64>);
-    else if (a.cache.dim <= 128)
+    else if (wide == 128)
       bf ? join(k_attn_join<DSV_BF16, 128>) : join(k_attn_join<DSV_F16, 128>);
     else
       bf ? join(k_attn_join<DSV_BF16, 256>) : join(k_attn_join<DSV_F16, 256>);
