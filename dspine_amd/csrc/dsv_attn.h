@@ -25,8 +25,8 @@
 
 namespace dsv {
 
-constexpr int AT_THREADS = 256;
-constexpr int AT_WAVES = AT_THREADS / WAVE;
+constexpr int AT_WAVES = 4;   // waves of a direct workgroup, and those that bring a staged tile
+constexpr int AT_MOST = 8;    // waves of a staged workgroup at most
 constexpr int AT_NODES = 64;
 constexpr int AT_STEP = 32;  // positions of a step: two tiles of the first product, one of the second
 constexpr int AT_TILE = 64;  // positions of a plan's unit, and of a staged tile
@@ -39,7 +39,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct AttnParams {
   dsv_tree_attention_args a;
-  int G, WR, RB;       // query heads a cache head; waves over the rows; row blocks of a request
+  int G, WR, RB;       // query heads a cache head; groups of rows a workgroup, row blocks of a request
   int most;            // ranges at most
   int least;           // tiles of a range at least (the last part of the batch may be less)
   uint32_t num_slots, k_step, v_step;  // slots; bytes from slot to slot
@@ -68,35 +68,58 @@ __device__ __forceinline__ int tiles_of(const Request& r) {
 }
 
 // The plan, computed by every wave from the batch's lengths: range i is the tiles [total * i / ranges,
-// total * (i + 1) / ranges) of the batch.
+// total * (i + 1) / ranges) of the batch.  Up to 64 requests are read once, a request a lane, and looked up among the
+// lanes; larger batches are read again where they are asked for.
 struct Plan {
   int64_t total;
   int ranges;
+  bool small;    // up to 64 requests
+  Request mine;  // this lane's, of a small batch
+  int tiles;     // its tiles
   __device__ __forceinline__ int64_t start(int i) const { return total * i / ranges; }
   // the range that holds a tile
   __device__ __forceinline__ int range_of(int64_t tile) const { return (int)(((tile + 1) * ranges + total - 1) / total) - 1; }
 };
 __device__ __forceinline__ Plan plan_of(const AttnParams& P, int lane) {
-  int64_t sum = 0;
-  for (int b = lane; b < P.a.bs; b += WAVE) sum += tiles_of(request_of(P.a, b));
   Plan p;
+  p.small = P.a.bs <= WAVE;
+  p.tiles = 0;
+  p.mine = Request{0, 0, 0};
+  int64_t sum = 0;
+  if (p.small) {
+    if (lane < P.a.bs) {
+      p.mine = request_of(P.a, lane);
+      p.tiles = tiles_of(p.mine);
+    }
+    sum = p.tiles;
+  } else {
+    for (int b = lane; b < P.a.bs; b += WAVE) sum += tiles_of(request_of(P.a, b));
+  }
   p.total = wave_sum(sum);
   const int64_t r = (p.total + P.least - 1) / P.least;
   p.ranges = (int)(r < 1 ? 1 : (r > P.most ? P.most : r));
   return p;
 }
+// Request b (the same in every lane).
+__device__ __forceinline__ Request request_in(const AttnParams& P, const Plan& p, int b) {
+  if (!p.small) return request_of(P.a, b);
+  return Request{readlane_at(p.mine.nodes, b), readlane_at(p.mine.prefix, b), readlane_at(p.mine.total, b)};
+}
 // Tiles of the requests before b.
-__device__ __forceinline__ int64_t tiles_before(const AttnParams& P, int b, int lane) {
+__device__ __forceinline__ int64_t tiles_before(const AttnParams& P, const Plan& p, int b, int lane) {
   int64_t sum = 0;
-  for (int i = lane; i < b; i += WAVE) sum += tiles_of(request_of(P.a, i));
+  if (p.small)
+    sum = lane < b ? p.tiles : 0;
+  else
+    for (int i = lane; i < b; i += WAVE) sum += tiles_of(request_of(P.a, i));
   return wave_sum(sum);
 }
 // The request of a tile (tile < total) and the tiles before it.
-__device__ __forceinline__ int request_at(const AttnParams& P, int64_t tile, int lane, int64_t& before) {
+__device__ __forceinline__ int request_at(const AttnParams& P, const Plan& p, int64_t tile, int lane, int64_t& before) {
   before = 0;
   for (int b0 = 0;; b0 += WAVE) {
     const int i = b0 + lane;
-    const int n = i < P.a.bs ? tiles_of(request_of(P.a, i)) : 0;
+    const int n = p.small ? p.tiles : (i < P.a.bs ? tiles_of(request_of(P.a, i)) : 0);
     const int64_t end = before + wave_incl_scan((int64_t)n);
     const uint64_t past = __ballot(end > tile);
     if (past) {
@@ -223,12 +246,16 @@ __device__ __forceinline__ uint64_t mask_of(const dsv_tree_attention_args& a, in
   return node >= 63 ? ~0ull : (2ull << node) - 1ull;
 }
 
-template <int XT, int CT, int DP, bool FULL, int R, bool STAGED, int OCC>
-__global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
+// FORM: direct, or staged with a wave (AT_ROWS) or two (AT_PAIRS) for a group of rows.
+enum { AT_DIRECT = 0, AT_PAIRS = 1, AT_ROWS = 2 };
+
+template <int XT, int CT, int DP, bool FULL, int R, int FORM, int WAVES, int OCC>
+__global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
   const dsv_tree_attention_args& a = P.a;
   const dsv_kv_cache& c = a.cache;
   const int dim = FULL ? DP : c.dim;  // (a constant for the common sizes: no test of it in the loop)
-  constexpr bool QUANT = CT == DSV_E4M3 || CT == DSV_I8;
+  constexpr bool QUANT = CT == DSV_E4M3 || CT == DSV_I8, STAGED = FORM != AT_DIRECT;
+  constexpr int WK = FORM == AT_DIRECT ? AT_WAVES : (FORM == AT_PAIRS ? 2 : 1);  // waves of the same rows
   constexpr int PT = CT == DSV_BF16 ? DSV_BF16 : DSV_F16;  // the weights' type
   // float16 weights are held 2^11 higher, so that what their range loses lies below 2^-35 of the row's largest
   constexpr float SHIFT = PT == DSV_F16 ? 11.f : 0.f, LIM = PT == DSV_F16 ? 4.f : 8.f;
@@ -241,9 +268,9 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
   constexpr int SET_ASIDE = STAGED ? AT_TILE : AT_STEP;
   constexpr int FRAGS = 4 * NK + 2 * EPL;  // operands of a staged tile: keys, then values, 16 bytes a lane each (values as
                                            // two halves of 8, so that their writes find all banks)
-  constexpr size_t SUMS = sizeof(float) * AT_WAVES * 16 * OS, TILES = STAGED ? sizeof(uint4) * 2 * FRAGS * WAVE : 0;
+  constexpr size_t SUMS = sizeof(float) * WAVES * 16 * OS, TILES = STAGED ? sizeof(uint4) * 2 * FRAGS * WAVE : 0;
   __shared__ __attribute__((aligned(16))) unsigned char s_mem[SUMS > TILES ? SUMS : TILES];
-  __shared__ float s_m[AT_WAVES][16 * R], s_l[AT_WAVES][16 * R];
+  __shared__ float s_m[WAVES][16 * R], s_l[WAVES][16 * R];
   __shared__ int s_odd;
   float(*const s_o)[16][OS] = reinterpret_cast<float(*)[16][OS]>(s_mem);
 
@@ -257,14 +284,14 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
   const int h = inner / P.RB, rb = inner - h * P.RB;
   const Plan plan = plan_of(P, lane);
   if (range >= plan.ranges || plan.total == 0) return;
-  const int WR = P.WR, WK = AT_WAVES / WR, wr = wave / WK, wk = wave - wr * WK;
-  const int block0 = rb * 16 * R * WR, row0 = block0 + wr * 16 * R;
+  const int wr = wave / WK, wk = wave - wr * WK;
+  const int block0 = rb * 16 * R * P.WR, row0 = block0 + wr * 16 * R;
   int64_t tile = plan.start(range), before;
   const int64_t stop = plan.start(range + 1);
-  int b = __builtin_amdgcn_readfirstlane(request_at(P, tile, lane, before));
+  int b = __builtin_amdgcn_readfirstlane(request_at(P, plan, tile, lane, before));
   // the range's requests, one after the other
   for (bool first = true; tile < stop; first = false) {
-  const Request req = request_of(a, b);
+  const Request req = request_in(P, plan, b);
   const int n_rows = req.nodes * P.G, tiles = tiles_of(req);
   const int t0 = (int)(tile - before), t1 = (int)(stop - before < tiles ? stop - before : tiles);
   const int request = b;
@@ -293,6 +320,16 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
       for (int i = 0; i < 4; ++i) qf[rt][kk][i] = w[i];
     }
   }
+
+  // Before the loops the queries must have come: a wait for them inside would be one for every load in flight.
+  auto queries_here = [&]() {
+#pragma unroll
+    for (int rt = 0; rt < R; ++rt)
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(qf[rt][kk][i]));
+  };
 
   const int32_t* table = a.page_table + (int64_t)request * a.page_stride;
   const uint8_t* kbase = reinterpret_cast<const uint8_t*>(c.k) + (int64_t)h * c.k_head_stride * ESZ + g * 16;
@@ -396,11 +433,12 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
   };
   // The positions' factors of a score (base 2) and of a weight.  Value scales are taken relative to a power of two at or
   // above the largest so far.
-  auto factors = [&](const float (&kf)[8], const float (&vf)[8], float (&cs)[8], float (&vn)[8]) {
+  auto factors = [&](const auto& kf, const auto& vf, auto& cs, auto& vn) {
     if constexpr (QUANT) {
+      constexpr int N = sizeof(kf) / sizeof(kf[0]);
       float top = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < N; ++j) {
         cs[j] = kf[j] * c0;
         const float v = fabsf(vf[j]);
         top = fmaxf(top, v < INFINITY ? v : 0.f);
@@ -422,23 +460,26 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
         }
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) vn[j] = vf[j] * vinv;
+      for (int j = 0; j < N; ++j) vn[j] = vf[j] * vinv;
     }
   };
-  // A step: scores of 32 positions' keys, weights, weighted values.  WHOLE: every row sees every position that holds
-  // anything (bit j of `here`: this lane's position j does).  `next` runs when the keys have been used.
-  auto step = [&](auto whole_, int base, uint32_t here, const float (&cs)[8], const float (&vn)[8], auto key, auto value,
-                  auto next) {
+  // A step, or n at once: scores of 32 n positions' keys, weights, weighted values.  WHOLE: every row sees every position
+  // that holds anything (bit j of `here`: this lane's position j does).  `next` runs when the keys have been used, `after` when the
+  // values' operand e has.
+  auto step = [&](auto whole_, auto n_, int base, uint32_t here, const auto& cs, const auto& vn, auto key, auto value,
+                  auto next, auto after) {
     constexpr bool WHOLE = decltype(whole_)::value;
-    f32x4 s[R][2];
+    constexpr int N = decltype(n_)::value, POS = 8 * N;  // positions a lane
+    constexpr uint32_t ALL = (1u << POS) - 1u;
+    f32x4 s[R][2 * N];
 #pragma unroll
     for (int rt = 0; rt < R; ++rt)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) s[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < 2 * N; ++i) s[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int kk = 0; kk < NK; ++kk)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 2 * N; ++i) {
         uint32_t ko[4];
         key(i, kk, ko);
 #pragma unroll
@@ -453,7 +494,7 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
         const uint64_t mask = r < n_rows ? mask_of(a, request, r / P.G) : 0ull;
         uint32_t bits = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < POS; ++j) {
           const int p = base + (j / 4) * 16 + g * 4 + (j & 3) - req.prefix;
           const bool sees = p < 0 || (p < 64 && ((mask >> (p & 63)) & 1));
           bits |= (sees ? 1u : 0u) << j;
@@ -467,19 +508,20 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
     for (int rt = 0; rt < R; ++rt) {
       const float ref = mref[rt] == AT_LOW ? 0.f : mref[rt];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < POS; ++j) {
         float x = fmaf(s[rt][j / 4][j & 3], QUANT ? cs[j] : c0, -ref);
         if (!WHOLE && !((seen[rt] >> j) & 1)) x = -INFINITY;
         s[rt][j / 4][j & 3] = x;
         over = fmaxf(over, x);
       }
     }
-    if (WHOLE && __any(here != 0xffu)) {
+    if (WHOLE && __any(here != ALL)) {
+      asm volatile("");  // (a branch: the selects are for bad slots only)
       over = AT_LOW;
 #pragma unroll
       for (int rt = 0; rt < R; ++rt)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
+        for (int j = 0; j < POS; ++j) {
           if (!((here >> j) & 1)) s[rt][j / 4][j & 3] = -INFINITY;
           over = fmaxf(over, s[rt][j / 4][j & 3]);
         }
@@ -490,7 +532,7 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
       for (int rt = 0; rt < R; ++rt) {
         float top = AT_LOW;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, s[rt][j / 4][j & 3]);
+        for (int j = 0; j < POS; ++j) top = fmaxf(top, s[rt][j / 4][j & 3]);
         top = across_groups_max(top);
         const bool unset = mref[rt] == AT_LOW;
         float move = top - SHIFT;  // of the reference: up, or anywhere from none
@@ -502,47 +544,64 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
 #pragma unroll
         for (int e = 0; e < EPL; ++e) o[rt][e] *= keep;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[rt][j / 4][j & 3] -= move;
+        for (int j = 0; j < POS; ++j) s[rt][j / 4][j & 3] -= move;
       }
       fresh = __any(none);
     }
-    uint32_t pf[R][4];
+    uint32_t pf[R][N][4];
 #pragma unroll
     for (int rt = 0; rt < R; ++rt) {
-      float w[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        w[j] = __builtin_amdgcn_exp2f(s[rt][j / 4][j & 3]);
-        l[rt] += w[j];
-        if constexpr (QUANT) {
-          w[j] *= vn[j];
-          if (!WHOLE && !((seen[rt] >> j) & 1)) w[j] = 0.f;
+      for (int j = 0; j < POS; j += 2) {
+        float w[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          w[u] = __builtin_amdgcn_exp2f(s[rt][j / 4][(j + u) & 3]);
+          l[rt] += w[u];
+          if constexpr (QUANT) {
+            w[u] *= vn[j + u];
+            if (!WHOLE && !((seen[rt] >> (j + u)) & 1)) w[u] = 0.f;
+          }
         }
+        pf[rt][j / 8][j % 8 / 2] = pack_act<PT>(w[0], w[1]);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) pf[rt][i] = pack_act<PT>(w[2 * i], w[2 * i + 1]);
     }
 #pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-      uint32_t vo[4];
-      value(e, vo);
+    for (int n = 0; n < N; ++n)
 #pragma unroll
-      for (int rt = 0; rt < R; ++rt) o[rt][e] = mfma<PT>(vo, pf[rt], o[rt][e]);
-    }
+      for (int e = 0; e < EPL; ++e) {
+        uint32_t vo[4];
+        value(n, e, vo);
+#pragma unroll
+        for (int rt = 0; rt < R; ++rt) o[rt][e] = mfma<PT>(vo, pf[rt][n], o[rt][e]);
+        after(e);
+      }
   };
 
   if constexpr (!STAGED) {
-    // (scales of positions that hold nothing are zeros)
-    auto load_scales = [&](const uint32_t (&vs)[8], float (&kf)[8], float (&vf)[8]) {
+    // The scales of a step's 32 positions: lane (m, g) loads the key's (g < 2) or the value's of position
+    // (g & 1) * 16 + m (zero where it holds nothing), and a lane's eight come back through LDS: 16 loads and their
+    // addresses a lane were most of the step's instructions.
+    __shared__ float s_scale[AT_WAVES][2][AT_STEP];
+    auto load_scale = [&](uint32_t k0, uint32_t k1) {
+      const uint32_t slot = g & 1 ? k1 : k0;
+      if constexpr (!QUANT) return 0.f;
+      const int64_t s = good(slot) ? slot : 0u;
+      const float f = g < 2 ? ksc[s * c.ks_slot_stride] : vsc[s * c.vs_slot_stride];
+      return good(slot) ? f : 0.f;
+    };
+    auto spread_scales = [&](float scale, float (&kf)[8], float (&vf)[8]) {
       if constexpr (QUANT) {
+        s_scale[wave][g >> 1][(g & 1) * 16 + m] = scale;
+        __builtin_amdgcn_wave_barrier();  // (the wave's own memory, in order)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool ok = good(vs[j]);
-          const uint32_t s = ok ? vs[j] : 0u;
-          kf[j] = ksc[(int64_t)s * c.ks_slot_stride];
-          vf[j] = vsc[(int64_t)s * c.vs_slot_stride];
-          if (!ok) kf[j] = vf[j] = 0.f;
+        for (int i = 0; i < 2; ++i) {
+          const float4 k4 = *reinterpret_cast<const float4*>(&s_scale[wave][0][i * 16 + g * 4]);
+          const float4 v4 = *reinterpret_cast<const float4*>(&s_scale[wave][1][i * 16 + g * 4]);
+          kf[4 * i] = k4.x, kf[4 * i + 1] = k4.y, kf[4 * i + 2] = k4.z, kf[4 * i + 3] = k4.w;
+          vf[4 * i] = v4.x, vf[4 * i + 1] = v4.y, vf[4 * i + 2] = v4.z, vf[4 * i + 3] = v4.w;
         }
+        __builtin_amdgcn_wave_barrier();
       }
     };
     auto holds = [&](const uint32_t (&vs)[8]) {
@@ -551,44 +610,58 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
       for (int j = 0; j < 8; ++j) here |= (good(vs[j]) ? 1u : 0u) << j;
       return here;
     };
+    queries_here();
     // steps of this wave: every WK-th
     int t = t0 * (AT_TILE / AT_STEP) + wk;
     int end = t1 * (AT_TILE / AT_STEP);
     const int some = (req.total + AT_STEP - 1) / AT_STEP;
     end = end < some ? end : some;
     if (row0 >= n_rows) t = end;
-    // Those in the context: a step's values are loaded at its beginning, the next one's keys and scales when its scores
-    // are done, the slots two steps ahead.
+    // Those in the context: the next step's keys, values and scales are loaded when this one's scores are done, the slots
+    // two steps ahead.
     const int whole = clear / AT_STEP < end ? clear / AT_STEP : end;
     if (t < whole) {
-      uint32_t ks[2], vs0[8], vs1[8], kw[2][KL][4], wv[8][VW];
-      float kf[8], vf[8], cs[8], vn[8];
-      key_slots(t * AT_STEP, ks[0], ks[1]);
-      value_slots(Int<1>{}, t * AT_STEP, vs0);
-      load_key(ks[0], kw[0]);
-      load_key(ks[1], kw[1]);
-      load_scales(vs0, kf, vf);
-      key_slots((t + WK < whole ? t + WK : t) * AT_STEP, ks[0], ks[1]);
-      value_slots(Int<1>{}, (t + WK < whole ? t + WK : t) * AT_STEP, vs1);
-      for (; t < whole; t += WK) {
+      uint32_t ks[2], vs[8], here0, here1, kw[2][KL][4], wv0[8][VW], wv1[8][VW];
+      float scale, cs[8], vn[8];
+      auto load_values = [&](uint32_t (&wv)[8][VW], uint32_t& here) {
+        here = holds(vs);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) load_value(vs0[j], wv[j]);
-        const uint32_t here = holds(vs0);
-        if (__any(here != 0xffu)) clear_values(here, false, wv);
+        for (int j = 0; j < 8; ++j) load_value(vs[j], wv[j]);
+      };
+      auto go = [&](uint32_t (&wv)[8][VW], uint32_t here, uint32_t (&then)[8][VW], uint32_t& then_here) {
+        float kf[8], vf[8];
+        spread_scales(scale, kf, vf);
         factors(kf, vf, cs, vn);
-        step(Int<1>{}, t * AT_STEP, here, cs, vn, [&](int i, int kk, uint32_t (&ko)[4]) { key_frag(kw[i], kk, ko); },
-             [&](int e, uint32_t (&vo)[4]) { value_operand<CT>(wv, e, vo); },
+        step(Int<1>{}, Int<1>{}, t * AT_STEP, here, cs, vn,
+             [&](int i, int kk, uint32_t (&ko)[4]) { key_frag(kw[i], kk, ko); },
+             [&](int, int e, uint32_t (&vo)[4]) { value_operand<CT>(wv, e, vo); },
              [&]() {
+               if (__any(here != 0xffu)) clear_values(here, false, wv);
                load_key(ks[0], kw[0]);
                load_key(ks[1], kw[1]);
-#pragma unroll
-               for (int j = 0; j < 8; ++j) vs0[j] = vs1[j];
-               load_scales(vs0, kf, vf);
+               scale = load_scale(ks[0], ks[1]);
+               load_values(then, then_here);
                const int ahead = t + 2 * WK < whole ? t + 2 * WK : t;
                ks[0] = (uint32_t)table[ahead * AT_STEP + m];
                ks[1] = (uint32_t)table[ahead * AT_STEP + 16 + m];
-               value_slots(Int<1>{}, ahead * AT_STEP, vs1);
-             });
+               value_slots(Int<1>{}, ahead * AT_STEP, vs);
+             },
+             [](int) {});
+        t += WK;
+      };
+      key_slots(t * AT_STEP, ks[0], ks[1]);
+      value_slots(Int<1>{}, t * AT_STEP, vs);
+      load_key(ks[0], kw[0]);
+      load_key(ks[1], kw[1]);
+      scale = load_scale(ks[0], ks[1]);
+      load_values(wv0, here0);
+      key_slots((t + WK < whole ? t + WK : t) * AT_STEP, ks[0], ks[1]);
+      value_slots(Int<1>{}, (t + WK < whole ? t + WK : t) * AT_STEP, vs);
+      while (true) {
+        go(wv0, here0, wv1, here1);
+        if (t >= whole) break;
+        go(wv1, here1, wv0, here0);
+        if (t >= whole) break;
       }
     }
     // The window's.
@@ -600,20 +673,21 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
       value_slots(Int<0>{}, base, vs);
       load_key(ks[0], kw[0]);
       load_key(ks[1], kw[1]);
-      load_scales(vs, kf, vf);
+      spread_scales(load_scale(ks[0], ks[1]), kf, vf);
 #pragma unroll
       for (int j = 0; j < 8; ++j) load_value(vs[j], wv[j]);
       const uint32_t here = holds(vs);
       clear_values(here, true, wv);
       factors(kf, vf, cs, vn);
-      step(Int<0>{}, base, here, cs, vn, [&](int i, int kk, uint32_t (&ko)[4]) { key_frag(kw[i], kk, ko); },
-           [&](int e, uint32_t (&vo)[4]) { value_operand<CT>(wv, e, vo); }, [] {});
+      step(Int<0>{}, Int<1>{}, base, here, cs, vn,
+           [&](int i, int kk, uint32_t (&ko)[4]) { key_frag(kw[i], kk, ko); },
+           [&](int, int e, uint32_t (&vo)[4]) { value_operand<CT>(wv, e, vo); }, [] {}, [](int) {});
     }
   } else {
     uint4(*const s_frag)[FRAGS][WAVE] = reinterpret_cast<uint4(*)[FRAGS][WAVE]>(s_mem);
     __shared__ float s_scale[2][2][AT_TILE];
     __shared__ uint32_t s_here[2][AT_WAVES];
-    // A wave brings 16 positions: lane (m, g) pieces of the key of position m, and of the values of g * 4 .. g * 4 + 3.
+    // Each of the first waves brings 16 positions: lane (m, g) pieces of the key of position m, and of the values of g * 4 .. g * 4 + 3.
     uint32_t kw[KL][4], wv[4][VW], kslot = ~0u, vslot[4];
     uint32_t have = 0;  // bits of the 16 positions
     float scale = 0.f;
@@ -662,27 +736,50 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
       if (lane == 0) s_here[buf][wave] = have;
     };
     int buf = 0;
-    fetch_slots(t0);
-    fetch();
-    if (t0 + 1 < t1) fetch_slots(t0 + 1);
-    put(t0, 0);
-    if (t0 + 1 < t1) {
+    const bool brings = wave < AT_WAVES;
+    if (brings) fetch_slots(t0);
+    queries_here();
+    if (brings) {
       fetch();
-      if (t0 + 2 < t1) fetch_slots(t0 + 2);
+      if (t0 + 1 < t1) fetch_slots(t0 + 1);
+      put(t0, 0);
+      if (t0 + 1 < t1) {
+        fetch();
+        if (t0 + 2 < t1) fetch_slots(t0 + 2);
+      }
     }
-    // A turn: the next tile into the other buffer, the loads of the one after it, the products of this one.
+    // A turn: the next tile into the other buffer, the loads of the one after it, the products of this one.  A step's keys
+    // are read from LDS while the step before it multiplies (the first step's while the next tile is put away), its values
+    // while its weights are computed, into the same registers: read where they are used, the reads' latencies were most
+    // of a turn.
+    constexpr bool AHEAD = R == 1 && DP <= 128;  // (with more rows the registers are not there, nor are the reads most of a step)
+    uint4 fr[EPL];
+    static_assert(2 * NK == EPL, "a step has as many key operands as value operands");
+    auto read_key = [&](int blk, int n) { fr[n] = s_frag[buf][blk * 2 * NK + n][lane]; };
+    auto read_value = [&](int blk, int e) {
+      const uint2* v = reinterpret_cast<const uint2*>(s_frag[buf][4 * NK + blk * EPL + e]);
+      const uint2 lo = v[lane], hi = v[WAVE + lane];
+      fr[e] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    };
     auto turn = [&](auto whole_, int t) {
       __syncthreads();
-      if (t + 1 < t1) {
+      const bool works = row0 < n_rows;
+      if constexpr (AHEAD) {
+        if (works)
+#pragma unroll
+          for (int n = 0; n < EPL; ++n) read_key(wk, n);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (brings && t + 1 < t1) {
         put(t + 1, buf ^ 1);
         if (t + 2 < t1) {
           fetch();
           if (t + 3 < t1) fetch_slots(t + 3);
         }
       }
-      if (row0 < n_rows) {
-        for (int blk = wk; blk < 2; blk += WK) {
-          const uint32_t all = __builtin_amdgcn_readfirstlane(s_here[buf][2 * blk] | s_here[buf][2 * blk + 1] << 16);
+      if (works) {
+        auto one = [&](int blk, auto more_) {
+          constexpr bool more = decltype(more_)::value;
           float cs[8], vn[8];
           if constexpr (QUANT) {
             float kf[8], vf[8];
@@ -695,18 +792,38 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
             }
             factors(kf, vf, cs, vn);
           }
-          const uint32_t here = ((all >> (g * 4)) & 0xfu) | (((all >> (16 + g * 4)) & 0xfu) << 4);
-          step(whole_, t * AT_TILE + blk * AT_STEP, here, cs, vn,
+          uint32_t here = 0;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            here |= ((__builtin_amdgcn_readfirstlane(s_here[buf][2 * blk + i]) >> (g * 4)) & 0xfu) << (4 * i);
+          step(whole_, Int<1>{}, t * AT_TILE + blk * AT_STEP, here, cs, vn,
                [&](int i, int kk, uint32_t (&ko)[4]) {
-                 const uint4 v = s_frag[buf][(blk * 2 + i) * NK + kk][lane];
+                 if constexpr (!AHEAD) read_key(blk, i * NK + kk);
+                 const uint4 v = fr[i * NK + kk];
                  ko[0] = v.x, ko[1] = v.y, ko[2] = v.z, ko[3] = v.w;
                },
-               [&](int e, uint32_t (&vo)[4]) {
-                 const uint2* v = reinterpret_cast<const uint2*>(s_frag[buf][4 * NK + blk * EPL + e]);
-                 vo[0] = v[lane].x, vo[1] = v[lane].y, vo[2] = v[WAVE + lane].x, vo[3] = v[WAVE + lane].y;
+               [&](int, int e, uint32_t (&vo)[4]) {
+                 if constexpr (!AHEAD) read_value(blk, e);
+                 const uint4 v = fr[e];
+                 vo[0] = v.x, vo[1] = v.y, vo[2] = v.z, vo[3] = v.w;
                },
-               [] {});
-        }
+               [&]() {
+                 if constexpr (AHEAD) {
+                   __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                   for (int e = 0; e < EPL; ++e) read_value(blk, e);
+                   __builtin_amdgcn_sched_barrier(0);
+                 }
+               },
+               [&](int e) {
+                 if constexpr (AHEAD && more) {
+                   read_key(blk + 1, e);
+                   __builtin_amdgcn_sched_barrier(0);
+                 }
+               });
+        };
+        one(wk, Int<WK == 1>{});
+        if constexpr (WK == 1) one(1, Int<0>{});
       }
       buf ^= 1;
     };
@@ -792,26 +909,32 @@ __global__ __launch_bounds__(AT_THREADS, OCC) void k_attn(AttnParams P) {
   }
 }
 
-// Row tiles a wave, waves over the rows and row blocks of T nodes with G query heads each.
+// How the rows of a request (T nodes of G query heads) are split: row tiles a wave, waves (or pairs) a workgroup, row
+// blocks.
 struct AttnShape {
-  int R, WR, RB;
-  bool staged;
+  int form, R, WR, RB;
+  int waves;  // of a workgroup
 };
+// Waves a SIMD the kernels' registers are held to.
+constexpr int attn_occupancy(int form, int R, int dim) {
+  return dim > 128 && form != AT_ROWS ? 1 : 2;
+}
 
 template <int XT, int CT>
 void launch_attn(const AttnParams& P, const AttnShape& s, unsigned blocks, hipStream_t stream) {
-  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3(blocks), dim3(AT_THREADS), 0, stream, P); };
+  auto go = [&](auto kern, int n) { hipLaunchKernelGGL(kern, dim3(blocks), dim3((unsigned)n * 64u), 0, stream, P); };
   const int D = P.a.cache.dim;
   auto width = [&](auto dp, auto full) {
     constexpr int DP = decltype(dp)::value;
     constexpr bool FULL = decltype(full)::value;
-    constexpr int OCC = DP > 128 ? 1 : 2;
-    if (!s.staged)
-      go(k_attn<XT, CT, DP, FULL, 1, false, OCC>);
+    if (s.form == AT_DIRECT)
+      go(k_attn<XT, CT, DP, FULL, 1, AT_DIRECT, AT_WAVES, attn_occupancy(AT_DIRECT, 1, DP)>, s.waves);
+    else if (s.form == AT_PAIRS)
+      go(k_attn<XT, CT, DP, FULL, 1, AT_PAIRS, AT_WAVES, attn_occupancy(AT_PAIRS, 1, DP)>, s.waves);
     else if (s.R == 1)
-      go(k_attn<XT, CT, DP, FULL, 1, true, OCC>);
-    else
-      go(k_attn<XT, CT, DP, FULL, 2, true, OCC>);
+      go(k_attn<XT, CT, DP, FULL, 1, AT_ROWS, AT_MOST, attn_occupancy(AT_ROWS, 1, DP)>, s.waves);
+    else if constexpr (DP <= 128)
+      go(k_attn<XT, CT, DP, FULL, 2, AT_ROWS, AT_MOST, attn_occupancy(AT_ROWS, 2, DP)>, s.waves);
   };
   if (D <= 64)
     D == 64 ? width(Int<64>{}, Int<1>{}) : width(Int<64>{}, Int<0>{});

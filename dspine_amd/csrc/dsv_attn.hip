@@ -11,22 +11,24 @@ extern template void launch_attn<DSV_F16, DSV_E4M3>(const AttnParams&, const Att
 extern template void launch_attn<DSV_BF16, DSV_I8>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
 extern template void launch_attn<DSV_F16, DSV_I8>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
 
+constexpr int AJ_THREADS = 256;
+
 // The parts of a request joined: 8 elements of a row a thread, the parts in their order.  Bound by latency (the plan's
 // lengths, the references, the sums) and by the sums' bytes.
 template <int XT, int DP>
-__global__ __launch_bounds__(AT_THREADS) void k_attn_join(AttnParams P) {
+__global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
   const dsv_tree_attention_args& a = P.a;
   const dsv_kv_cache& c = a.cache;
-  constexpr int PER = DP / 8, ROWS = AT_THREADS / PER;
+  constexpr int PER = DP / 8, ROWS = AJ_THREADS / PER;
   const int lane = threadIdx.x & (WAVE - 1);
   const int rows = a.T * P.G, blocks = (rows + ROWS - 1) / ROWS;
   const int b = (int)(blockIdx.x / (c.heads * blocks)), in = (int)(blockIdx.x - (int64_t)b * c.heads * blocks);
   const int h = in / blocks, r = (in - h * blocks) * ROWS + (int)threadIdx.x / PER, d = (int)threadIdx.x % PER * 8;
-  const Request req = request_of(a, b);
+  const Plan plan = plan_of(P, lane);
+  const Request req = request_in(P, plan, b);
   const int tiles = tiles_of(req);
   if ((in - h * blocks) * ROWS >= req.nodes * P.G) return;
-  const Plan plan = plan_of(P, lane);
-  const int64_t before = tiles_before(P, b, lane);
+  const int64_t before = tiles_before(P, plan, b, lane);
   const int i0 = plan.range_of(before), i1 = plan.range_of(before + tiles - 1);
   if (i0 == i1 || r >= req.nodes * P.G || d >= c.dim) return;
   const int node = r / P.G, qh = h * P.G + r - node * P.G;
@@ -62,10 +64,25 @@ __global__ __launch_bounds__(AT_THREADS) void k_attn_join(AttnParams P) {
   if (d == 0 && a.lse) a.lse[row * a.q_heads + qh] = lt == 0.f ? -INFINITY : (top + log2f(lt)) * 0.693147180559945309f;
 }
 
+static AttnShape attn_shape(int T, int G, int dim) {
+  const int tiles = (T * G + 15) / 16;
+  AttnShape s;
+  s.form = tiles == 1 ? AT_DIRECT : (tiles == 2 ? AT_PAIRS : AT_ROWS);
+  s.R = tiles > AT_MOST && dim <= 128 ? 2 : 1;
+  const int groups = (tiles + s.R - 1) / s.R;
+  s.WR = groups < AT_MOST ? groups : AT_MOST;
+  s.RB = (groups + s.WR - 1) / s.WR;
+  s.waves = s.WR > AT_WAVES ? s.WR : AT_WAVES;
+  return s;
+}
+
 // Ranges at most: as many as workgroups run at once (or a few times as many where the heads and row blocks leave too
 // many of those idle otherwise).
-static int attn_ranges(int heads, int RB, bool wide) {
-  const int64_t slots = wide ? 256 : 512, hb = (int64_t)heads * RB;
+static int attn_ranges(const AttnShape& s, int heads, int dim) {
+  const int lds = s.form == AT_DIRECT ? (dim > 128 ? 2 : 4) : (dim > 128 ? 1 : (dim > 64 ? 2 : 4));
+  int per = 4 * attn_occupancy(s.form, s.R, dim) / s.waves;  // workgroups a CU
+  per = per < 1 ? 1 : (per > lds ? lds : per);
+  const int64_t slots = 256 * per, hb = (int64_t)heads * s.RB;
   int64_t best = 1;
   double use = 0.0;
   for (int k = 1; k <= 4; ++k) {
@@ -76,17 +93,6 @@ static int attn_ranges(int heads, int RB, bool wide) {
   return (int)best;
 }
 
-static AttnShape attn_shape(int T, int G) {
-  const int tiles = (T * G + 15) / 16;
-  AttnShape s;
-  s.staged = tiles > 1;
-  s.R = tiles > 4 ? 2 : 1;
-  const int groups = (tiles + s.R - 1) / s.R;
-  s.WR = !s.staged ? 1 : (groups > 2 ? 4 : 2);  // (a staged tile has two steps for waves of the same rows)
-  s.RB = (groups + s.WR - 1) / s.WR;
-  return s;
-}
-
 }  // namespace dsv
 
 using namespace dsv;
@@ -94,8 +100,8 @@ using namespace dsv;
 extern "C" int64_t dsv_tree_attention_workspace_bytes(int32_t bs, int32_t T, int32_t heads, int32_t q_heads,
                                                       int32_t dim) {
   if (bs < 1 || T < 1 || heads < 1 || q_heads < heads || dim < 1) return 0;
-  const AttnShape s = attn_shape(T, q_heads / heads);
-  const int64_t rows = 2 * (int64_t)attn_ranges(heads, s.RB, dim > 128) * q_heads * T;
+  const AttnShape s = attn_shape(T, q_heads / heads, dim);
+  const int64_t rows = 2 * (int64_t)attn_ranges(s, heads, dim) * q_heads * T;
   return rows * (dim * (int64_t)sizeof(float) + (int64_t)sizeof(float2));
 }
 
@@ -127,13 +133,13 @@ extern "C" int dsv_tree_attention(const dsv_tree_attention_args* args, dsv_strea
   AttnParams P;
   P.a = a;
   P.G = a.q_heads / a.cache.heads;
-  const AttnShape s = attn_shape(a.T, P.G);
+  const AttnShape s = attn_shape(a.T, P.G, a.cache.dim);
   P.WR = s.WR;
   P.RB = s.RB;
-  P.most = attn_ranges(a.cache.heads, s.RB, a.cache.dim > 128);
+  P.most = attn_ranges(s, a.cache.heads, a.cache.dim);
   P.least = 2;
   const int64_t blocks = (P.most + 7) / 8 * 8 * (int64_t)a.cache.heads * s.RB;
-  const int64_t wide = a.cache.dim <= 64 ? 64 : (a.cache.dim <= 128 ? 128 : 256), per = AT_THREADS / (wide / 8);
+  const int64_t wide = a.cache.dim <= 64 ? 64 : (a.cache.dim <= 128 ? 128 : 256), per = AJ_THREADS / (wide / 8);
   const int64_t joins = (a.T * (int64_t)P.G + per - 1) / per * a.cache.heads * a.bs;
   if (blocks > 0x7fffffffll || joins > 0x7fffffffll)
     DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: too many nodes for one call");
@@ -156,7 +162,7 @@ extern "C" int dsv_tree_attention(const dsv_tree_attention_args* args, dsv_strea
     bf ? launch_attn<DSV_BF16, DSV_BF16>(P, s, (unsigned)blocks, stream) : launch_attn<DSV_F16, DSV_F16>(P, s, (unsigned)blocks, stream);
   DSV_CHECK_LAUNCH("k_attn");
   if (P.most > 1) {
-    auto join = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)joins), dim3(AT_THREADS), 0, stream, P); };
+    auto join = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)joins), dim3(AJ_THREADS), 0, stream, P); };
     if (wide == 64)
       bf ? join(k_attn_join<DSV_BF16, 64>) : join(k_attn_join<DSV_F16, 64>);
     else if (wide == 128)
