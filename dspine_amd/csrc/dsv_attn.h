@@ -248,6 +248,7 @@ __device__ __forceinline__ uint64_t mask_of(const dsv_tree_attention_args& a, in
 
 // FORM: direct, or staged with a wave (AT_ROWS) or two (AT_PAIRS) for a group of rows.
 enum { AT_DIRECT = 0, AT_PAIRS = 1, AT_ROWS = 2 };
+constexpr int AT_DEPTH(int R, int DP) { return R == 1 && DP <= 128 ? 2 : 1; }
 
 template <int XT, int CT, int DP, bool FULL, int R, int FORM, int WAVES, int OCC>
 __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
@@ -303,26 +304,25 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
   if (tid == 0) s_odd = 0;
   __syncthreads();
 
-  // queries, in the order of the keys' elements
+  // Queries, in the order of the keys' elements.  They are waited for here, before the loops: a wait inside would be one
+  // for every load in flight.
   uint32_t qf[R][NK][4];
+  auto load_queries = [&]() {
 #pragma unroll
-  for (int rt = 0; rt < R; ++rt) {
-    const int r = row0 + rt * 16 + m;
-    const int64_t row = r < n_rows ? row_of(a, request, r / P.G) : -1;
-    const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (row < 0 ? 0 : row) * a.q_row_stride +
-                        (int64_t)(h * P.G + r % P.G) * a.q_head_stride;
+    for (int rt = 0; rt < R; ++rt) {
+      const int r = row0 + rt * 16 + m;
+      const int64_t row = r < n_rows ? row_of(a, request, r / P.G) : -1;
+      const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (row < 0 ? 0 : row) * a.q_row_stride +
+                          (int64_t)(h * P.G + r % P.G) * a.q_head_stride;
 #pragma unroll
-    for (int kk = 0; kk < NK; ++kk) {
-      const int d = QUANT ? (kk / 2) * 64 + g * 16 + (kk & 1) * 8 : kk * 32 + g * 8;
-      uint32_t w[4] = {0, 0, 0, 0};
-      if (row >= 0 && d < dim) load_words<4>(q + d, w);
+      for (int kk = 0; kk < NK; ++kk) {
+        const int d = QUANT ? (kk / 2) * 64 + g * 16 + (kk & 1) * 8 : kk * 32 + g * 8;
+        uint32_t w[4] = {0, 0, 0, 0};
+        if (row >= 0 && d < dim) load_words<4>(q + d, w);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) qf[rt][kk][i] = w[i];
+        for (int i = 0; i < 4; ++i) qf[rt][kk][i] = w[i];
+      }
     }
-  }
-
-  // Before the loops the queries must have come: a wait for them inside would be one for every load in flight.
-  auto queries_here = [&]() {
 #pragma unroll
     for (int rt = 0; rt < R; ++rt)
 #pragma unroll
@@ -610,7 +610,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       for (int j = 0; j < 8; ++j) here |= (good(vs[j]) ? 1u : 0u) << j;
       return here;
     };
-    queries_here();
+    load_queries();
     // steps of this wave: every WK-th
     int t = t0 * (AT_TILE / AT_STEP) + wk;
     int end = t1 * (AT_TILE / AT_STEP);
@@ -621,46 +621,48 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
     // two steps ahead.
     const int whole = clear / AT_STEP < end ? clear / AT_STEP : end;
     if (t < whole) {
-      uint32_t ks[2], vs[8], here0, here1, kw[2][KL][4], wv0[8][VW], wv1[8][VW];
-      float scale, cs[8], vn[8];
-      auto load_values = [&](uint32_t (&wv)[8][VW], uint32_t& here) {
+      uint32_t ks0[2], vs0[8], ks1[2], vs1[8], here0, here1, kw[2][KL][4], wv0[8][VW], wv1[8][VW];
+      float scale;
+      auto slots = [&](int i, uint32_t (&ks)[2], uint32_t (&vs)[8]) {
+        ks[0] = (uint32_t)table[i * AT_STEP + m];
+        ks[1] = (uint32_t)table[i * AT_STEP + 16 + m];
+        value_slots(Int<1>{}, i * AT_STEP, vs);
+      };
+      auto load = [&](const uint32_t (&ks)[2], const uint32_t (&vs)[8], uint32_t (&wv)[8][VW], uint32_t& here) {
+        load_key(ks[0], kw[0]);
+        load_key(ks[1], kw[1]);
+        scale = load_scale(ks[0], ks[1]);
         here = holds(vs);
 #pragma unroll
         for (int j = 0; j < 8; ++j) load_value(vs[j], wv[j]);
       };
-      auto go = [&](uint32_t (&wv)[8][VW], uint32_t here, uint32_t (&then)[8][VW], uint32_t& then_here) {
-        float kf[8], vf[8];
+      // (the slots of the step after the next are asked for before the next one's data: a wait for them, loads being
+      // counted in order, is none for that data)
+      auto go = [&](uint32_t (&wv)[8][VW], uint32_t here, uint32_t (&then)[8][VW], uint32_t& then_here, uint32_t (&ks)[2],
+                    uint32_t (&vs)[8], uint32_t (&then_ks)[2], uint32_t (&then_vs)[8]) {
+        float kf[8], vf[8], cs[8], vn[8];
         spread_scales(scale, kf, vf);
         factors(kf, vf, cs, vn);
         step(Int<1>{}, Int<1>{}, t * AT_STEP, here, cs, vn,
              [&](int i, int kk, uint32_t (&ko)[4]) { key_frag(kw[i], kk, ko); },
              [&](int, int e, uint32_t (&vo)[4]) { value_operand<CT>(wv, e, vo); },
              [&]() {
+               slots(t + 2 * WK < whole ? t + 2 * WK : t, then_ks, then_vs);
+               __builtin_amdgcn_sched_barrier(0);
+               load(ks, vs, then, then_here);
+               __builtin_amdgcn_sched_barrier(0);
                if (__any(here != 0xffu)) clear_values(here, false, wv);
-               load_key(ks[0], kw[0]);
-               load_key(ks[1], kw[1]);
-               scale = load_scale(ks[0], ks[1]);
-               load_values(then, then_here);
-               const int ahead = t + 2 * WK < whole ? t + 2 * WK : t;
-               ks[0] = (uint32_t)table[ahead * AT_STEP + m];
-               ks[1] = (uint32_t)table[ahead * AT_STEP + 16 + m];
-               value_slots(Int<1>{}, ahead * AT_STEP, vs);
              },
              [](int) {});
         t += WK;
       };
-      key_slots(t * AT_STEP, ks[0], ks[1]);
-      value_slots(Int<1>{}, t * AT_STEP, vs);
-      load_key(ks[0], kw[0]);
-      load_key(ks[1], kw[1]);
-      scale = load_scale(ks[0], ks[1]);
-      load_values(wv0, here0);
-      key_slots((t + WK < whole ? t + WK : t) * AT_STEP, ks[0], ks[1]);
-      value_slots(Int<1>{}, (t + WK < whole ? t + WK : t) * AT_STEP, vs);
+      slots(t, ks0, vs0);
+      slots(t + WK < whole ? t + WK : t, ks1, vs1);
+      load(ks0, vs0, wv0, here0);
       while (true) {
-        go(wv0, here0, wv1, here1);
+        go(wv0, here0, wv1, here1, ks1, vs1, ks0, vs0);
         if (t >= whole) break;
-        go(wv1, here1, wv0, here0);
+        go(wv1, here1, wv0, here0, ks0, vs0, ks1, vs1);
         if (t >= whole) break;
       }
     }
@@ -687,66 +689,81 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
     uint4(*const s_frag)[FRAGS][WAVE] = reinterpret_cast<uint4(*)[FRAGS][WAVE]>(s_mem);
     __shared__ float s_scale[2][2][AT_TILE];
     __shared__ uint32_t s_here[2][AT_WAVES];
-    // Each of the first waves brings 16 positions: lane (m, g) pieces of the key of position m, and of the values of g * 4 .. g * 4 + 3.
-    uint32_t kw[KL][4], wv[4][VW], kslot = ~0u, vslot[4];
-    uint32_t have = 0;  // bits of the 16 positions
-    float scale = 0.f;
-    auto fetch_slots = [&](int t) {
+    // Each of the first waves brings 16 positions: lane (m, g) pieces of the key of position m, and of the values of
+    // g * 4 .. g * 4 + 3.  The loads run DEPTH tiles ahead of the one that is put away (in two sets of registers where
+    // there are that many).
+    constexpr int DEPTH = AT_DEPTH(R, DP);
+    struct Brought {
+      uint32_t kw[KL][4], wv[4][VW];
+      uint32_t kslot, vslot[4];  // of the next tile to be loaded
+      uint32_t have;             // bits of the 16 positions
+      float scale;
+    };
+    Brought sets[DEPTH];
+    auto fetch_slots = [&](Brought& f, int t) {
+      if (t >= t1) return;
       const int base = t * AT_TILE + wave * 16;
       if (base + 16 <= req.total) {
-        kslot = (uint32_t)table[base + m];
+        f.kslot = (uint32_t)table[base + m];
         uint4 v;
         __builtin_memcpy(&v, table + base + g * 4, 16);
-        vslot[0] = v.x, vslot[1] = v.y, vslot[2] = v.z, vslot[3] = v.w;
+        f.vslot[0] = v.x, f.vslot[1] = v.y, f.vslot[2] = v.z, f.vslot[3] = v.w;
       } else {
-        kslot = base + m <= last ? (uint32_t)table[base + m] : ~0u;
+        f.kslot = base + m <= last ? (uint32_t)table[base + m] : ~0u;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) vslot[j] = base + g * 4 + j <= last ? (uint32_t)table[base + g * 4 + j] : ~0u;
+        for (int j = 0; j < 4; ++j) f.vslot[j] = base + g * 4 + j <= last ? (uint32_t)table[base + g * 4 + j] : ~0u;
       }
     };
-    auto fetch = [&]() {
-      load_key(kslot, kw);
+    auto fetch = [&](Brought& f) {
+      load_key(f.kslot, f.kw);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) load_value(vslot[j], wv[j]);
-      have = (uint32_t)__ballot(good(kslot)) & 0xffffu;
+      for (int j = 0; j < 4; ++j) load_value(f.vslot[j], f.wv[j]);
+      f.have = (uint32_t)__ballot(good(f.kslot)) & 0xffffu;
       if constexpr (QUANT) {
-        const int64_t s = good(kslot) ? kslot : 0u;
-        if (g < 2) scale = g == 0 ? ksc[s * c.ks_slot_stride] : vsc[s * c.vs_slot_stride];
-        if (!good(kslot)) scale = 0.f;
+        const int64_t s = good(f.kslot) ? f.kslot : 0u;
+        if (g < 2) f.scale = g == 0 ? ksc[s * c.ks_slot_stride] : vsc[s * c.vs_slot_stride];
+        if (!good(f.kslot)) f.scale = 0.f;
       }
     };
-    auto put = [&](int t, int buf) {
-      uint4(*const f)[WAVE] = s_frag[buf];
+    auto put = [&](Brought& f, int t, int buf) {
+      uint4(*const to)[WAVE] = s_frag[buf];
       const bool aside = t * AT_TILE + SET_ASIDE > clear;
-      if (aside || have != 0xffffu) clear_values(have >> (g * 4), aside, wv);
+      if (aside || f.have != 0xffffu) clear_values(f.have >> (g * 4), aside, f.wv);
 #pragma unroll
       for (int kk = 0; kk < NK; ++kk) {
         uint32_t ko[4];
-        key_frag(kw, kk, ko);
-        f[wave * NK + kk][lane] = make_uint4(ko[0], ko[1], ko[2], ko[3]);
+        key_frag(f.kw, kk, ko);
+        to[wave * NK + kk][lane] = make_uint4(ko[0], ko[1], ko[2], ko[3]);
       }
 #pragma unroll
       for (int e = 0; e < EPL; ++e) {
         uint32_t vo[2];
-        value_operand<CT>(wv, e, vo);
-        reinterpret_cast<uint2*>(f[4 * NK + (wave / 2) * EPL + e])[(wave & 1) * WAVE + lane] = make_uint2(vo[0], vo[1]);
+        value_operand<CT>(f.wv, e, vo);
+        reinterpret_cast<uint2*>(to[4 * NK + (wave / 2) * EPL + e])[(wave & 1) * WAVE + lane] = make_uint2(vo[0], vo[1]);
       }
       if constexpr (QUANT)
-        if (g < 2) s_scale[buf][g][wave * 16 + m] = scale;
-      if (lane == 0) s_here[buf][wave] = have;
+        if (g < 2) s_scale[buf][g][wave * 16 + m] = f.scale;
+      if (lane == 0) s_here[buf][wave] = f.have;
     };
     int buf = 0;
     const bool brings = wave < AT_WAVES;
-    if (brings) fetch_slots(t0);
-    queries_here();
-    if (brings) {
-      fetch();
-      if (t0 + 1 < t1) fetch_slots(t0 + 1);
-      put(t0, 0);
-      if (t0 + 1 < t1) {
-        fetch();
-        if (t0 + 2 < t1) fetch_slots(t0 + 2);
+    // the loads of tile t and the slots of the set's next one
+    auto ask = [&](Brought& f, int t) {
+      if (t < t1) {
+        fetch(f);
+        fetch_slots(f, t + DEPTH);
       }
+    };
+    if (brings) {
+      fetch_slots(sets[0], t0);
+      if constexpr (DEPTH > 1) fetch_slots(sets[1], t0 + 1);
+      ask(sets[0], t0);
+      if constexpr (DEPTH > 1) ask(sets[1], t0 + 1);
+    }
+    load_queries();
+    if (brings) {
+      put(sets[0], t0, 0);
+      ask(sets[0], t0 + DEPTH);
     }
     // A turn: the next tile into the other buffer, the loads of the one after it, the products of this one.  A step's keys
     // are read from LDS while the step before it multiplies (the first step's while the next tile is put away), its values
@@ -761,7 +778,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       const uint2 lo = v[lane], hi = v[WAVE + lane];
       fr[e] = make_uint4(lo.x, lo.y, hi.x, hi.y);
     };
-    auto turn = [&](auto whole_, int t) {
+    auto turn = [&](auto whole_, Brought& next, int t) {
       __syncthreads();
       const bool works = row0 < n_rows;
       if constexpr (AHEAD) {
@@ -771,11 +788,8 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
         __builtin_amdgcn_sched_barrier(0);
       }
       if (brings && t + 1 < t1) {
-        put(t + 1, buf ^ 1);
-        if (t + 2 < t1) {
-          fetch();
-          if (t + 3 < t1) fetch_slots(t + 3);
-        }
+        put(next, t + 1, buf ^ 1);
+        ask(next, t + 1 + DEPTH);
       }
       if (works) {
         auto one = [&](int blk, auto more_) {
@@ -829,8 +843,20 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
     };
     const int whole = clear / AT_TILE < t1 ? clear / AT_TILE : t1;
     int t = t0;
-    for (; t < whole; ++t) turn(Int<1>{}, t);
-    for (; t < t1; ++t) turn(Int<0>{}, t);
+    if constexpr (DEPTH == 1) {
+      for (; t < whole; ++t) turn(Int<1>{}, sets[0], t);
+      for (; t < t1; ++t) turn(Int<0>{}, sets[0], t);
+    } else {
+      // (turn t puts away the set of t + 1 - t0)
+      for (; t + 1 < whole; t += 2) {
+        turn(Int<1>{}, sets[1], t);
+        turn(Int<1>{}, sets[0], t + 1);
+      }
+      for (; t < t1; t += 2) {
+        turn(Int<0>{}, sets[1], t);
+        if (t + 1 < t1) turn(Int<0>{}, sets[0], t + 1);
+      }
+    }
   }
 
   // The waves of the same rows join: their references, then the sums of one row tile after another through LDS.

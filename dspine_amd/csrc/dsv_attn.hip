@@ -137,7 +137,7 @@ extern "C" int dsv_tree_attention(const dsv_tree_attention_args* args, dsv_strea
   P.WR = s.WR;
   P.RB = s.RB;
   P.most = attn_ranges(s, a.cache.heads, a.cache.dim);
-  P.least = 2;
+  P.least = s.form == AT_ROWS ? 4 : 2;
   const int64_t blocks = (P.most + 7) / 8 * 8 * (int64_t)a.cache.heads * s.RB;
   const int64_t wide = a.cache.dim <= 64 ? 64 : (a.cache.dim <= 128 ? 128 : 256), per = AJ_THREADS / (wide / 8);
   const int64_t joins = (a.T * (int64_t)P.G + per - 1) / per * a.cache.heads * a.bs;
