@@ -248,6 +248,18 @@ def stream_of(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def launch(what: str, device: torch.device, call, *args) -> None:
+    """``call(*args, stream)`` on the device's current stream, that device being the current one
+    during the call."""
+    if torch.cuda.current_device() == device.index:
+        rc = call(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = call(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if rc != DSV_OK:
+        check(rc, what)
+
+
 def dtype_code(t: torch.Tensor) -> int:
     if t.dtype == torch.bfloat16:
         return DSV_BF16

@@ -40,45 +40,89 @@ __global__ __launch_bounds__(256) void k_tree_masks(const int32_t* parents, int 
   }
 }
 
-// The largest logit of a piece of a row as (value key, ~id): the maximum is the row's first argmax.  One pass
-// over the logits, bound by memory; rows at or past their request's length are not read.
+// The largest logit of a piece of a row as (value key, ~id): the maximum is the row's first argmax.  One pass over
+// the logits, bound by memory: 16-byte vectors of the row's aligned part, TA_VECS in flight a thread; a thread keeps
+// its best vector and looks into it at the end (with a key for every logit the pass ran at 1.5 TB/s).  Rows at or
+// past their request's length are not read.
 constexpr int TA_THREADS = 256;
-constexpr int TA_VECS = 8;  // 16-byte vectors a thread has in flight
+constexpr int TA_VECS = 8;
 
+template <int DT>
+__host__ __device__ constexpr int ta_per() {
+  return DT == DSV_BF16 ? 8 : 4;  // logits of a vector
+}
 template <int DT>
 __host__ __device__ constexpr int64_t ta_piece() {
-  return (int64_t)TA_THREADS * TA_VECS * (DT == DSV_BF16 ? 8 : 4);
+  return (int64_t)TA_THREADS * TA_VECS * ta_per<DT>();
 }
 
 template <int DT>
-__device__ __forceinline__ uint64_t arg_key(uint32_t bits, uint32_t id) {
-  const uint32_t k = DT == DSV_BF16 ? f32_key(bf16_bits_to_f32(bits)) : f32_key(__uint_as_float(bits));
-  return ((uint64_t)k << 32) | (uint32_t)~id;
+__device__ __forceinline__ float ta_value(const uint4& v, int i) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  if constexpr (DT == DSV_BF16)
+    return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+  else
+    return __uint_as_float(w[i]);
 }
+__device__ __forceinline__ uint64_t ta_key(float x, uint32_t id) { return ((uint64_t)f32_key(x) << 32) | (uint32_t)~id; }
 
 template <int DT>
 __global__ __launch_bounds__(TA_THREADS) void k_tree_argmax(const void* logits, int64_t vocab, int64_t stride, int T,
                                                             const int32_t* lens, int C, uint64_t* best) {
   using elem = typename std::conditional<DT == DSV_BF16, uint16_t, uint32_t>::type;
+  constexpr int PER = ta_per<DT>();
   __shared__ uint64_t s_best[TA_THREADS / WAVE];
-  const int64_t row = blockIdx.x / C;
-  const int c = (int)(blockIdx.x - row * C);
+  const int row = (int)(blockIdx.x / (unsigned)C), c = (int)(blockIdx.x - (unsigned)row * (unsigned)C);
   if (lens) {
-    const int64_t b = row / T;
-    const int i = (int)(row - b * T);
-    const int n = lens[b];
-    if (i > 0 && i >= n) return;
+    const int b = row / T, i = row - b * T;
+    if (i > 0 && i >= lens[b]) return;
   }
   const elem* x = reinterpret_cast<const elem*>(logits) + row * stride;
-  const int64_t from = c * ta_piece<DT>();
-  const int64_t to = from + ta_piece<DT>() < vocab ? from + ta_piece<DT>() : vocab;
-  uint64_t m = 0;
-  for (int64_t i = from + threadIdx.x; i < to; i += TA_THREADS) {
-    const uint64_t k = arg_key<DT>(x[i], (uint32_t)i);
-    m = k > m ? k : m;
+  const int tid = threadIdx.x;
+  // logits before the first 16-byte boundary, whole vectors, logits behind them
+  int lead = (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(elem);
+  lead = lead < vocab ? lead : (int)vocab;
+  const int vecs = (int)((vocab - lead) / PER);
+  const uint4* v = reinterpret_cast<const uint4*>(x + lead);
+  uint4 got[TA_VECS];
+  const int first = c * TA_THREADS * TA_VECS + tid;
+#pragma unroll
+  for (int u = 0; u < TA_VECS; ++u) {
+    const int i = first + u * TA_THREADS;
+    if (i < vecs) got[u] = v[i];
   }
-  m = block_max_u64<TA_THREADS / WAVE>(m, s_best);
-  if (threadIdx.x == 0) best[row * C + c] = m;
+  float top = -INFINITY;
+  int at = -1;
+  uint4 which = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int u = 0; u < TA_VECS; ++u) {
+    const int i = first + u * TA_THREADS;
+    float m = ta_value<DT>(got[u], 0);
+#pragma unroll
+    for (int k = 1; k < PER; ++k) m = fmaxf(m, ta_value<DT>(got[u], k));
+    if (i < vecs && (m > top || at < 0)) {
+      top = m;
+      at = i;
+      which = got[u];
+    }
+  }
+  uint64_t key = 0;
+  if (at >= 0) {
+#pragma unroll
+    for (int k = PER - 1; k >= 0; --k)  // (the first of equal ones is left)
+      if (ta_value<DT>(which, k) == top) key = ta_key(top, (uint32_t)(lead + at * PER + k));
+  }
+  if (c == 0) {  // the row's ends
+    const int behind = (int)(vocab - lead) - vecs * PER;
+    if (tid < lead + behind) {
+      const int id = tid < lead ? tid : (int)vocab - behind + (tid - lead);
+      const float y = DT == DSV_BF16 ? bf16_bits_to_f32(x[id]) : __uint_as_float(x[id]);
+      const uint64_t k = ta_key(y, (uint32_t)id);
+      key = k > key ? k : key;
+    }
+  }
+  key = block_max_u64<TA_THREADS / WAVE>(key, s_best);
+  if (tid == 0) best[(int64_t)row * C + c] = key;
 }
 
 // The walk, without walking: node i fits when its token is its parent's argmax, no sibling before it carries the

@@ -11,7 +11,7 @@ import math
 import torch
 
 from dspine_amd import _lib
-from dspine_amd.kernels.cache import _ACT, QUANTISED, KVCache, _distinct, _rows, _strides, cache_fields, tensors_of
+from dspine_amd.kernels.cache import _ACT, QUANTISED, KVCache, _distinct, _rows, cache_fields, tensors_of
 from dspine_amd.verify import Workspace
 
 MAX_NODES = 64
@@ -77,27 +77,19 @@ def tree_attention(q: torch.Tensor, cache: KVCache, *, T: int, page_table: torch
     if lse is not None and (lse.shape != (rows, heads) or lse.dtype != torch.float32 or not lse.is_contiguous()):
         raise ValueError("lse must be contiguous float32 [rows, q_heads]")
     if rows:
-        _rows(q, "q")
-        _rows(out, "out")
+        q_at, q_row, q_head = _rows(q, "q")
+        out_at, out_row, out_head = _rows(out, "out")
         _distinct(out, "out")
     dev = _lib.require_cuda(q, *tensors_of(cache), page_table, prefix_lens, verify_lens, row_offsets, masks, out, lse)
     if rows == 0:
         return out
     lib = _lib.load()
-    a = _lib.TreeAttentionArgs()
-    a.cache = c
-    a.q, a.out, a.lse = q.data_ptr(), out.data_ptr(), _lib.ptr(lse)
-    a.dtype, a.q_heads, a.rows = _ACT[q.dtype], heads, rows
-    a.q_row_stride, a.q_head_stride = _strides(q)
-    a.out_row_stride, a.out_head_stride = _strides(out)
-    a.bs, a.T = bs, T
-    a.prefix_lens, a.verify_lens = prefix_lens.data_ptr(), _lib.ptr(verify_lens)
-    a.row_offsets = _lib.ptr(row_offsets)
-    a.row_offsets_i64 = int(row_offsets is not None and row_offsets.dtype == torch.int64)
-    a.scale, a.masks = scale, _lib.ptr(masks)
-    a.page_table, a.page_stride, a.page_cols = page_table.data_ptr(), page_table.stride(0), page_table.shape[1]
-    wbuf = (workspace or Workspace()).get(int(lib.dsv_tree_attention_workspace_bytes(bs, T, c.heads, heads, dim)), dev)
-    a.workspace, a.workspace_bytes = wbuf.data_ptr(), wbuf.numel()
-    with torch.cuda.device(dev):
-        _lib.check(lib.dsv_tree_attention(a, _lib.stream_of(dev)), "dsv_tree_attention")
+    ptr = _lib.ptr
+    wbuf = (workspace or Workspace()).get(lib.dsv_tree_attention_workspace_bytes(bs, T, c.heads, heads, dim), dev)
+    a = _lib.TreeAttentionArgs(
+        c, q_at, out_at, ptr(lse), _ACT[q.dtype], heads, rows, q_row, q_head, out_row, out_head, bs, T,
+        prefix_lens.data_ptr(), ptr(verify_lens), ptr(row_offsets),
+        int(row_offsets is not None and row_offsets.dtype == torch.int64), scale, ptr(masks), page_table.data_ptr(),
+        page_table.stride(0), page_table.shape[1], wbuf.data_ptr(), wbuf.numel())
+    _lib.launch("dsv_tree_attention", dev, lib.dsv_tree_attention, a)
     return out

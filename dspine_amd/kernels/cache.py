@@ -45,21 +45,26 @@ def new_cache(num_slots: int, heads: int, dim: int, *, dtype: torch.dtype = torc
 
 
 def _rows(t, name):
-    """Whether t [., heads, dim] has contiguous rows on 16-byte boundaries."""
-    if t.stride(2) != 1 and t.shape[2] != 1:
-        raise ValueError(f"{name} must have a contiguous last dimension")
-    size = t.element_size()
-    if t.data_ptr() % 16 or any(t.stride(i) * size % 16 for i in (0, 1) if t.shape[i] > 1):
+    """(address, row stride, head stride) of t [., heads, dim]; its rows must be contiguous and start
+    on 16-byte boundaries.  The stride of a dimension of one says nothing: 0."""
+    at, size = t.data_ptr(), t.element_size()
+    n, heads, dim = t.shape
+    if t.is_contiguous():
+        row, head = heads * dim, dim
+    else:
+        row, head, last = t.stride()
+        if last != 1 and dim != 1:
+            raise ValueError(f"{name} must have a contiguous last dimension")
+        row, head = row if n > 1 else 0, head if heads > 1 else 0
+    if at % 16 or row * size % 16 or head * size % 16:
         raise ValueError(f"{name} must have its rows on 16-byte boundaries")
-
-
-def _strides(t):
-    """(row, head) strides; 0 for a dimension of one, whose stride says nothing."""
-    return tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in (0, 1))
+    return at, row, head
 
 
 def _distinct(t, name):
     """Refuse a tensor to be written whose elements share memory."""
+    if t.is_contiguous():
+        return
     reach = 1
     for stride, size in sorted((t.stride(i), t.shape[i]) for i in range(t.ndim) if t.shape[i] > 1):
         if stride < reach:
@@ -74,32 +79,29 @@ def tensors_of(cache: KVCache):
 def cache_fields(cache: KVCache, *, write: bool = False) -> _lib.KvCache:
     """The ``dsv_kv_cache`` of a cache, checked but for its device."""
     k, v, ks, vs = cache.k, cache.v, cache.k_scale, cache.v_scale
-    if k.ndim != 3 or v.shape != k.shape or k.dtype not in _CACHE or v.dtype != k.dtype:
+    shape, dtype = k.shape, k.dtype
+    code = _CACHE.get(dtype)
+    if len(shape) != 3 or v.shape != shape or code is None or v.dtype != dtype:
         raise ValueError("a cache's k and v must be [num_slots, heads, dim] of one supported dtype")
-    if k.shape[2] % 16 or not 16 <= k.shape[2] <= 256 or k.shape[0] < 1 or k.shape[1] < 1:
+    slots, heads, dim = shape
+    if dim % 16 or not 16 <= dim <= 256 or slots < 1 or heads < 1:
         raise ValueError("a cache needs slots, heads and a dim that is a multiple of 16 up to 256")
-    for name, t in (("cache k", k), ("cache v", v)):
-        _rows(t, name)
-    quant = k.dtype in QUANTISED
-    for name, t in (("k_scale", ks), ("v_scale", vs)):
-        if (t is not None) != quant:
-            raise ValueError("scales belong to the 8-bit caches, both of them")
-        if quant and (t.shape != k.shape[:2] or t.dtype != torch.float32):
-            raise ValueError(f"{name} must be float32 [num_slots, heads]")
+    k_at, k_slot, k_head = _rows(k, "cache k")
+    v_at, v_slot, v_head = _rows(v, "cache v")
+    quant = code in (_lib.DSV_E4M3, _lib.DSV_I8)
+    if (ks is not None) != quant or (vs is not None) != quant:
+        raise ValueError("scales belong to the 8-bit caches, both of them")
+    scales = (None, None, 0, 0, 0, 0)
+    if quant:
+        for name, t in (("k_scale", ks), ("v_scale", vs)):
+            if t.shape != shape[:2] or t.dtype != torch.float32:
+                raise ValueError(f"{name} must be float32 [num_slots, heads]")
+        scales = (ks.data_ptr(), vs.data_ptr(), *ks.stride(), *vs.stride())
     if write:
         for name, t in (("cache k", k), ("cache v", v), ("k_scale", ks), ("v_scale", vs)):
             if t is not None:
                 _distinct(t, name)
-    c = _lib.KvCache()
-    c.k, c.v, c.dtype = k.data_ptr(), v.data_ptr(), _CACHE[k.dtype]
-    c.num_slots, c.heads, c.dim = k.shape
-    c.k_slot_stride, c.k_head_stride = _strides(k)
-    c.v_slot_stride, c.v_head_stride = _strides(v)
-    if quant:
-        c.k_scale, c.v_scale = ks.data_ptr(), vs.data_ptr()
-        c.ks_slot_stride, c.ks_head_stride = _strides(ks)
-        c.vs_slot_stride, c.vs_head_stride = _strides(vs)
-    return c
+    return _lib.KvCache(k_at, v_at, code, heads, dim, 0, slots, k_slot, k_head, v_slot, v_head, *scales)
 
 
 def _check_slots(slots):
@@ -124,13 +126,13 @@ def write_kv(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tens
         raise ValueError("k and v must be bfloat16 or float16 [len(slots), heads, dim]")
     if cache.k.dtype not in QUANTISED and cache.k.dtype != k.dtype:
         raise ValueError("a 16-bit cache holds its own dtype only")
-    for name, t in (("k", k), ("v", v)):
-        if shape[0]:
-            _rows(t, name)
+    if shape[0] == 0:
+        return
+    k_at, k_row, k_head = _rows(k, "k")
+    v_at, v_row, v_head = _rows(v, "v")
     dev = _lib.require_cuda(*tensors_of(cache), k, v, slots)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().dsv_kv_write(c, k.data_ptr(), v.data_ptr(), _ACT[k.dtype], shape[0], *_strides(k),
-                                            *_strides(v), slots.data_ptr(), i64, _lib.stream_of(dev)), "dsv_kv_write")
+    _lib.launch("dsv_kv_write", dev, _lib.load().dsv_kv_write, c, k_at, v_at, _ACT[k.dtype], shape[0], k_row, k_head, v_row,
+                v_head, slots.data_ptr(), i64)
 
 
 def read_kv(cache: KVCache, slots: torch.Tensor, *, dtype: torch.dtype = torch.bfloat16, out=None):
@@ -151,7 +153,6 @@ def read_kv(cache: KVCache, slots: torch.Tensor, *, dtype: torch.dtype = torch.b
         if shape[0] and t.data_ptr() % 16:
             raise ValueError("out must start on a 16-byte boundary")
     dev = _lib.require_cuda(*tensors_of(cache), k, v, slots)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().dsv_kv_read(c, k.data_ptr(), v.data_ptr(), _OUT[k.dtype], shape[0], slots.data_ptr(),
-                                           i64, _lib.stream_of(dev)), "dsv_kv_read")
+    _lib.launch("dsv_kv_read", dev, _lib.load().dsv_kv_read, c, k.data_ptr(), v.data_ptr(), _OUT[k.dtype], shape[0],
+                slots.data_ptr(), i64)
     return k, v

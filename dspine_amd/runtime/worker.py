@@ -332,14 +332,12 @@ def commit_accept(outputs, *, prefix_lens, req_pool_indices, req_to_token, out_c
     elif free_count.dtype != torch.int32 or free_count.numel() < 1:
         raise ValueError("free_count must be int32 [1]")
     if path is not None:
-        with torch.cuda.device(dev):
-            _lib.check(_lib.load().dsv_commit_tree(
-                bs, T, accept.data_ptr(), path.data_ptr(), _lib.ptr(verify_lens), prefix_lens.data_ptr(),
-                int(prefix_lens.dtype == torch.int64), req_pool_indices.data_ptr(),
-                int(req_pool_indices.dtype == torch.int64), req_to_token.data_ptr(), req_to_token.stride(0),
-                req_to_token.shape[1], _lib.ptr(out_cache_loc), _lib.ptr(slot_offsets), _lib.ptr(seq_lens),
-                int(seq_lens is not None and seq_lens.dtype == torch.int64), free_slots.data_ptr(),
-                free_count.data_ptr(), _lib.stream_of(dev)), "dsv_commit_tree")
+        _lib.launch("dsv_commit_tree", dev, _lib.load().dsv_commit_tree, bs, T, accept.data_ptr(), path.data_ptr(),
+                    _lib.ptr(verify_lens), prefix_lens.data_ptr(), int(prefix_lens.dtype == torch.int64),
+                    req_pool_indices.data_ptr(), int(req_pool_indices.dtype == torch.int64), req_to_token.data_ptr(),
+                    req_to_token.stride(0), req_to_token.shape[1], _lib.ptr(out_cache_loc), _lib.ptr(slot_offsets),
+                    _lib.ptr(seq_lens), int(seq_lens is not None and seq_lens.dtype == torch.int64),
+                    free_slots.data_ptr(), free_count.data_ptr())
         return free_slots, free_count
     _lib.check(_lib.load().dsv_commit_accept(
         bs, T, accept.data_ptr(), _lib.ptr(verify_lens), prefix_lens.data_ptr(),

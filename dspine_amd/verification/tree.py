@@ -37,9 +37,8 @@ def tree_masks(parents: torch.Tensor, masks: torch.Tensor | None = None, depths:
         if t.shape != parents.shape or t.dtype != dtype or not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous {dtype} [bs, T]")
     dev = _lib.require_cuda(parents, masks, depths)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().dsv_tree_masks(parents.data_ptr(), parents.shape[0], parents.shape[1], masks.data_ptr(),
-                                              depths.data_ptr(), _lib.stream_of(dev)), "dsv_tree_masks")
+    _lib.launch("dsv_tree_masks", dev, _lib.load().dsv_tree_masks, parents.data_ptr(), parents.shape[0],
+                parents.shape[1], masks.data_ptr(), depths.data_ptr())
     return masks, depths
 
 
@@ -92,10 +91,8 @@ def accept_greedy_tree(*, candidates: torch.Tensor, parents: torch.Tensor, next_
     lib = _lib.load()
     V = logits.shape[1]
     stride = logits.stride(0) if logits.shape[0] > 1 else V
-    wbuf = (workspace or Workspace()).get(int(lib.dsv_tree_verify_workspace_bytes(bs * T, V)), dev)
-    with torch.cuda.device(dev):
-        _lib.check(lib.dsv_tree_verify(
-            logits.data_ptr(), code, bs * T, V, stride, bs, T, candidates.data_ptr(),
-            parents.data_ptr(), _lib.ptr(verify_lens), prefix_lens.data_ptr(), *(t.data_ptr() for t in outputs),
-            path.data_ptr(), wbuf.data_ptr(), wbuf.numel(), _lib.stream_of(dev)), "dsv_tree_verify")
+    wbuf = (workspace or Workspace()).get(lib.dsv_tree_verify_workspace_bytes(bs * T, V), dev)
+    _lib.launch("dsv_tree_verify", dev, lib.dsv_tree_verify, logits.data_ptr(), code, bs * T, V, stride, bs, T,
+                candidates.data_ptr(), parents.data_ptr(), _lib.ptr(verify_lens), prefix_lens.data_ptr(),
+                *(t.data_ptr() for t in outputs), path.data_ptr(), wbuf.data_ptr(), wbuf.numel())
     return outputs, path
