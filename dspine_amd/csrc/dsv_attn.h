@@ -39,9 +39,10 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 struct AttnParams {
   dsv_tree_attention_args a;
-  int G, WR, RB;       // query heads a cache head; groups of rows a workgroup, row blocks of a request
+  FastDiv G;           // query heads a cache head
+  int WR, RB;            // groups of rows a workgroup, row blocks of a request
   int most;            // ranges at most
-  int least;           // tiles of a range at least (the last part of the batch may be less)
+  FastDiv least;       // tiles of a range at least (a batch of fewer is one range)
   uint32_t num_slots, k_step, v_step;  // slots; bytes from slot to slot
   float* part_o;       // [2 * range + (the range's last request, not its first)][head][row][dim]
   float2* part_ml;     // the same of [row]: reference, sum
@@ -67,25 +68,28 @@ __device__ __forceinline__ int tiles_of(const Request& r) {
   return r.nodes == 0 ? 0 : (t < 1 ? 1 : t);
 }
 
-// The plan, computed by every wave from the batch's lengths: range i is the tiles [total * i / ranges,
-// total * (i + 1) / ranges) of the batch.  Up to 64 requests are read once, a request a lane, and looked up among the
-// lanes; larger batches are read again where they are asked for.
+// The plan, computed by every wave from the batch's lengths: the first `more` ranges are `size` + 1 tiles, the others
+// `size`.  Up to 64 requests are read once, a request a lane, and looked up among the lanes; larger batches are read
+// again where they are asked for.
 struct Plan {
-  int64_t total;
-  int ranges;
+  int total, ranges, size, more;
   bool small;    // up to 64 requests
   Request mine;  // this lane's, of a small batch
   int tiles;     // its tiles
-  __device__ __forceinline__ int64_t start(int i) const { return total * i / ranges; }
+  __device__ __forceinline__ int start(int i) const { return i * size + (i < more ? i : more); }
   // the range that holds a tile
-  __device__ __forceinline__ int range_of(int64_t tile) const { return (int)(((tile + 1) * ranges + total - 1) / total) - 1; }
+  __device__ __forceinline__ int range_of(int tile) const {
+    const int wide = more * (size + 1);
+    return tile < wide ? (int)((uint32_t)tile / (uint32_t)(size + 1))
+                       : more + (int)((uint32_t)(tile - wide) / (uint32_t)(size < 1 ? 1 : size));
+  }
 };
 __device__ __forceinline__ Plan plan_of(const AttnParams& P, int lane) {
   Plan p;
   p.small = P.a.bs <= WAVE;
   p.tiles = 0;
   p.mine = Request{0, 0, 0};
-  int64_t sum = 0;
+  int sum = 0;
   if (p.small) {
     if (lane < P.a.bs) {
       p.mine = request_of(P.a, lane);
@@ -96,8 +100,10 @@ __device__ __forceinline__ Plan plan_of(const AttnParams& P, int lane) {
     for (int b = lane; b < P.a.bs; b += WAVE) sum += tiles_of(request_of(P.a, b));
   }
   p.total = wave_sum(sum);
-  const int64_t r = (p.total + P.least - 1) / P.least;
-  p.ranges = (int)(r < 1 ? 1 : (r > P.most ? P.most : r));
+  const int r = (int)P.least.div((uint32_t)p.total + P.least.d - 1);
+  p.ranges = r < 1 ? 1 : (r > P.most ? P.most : r);
+  p.size = (int)((uint32_t)p.total / (uint32_t)p.ranges);
+  p.more = p.total - p.size * p.ranges;
   return p;
 }
 // Request b (the same in every lane).
@@ -106,8 +112,8 @@ __device__ __forceinline__ Request request_in(const AttnParams& P, const Plan& p
   return Request{readlane_at(p.mine.nodes, b), readlane_at(p.mine.prefix, b), readlane_at(p.mine.total, b)};
 }
 // Tiles of the requests before b.
-__device__ __forceinline__ int64_t tiles_before(const AttnParams& P, const Plan& p, int b, int lane) {
-  int64_t sum = 0;
+__device__ __forceinline__ int tiles_before(const AttnParams& P, const Plan& p, int b, int lane) {
+  int sum = 0;
   if (p.small)
     sum = lane < b ? p.tiles : 0;
   else
@@ -115,12 +121,12 @@ __device__ __forceinline__ int64_t tiles_before(const AttnParams& P, const Plan&
   return wave_sum(sum);
 }
 // The request of a tile (tile < total) and the tiles before it.
-__device__ __forceinline__ int request_at(const AttnParams& P, const Plan& p, int64_t tile, int lane, int64_t& before) {
+__device__ __forceinline__ int request_at(const AttnParams& P, const Plan& p, int tile, int lane, int& before) {
   before = 0;
   for (int b0 = 0;; b0 += WAVE) {
     const int i = b0 + lane;
     const int n = p.small ? p.tiles : (i < P.a.bs ? tiles_of(request_of(P.a, i)) : 0);
-    const int64_t end = before + wave_incl_scan((int64_t)n);
+    const int end = before + wave_incl_scan(n);
     const uint64_t past = __ballot(end > tile);
     if (past) {
       const int l = __ffsll((unsigned long long)past) - 1;
@@ -272,6 +278,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
   constexpr size_t SUMS = sizeof(float) * WAVES * 16 * OS, TILES = STAGED ? sizeof(uint4) * 2 * FRAGS * WAVE : 0;
   __shared__ __attribute__((aligned(16))) unsigned char s_mem[SUMS > TILES ? SUMS : TILES];
   __shared__ float s_m[WAVES][16 * R], s_l[WAVES][16 * R];
+  __shared__ uint64_t s_mask[WAVES][16 * R];  // of the wave's rows
   __shared__ int s_odd;
   float(*const s_o)[16][OS] = reinterpret_cast<float(*)[16][OS]>(s_mem);
 
@@ -287,14 +294,14 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
   if (range >= plan.ranges || plan.total == 0) return;
   const int wr = wave / WK, wk = wave - wr * WK;
   const int block0 = rb * 16 * R * P.WR, row0 = block0 + wr * 16 * R;
-  int64_t tile = plan.start(range), before;
-  const int64_t stop = plan.start(range + 1);
+  int tile = plan.start(range), before;
+  const int stop = plan.start(range + 1);
   int b = __builtin_amdgcn_readfirstlane(request_at(P, plan, tile, lane, before));
   // the range's requests, one after the other
   for (bool first = true; tile < stop; first = false) {
   const Request req = request_in(P, plan, b);
-  const int n_rows = req.nodes * P.G, tiles = tiles_of(req);
-  const int t0 = (int)(tile - before), t1 = (int)(stop - before < tiles ? stop - before : tiles);
+  const int n_rows = req.nodes * (int)P.G.d, tiles = tiles_of(req);
+  const int t0 = tile - before, t1 = stop - before < tiles ? stop - before : tiles;
   const int request = b;
   before += tiles;
   tile += t1 - t0;
@@ -310,10 +317,9 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
   auto load_queries = [&]() {
 #pragma unroll
     for (int rt = 0; rt < R; ++rt) {
-      const int r = row0 + rt * 16 + m;
-      const int64_t row = r < n_rows ? row_of(a, request, r / P.G) : -1;
-      const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (row < 0 ? 0 : row) * a.q_row_stride +
-                          (int64_t)(h * P.G + r % P.G) * a.q_head_stride;
+      const int r = row0 + rt * 16 + m, node = (int)P.G.div((uint32_t)r), head = h * (int)P.G.d + r - node * (int)P.G.d;
+      const int64_t row = r < n_rows ? row_of(a, request, node) : -1;
+      const uint16_t* q = reinterpret_cast<const uint16_t*>(a.q) + (row < 0 ? 0 : row * a.q_row_stride + head * a.q_head_stride);
 #pragma unroll
       for (int kk = 0; kk < NK; ++kk) {
         const int d = QUANT ? (kk / 2) * 64 + g * 16 + (kk & 1) * 8 : kk * 32 + g * 8;
@@ -322,6 +328,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) qf[rt][kk][i] = w[i];
       }
+      if (g == 0) s_mask[wave][rt * 16 + m] = r < n_rows ? mask_of(a, request, node) : 0ull;
     }
 #pragma unroll
     for (int rt = 0; rt < R; ++rt)
@@ -343,7 +350,9 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
 
   f32x4 o[R][EPL];
   float mref[R], l[R];
-  float vref = 0.f, vinv = 0.f;
+  // The largest value scale so far is held as a power of two 2^vlog; weights are 2^vlog smaller than they would be, by the
+  // rows' references, so that with their scales they stay within float16.
+  float vlog = -60.f, vtop = 8.673617379884035e-19f;  // (2^-60)
   bool fresh = true;  // some row has no reference yet
 #pragma unroll
   for (int rt = 0; rt < R; ++rt) {
@@ -431,55 +440,45 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       }
     if (odd) s_odd = 1;
   };
-  // The positions' factors of a score (base 2) and of a weight.  Value scales are taken relative to a power of two at or
-  // above the largest so far.
-  auto factors = [&](const auto& kf, const auto& vf, auto& cs, auto& vn) {
+  // v: magnitudes of value scales, over the lanes.
+  auto meet_scales = [&](float v) {
     if constexpr (QUANT) {
-      constexpr int N = sizeof(kf) / sizeof(kf[0]);
-      float top = 0.f;
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        cs[j] = kf[j] * c0;
-        const float v = fabsf(vf[j]);
-        top = fmaxf(top, v < INFINITY ? v : 0.f);
-      }
-      if (__any(top > vref)) {
-        top = wave_max_f32(top);
+      if (__any(v > vtop)) {
+        const float top = wave_max_f32(v < INFINITY ? v : 0.f);
         int ex;
         (void)frexpf(top, &ex);
-        ex = ex > 120 ? 120 : (ex < -120 ? -120 : ex);
-        const float up = ldexpf(1.f, ex);
-        if (up > vref) {
-          const float keep = vref / up;
+        const float up = (float)ex;
+        if (top > vtop && up > vlog) {
+          const float keep = __builtin_amdgcn_exp2f(vlog - up);
 #pragma unroll
-          for (int rt = 0; rt < R; ++rt)
+          for (int rt = 0; rt < R; ++rt) {
+            if (mref[rt] != AT_LOW) mref[rt] += up - vlog;
+            l[rt] *= keep;
 #pragma unroll
             for (int e = 0; e < EPL; ++e) o[rt][e] *= keep;
-          vref = up;
-          vinv = 1.f / up;
+          }
+          vlog = up;
+          vtop = __builtin_amdgcn_exp2f(up);
         }
       }
-#pragma unroll
-      for (int j = 0; j < N; ++j) vn[j] = vf[j] * vinv;
     }
   };
-  // A step, or n at once: scores of 32 n positions' keys, weights, weighted values.  WHOLE: every row sees every position
-  // that holds anything (bit j of `here`: this lane's position j does).  `next` runs when the keys have been used, `after` when the
+  // A step: scores of 32 positions' keys, weights, weighted values.  WHOLE: every row sees every position that holds
+  // anything (`full`: all do; bit j of here_(): this lane's position j does).  cs: the positions' factors of a score
+  // (base 2), vs: their value scales.  `next` runs when the keys have been used, `after` when the
   // values' operand e has.
-  auto step = [&](auto whole_, auto n_, int base, uint32_t here, const auto& cs, const auto& vn, auto key, auto value,
+  auto step = [&](auto whole_, int base, bool full, auto here_, const auto& cs, const auto& vs, auto key, auto value,
                   auto next, auto after) {
     constexpr bool WHOLE = decltype(whole_)::value;
-    constexpr int N = decltype(n_)::value, POS = 8 * N;  // positions a lane
-    constexpr uint32_t ALL = (1u << POS) - 1u;
-    f32x4 s[R][2 * N];
+    f32x4 s[R][2];
 #pragma unroll
     for (int rt = 0; rt < R; ++rt)
 #pragma unroll
-      for (int i = 0; i < 2 * N; ++i) s[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < 2; ++i) s[rt][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int kk = 0; kk < NK; ++kk)
 #pragma unroll
-      for (int i = 0; i < 2 * N; ++i) {
+      for (int i = 0; i < 2; ++i) {
         uint32_t ko[4];
         key(i, kk, ko);
 #pragma unroll
@@ -488,13 +487,13 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
     next();
     uint32_t seen[R];  // bit j: the row sees this lane's position j
     if constexpr (!WHOLE) {
+      const uint32_t here = here_();
 #pragma unroll
       for (int rt = 0; rt < R; ++rt) {
-        const int r = row0 + rt * 16 + m;
-        const uint64_t mask = r < n_rows ? mask_of(a, request, r / P.G) : 0ull;
+        const uint64_t mask = s_mask[wave][rt * 16 + m];
         uint32_t bits = 0;
 #pragma unroll
-        for (int j = 0; j < POS; ++j) {
+        for (int j = 0; j < 8; ++j) {
           const int p = base + (j / 4) * 16 + g * 4 + (j & 3) - req.prefix;
           const bool sees = p < 0 || (p < 64 && ((mask >> (p & 63)) & 1));
           bits |= (sees ? 1u : 0u) << j;
@@ -508,34 +507,35 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
     for (int rt = 0; rt < R; ++rt) {
       const float ref = mref[rt] == AT_LOW ? 0.f : mref[rt];
 #pragma unroll
-      for (int j = 0; j < POS; ++j) {
+      for (int j = 0; j < 8; ++j) {
         float x = fmaf(s[rt][j / 4][j & 3], QUANT ? cs[j] : c0, -ref);
         if (!WHOLE && !((seen[rt] >> j) & 1)) x = -INFINITY;
         s[rt][j / 4][j & 3] = x;
         over = fmaxf(over, x);
       }
     }
-    if (WHOLE && __any(here != ALL)) {
+    if (WHOLE && !full) {
       asm volatile("");  // (a branch: the selects are for bad slots only)
+      const uint32_t here = here_();
       over = AT_LOW;
 #pragma unroll
       for (int rt = 0; rt < R; ++rt)
 #pragma unroll
-        for (int j = 0; j < POS; ++j) {
+        for (int j = 0; j < 8; ++j) {
           if (!((here >> j) & 1)) s[rt][j / 4][j & 3] = -INFINITY;
           over = fmaxf(over, s[rt][j / 4][j & 3]);
         }
     }
-    if (fresh || __any(over > SHIFT + LIM)) {
+    if (fresh || __any(over > SHIFT + LIM - (QUANT ? vlog : 0.f))) {
       bool none = false;
 #pragma unroll
       for (int rt = 0; rt < R; ++rt) {
         float top = AT_LOW;
 #pragma unroll
-        for (int j = 0; j < POS; ++j) top = fmaxf(top, s[rt][j / 4][j & 3]);
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, s[rt][j / 4][j & 3]);
         top = across_groups_max(top);
         const bool unset = mref[rt] == AT_LOW;
-        float move = top - SHIFT;  // of the reference: up, or anywhere from none
+        float move = top - SHIFT + (QUANT ? vlog : 0.f);  // of the reference: up, or anywhere from none
         if (top == AT_LOW || (!unset && move < 0.f)) move = 0.f;
         if (top != AT_LOW || !unset) mref[rt] = (unset ? 0.f : mref[rt]) + move;
         none |= mref[rt] == AT_LOW;
@@ -544,38 +544,36 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
 #pragma unroll
         for (int e = 0; e < EPL; ++e) o[rt][e] *= keep;
 #pragma unroll
-        for (int j = 0; j < POS; ++j) s[rt][j / 4][j & 3] -= move;
+        for (int j = 0; j < 8; ++j) s[rt][j / 4][j & 3] -= move;
       }
       fresh = __any(none);
     }
-    uint32_t pf[R][N][4];
+    uint32_t pf[R][4];
 #pragma unroll
     for (int rt = 0; rt < R; ++rt) {
 #pragma unroll
-      for (int j = 0; j < POS; j += 2) {
+      for (int j = 0; j < 8; j += 2) {
         float w[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           w[u] = __builtin_amdgcn_exp2f(s[rt][j / 4][(j + u) & 3]);
           l[rt] += w[u];
           if constexpr (QUANT) {
-            w[u] *= vn[j + u];
+            w[u] *= vs[j + u];
             if (!WHOLE && !((seen[rt] >> (j + u)) & 1)) w[u] = 0.f;
           }
         }
-        pf[rt][j / 8][j % 8 / 2] = pack_act<PT>(w[0], w[1]);
+        pf[rt][j / 2] = pack_act<PT>(w[0], w[1]);
       }
     }
 #pragma unroll
-    for (int n = 0; n < N; ++n)
+    for (int e = 0; e < EPL; ++e) {
+      uint32_t vo[4];
+      value(e, vo);
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) {
-        uint32_t vo[4];
-        value(n, e, vo);
-#pragma unroll
-        for (int rt = 0; rt < R; ++rt) o[rt][e] = mfma<PT>(vo, pf[rt][n], o[rt][e]);
-        after(e);
-      }
+      for (int rt = 0; rt < R; ++rt) o[rt][e] = mfma<PT>(vo, pf[rt], o[rt][e]);
+      after(e);
+    }
   };
 
   if constexpr (!STAGED) {
@@ -592,7 +590,8 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
     };
     auto spread_scales = [&](float scale, float (&kf)[8], float (&vf)[8]) {
       if constexpr (QUANT) {
-        s_scale[wave][g >> 1][(g & 1) * 16 + m] = scale;
+        meet_scales(g < 2 ? 0.f : fabsf(scale));
+        s_scale[wave][g >> 1][(g & 1) * 16 + m] = g < 2 ? scale * c0 : scale;
         __builtin_amdgcn_wave_barrier();  // (the wave's own memory, in order)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -639,19 +638,19 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       // (the slots of the step after the next are asked for before the next one's data: a wait for them, loads being
       // counted in order, is none for that data)
       auto go = [&](uint32_t (&wv)[8][VW], uint32_t here, uint32_t (&then)[8][VW], uint32_t& then_here, uint32_t (&ks)[2],
-                    uint32_t (&vs)[8], uint32_t (&then_ks)[2], uint32_t (&then_vs)[8]) {
-        float kf[8], vf[8], cs[8], vn[8];
-        spread_scales(scale, kf, vf);
-        factors(kf, vf, cs, vn);
-        step(Int<1>{}, Int<1>{}, t * AT_STEP, here, cs, vn,
+                    uint32_t (&slot)[8], uint32_t (&then_ks)[2], uint32_t (&then_slot)[8]) {
+        float cs[8], vs[8];
+        spread_scales(scale, cs, vs);
+        const bool full = !__any(here != 0xffu);
+        step(Int<1>{}, t * AT_STEP, full, [&]() { return here; }, cs, vs,
              [&](int i, int kk, uint32_t (&ko)[4]) { key_frag(kw[i], kk, ko); },
-             [&](int, int e, uint32_t (&vo)[4]) { value_operand<CT>(wv, e, vo); },
+             [&](int e, uint32_t (&vo)[4]) { value_operand<CT>(wv, e, vo); },
              [&]() {
-               slots(t + 2 * WK < whole ? t + 2 * WK : t, then_ks, then_vs);
+               slots(t + 2 * WK < whole ? t + 2 * WK : t, then_ks, then_slot);
                __builtin_amdgcn_sched_barrier(0);
-               load(ks, vs, then, then_here);
+               load(ks, slot, then, then_here);
                __builtin_amdgcn_sched_barrier(0);
-               if (__any(here != 0xffu)) clear_values(here, false, wv);
+               if (!full) clear_values(here, false, wv);
              },
              [](int) {});
         t += WK;
@@ -668,22 +667,21 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
     }
     // The window's.
     for (; t < end; t += WK) {
-      uint32_t ks[2], vs[8], kw[2][KL][4], wv[8][VW];
-      float kf[8], vf[8], cs[8], vn[8];
+      uint32_t ks[2], slot[8], kw[2][KL][4], wv[8][VW];
+      float cs[8], vs[8];
       const int base = t * AT_STEP;
       key_slots(base, ks[0], ks[1]);
-      value_slots(Int<0>{}, base, vs);
+      value_slots(Int<0>{}, base, slot);
       load_key(ks[0], kw[0]);
       load_key(ks[1], kw[1]);
-      spread_scales(load_scale(ks[0], ks[1]), kf, vf);
+      spread_scales(load_scale(ks[0], ks[1]), cs, vs);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) load_value(vs[j], wv[j]);
-      const uint32_t here = holds(vs);
+      for (int j = 0; j < 8; ++j) load_value(slot[j], wv[j]);
+      const uint32_t here = holds(slot);
       clear_values(here, true, wv);
-      factors(kf, vf, cs, vn);
-      step(Int<0>{}, Int<1>{}, base, here, cs, vn,
+      step(Int<0>{}, base, false, [&]() { return here; }, cs, vs,
            [&](int i, int kk, uint32_t (&ko)[4]) { key_frag(kw[i], kk, ko); },
-           [&](int, int e, uint32_t (&vo)[4]) { value_operand<CT>(wv, e, vo); }, [] {}, [](int) {});
+           [&](int e, uint32_t (&vo)[4]) { value_operand<CT>(wv, e, vo); }, [] {}, [](int) {});
     }
   } else {
     uint4(*const s_frag)[FRAGS][WAVE] = reinterpret_cast<uint4(*)[FRAGS][WAVE]>(s_mem);
@@ -742,7 +740,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
         reinterpret_cast<uint2*>(to[4 * NK + (wave / 2) * EPL + e])[(wave & 1) * WAVE + lane] = make_uint2(vo[0], vo[1]);
       }
       if constexpr (QUANT)
-        if (g < 2) s_scale[buf][g][wave * 16 + m] = f.scale;
+        if (g < 2) s_scale[buf][g][wave * 16 + m] = g == 0 ? f.scale * c0 : f.scale;
       if (lane == 0) s_here[buf][wave] = f.have;
     };
     int buf = 0;
@@ -794,29 +792,27 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       if (works) {
         auto one = [&](int blk, auto more_) {
           constexpr bool more = decltype(more_)::value;
-          float cs[8], vn[8];
+          float cs[8], vs[8];
           if constexpr (QUANT) {
-            float kf[8], vf[8];
+            meet_scales(fabsf(s_scale[buf][1][blk * AT_STEP + (lane & 31)]));
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const float4 k4 = *reinterpret_cast<const float4*>(&s_scale[buf][0][blk * AT_STEP + i * 16 + g * 4]);
               const float4 v4 = *reinterpret_cast<const float4*>(&s_scale[buf][1][blk * AT_STEP + i * 16 + g * 4]);
-              kf[4 * i] = k4.x, kf[4 * i + 1] = k4.y, kf[4 * i + 2] = k4.z, kf[4 * i + 3] = k4.w;
-              vf[4 * i] = v4.x, vf[4 * i + 1] = v4.y, vf[4 * i + 2] = v4.z, vf[4 * i + 3] = v4.w;
+              cs[4 * i] = k4.x, cs[4 * i + 1] = k4.y, cs[4 * i + 2] = k4.z, cs[4 * i + 3] = k4.w;
+              vs[4 * i] = v4.x, vs[4 * i + 1] = v4.y, vs[4 * i + 2] = v4.z, vs[4 * i + 3] = v4.w;
             }
-            factors(kf, vf, cs, vn);
           }
-          uint32_t here = 0;
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            here |= ((__builtin_amdgcn_readfirstlane(s_here[buf][2 * blk + i]) >> (g * 4)) & 0xfu) << (4 * i);
-          step(whole_, Int<1>{}, t * AT_TILE + blk * AT_STEP, here, cs, vn,
+          const uint32_t h0 = __builtin_amdgcn_readfirstlane(s_here[buf][2 * blk]);
+          const uint32_t h1 = __builtin_amdgcn_readfirstlane(s_here[buf][2 * blk + 1]);
+          step(whole_, t * AT_TILE + blk * AT_STEP, (h0 & h1) == 0xffffu,
+               [&]() { return ((h0 >> (g * 4)) & 0xfu) | (((h1 >> (g * 4)) & 0xfu) << 4); }, cs, vs,
                [&](int i, int kk, uint32_t (&ko)[4]) {
                  if constexpr (!AHEAD) read_key(blk, i * NK + kk);
                  const uint4 v = fr[i * NK + kk];
                  ko[0] = v.x, ko[1] = v.y, ko[2] = v.z, ko[3] = v.w;
                },
-               [&](int, int e, uint32_t (&vo)[4]) {
+               [&](int e, uint32_t (&vo)[4]) {
                  if constexpr (!AHEAD) read_value(blk, e);
                  const uint4 v = fr[e];
                  vo[0] = v.x, vo[1] = v.y, vo[2] = v.z, vo[3] = v.w;
@@ -869,7 +865,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
     }
   }
   __syncthreads();
-  const float unit = QUANT ? vref * (CT == DSV_I8 ? I8_UNIT : 1.f) : 1.f;
+  constexpr float unit = CT == DSV_I8 ? I8_UNIT : 1.f;
   // the positions whose values were set aside where they are not finite
   const int aside0 = clear / SET_ASIDE * SET_ASIDE > t0 * AT_TILE ? clear / SET_ASIDE * SET_ASIDE : t0 * AT_TILE;
   const int aside1 = t1 * AT_TILE < req.total ? t1 * AT_TILE : req.total;
@@ -897,7 +893,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
 #pragma unroll
         for (int u = 0; u < 8; ++u) sum[u] += s_o[wr * WK + k][rr][d + u];
       }
-      const int node = r / P.G, qh = h * P.G + r - node * P.G;
+      const int node = (int)P.G.div((uint32_t)r), qh = h * (int)P.G.d + r - node * (int)P.G.d;
       if (CT != DSV_I8 && s_odd) {
         const uint64_t mask = mask_of(a, request, node);
         for (int p = aside0; p < aside1; ++p) {
@@ -913,7 +909,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       }
       if (t1 - t0 < tiles) {
         // (its first part is its range's last request's, unless it begins the range; the others begin theirs)
-        const int64_t at = ((int64_t)(2 * range + (first ? 0 : 1)) * c.heads + h) * (a.T * P.G) + r;
+        const int64_t at = ((int64_t)(2 * range + (first ? 0 : 1)) * c.heads + h) * (a.T * (int)P.G.d) + r;
         float* po = P.part_o + at * dim + d;
         *reinterpret_cast<float4*>(po) = make_float4(sum[0], sum[1], sum[2], sum[3]);
         *reinterpret_cast<float4*>(po + 4) = make_float4(sum[4], sum[5], sum[6], sum[7]);

@@ -21,17 +21,17 @@ __global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
   const dsv_kv_cache& c = a.cache;
   constexpr int PER = DP / 8, ROWS = AJ_THREADS / PER;
   const int lane = threadIdx.x & (WAVE - 1);
-  const int rows = a.T * P.G, blocks = (rows + ROWS - 1) / ROWS;
+  const int rows = a.T * (int)P.G.d, blocks = (rows + ROWS - 1) / ROWS;
   const int b = (int)(blockIdx.x / (c.heads * blocks)), in = (int)(blockIdx.x - (int64_t)b * c.heads * blocks);
   const int h = in / blocks, r = (in - h * blocks) * ROWS + (int)threadIdx.x / PER, d = (int)threadIdx.x % PER * 8;
   const Plan plan = plan_of(P, lane);
   const Request req = request_in(P, plan, b);
   const int tiles = tiles_of(req);
-  if ((in - h * blocks) * ROWS >= req.nodes * P.G) return;
-  const int64_t before = tiles_before(P, plan, b, lane);
+  if ((in - h * blocks) * ROWS >= req.nodes * (int)P.G.d) return;
+  const int before = tiles_before(P, plan, b, lane);
   const int i0 = plan.range_of(before), i1 = plan.range_of(before + tiles - 1);
-  if (i0 == i1 || r >= req.nodes * P.G || d >= c.dim) return;
-  const int node = r / P.G, qh = h * P.G + r - node * P.G;
+  if (i0 == i1 || r >= req.nodes * (int)P.G.d || d >= c.dim) return;
+  const int node = (int)P.G.div((uint32_t)r), qh = h * (int)P.G.d + r - node * (int)P.G.d;
   const int64_t row = row_of(a, b, node);
   if (row < 0) return;
   // the request's part of range i: the last of its range where that begins before it
@@ -132,17 +132,19 @@ extern "C" int dsv_tree_attention(const dsv_tree_attention_args* args, dsv_strea
     DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: slots are too far apart");
   AttnParams P;
   P.a = a;
-  P.G = a.q_heads / a.cache.heads;
-  const AttnShape s = attn_shape(a.T, P.G, a.cache.dim);
+  const int G = a.q_heads / a.cache.heads;
+  P.G = fast_div((uint32_t)G);
+  const AttnShape s = attn_shape(a.T, G, a.cache.dim);
   P.WR = s.WR;
   P.RB = s.RB;
   P.most = attn_ranges(s, a.cache.heads, a.cache.dim);
-  P.least = s.form == AT_ROWS ? 4 : 2;
+  P.least = fast_div(s.form == AT_ROWS ? 4 : 2);
   const int64_t blocks = (P.most + 7) / 8 * 8 * (int64_t)a.cache.heads * s.RB;
   const int64_t wide = a.cache.dim <= 64 ? 64 : (a.cache.dim <= 128 ? 128 : 256), per = AJ_THREADS / (wide / 8);
-  const int64_t joins = (a.T * (int64_t)P.G + per - 1) / per * a.cache.heads * a.bs;
-  if (blocks > 0x7fffffffll || joins > 0x7fffffffll)
-    DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: too many nodes for one call");
+  const int64_t joins = (a.T * (int64_t)G + per - 1) / per * a.cache.heads * a.bs;
+  const int64_t tiles = ((a.page_cols + AT_TILE - 1) / AT_TILE + 1) * a.bs;  // at most
+  if (blocks > 0x7fffffffll || joins > 0x7fffffffll || tiles > 0x7fffff00ll)
+    DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: too many nodes or positions for one call");
   const int64_t need = dsv_tree_attention_workspace_bytes(a.bs, a.T, a.cache.heads, a.q_heads, a.cache.dim);
   if (!a.workspace || (uintptr_t)a.workspace % 16)
     DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: a 16-byte-aligned workspace is required");

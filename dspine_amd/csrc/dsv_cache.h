@@ -20,6 +20,21 @@ __device__ __forceinline__ int64_t load_index(const void* p, int i64, int64_t i)
   return i64 ? reinterpret_cast<const int64_t*>(p)[i] : (int64_t) reinterpret_cast<const int32_t*>(p)[i];
 }
 
+// r / d for r < 2^31.
+struct FastDiv {
+  uint32_t d, mul, shift;
+  __device__ __forceinline__ uint32_t div(uint32_t r) const { return (uint32_t)(((uint64_t)r * mul) >> shift); }
+};
+inline FastDiv fast_div(uint32_t d) {
+  FastDiv f;
+  int log = 0;
+  while ((1ull << log) < d) ++log;
+  f.d = d;
+  f.shift = 31 + log;
+  f.mul = (uint32_t)(((1ull << f.shift) + d - 1) / d);
+  return f;
+}
+
 // 16 bits of an activation as float32.
 template <int XT>
 __device__ __forceinline__ float act_to_f32(uint32_t bits) {

@@ -12,21 +12,6 @@ namespace dsv {
 constexpr int KV_THREADS = 256;
 constexpr int KV_ROWS = 2;
 
-// r / d for r < 2^31.
-struct FastDiv {
-  uint32_t d, mul, shift;
-  __device__ __forceinline__ uint32_t div(uint32_t r) const { return (uint32_t)(((uint64_t)r * mul) >> shift); }
-};
-static FastDiv fast_div(uint32_t d) {
-  FastDiv f;
-  int log = 0;
-  while ((1ull << log) < d) ++log;
-  f.d = d;
-  f.shift = 31 + log;
-  f.mul = (uint32_t)(((1ull << f.shift) + d - 1) / d);
-  return f;
-}
-
 // Keys or values: the cache's tensor, its scales, and the activations (read by the write, written by the read).
 struct KvSide {
   void* base;
