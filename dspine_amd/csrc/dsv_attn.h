@@ -40,7 +40,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 struct AttnParams {
   dsv_tree_attention_args a;
   FastDiv G;           // query heads a cache head
-  int WR, RB;            // groups of rows a workgroup, row blocks of a request
+  int WR, RB;          // groups of rows a workgroup, row blocks of a request
   int most;            // ranges at most
   FastDiv least;       // tiles of a range at least (a batch of fewer is one range)
   uint32_t num_slots, k_step, v_step;  // slots; bytes from slot to slot
@@ -120,10 +120,10 @@ __device__ __forceinline__ int tiles_before(const AttnParams& P, const Plan& p, 
     for (int i = lane; i < b; i += WAVE) sum += tiles_of(request_of(P.a, i));
   return wave_sum(sum);
 }
-// The request of a tile (tile < total) and the tiles before it.
+// The request of a tile (tile < total) and the tiles before it; -1 if there is none (lengths that change under the call).
 __device__ __forceinline__ int request_at(const AttnParams& P, const Plan& p, int tile, int lane, int& before) {
   before = 0;
-  for (int b0 = 0;; b0 += WAVE) {
+  for (int b0 = 0; b0 < P.a.bs; b0 += WAVE) {
     const int i = b0 + lane;
     const int n = p.small ? p.tiles : (i < P.a.bs ? tiles_of(request_of(P.a, i)) : 0);
     const int end = before + wave_incl_scan(n);
@@ -135,6 +135,7 @@ __device__ __forceinline__ int request_at(const AttnParams& P, const Plan& p, in
     }
     before = readlane<WAVE - 1>(end);
   }
+  return -1;
 }
 
 template <int XT>
@@ -298,7 +299,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
   const int stop = plan.start(range + 1);
   int b = __builtin_amdgcn_readfirstlane(request_at(P, plan, tile, lane, before));
   // the range's requests, one after the other
-  for (bool first = true; tile < stop; first = false) {
+  for (bool first = true; tile < stop && b >= 0 && b < a.bs; first = false) {
   const Request req = request_in(P, plan, b);
   const int n_rows = req.nodes * (int)P.G.d, tiles = tiles_of(req);
   const int t0 = tile - before, t1 = stop - before < tiles ? stop - before : tiles;
