@@ -255,6 +255,9 @@ __device__ __forceinline__ uint64_t mask_of(const dsv_tree_attention_args& a, in
 
 // FORM: direct, or staged with a wave (AT_ROWS) or two (AT_PAIRS) for a group of rows.
 enum { AT_DIRECT = 0, AT_PAIRS = 1, AT_ROWS = 2 };
+// Tiles a turn: two row tiles a wave leave one workgroup of eight waves a CU, and LDS for four staged tiles: its first four
+// waves bring one tile and the others the next, so that all do the same work between two barriers.
+constexpr int AT_TILES(int FORM, int R) { return FORM == 2 && R == 2 ? 2 : 1; }
 constexpr int AT_DEPTH(int R, int DP) { return R == 1 && DP <= 128 ? 2 : 1; }
 
 template <int XT, int CT, int DP, bool FULL, int R, int FORM, int WAVES, int OCC>
@@ -276,7 +279,8 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
   constexpr int SET_ASIDE = STAGED ? AT_TILE : AT_STEP;
   constexpr int FRAGS = 4 * NK + 2 * EPL;  // operands of a staged tile: keys, then values, 16 bytes a lane each (values as
                                            // two halves of 8, so that their writes find all banks)
-  constexpr size_t SUMS = sizeof(float) * WAVES * 16 * OS, TILES = STAGED ? sizeof(uint4) * 2 * FRAGS * WAVE : 0;
+  constexpr int NT = AT_TILES(FORM, R);
+  constexpr size_t SUMS = sizeof(float) * WAVES * 16 * OS, TILES = STAGED ? sizeof(uint4) * 2 * NT * FRAGS * WAVE : 0;
   __shared__ __attribute__((aligned(16))) unsigned char s_mem[SUMS > TILES ? SUMS : TILES];
   __shared__ float s_m[WAVES][16 * R], s_l[WAVES][16 * R];
   __shared__ uint64_t s_mask[WAVES][16 * R];  // of the wave's rows
@@ -686,8 +690,8 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
     }
   } else {
     uint4(*const s_frag)[FRAGS][WAVE] = reinterpret_cast<uint4(*)[FRAGS][WAVE]>(s_mem);
-    __shared__ float s_scale[2][2][AT_TILE];
-    __shared__ uint32_t s_here[2][AT_WAVES];
+    __shared__ float s_scale[2 * NT][2][AT_TILE];
+    __shared__ uint32_t s_here[2 * NT][AT_WAVES];
     // Each of the first waves brings 16 positions: lane (m, g) pieces of the key of position m, and of the values of
     // g * 4 .. g * 4 + 3.  The loads run DEPTH tiles ahead of the one that is put away (in two sets of registers where
     // there are that many).
@@ -699,9 +703,11 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       float scale;
     };
     Brought sets[DEPTH];
+    const bool brings = wave < AT_WAVES * NT;
+    const int piece = wave % AT_WAVES, ahead = NT > 1 ? wave / AT_WAVES : 0;  // what of a turn's which tile
     auto fetch_slots = [&](Brought& f, int t) {
       if (t >= t1) return;
-      const int base = t * AT_TILE + wave * 16;
+      const int base = t * AT_TILE + piece * 16;
       if (base + 16 <= req.total) {
         f.kslot = (uint32_t)table[base + m];
         uint4 v;
@@ -724,56 +730,57 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
         if (!good(f.kslot)) f.scale = 0.f;
       }
     };
-    auto put = [&](Brought& f, int t, int buf) {
-      uint4(*const to)[WAVE] = s_frag[buf];
+    auto put = [&](Brought& f, int t, int to_buf) {
+      const int at = to_buf * NT + ahead;
+      uint4(*const to)[WAVE] = s_frag[at];
       const bool aside = t * AT_TILE + SET_ASIDE > clear;
       if (aside || f.have != 0xffffu) clear_values(f.have >> (g * 4), aside, f.wv);
 #pragma unroll
       for (int kk = 0; kk < NK; ++kk) {
         uint32_t ko[4];
         key_frag(f.kw, kk, ko);
-        to[wave * NK + kk][lane] = make_uint4(ko[0], ko[1], ko[2], ko[3]);
+        to[piece * NK + kk][lane] = make_uint4(ko[0], ko[1], ko[2], ko[3]);
       }
 #pragma unroll
       for (int e = 0; e < EPL; ++e) {
         uint32_t vo[2];
         value_operand<CT>(f.wv, e, vo);
-        reinterpret_cast<uint2*>(to[4 * NK + (wave / 2) * EPL + e])[(wave & 1) * WAVE + lane] = make_uint2(vo[0], vo[1]);
+        reinterpret_cast<uint2*>(to[4 * NK + (piece / 2) * EPL + e])[(piece & 1) * WAVE + lane] = make_uint2(vo[0], vo[1]);
       }
       if constexpr (QUANT)
-        if (g < 2) s_scale[buf][g][wave * 16 + m] = g == 0 ? f.scale * c0 : f.scale;
-      if (lane == 0) s_here[buf][wave] = f.have;
+        if (g < 2) s_scale[at][g][piece * 16 + m] = g == 0 ? f.scale * c0 : f.scale;
+      if (lane == 0) s_here[at][piece] = f.have;
     };
     int buf = 0;
-    const bool brings = wave < AT_WAVES;
     // the loads of tile t and the slots of the set's next one
     auto ask = [&](Brought& f, int t) {
       if (t < t1) {
         fetch(f);
-        fetch_slots(f, t + DEPTH);
+        fetch_slots(f, t + NT * DEPTH);
       }
     };
     if (brings) {
-      fetch_slots(sets[0], t0);
+      fetch_slots(sets[0], t0 + ahead);
       if constexpr (DEPTH > 1) fetch_slots(sets[1], t0 + 1);
-      ask(sets[0], t0);
+      ask(sets[0], t0 + ahead);
       if constexpr (DEPTH > 1) ask(sets[1], t0 + 1);
     }
     load_queries();
-    if (brings) {
-      put(sets[0], t0, 0);
-      ask(sets[0], t0 + DEPTH);
+    if (brings && t0 + ahead < t1) {
+      put(sets[0], t0 + ahead, 0);
+      ask(sets[0], t0 + ahead + NT * DEPTH);
     }
-    // A turn: the next tile into the other buffer, the loads of the one after it, the products of this one.  A step's keys
+    static_assert(NT == 1 || DEPTH == 1, "one set a wave");
+    // A turn: the next tile (or two) into the other buffer, the loads of the one after it, the products of this one.  A step's keys
     // are read from LDS while the step before it multiplies (the first step's while the next tile is put away), its values
     // while its weights are computed, into the same registers: read where they are used, the reads' latencies were most
     // of a turn.
     constexpr bool AHEAD = R == 1 && DP <= 128;  // (with more rows the registers are not there, nor are the reads most of a step)
     uint4 fr[EPL];
     static_assert(2 * NK == EPL, "a step has as many key operands as value operands");
-    auto read_key = [&](int blk, int n) { fr[n] = s_frag[buf][blk * 2 * NK + n][lane]; };
-    auto read_value = [&](int blk, int e) {
-      const uint2* v = reinterpret_cast<const uint2*>(s_frag[buf][4 * NK + blk * EPL + e]);
+    auto read_key = [&](int cur, int blk, int n) { fr[n] = s_frag[cur][blk * 2 * NK + n][lane]; };
+    auto read_value = [&](int cur, int blk, int e) {
+      const uint2* v = reinterpret_cast<const uint2*>(s_frag[cur][4 * NK + blk * EPL + e]);
       const uint2 lo = v[lane], hi = v[WAVE + lane];
       fr[e] = make_uint4(lo.x, lo.y, hi.x, hi.y);
     };
@@ -783,38 +790,39 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       if constexpr (AHEAD) {
         if (works)
 #pragma unroll
-          for (int n = 0; n < EPL; ++n) read_key(wk, n);
+          for (int n = 0; n < EPL; ++n) read_key(buf, wk, n);
         __builtin_amdgcn_sched_barrier(0);
       }
-      if (brings && t + 1 < t1) {
-        put(next, t + 1, buf ^ 1);
-        ask(next, t + 1 + DEPTH);
+      const int own = t + NT + ahead;
+      if (brings && own < t1) {
+        put(next, own, buf ^ 1);
+        ask(next, own + NT * DEPTH);
       }
       if (works) {
-        auto one = [&](int blk, auto more_) {
+        auto one = [&](int cur, int tile, int blk, auto more_) {
           constexpr bool more = decltype(more_)::value;
           float cs[8], vs[8];
           if constexpr (QUANT) {
-            meet_scales(fabsf(s_scale[buf][1][blk * AT_STEP + (lane & 31)]));
+            meet_scales(fabsf(s_scale[cur][1][blk * AT_STEP + (lane & 31)]));
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const float4 k4 = *reinterpret_cast<const float4*>(&s_scale[buf][0][blk * AT_STEP + i * 16 + g * 4]);
-              const float4 v4 = *reinterpret_cast<const float4*>(&s_scale[buf][1][blk * AT_STEP + i * 16 + g * 4]);
+              const float4 k4 = *reinterpret_cast<const float4*>(&s_scale[cur][0][blk * AT_STEP + i * 16 + g * 4]);
+              const float4 v4 = *reinterpret_cast<const float4*>(&s_scale[cur][1][blk * AT_STEP + i * 16 + g * 4]);
               cs[4 * i] = k4.x, cs[4 * i + 1] = k4.y, cs[4 * i + 2] = k4.z, cs[4 * i + 3] = k4.w;
               vs[4 * i] = v4.x, vs[4 * i + 1] = v4.y, vs[4 * i + 2] = v4.z, vs[4 * i + 3] = v4.w;
             }
           }
-          const uint32_t h0 = __builtin_amdgcn_readfirstlane(s_here[buf][2 * blk]);
-          const uint32_t h1 = __builtin_amdgcn_readfirstlane(s_here[buf][2 * blk + 1]);
-          step(whole_, t * AT_TILE + blk * AT_STEP, (h0 & h1) == 0xffffu,
+          const uint32_t h0 = __builtin_amdgcn_readfirstlane(s_here[cur][2 * blk]);
+          const uint32_t h1 = __builtin_amdgcn_readfirstlane(s_here[cur][2 * blk + 1]);
+          step(whole_, tile * AT_TILE + blk * AT_STEP, (h0 & h1) == 0xffffu,
                [&]() { return ((h0 >> (g * 4)) & 0xfu) | (((h1 >> (g * 4)) & 0xfu) << 4); }, cs, vs,
                [&](int i, int kk, uint32_t (&ko)[4]) {
-                 if constexpr (!AHEAD) read_key(blk, i * NK + kk);
+                 if constexpr (!AHEAD) read_key(cur, blk, i * NK + kk);
                  const uint4 v = fr[i * NK + kk];
                  ko[0] = v.x, ko[1] = v.y, ko[2] = v.z, ko[3] = v.w;
                },
                [&](int e, uint32_t (&vo)[4]) {
-                 if constexpr (!AHEAD) read_value(blk, e);
+                 if constexpr (!AHEAD) read_value(cur, blk, e);
                  const uint4 v = fr[e];
                  vo[0] = v.x, vo[1] = v.y, vo[2] = v.z, vo[3] = v.w;
                },
@@ -822,27 +830,30 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
                  if constexpr (AHEAD) {
                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                   for (int e = 0; e < EPL; ++e) read_value(blk, e);
+                   for (int e = 0; e < EPL; ++e) read_value(cur, blk, e);
                    __builtin_amdgcn_sched_barrier(0);
                  }
                },
                [&](int e) {
                  if constexpr (AHEAD && more) {
-                   read_key(blk + 1, e);
+                   read_key(cur, blk + 1, e);
                    __builtin_amdgcn_sched_barrier(0);
                  }
                });
         };
-        one(wk, Int<WK == 1>{});
-        if constexpr (WK == 1) one(1, Int<0>{});
+#pragma unroll 1
+        for (int i = 0; i < NT && t + i < t1; ++i) {
+          one(buf * NT + i, t + i, wk, Int<WK == 1>{});
+          if constexpr (WK == 1) one(buf * NT + i, t + i, 1, Int<0>{});
+        }
       }
       buf ^= 1;
     };
     const int whole = clear / AT_TILE < t1 ? clear / AT_TILE : t1;
     int t = t0;
     if constexpr (DEPTH == 1) {
-      for (; t < whole; ++t) turn(Int<1>{}, sets[0], t);
-      for (; t < t1; ++t) turn(Int<0>{}, sets[0], t);
+      for (; t + NT <= whole; t += NT) turn(Int<1>{}, sets[0], t);
+      for (; t < t1; t += NT) turn(Int<0>{}, sets[0], t);
     } else {
       // (turn t puts away the set of t + 1 - t0)
       for (; t + 1 < whole; t += 2) {

@@ -72,16 +72,17 @@ static AttnShape attn_shape(int T, int G, int dim) {
   const int groups = (tiles + s.R - 1) / s.R;
   s.WR = groups < AT_MOST ? groups : AT_MOST;
   s.RB = (groups + s.WR - 1) / s.WR;
-  s.waves = s.WR > AT_WAVES ? s.WR : AT_WAVES;
+  s.waves = s.R == 2 ? AT_MOST : (s.WR > AT_WAVES ? s.WR : AT_WAVES);  // (those without rows bring positions)
   return s;
 }
 
 // Ranges at most: as many as workgroups run at once (or a few times as many where the heads and row blocks leave too
 // many of those idle otherwise).
 static int attn_ranges(const AttnShape& s, int heads, int dim) {
-  const int lds = s.form == AT_DIRECT ? (dim > 128 ? 2 : 4) : (dim > 128 ? 1 : (dim > 64 ? 2 : 4));
+  const int lds = s.form == AT_DIRECT ? (dim > 128 ? 2 : 4) : (dim > 128 ? 1 : (dim > 64 ? 2 : 4)) / s.R;
   int per = 4 * attn_occupancy(s.form, s.R, dim) / s.waves;  // workgroups a CU
-  per = per < 1 ? 1 : (per > lds ? lds : per);
+  per = per > lds ? lds : per;
+  per = per < 1 ? 1 : per;
   const int64_t slots = 256 * per, hb = (int64_t)heads * s.RB;
   int64_t best = 1;
   double use = 0.0;
