@@ -11,7 +11,7 @@ extern template void launch_attn<DSV_F16, DSV_E4M3>(const AttnParams&, const Att
 extern template void launch_attn<DSV_BF16, DSV_I8>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
 extern template void launch_attn<DSV_F16, DSV_I8>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
 
-constexpr int AJ_THREADS = 256;
+constexpr int AJ_THREADS = 256, AJ_PARTS = 4;
 
 // The parts of a request joined: 8 elements of a row a thread, the parts in their order.  Bound by latency (the plan's
 // lengths, the references, the sums) and by the sums' bytes.
@@ -38,21 +38,32 @@ __global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
   auto part = [&](int i) {
     return ((int64_t)(2 * i + (i == i0 && plan.start(i) < before ? 1 : 0)) * c.heads + h) * rows + r;
   };
-  float top = AT_LOW;
-#pragma unroll 4
-  for (int i = i0; i <= i1; ++i) top = fmaxf(top, P.part_ml[part(i)].x);
-  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, lt = 0.f;
-#pragma unroll 4
-  for (int i = i0; i <= i1; ++i) {
-    const int64_t at = part(i);
-    const float2 ml = P.part_ml[at];
-    const float4 x = *reinterpret_cast<const float4*>(P.part_o + at * c.dim + d);
-    const float4 y = *reinterpret_cast<const float4*>(P.part_o + at * c.dim + d + 4);
-    const float f = __builtin_amdgcn_exp2f(ml.x - top);
-    lt = fmaf(ml.y, f, lt);
-    const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  float top = AT_LOW, lt = 0.f, sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (int i = i0; i <= i1; i += AJ_PARTS) {  // (the references and the sums of a few parts are asked for at once)
+    float2 ml[AJ_PARTS];
+    f32x4 x[AJ_PARTS][2];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) sum[u] = fmaf(v[u], f, sum[u]);
+    for (int j = 0; j < AJ_PARTS; ++j) {
+      const int64_t at = part(i + j <= i1 ? i + j : i1);
+      ml[j] = P.part_ml[at];
+      x[j][0] = *reinterpret_cast<const f32x4*>(P.part_o + at * c.dim + d);
+      x[j][1] = *reinterpret_cast<const f32x4*>(P.part_o + at * c.dim + d + 4);
+    }
+    const float old = top;
+#pragma unroll
+    for (int j = 0; j < AJ_PARTS; ++j) top = fmaxf(top, ml[j].x);  // (the last part again, where there are fewer)
+    const float keep = __builtin_amdgcn_exp2f(old - top);
+    lt *= keep;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) sum[u] *= keep;
+#pragma unroll
+    for (int j = 0; j < AJ_PARTS; ++j) {
+      if (i + j > i1) break;
+      const float f = __builtin_amdgcn_exp2f(ml[j].x - top);
+      lt = fmaf(ml[j].y, f, lt);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) sum[u] = fmaf(x[j][u / 4][u & 3], f, sum[u]);
+    }
   }
   const float inv = lt == 0.f ? 0.f : 1.f / lt;
   uint4 v;
