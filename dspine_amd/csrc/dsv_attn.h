@@ -364,14 +364,18 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
 
   f32x4 o[R][EPL];
   float mref[R], l[R];
-  // The largest value scale so far is held as a power of two 2^vlog; weights are 2^vlog smaller than they would be, by the
-  // rows' references, so that with their scales they stay within float16.
-  float vlog = -60.f, vtop = 8.673617379884035e-19f;  // (2^-60)
+  // The largest value scale that the lane's row has seen is held as a power of two, vtop = 2^vlog; its weights are 2^vlog
+  // smaller than they would be, by its reference, so that with their scales they stay within float16.  (A row's own:
+  // one large scale of a node that it does not see would push its weights out of float16's range.)  The sum l is kept
+  // without that factor, so that scales of any distance leave it whole.
+  float vlog[R], vtop[R];
   bool fresh = true;  // some row has no reference yet
 #pragma unroll
   for (int rt = 0; rt < R; ++rt) {
     mref[rt] = AT_LOW;
     l[rt] = 0.f;
+    vlog[rt] = -100.f;  // (scales far below lose bits)
+    vtop[rt] = 0x1p-100f;
 #pragma unroll
     for (int e = 0; e < EPL; ++e) o[rt][e] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -454,26 +458,28 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       }
     if (odd) s_odd = 1;
   };
-  // v: magnitudes of value scales, over the lanes.
+  // the lane's row rt sees value scales up to `top` (finite)
+  auto raise = [&](int rt, float top) {
+    int ex;
+    (void)frexpf(top, &ex);
+    const float up = top > vtop[rt] ? (float)(ex < 127 ? ex : 127) : vlog[rt], keep = __builtin_amdgcn_exp2f(vlog[rt] - up);
+    if (mref[rt] != AT_LOW) mref[rt] += up - vlog[rt];
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) o[rt][e] *= keep;
+    vlog[rt] = up;
+    vtop[rt] = __builtin_amdgcn_exp2f(up);
+  };
+  // a step's value scales, spread over the lanes, which every row sees
   auto meet_scales = [&](float v) {
     if constexpr (QUANT) {
-      if (__any(v > vtop)) {
-        const float top = wave_max_f32(v < INFINITY ? v : 0.f);
-        int ex;
-        (void)frexpf(top, &ex);
-        const float up = (float)ex;
-        if (top > vtop && up > vlog) {
-          const float keep = __builtin_amdgcn_exp2f(vlog - up);
+      v = v < INFINITY ? v : 0.f;
+      bool more = false;
 #pragma unroll
-          for (int rt = 0; rt < R; ++rt) {
-            if (mref[rt] != AT_LOW) mref[rt] += up - vlog;
-            l[rt] *= keep;
+      for (int rt = 0; rt < R; ++rt) more |= v > vtop[rt];
+      if (__any(more)) {
+        const float top = wave_max_f32(v);
 #pragma unroll
-            for (int e = 0; e < EPL; ++e) o[rt][e] *= keep;
-          }
-          vlog = up;
-          vtop = __builtin_amdgcn_exp2f(up);
-        }
+        for (int rt = 0; rt < R; ++rt) raise(rt, top);
       }
     }
   };
@@ -515,6 +521,16 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
           bits |= (sees ? 1u : 0u) << j;
         }
         seen[rt] = bits & here;
+        if constexpr (QUANT) {
+          float top = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float v = (seen[rt] >> j) & 1 ? fabsf(vs[j]) : 0.f;
+            top = fmaxf(top, v < INFINITY ? v : 0.f);
+          }
+          top = across_groups_max(top);
+          if (__any(top > vtop[rt])) raise(rt, top);
+        }
       }
     }
     // scores against the rows' references
@@ -522,27 +538,32 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
 #pragma unroll
     for (int rt = 0; rt < R; ++rt) {
       const float ref = mref[rt] == AT_LOW ? 0.f : mref[rt];
+      float top = AT_LOW;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         float x = fmaf(s[rt][j / 4][j & 3], QUANT ? cs[j] : c0, -ref);
         if (!WHOLE && !((seen[rt] >> j) & 1)) x = -INFINITY;
         s[rt][j / 4][j & 3] = x;
-        over = fmaxf(over, x);
+        top = fmaxf(top, x);
       }
+      over = fmaxf(over, QUANT ? top + vlog[rt] : top);
     }
     if (WHOLE && !full) {
       asm volatile("");  // (a branch: the selects are for bad slots only)
       const uint32_t here = here_();
       over = AT_LOW;
 #pragma unroll
-      for (int rt = 0; rt < R; ++rt)
+      for (int rt = 0; rt < R; ++rt) {
+        float top = AT_LOW;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           if (!((here >> j) & 1)) s[rt][j / 4][j & 3] = -INFINITY;
-          over = fmaxf(over, s[rt][j / 4][j & 3]);
+          top = fmaxf(top, s[rt][j / 4][j & 3]);
         }
+        over = fmaxf(over, QUANT ? top + vlog[rt] : top);
+      }
     }
-    if (fresh || __any(over > SHIFT + LIM - (QUANT ? vlog : 0.f))) {
+    if (fresh || __any(over > SHIFT + LIM)) {
       bool none = false;
 #pragma unroll
       for (int rt = 0; rt < R; ++rt) {
@@ -551,7 +572,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
         for (int j = 0; j < 8; ++j) top = fmaxf(top, s[rt][j / 4][j & 3]);
         top = across_groups_max(top);
         const bool unset = mref[rt] == AT_LOW;
-        float move = top - SHIFT + (QUANT ? vlog : 0.f);  // of the reference: up, or anywhere from none
+        float move = top - SHIFT + (QUANT ? vlog[rt] : 0.f);  // of the reference: up, or anywhere from none
         if (top == AT_LOW || (!unset && move < 0.f)) move = 0.f;
         if (top != AT_LOW || !unset) mref[rt] = (unset ? 0.f : mref[rt]) + move;
         none |= mref[rt] == AT_LOW;
@@ -567,13 +588,14 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
     uint32_t pf[R][4];
 #pragma unroll
     for (int rt = 0; rt < R; ++rt) {
+      float sum = QUANT ? 0.f : l[rt];
 #pragma unroll
       for (int j = 0; j < 8; j += 2) {
         float w[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           w[u] = __builtin_amdgcn_exp2f(s[rt][j / 4][(j + u) & 3]);
-          l[rt] += w[u];
+          sum += w[u];
           if constexpr (QUANT) {
             w[u] *= vs[j + u];
             if (!WHOLE && !((seen[rt] >> (j + u)) & 1)) w[u] = 0.f;
@@ -581,6 +603,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
         }
         pf[rt][j / 2] = pack_act<PT>(w[0], w[1]);
       }
+      l[rt] = QUANT ? fmaf(sum, vtop[rt], l[rt]) : sum;
     }
 #pragma unroll
     for (int e0 = 0; e0 < EPL; e0 += GRP) {
@@ -608,9 +631,9 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       const float f = g < 2 ? ksc[s * c.ks_slot_stride] : vsc[s * c.vs_slot_stride];
       return good(slot) ? f : 0.f;
     };
-    auto spread_scales = [&](float scale, float (&kf)[8], float (&vf)[8]) {
+    auto spread_scales = [&](auto whole_, float scale, float (&kf)[8], float (&vf)[8]) {
       if constexpr (QUANT) {
-        meet_scales(g < 2 ? 0.f : fabsf(scale));
+        if (decltype(whole_)::value) meet_scales(g < 2 ? 0.f : fabsf(scale));
         s_scale[wave][g >> 1][(g & 1) * 16 + m] = g < 2 ? scale * c0 : scale;
         __builtin_amdgcn_wave_barrier();  // (the wave's own memory, in order)
 #pragma unroll
@@ -660,7 +683,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       auto go = [&](uint32_t (&wv)[8][VW], uint32_t here, uint32_t (&then)[8][VW], uint32_t& then_here, uint32_t (&ks)[2],
                     uint32_t (&slot)[8], uint32_t (&then_ks)[2], uint32_t (&then_slot)[8]) {
         float cs[8], vs[8];
-        spread_scales(scale, cs, vs);
+        spread_scales(Int<1>{}, scale, cs, vs);
         const bool full = !__any(here != 0xffu);
         step(Int<1>{}, t * AT_STEP, full, [&]() { return here; }, cs, vs,
              [&](int i, int kk, uint32_t (&ko)[4]) { key_frag(kw[i], kk, ko); },
@@ -694,7 +717,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       value_slots(Int<0>{}, base, slot);
       load_key(ks[0], kw[0]);
       load_key(ks[1], kw[1]);
-      spread_scales(load_scale(ks[0], ks[1]), cs, vs);
+      spread_scales(Int<0>{}, load_scale(ks[0], ks[1]), cs, vs);
 #pragma unroll
       for (int j = 0; j < 8; ++j) load_value(slot[j], wv[j]);
       const uint32_t here = holds(slot);
@@ -818,7 +841,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
           constexpr bool more = decltype(more_)::value;
           float cs[8], vs[8];
           if constexpr (QUANT) {
-            meet_scales(fabsf(s_scale[cur][1][blk * AT_STEP + (lane & 31)]));
+            if (decltype(whole_)::value) meet_scales(fabsf(s_scale[cur][1][blk * AT_STEP + (lane & 31)]));
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const float4 k4 = *reinterpret_cast<const float4*>(&s_scale[cur][0][blk * AT_STEP + i * 16 + g * 4]);
@@ -886,6 +909,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
 #pragma unroll
   for (int rt = 0; rt < R; ++rt) {
     l[rt] = across_groups_sum(l[rt]);
+    if (QUANT && mref[rt] != AT_LOW) mref[rt] -= vlog[rt];
     if (g == 0) {
       s_m[wave][rt * 16 + m] = mref[rt];
       s_l[wave][rt * 16 + m] = l[rt];
@@ -900,7 +924,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
   for (int rt = 0; rt < R; ++rt) {
     float top = AT_LOW;
     for (int k = 0; k < WK; ++k) top = fmaxf(top, s_m[wr * WK + k][rt * 16 + m]);
-    const float f = __builtin_amdgcn_exp2f(mref[rt] - top) * unit;
+    const float f = __builtin_amdgcn_exp2f(mref[rt] - top) * (QUANT ? vtop[rt] * unit : unit);
     if (rt) __syncthreads();
 #pragma unroll
     for (int r = 0; r < 4; ++r)
