@@ -21,9 +21,9 @@
 // finished there; the parts of the others are left as sums and joined by k_attn_join.
 //
 // Measured, both launches of a call (8 cache heads, dim 128; the card copies at 4.8 TB/s and multiplies at 1.36 PF):
-//   64 requests, 17 nodes, 4 query heads a cache head, bf16, 1k to 8k positions   267 us   4.5 TB/s: memory
-//   8 requests, 1 node, int8, 16k to 64k positions                                181 us   3.7 TB/s: memory, and 8 to 16 bits
-//   16 requests, 64 nodes, 8 query heads a cache head, e4m3, 4k to 12k            419 us   0.64 PF: a wave's own chain of LDS
+//   64 requests, 17 nodes, 4 query heads a cache head, bf16, 1k to 8k positions   270 us   4.4 TB/s: memory
+//   8 requests, 1 node, int8, 16k to 64k positions                                175 us   3.9 TB/s: memory, and 8 to 16 bits
+//   16 requests, 64 nodes, 8 query heads a cache head, e4m3, 4k to 12k            438 us   0.61 PF: a wave's own chain of LDS
 //       reads, products, exponentials and products (matrix pipe busy a quarter of the time, VALU a third)
 //   4 requests, 25 nodes, bf16, 1.5k to 4.7k                                       35 us   1.5 TB/s: latency (the plan, the
 //       first loads, the outputs and the second launch take longer than a workgroup's six tiles)
@@ -490,7 +490,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
   auto step = [&](auto whole_, int base, bool full, auto here_, const auto& cs, const auto& vs, auto key, auto value,
                   auto next, auto after) {
     constexpr bool WHOLE = decltype(whole_)::value;
-    constexpr int GRP = R == 2 ? 4 : 1;  // operands asked for together (one, with two row tiles: 445 us for 424 below)
+    constexpr int GRP = R == 2 ? 4 : 1;  // operands asked for together (one, with two row tiles: 5 % slower)
     f32x4 s[R][2];
 #pragma unroll
     for (int rt = 0; rt < R; ++rt)

@@ -82,8 +82,8 @@ __global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
 //   17 to 32: staged, two waves for the same rows.  32 rows, 1 x 640 positions: 18.0 us, 19.3 with one wave for them
 //     and two that only bring; 16 x 2k to 8k: 87 and 88.
 //   up to 128: staged, a wave for each 16.  With 32 a wave: 305 us for 277 (68 rows), 44.6 for 40.2 (100 rows).
-//   more: staged, 32 a wave (half the LDS reads a product).  With 16: 570 us for 421 (512 rows, e4m3), 178 for 157
-//     (132 rows).  Dims above 128 have no registers for it.
+//   more: staged, 32 a wave (half the LDS reads a product).  With 16: 570 us for 421 (512 rows, e4m3, one value scale
+//     for a wave's rows; 438 with one a row), 178 for 157 (132 rows, bf16).  Dims above 128 have no registers for it.
 static AttnShape attn_shape(int T, int G, int dim) {
   const int tiles = (T * G + 15) / 16;
   AttnShape s;
