@@ -3,7 +3,8 @@
 // For request b, cache head h and the query rows r = (node, query head of h's group), with s = scale * q.k:
 // out = sum_p e^(s_p - m) v_p / sum_p e^(s_p - m), in one pass over the positions with a reference m of the softmax
 // that moves up where a score exceeds it by more than a few powers of two (the weights are then at most 2^LIM, and the
-// partial sums are rescaled; most steps only compare).
+// partial sums are rescaled; most steps only compare).  With value scales the weighted values have a reference of their
+// own, the largest weight times scale: a scale counts by the weight of its position.
 //
 // The matrix cores take keys as they lie in memory: S^T = K Q^T with the positions on the rows of the tile, so that a
 // lane holds, for one query row, the weights of the four (twice: eight) positions that the second product
@@ -54,7 +55,7 @@ struct AttnParams {
   FastDiv least;       // tiles of a range at least (a batch of fewer is one range)
   uint32_t num_slots, k_step, v_step;  // slots; bytes from slot to slot
   float* part_o;       // [2 * range + (the range's last request, not its first)][head][row][dim]
-  float2* part_ml;     // the same of [row]: reference, sum
+  float4* part_ml;     // the same of [row]: reference of the scores, sum of the weights, reference of the weighted values
 };
 
 // The request's nodes, its context and its positions (context and window) that the page table has.
@@ -291,7 +292,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
   constexpr int NT = AT_TILES(FORM, R);
   constexpr size_t SUMS = sizeof(float) * WAVES * 16 * OS, TILES = STAGED ? sizeof(uint4) * 2 * NT * FRAGS * WAVE : 0;
   __shared__ __attribute__((aligned(16))) unsigned char s_mem[SUMS > TILES ? SUMS : TILES];
-  __shared__ float s_m[WAVES][16 * R], s_l[WAVES][16 * R];
+  __shared__ float s_m[WAVES][16 * R], s_l[WAVES][16 * R], s_r[WAVES][16 * R];
   __shared__ uint64_t s_mask[WAVES][16 * R];  // of the wave's rows
   __shared__ int s_odd;
   float(*const s_o)[16][OS] = reinterpret_cast<float(*)[16][OS]>(s_mem);
@@ -364,18 +365,18 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
 
   f32x4 o[R][EPL];
   float mref[R], l[R];
-  // The largest value scale that the lane's row has seen is held as a power of two, vtop = 2^vlog; its weights are 2^vlog
-  // smaller than they would be, by its reference, so that with their scales they stay within float16.  (A row's own:
-  // one large scale of a node that it does not see would push its weights out of float16's range.)  The sum l is kept
-  // without that factor, so that scales of any distance leave it whole.
+  // With value scales the row has two references, both powers of two that only move up: m of its scores, 2^4 at most below
+  // any, for the sum l of the weights, and `mref` of weight times scale, for the float16 operands: those of the positions that
+  // count lie within [2^10, 2^15] at their largest, whatever scales positions without weight have.  A score is taken against
+  // mref, and mref - m = vlog (vtop = 2^vlog) is put back into l.  vlog >= -120: the weights stay within float32.
   float vlog[R], vtop[R];
   bool fresh = true;  // some row has no reference yet
 #pragma unroll
   for (int rt = 0; rt < R; ++rt) {
     mref[rt] = AT_LOW;
     l[rt] = 0.f;
-    vlog[rt] = -100.f;  // (scales far below lose bits)
-    vtop[rt] = 0x1p-100f;
+    vlog[rt] = 0.f;
+    vtop[rt] = 1.f;
 #pragma unroll
     for (int e = 0; e < EPL; ++e) o[rt][e] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -458,31 +459,6 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       }
     if (odd) s_odd = 1;
   };
-  // the lane's row rt sees value scales up to `top` (finite)
-  auto raise = [&](int rt, float top) {
-    int ex;
-    (void)frexpf(top, &ex);
-    const float up = top > vtop[rt] ? (float)(ex < 127 ? ex : 127) : vlog[rt], keep = __builtin_amdgcn_exp2f(vlog[rt] - up);
-    if (mref[rt] != AT_LOW) mref[rt] += up - vlog[rt];
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) o[rt][e] *= keep;
-    vlog[rt] = up;
-    vtop[rt] = __builtin_amdgcn_exp2f(up);
-  };
-  // a step's value scales, spread over the lanes, which every row sees
-  auto meet_scales = [&](float v) {
-    if constexpr (QUANT) {
-      v = v < INFINITY ? v : 0.f;
-      bool more = false;
-#pragma unroll
-      for (int rt = 0; rt < R; ++rt) more |= v > vtop[rt];
-      if (__any(more)) {
-        const float top = wave_max_f32(v);
-#pragma unroll
-        for (int rt = 0; rt < R; ++rt) raise(rt, top);
-      }
-    }
-  };
   // A step: scores of 32 positions' keys, weights, weighted values.  WHOLE: every row sees every position that holds
   // anything (`full`: all do; bit j of here_(): this lane's position j does).  cs: the positions' factors of a score
   // (base 2), vs: their value scales.  `next` runs when the keys have been used, `after` when the
@@ -521,17 +497,16 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
           bits |= (sees ? 1u : 0u) << j;
         }
         seen[rt] = bits & here;
-        if constexpr (QUANT) {
-          float top = 0.f;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float v = (seen[rt] >> j) & 1 ? fabsf(vs[j]) : 0.f;
-            top = fmaxf(top, v < INFINITY ? v : 0.f);
-          }
-          top = across_groups_max(top);
-          if (__any(top > vtop[rt])) raise(rt, top);
-        }
       }
+    }
+    // The largest value scale of the lane's positions, as a power of two: with the lane's largest score it bounds weight times
+    // scale from above, so most steps need no more to know that their operands stay within float16.
+    float lift = -INFINITY;
+    if constexpr (QUANT) {
+      float v = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v = fmaxf(v, fabsf(vs[j]));
+      lift = __builtin_amdgcn_logf(v);
     }
     // scores against the rows' references
     float over = AT_LOW;
@@ -546,7 +521,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
         s[rt][j / 4][j & 3] = x;
         top = fmaxf(top, x);
       }
-      over = fmaxf(over, QUANT ? top + vlog[rt] : top);
+      over = fmaxf(over, QUANT ? top + fmaxf(vlog[rt] + SHIFT, lift) : top);
     }
     if (WHOLE && !full) {
       asm volatile("");  // (a branch: the selects are for bad slots only)
@@ -560,7 +535,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
           if (!((here >> j) & 1)) s[rt][j / 4][j & 3] = -INFINITY;
           top = fmaxf(top, s[rt][j / 4][j & 3]);
         }
-        over = fmaxf(over, QUANT ? top + vlog[rt] : top);
+        over = fmaxf(over, QUANT ? top + fmaxf(vlog[rt] + SHIFT, lift) : top);
       }
     }
     if (fresh || __any(over > SHIFT + LIM)) {
@@ -572,12 +547,30 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
         for (int j = 0; j < 8; ++j) top = fmaxf(top, s[rt][j / 4][j & 3]);
         top = across_groups_max(top);
         const bool unset = mref[rt] == AT_LOW;
-        float move = top - SHIFT + (QUANT ? vlog[rt] : 0.f);  // of the reference: up, or anywhere from none
-        if (top == AT_LOW || (!unset && move < 0.f)) move = 0.f;
+        float move, keep_l;  // of the reference: up, or anywhere from none
+        if constexpr (QUANT) {
+          float high = -INFINITY;  // weight times scale
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float v = fabsf(vs[j]);
+            high = fmaxf(high, s[rt][j / 4][j & 3] + (v < INFINITY ? __builtin_amdgcn_logf(v) : -INFINITY));
+          }
+          high = across_groups_max(high);
+          const bool any = top != AT_LOW;
+          const float old = -vlog[rt], low = !any ? old : (unset ? ceilf(top) : fmaxf(old, ceilf(top)));  // the scores'
+          move = fmaxf(ceilf(high) - SHIFT, low - 120.f);
+          if (!any || (!unset && move < 0.f)) move = 0.f;
+          keep_l = unset ? 0.f : __builtin_amdgcn_exp2f(old - low);
+          if (any) vlog[rt] = move - low;
+          vtop[rt] = __builtin_amdgcn_exp2f(vlog[rt]);
+        } else {
+          move = top - SHIFT;
+          if (top == AT_LOW || (!unset && move < 0.f)) move = 0.f;
+        }
         if (top != AT_LOW || !unset) mref[rt] = (unset ? 0.f : mref[rt]) + move;
         none |= mref[rt] == AT_LOW;
         const float keep = unset ? 0.f : __builtin_amdgcn_exp2f(-move);
-        l[rt] *= keep;
+        l[rt] *= QUANT ? keep_l : keep;
 #pragma unroll
         for (int e = 0; e < EPL; ++e) o[rt][e] *= keep;
 #pragma unroll
@@ -631,9 +624,8 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       const float f = g < 2 ? ksc[s * c.ks_slot_stride] : vsc[s * c.vs_slot_stride];
       return good(slot) ? f : 0.f;
     };
-    auto spread_scales = [&](auto whole_, float scale, float (&kf)[8], float (&vf)[8]) {
+    auto spread_scales = [&](float scale, float (&kf)[8], float (&vf)[8]) {
       if constexpr (QUANT) {
-        if (decltype(whole_)::value) meet_scales(g < 2 ? 0.f : fabsf(scale));
         s_scale[wave][g >> 1][(g & 1) * 16 + m] = g < 2 ? scale * c0 : scale;
         __builtin_amdgcn_wave_barrier();  // (the wave's own memory, in order)
 #pragma unroll
@@ -683,7 +675,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       auto go = [&](uint32_t (&wv)[8][VW], uint32_t here, uint32_t (&then)[8][VW], uint32_t& then_here, uint32_t (&ks)[2],
                     uint32_t (&slot)[8], uint32_t (&then_ks)[2], uint32_t (&then_slot)[8]) {
         float cs[8], vs[8];
-        spread_scales(Int<1>{}, scale, cs, vs);
+        spread_scales(scale, cs, vs);
         const bool full = !__any(here != 0xffu);
         step(Int<1>{}, t * AT_STEP, full, [&]() { return here; }, cs, vs,
              [&](int i, int kk, uint32_t (&ko)[4]) { key_frag(kw[i], kk, ko); },
@@ -717,7 +709,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       value_slots(Int<0>{}, base, slot);
       load_key(ks[0], kw[0]);
       load_key(ks[1], kw[1]);
-      spread_scales(Int<0>{}, load_scale(ks[0], ks[1]), cs, vs);
+      spread_scales(load_scale(ks[0], ks[1]), cs, vs);
 #pragma unroll
       for (int j = 0; j < 8; ++j) load_value(slot[j], wv[j]);
       const uint32_t here = holds(slot);
@@ -841,7 +833,6 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
           constexpr bool more = decltype(more_)::value;
           float cs[8], vs[8];
           if constexpr (QUANT) {
-            if (decltype(whole_)::value) meet_scales(fabsf(s_scale[cur][1][blk * AT_STEP + (lane & 31)]));
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const float4 k4 = *reinterpret_cast<const float4*>(&s_scale[cur][0][blk * AT_STEP + i * 16 + g * 4]);
@@ -909,9 +900,9 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
 #pragma unroll
   for (int rt = 0; rt < R; ++rt) {
     l[rt] = across_groups_sum(l[rt]);
-    if (QUANT && mref[rt] != AT_LOW) mref[rt] -= vlog[rt];
     if (g == 0) {
-      s_m[wave][rt * 16 + m] = mref[rt];
+      s_r[wave][rt * 16 + m] = mref[rt];
+      s_m[wave][rt * 16 + m] = QUANT && mref[rt] != AT_LOW ? mref[rt] - vlog[rt] : mref[rt];
       s_l[wave][rt * 16 + m] = l[rt];
     }
   }
@@ -923,8 +914,8 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
 #pragma unroll
   for (int rt = 0; rt < R; ++rt) {
     float top = AT_LOW;
-    for (int k = 0; k < WK; ++k) top = fmaxf(top, s_m[wr * WK + k][rt * 16 + m]);
-    const float f = __builtin_amdgcn_exp2f(mref[rt] - top) * (QUANT ? vtop[rt] * unit : unit);
+    for (int k = 0; k < WK; ++k) top = fmaxf(top, s_r[wr * WK + k][rt * 16 + m]);
+    const float f = __builtin_amdgcn_exp2f(mref[rt] - top) * unit;
     if (rt) __syncthreads();
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -937,8 +928,11 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       const int rr = i / (DP / 8), d = i % (DP / 8) * 8, r = row0 + rt * 16 + rr;
       if (r >= n_rows || d >= dim) continue;
       float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      float mt = AT_LOW, lt = 0.f;
-      for (int k = 0; k < WK; ++k) mt = fmaxf(mt, s_m[wr * WK + k][rt * 16 + rr]);
+      float mt = AT_LOW, lt = 0.f, ref = AT_LOW;
+      for (int k = 0; k < WK; ++k) {
+        mt = fmaxf(mt, s_m[wr * WK + k][rt * 16 + rr]);
+        ref = fmaxf(ref, s_r[wr * WK + k][rt * 16 + rr]);
+      }
       for (int k = 0; k < WK; ++k) {
         lt += s_l[wr * WK + k][rt * 16 + rr] * __builtin_amdgcn_exp2f(s_m[wr * WK + k][rt * 16 + rr] - mt);
 #pragma unroll
@@ -964,16 +958,24 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
         float* po = P.part_o + at * dim + d;
         *reinterpret_cast<float4*>(po) = make_float4(sum[0], sum[1], sum[2], sum[3]);
         *reinterpret_cast<float4*>(po + 4) = make_float4(sum[4], sum[5], sum[6], sum[7]);
-        if (d == 0) P.part_ml[at] = make_float2(mt, lt);
+        if (d == 0) P.part_ml[at] = make_float4(mt, lt, ref, 0.f);
       } else {
         const int64_t row = row_of(a, request, node);
         if (row < 0) continue;
         const float inv = lt == 0.f ? 0.f : 1.f / lt;
+        if constexpr (QUANT) {  // (two steps: either factor alone may leave float32 where the product does not)
+          const float up = __builtin_amdgcn_exp2f(ref - mt);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) sum[u] = sum[u] * inv * up;
+        } else {
+#pragma unroll
+          for (int u = 0; u < 8; ++u) sum[u] *= inv;
+        }
         uint4 v;
-        v.x = pack_act<XT>(sum[0] * inv, sum[1] * inv);
-        v.y = pack_act<XT>(sum[2] * inv, sum[3] * inv);
-        v.z = pack_act<XT>(sum[4] * inv, sum[5] * inv);
-        v.w = pack_act<XT>(sum[6] * inv, sum[7] * inv);
+        v.x = pack_act<XT>(sum[0], sum[1]);
+        v.y = pack_act<XT>(sum[2], sum[3]);
+        v.z = pack_act<XT>(sum[4], sum[5]);
+        v.w = pack_act<XT>(sum[6], sum[7]);
         *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + row * a.out_row_stride + qh * a.out_head_stride + d) = v;
         if (d == 0 && a.lse) a.lse[row * a.q_heads + qh] = lt == 0.f ? -INFINITY : (mt + log2f(lt)) * 0.693147180559945309f;
       }

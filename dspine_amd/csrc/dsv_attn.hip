@@ -40,9 +40,9 @@ __global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
   auto part = [&](int i) {
     return ((int64_t)(2 * i + (i == i0 && plan.start(i) < before ? 1 : 0)) * c.heads + h) * rows + r;
   };
-  float top = AT_LOW, lt = 0.f, sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  float top = AT_LOW, ref = AT_LOW, lt = 0.f, sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int i = i0; i <= i1; i += AJ_PARTS) {  // (the references and the sums of a few parts are asked for at once)
-    float2 ml[AJ_PARTS];
+    float4 ml[AJ_PARTS];
     f32x4 x[AJ_PARTS][2];
 #pragma unroll
     for (int j = 0; j < AJ_PARTS; ++j) {
@@ -51,28 +51,34 @@ __global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
       x[j][0] = *reinterpret_cast<const f32x4*>(P.part_o + at * c.dim + d);
       x[j][1] = *reinterpret_cast<const f32x4*>(P.part_o + at * c.dim + d + 4);
     }
-    const float old = top;
+    const float old = top, old_ref = ref;
 #pragma unroll
-    for (int j = 0; j < AJ_PARTS; ++j) top = fmaxf(top, ml[j].x);  // (the last part again, where there are fewer)
-    const float keep = __builtin_amdgcn_exp2f(old - top);
-    lt *= keep;
+    for (int j = 0; j < AJ_PARTS; ++j) {  // (the last part again, where there are fewer)
+      top = fmaxf(top, ml[j].x);
+      ref = fmaxf(ref, ml[j].z);
+    }
+    const float keep = __builtin_amdgcn_exp2f(old_ref - ref);
+    lt *= __builtin_amdgcn_exp2f(old - top);
 #pragma unroll
     for (int u = 0; u < 8; ++u) sum[u] *= keep;
 #pragma unroll
     for (int j = 0; j < AJ_PARTS; ++j) {
       if (i + j > i1) break;
-      const float f = __builtin_amdgcn_exp2f(ml[j].x - top);
-      lt = fmaf(ml[j].y, f, lt);
+      const float f = __builtin_amdgcn_exp2f(ml[j].z - ref);
+      lt = fmaf(ml[j].y, __builtin_amdgcn_exp2f(ml[j].x - top), lt);
 #pragma unroll
       for (int u = 0; u < 8; ++u) sum[u] = fmaf(x[j][u / 4][u & 3], f, sum[u]);
     }
   }
-  const float inv = lt == 0.f ? 0.f : 1.f / lt;
+  // (two steps: either factor alone may leave float32 where the product does not)
+  const float inv = lt == 0.f ? 0.f : 1.f / lt, up = __builtin_amdgcn_exp2f(ref - top);
+#pragma unroll
+  for (int u = 0; u < 8; ++u) sum[u] = sum[u] * inv * up;
   uint4 v;
-  v.x = pack_act<XT>(sum[0] * inv, sum[1] * inv);
-  v.y = pack_act<XT>(sum[2] * inv, sum[3] * inv);
-  v.z = pack_act<XT>(sum[4] * inv, sum[5] * inv);
-  v.w = pack_act<XT>(sum[6] * inv, sum[7] * inv);
+  v.x = pack_act<XT>(sum[0], sum[1]);
+  v.y = pack_act<XT>(sum[2], sum[3]);
+  v.z = pack_act<XT>(sum[4], sum[5]);
+  v.w = pack_act<XT>(sum[6], sum[7]);
   *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + row * a.out_row_stride + qh * a.out_head_stride + d) = v;
   if (d == 0 && a.lse) a.lse[row * a.q_heads + qh] = lt == 0.f ? -INFINITY : (top + log2f(lt)) * 0.693147180559945309f;
 }
@@ -123,7 +129,7 @@ extern "C" int64_t dsv_tree_attention_workspace_bytes(int32_t bs, int32_t T, int
   if (bs < 1 || T < 1 || heads < 1 || q_heads < heads || dim < 1) return 0;
   const AttnShape s = attn_shape(T, q_heads / heads, dim);
   const int64_t rows = 2 * (int64_t)attn_ranges(s, heads, dim) * q_heads * T;
-  return rows * (dim * (int64_t)sizeof(float) + (int64_t)sizeof(float2));
+  return rows * (dim * (int64_t)sizeof(float) + (int64_t)sizeof(float4));
 }
 
 extern "C" int dsv_tree_attention(const dsv_tree_attention_args* args, dsv_stream_t stream_) {
@@ -177,7 +183,7 @@ extern "C" int dsv_tree_attention(const dsv_tree_attention_args* args, dsv_strea
   P.k_step = (uint32_t)(a.cache.k_slot_stride * esize);
   P.v_step = (uint32_t)(a.cache.v_slot_stride * esize);
   P.part_o = reinterpret_cast<float*>(a.workspace);
-  P.part_ml = reinterpret_cast<float2*>(P.part_o + 2 * (int64_t)P.most * a.q_heads * a.T * a.cache.dim);
+  P.part_ml = reinterpret_cast<float4*>(P.part_o + 2 * (int64_t)P.most * a.q_heads * a.T * a.cache.dim);
   const bool bf = a.dtype == DSV_BF16;
   if (a.cache.dtype == DSV_E4M3)
     bf ? launch_attn<DSV_BF16, DSV_E4M3>(P, s, (unsigned)blocks, stream) : launch_attn<DSV_F16, DSV_E4M3>(P, s, (unsigned)blocks, stream);
