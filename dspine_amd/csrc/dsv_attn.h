@@ -368,7 +368,9 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
   // With value scales the row has two references, both powers of two that only move up: m of its scores, 2^4 at most below
   // any, for the sum l of the weights, and `mref` of weight times scale, for the float16 operands: those of the positions that
   // count lie within [2^10, 2^15] at their largest, whatever scales positions without weight have.  A score is taken against
-  // mref, and mref - m = vlog (vtop = 2^vlog) is put back into l.  vlog >= -120: the weights stay within float32.
+  // mref, and mref - m = vlog (vtop = 2^vlog) is put back into l.  -120 <= vlog, so that the weights stay within float32, and
+  // vlog <= 117 for any finite scale: weights down to 2^-32 of the row's largest are then float32 numbers, subnormal ones
+  // at the far end, and count in l.
   float vlog[R], vtop[R];
   bool fresh = true;  // some row has no reference yet
 #pragma unroll

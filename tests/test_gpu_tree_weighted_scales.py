@@ -102,3 +102,43 @@ def test_a_context_of_zero_scales(device, T, G, dtype):
     want, wl, otol, ltol = _reference(d)
     R.close(out.cpu(), want, otol)
     R.close(lse.cpu(), wl, ltol)
+
+
+@pytest.mark.parametrize("dtype", [E4, I8])
+@pytest.mark.parametrize("T, G", FORMS)
+def test_values_up_to_the_largest_of_their_type(device, T, G, dtype):
+    """Rows that write_kv takes near bfloat16's largest: outputs are finite and right, as the rows read back are."""
+    from dspine_amd.kernels.cache import new_cache, read_kv, write_kv
+
+    d = _round(54, bs=2, T=T, H=2, G=G, D=64, act=BF, dtype=dtype, lens=[300, 40], tree=True)
+    n = d["cache"][0].shape[0]
+    x = torch.randn(n, 2, 64, generator=torch.Generator().manual_seed(55))
+    x = (x * (3e38 / x.abs().amax(-1, keepdim=True))).to(BF)
+    cache, slots = new_cache(n, 2, 64, dtype=dtype, device=device), torch.arange(n, device=device)
+    write_kv(cache, x.to(device), x.to(device), slots)
+    assert bool(torch.isfinite(read_kv(cache, slots, dtype=torch.float32)[1]).all())
+    d["cache"] = (*d["cache"][:1], cache.v.cpu(), d["cache"][2], cache.v_scale.cpu())
+    out, lse = _call(d, device)
+    want, wl, otol, ltol = _reference(d)
+    assert bool(torch.isfinite(out).all())
+    R.close(out.cpu(), want, otol)
+    R.close(lse.cpu(), wl, ltol)
+
+
+@pytest.mark.parametrize("dtype", [E4, I8])
+@pytest.mark.parametrize("T, G", FORMS)
+@pytest.mark.parametrize("power", [119, -108])
+def test_small_weights_count_whatever_the_scales(device, power, T, G, dtype):
+    """4096 weights of e^-13.5 beside one of 1, every scale near the end of write_kv's range: they are half a percent of
+    the sum, and all of it is there."""
+    d = _round(56, bs=1, T=T, H=1, G=G, D=64, act=BF, dtype=dtype, lens=[4097], tree=True)
+    k, v, ks, vs = d["cache"]
+    _lower(d, list(range(4096)), 13.5, 0)
+    at = d["page_table"][0].long()
+    k[at[4096:]] = torch.zeros_like(k[at[4096:]])
+    d["masks"][:] = 0  # (the context alone)
+    vs[:] = 2.0 ** power
+    out, lse = _call(d, device)
+    want, wl, otol, ltol = _reference(d)
+    R.close(out.cpu(), want, otol)
+    R.close(lse.cpu(), wl, ltol)
