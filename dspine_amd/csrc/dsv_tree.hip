@@ -192,7 +192,8 @@ __device__ __forceinline__ int64_t load_i(const void* p, int i64, int64_t i) {
 }
 
 // The commit of the accepted paths: one workgroup, requests in contiguous ranges a thread, a block scan places
-// each request's freed slots (as the chain's commit does).
+// each request's freed slots (as the chain's commit does).  The path of a tree ascends, so its slots can be moved down inside
+// the table one after the other; a caller's own order is read whole before the first position is written.
 constexpr int CT_THREADS = 1024;
 __global__ __launch_bounds__(CT_THREADS) void k_commit_tree(int bs, int T, const int32_t* accept, const int32_t* path,
                                                             const int32_t* verify_lens, const void* prefix_lens,
@@ -205,30 +206,37 @@ __global__ __launch_bounds__(CT_THREADS) void k_commit_tree(int bs, int T, const
   const int tid = threadIdx.x;
   const int per = (bs + CT_THREADS - 1) / CT_THREADS;
   const int b0 = tid * per < bs ? tid * per : bs, b1 = b0 + per < bs ? b0 + per : bs;
-  // the request's nodes n, its commit c (clamped into [1, n]) and the nodes that are kept
-  auto of = [&](int b, int& n, int& c) {
+  // the request's nodes n, its commit c (clamped into [1, n]) and the nodes that are kept: `take` gets the places and nodes of the
+  // path's entries, without those outside the window and those named before
+  auto of = [&](int b, int& n, int& c, auto take) {
     n = verify_lens ? verify_lens[b] : T;
     n = n < 1 ? 1 : (n > T ? T : n);
     c = accept[b] + 1;
     c = c < 1 ? 1 : (c > n ? n : c);
     uint64_t kept = 0;
-    for (int i = 0; i < c; ++i) {
+    for (int i = 0, at = 0; i < c; ++i) {
       const int node = path[(int64_t)b * T + i];
-      if (node >= 0 && node < n) kept |= 1ull << node;
+      if (node < 0 || node >= n || (kept >> node) & 1) continue;
+      kept |= 1ull << node;
+      take(at++, node);
     }
     return kept;
   };
   int mine = 0;
   for (int b = b0; b < b1; ++b) {
     int n, c;
-    const uint64_t kept = of(b, n, c);
+    const uint64_t kept = of(b, n, c, [](int, int) {});
     mine += n - __popcll(kept);
   }
   int total = 0;
   int at = block_excl_scan<CT_THREADS / WAVE>(mine, sred, &total);
   for (int b = b0; b < b1; ++b) {
-    int n, c;
-    const uint64_t kept = of(b, n, c);
+    int n, c, before = -1;
+    bool rises = true;
+    const uint64_t kept = of(b, n, c, [&](int, int node) {
+      rises &= node > before;
+      before = node;
+    });
     const int64_t row = load_i(req_pool, req_i64, b);
     const int64_t pre = load_i(prefix_lens, prefix_i64, b);
     int32_t* rt = req_to_token + row * rt_stride;
@@ -241,18 +249,23 @@ __global__ __launch_bounds__(CT_THREADS) void k_commit_tree(int bs, int T, const
     if (free_slots)  // (before the table changes: the slots may be read from it)
       for (int i = 0; i < n; ++i)
         if (!((kept >> i) & 1)) free_slots[at++] = slot_of(i);
-    // kept nodes in ascending order: a position is written after every read at or before it
-    int i = 0;
-    for (uint64_t left = kept; left; left &= left - 1, ++i) {
-      const int64_t slot = slot_of(__ffsll((unsigned long long)left) - 1);
+    auto write = [&](int i, int64_t slot) {
       const int64_t pos = pre + i;
       if (pos >= 0 && pos < rt_cols) rt[pos] = (int32_t)slot;
+    };
+    const int left = __popcll(kept);
+    if (rises || out_cache_loc) {  // (rising: a position is written after every read at or before it)
+      of(b, n, c, [&](int i, int node) { write(i, slot_of(node)); });
+    } else {
+      int32_t slots[TREE_MAX];
+      of(b, n, c, [&](int i, int node) { slots[i] = (int32_t)slot_of(node); });
+      for (int i = 0; i < left; ++i) write(i, slots[i]);
     }
     if (seq_lens) {
       if (seq_i64)
-        reinterpret_cast<int64_t*>(seq_lens)[row] = pre + i;
+        reinterpret_cast<int64_t*>(seq_lens)[row] = pre + left;
       else
-        reinterpret_cast<int32_t*>(seq_lens)[row] = (int32_t)(pre + i);
+        reinterpret_cast<int32_t*>(seq_lens)[row] = (int32_t)(pre + left);
     }
   }
   if (tid == 0 && free_count) *free_count = total;

@@ -297,7 +297,8 @@ def commit_accept(outputs, *, prefix_lens, req_pool_indices, req_to_token, out_c
 
     ``path`` (int32 [bs, T], T <= 64; ``accept_greedy_tree``'s) commits a drafted tree: the accepted
     positions are the nodes ``path[b, :accept[b] + 1]`` of the window, in that order, and the slots of
-    its other nodes are freed (``dsv_commit_tree``)."""
+    its other nodes are freed (``dsv_commit_tree``).  Entries outside the window and nodes named before
+    are left out; what follows moves up, and the length counts the entries that remain."""
     accept, output = outputs[0], outputs[3]
     bs, T = output.shape
     dev = _lib.require_cuda(accept, prefix_lens, req_pool_indices, req_to_token, out_cache_loc, verify_lens,

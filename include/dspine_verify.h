@@ -505,9 +505,10 @@ int dsv_tree_verify(const void* logits, int32_t logits_dtype, int64_t rows, int6
 int64_t dsv_tree_verify_workspace_bytes(int64_t rows, int64_t vocab);
 
 /* dsv_commit_accept where the accepted positions are the nodes path[b, i] (int32 [bs, T], T <= 64) */
-/* of the window: table position prefix + i takes the slot of node path[b, i], the slots of the    */
-/* window's other nodes go to free_slots in node order.  A path entry outside the window is left   */
-/* out.                                                                                            */
+/* of the window: table position prefix + i takes the slot of node path[b, i], in whatever order   */
+/* the path names them; the slots of the window's other nodes go to free_slots in node order.  A   */
+/* path entry outside the window and one that names a node again are left out: what follows moves  */
+/* up, and the sequence length is prefix + the entries that remain.                                 */
 int dsv_commit_tree(int32_t bs, int32_t T, const int32_t* accept, const int32_t* path, const int32_t* verify_lens,
                     const void* prefix_lens, int32_t prefix_i64, const void* req_pool_indices,
                     int32_t req_pool_i64, int32_t* req_to_token, int64_t rt_stride, int64_t rt_cols,
