@@ -49,8 +49,8 @@ def accept_greedy_tree(*, candidates: torch.Tensor, parents: torch.Tensor, next_
 
     candidates [bs, T] int64: the nodes' tokens, node 0 the last accepted one; next_token_logits
     [bs*T, V] (bfloat16 or float32): row ``b*T + i`` follows node i.  From node 0 the path moves to the child
-    that carries the argmax of the node it is at (lowest id on ties; of several such children the
-    first) until none does; nodes at or past ``verify_lens[b]`` (int32 [bs], clamped into [1, T]) are not
+    that carries the argmax of the node it is at (lowest id on ties, NaN as -inf; of several such children
+    the first) until none does; nodes at or past ``verify_lens[b]`` (int32 [bs], clamped into [1, T]) are not
     there and their rows are not read.  accept counts the moves, bonus is the last node's argmax, output holds the
     accepted tokens, the bonus, then zeros; ``path`` the nodes of the path (node 0 first), then -1 --
     what ``commit_accept(path=...)`` and a caller that gathers the path's hidden states take."""

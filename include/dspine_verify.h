@@ -492,7 +492,8 @@ int dsv_tree_masks(const int32_t* parents, int32_t bs, int32_t T, int64_t* masks
                    dsv_stream_t stream);
 
 /* Greedy acceptance of drafted trees.  candidates [bs, T] int64: node tokens (node 0 the last      */
-/* accepted token); logits row b * T + i follows node i, top1 = its first argmax.  From node 0 the */
+/* accepted token); logits row b * T + i follows node i, top1 = its first argmax (a NaN counts as  */
+/* -infinity).  From node 0 the                                                                     */
 /* path moves to the child that carries top1 of the node it is at (of several the first; children  */
 /* at or past verify_lens[b], clamped into [1, T], do not count) until none does.  accept = moves, */
 /* commit = accept + 1, bonus = top1 of the last node, output = the accepted tokens, the bonus,    */
