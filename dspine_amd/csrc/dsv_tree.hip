@@ -193,7 +193,9 @@ __device__ __forceinline__ int64_t load_i(const void* p, int i64, int64_t i) {
 
 // The commit of the accepted paths: one workgroup, requests in contiguous ranges a thread, a block scan places
 // each request's freed slots (as the chain's commit does).  The path of a tree ascends, so its slots can be moved down inside
-// the table one after the other; a caller's own order is read whole before the first position is written.
+// the table one after the other; a caller's own order is left to the wave, an entry a lane, so that it is read whole before the
+// first position is written (an array of the thread's own cost every call scratch memory: 8.9 us for 8.4 at 64 requests of
+// 17 nodes; 8.1 where no order is kept).
 constexpr int CT_THREADS = 1024;
 __global__ __launch_bounds__(CT_THREADS) void k_commit_tree(int bs, int T, const int32_t* accept, const int32_t* path,
                                                             const int32_t* verify_lens, const void* prefix_lens,
@@ -206,66 +208,88 @@ __global__ __launch_bounds__(CT_THREADS) void k_commit_tree(int bs, int T, const
   const int tid = threadIdx.x;
   const int per = (bs + CT_THREADS - 1) / CT_THREADS;
   const int b0 = tid * per < bs ? tid * per : bs, b1 = b0 + per < bs ? b0 + per : bs;
-  // the request's nodes n, its commit c (clamped into [1, n]) and the nodes that are kept: `take` gets the places and nodes of the
-  // path's entries, without those outside the window and those named before
-  auto of = [&](int b, int& n, int& c, auto take) {
+  // the request's nodes n, its commit c (clamped into [1, n]), the nodes that are kept, and whether the path names them in
+  // ascending order
+  auto of = [&](int b, int& n, int& c, bool& rises) {
     n = verify_lens ? verify_lens[b] : T;
     n = n < 1 ? 1 : (n > T ? T : n);
     c = accept[b] + 1;
     c = c < 1 ? 1 : (c > n ? n : c);
     uint64_t kept = 0;
-    for (int i = 0, at = 0; i < c; ++i) {
+    rises = true;
+    for (int i = 0; i < c; ++i) {
       const int node = path[(int64_t)b * T + i];
-      if (node < 0 || node >= n || (kept >> node) & 1) continue;
-      kept |= 1ull << node;
-      take(at++, node);
+      const uint64_t bit = node >= 0 && node < n ? 1ull << node : 0ull;
+      rises &= bit == 0 || kept < bit;  // (none at or past it so far)
+      kept |= bit;
     }
     return kept;
   };
   int mine = 0;
   for (int b = b0; b < b1; ++b) {
     int n, c;
-    const uint64_t kept = of(b, n, c, [](int, int) {});
+    bool rises;
+    const uint64_t kept = of(b, n, c, rises);
     mine += n - __popcll(kept);
   }
   int total = 0;
   int at = block_excl_scan<CT_THREADS / WAVE>(mine, sred, &total);
-  for (int b = b0; b < b1; ++b) {
-    int n, c, before = -1;
-    bool rises = true;
-    const uint64_t kept = of(b, n, c, [&](int, int node) {
-      rises &= node > before;
-      before = node;
-    });
-    const int64_t row = load_i(req_pool, req_i64, b);
-    const int64_t pre = load_i(prefix_lens, prefix_i64, b);
-    int32_t* rt = req_to_token + row * rt_stride;
-    const int64_t base = slot_offsets ? slot_offsets[b] : (int64_t)b * T;
-    auto slot_of = [&](int node) -> int64_t {
-      if (out_cache_loc) return out_cache_loc[base + node];
+  // a request's table row and window: node's slot, and a slot to the i-th of its new positions
+  struct Window {
+    int64_t row, pre, base, cols;
+    int32_t* rt;
+    const int64_t* loc;
+    __device__ __forceinline__ int64_t slot_of(int node) const {
+      if (loc) return loc[base + node];
       const int64_t pos = pre + node;
-      return pos >= 0 && pos < rt_cols ? (int64_t)rt[pos] : -1;
-    };
-    if (free_slots)  // (before the table changes: the slots may be read from it)
-      for (int i = 0; i < n; ++i)
-        if (!((kept >> i) & 1)) free_slots[at++] = slot_of(i);
-    auto write = [&](int i, int64_t slot) {
-      const int64_t pos = pre + i;
-      if (pos >= 0 && pos < rt_cols) rt[pos] = (int32_t)slot;
-    };
-    const int left = __popcll(kept);
-    if (rises || out_cache_loc) {  // (rising: a position is written after every read at or before it)
-      of(b, n, c, [&](int i, int node) { write(i, slot_of(node)); });
-    } else {
-      int32_t slots[TREE_MAX];
-      of(b, n, c, [&](int i, int node) { slots[i] = (int32_t)slot_of(node); });
-      for (int i = 0; i < left; ++i) write(i, slots[i]);
+      return pos >= 0 && pos < cols ? (int64_t)rt[pos] : -1;
     }
-    if (seq_lens) {
-      if (seq_i64)
-        reinterpret_cast<int64_t*>(seq_lens)[row] = pre + left;
-      else
-        reinterpret_cast<int32_t*>(seq_lens)[row] = (int32_t)(pre + left);
+    __device__ __forceinline__ void write(int i, int64_t slot) const {
+      const int64_t pos = pre + i;
+      if (pos >= 0 && pos < cols) rt[pos] = (int32_t)slot;
+    }
+  };
+  auto window_of = [&](int b) {
+    const int64_t row = load_i(req_pool, req_i64, b), pre = load_i(prefix_lens, prefix_i64, b);
+    return Window{row, pre, slot_offsets ? slot_offsets[b] : (int64_t)b * T, rt_cols, req_to_token + row * rt_stride, out_cache_loc};
+  };
+  for (int step = 0; step < per; ++step) {
+    const int b = b0 + step;
+    int n = 0, c = 0;
+    bool rises = true;
+    if (b < b1) {
+      const uint64_t kept = of(b, n, c, rises);
+      const Window w = window_of(b);
+      if (free_slots)  // (before the table changes: the slots may be read from it)
+        for (int i = 0; i < n; ++i)
+          if (!((kept >> i) & 1)) free_slots[at++] = w.slot_of(i);
+      // kept nodes in ascending order: a position is written after every read at or before it
+      int i = 0;
+      if (rises)
+        for (uint64_t left = kept; left; left &= left - 1, ++i) w.write(i, w.slot_of(__ffsll((unsigned long long)left) - 1));
+      if (seq_lens) {
+        const int64_t len = w.pre + __popcll(kept);
+        if (seq_i64)
+          reinterpret_cast<int64_t*>(seq_lens)[w.row] = len;
+        else
+          reinterpret_cast<int32_t*>(seq_lens)[w.row] = (int32_t)len;
+      }
+    }
+    const int lane = tid & (WAVE - 1);
+    for (uint64_t odd = __ballot(!rises); odd; odd &= odd - 1) {
+      const int from = __ffsll((unsigned long long)odd) - 1, rb = readlane_at(b, from), rn = readlane_at(n, from),
+                rc = readlane_at(c, from);
+      const int node = lane < rc ? path[(int64_t)rb * T + lane] : -1;
+      bool take = node >= 0 && node < rn;
+      for (int j = 0; j < rc; ++j) {
+        const int other = readlane_at(node, j);
+        if (j < lane && other == node) take = false;
+      }
+      const Window w = window_of(rb);
+      const uint64_t taken = __ballot(take);
+      const int64_t slot = take ? w.slot_of(node) : 0;
+      __builtin_amdgcn_wave_barrier();  // (every lane's slot has been asked for before any position is written)
+      if (take) w.write(__popcll(taken & ((1ull << lane) - 1ull)), slot);
     }
   }
   if (tid == 0 && free_count) *free_count = total;
