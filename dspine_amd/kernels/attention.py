@@ -36,7 +36,8 @@ def tree_attention(q: torch.Tensor, cache: KVCache, *, T: int, page_table: torch
 
     The work is split over the positions, so a call needs scratch memory, which it allocates on the
     current stream (in a captured graph: in the graph's own pool) or takes from ``workspace``; two calls
-    that may run at once must not be given one workspace."""
+    that may run at once must not be given one workspace, and one whose buffer a captured graph uses must live as
+    long as the graph."""
     if q.ndim != 3 or q.dtype not in _ACT:
         raise ValueError("q must be bfloat16 or float16 [rows, q_heads, dim]")
     c = cache_fields(cache)

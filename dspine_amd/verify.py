@@ -47,16 +47,28 @@ def new_outputs(bs: int, T: int, device, kv_slots: bool = True):
 
 class Workspace:
     """Grow-only scratch owned by the caller (like TargetDistribution.scratch,
-    sampling/target.py:94-104)."""
+    sampling/target.py:94-104).  A captured graph keeps the address of the buffer its call was given, so
+    every buffer lives as long as the workspace: those that larger ones replaced, each at most half of
+    the next, together hold less than the last."""
 
     def __init__(self):
-        self.buf = None
+        self.buf = None  # the one given last
+        self.all = []
 
     def get(self, nbytes: int, device) -> torch.Tensor:
         if self.buf is None or self.buf.device != device or self.buf.numel() < nbytes:
-            size = max(nbytes, 2 * self.buf.numel() if self.buf is not None else 0)
-            self.buf = torch.empty(size, dtype=torch.uint8, device=device)
+            self.buf = self._larger(nbytes, device)
         return self.buf
+
+    def _larger(self, nbytes, device):
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        own = [b for b in self.all if b.device == device]
+        if not own or own[-1].numel() < nbytes:
+            own.append(torch.empty(max(nbytes, 2 * own[-1].numel() if own else 0), dtype=torch.uint8, device=device))
+            self.all.append(own[-1])
+        return own[-1]
 
 
 _default_ws: dict = {}
