@@ -153,7 +153,9 @@ extern "C" int dsv_tree_attention(const dsv_tree_attention_args* args, dsv_strea
   if ((uintptr_t)a.q % 16 || (uintptr_t)a.out % 16 || a.q_row_stride % 8 || a.q_head_stride % 8 ||
       a.out_row_stride % 8 || a.out_head_stride % 8)
     DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: rows of q and out must start on 16-byte boundaries");
-  if (!(a.scale >= -3.4e38f && a.scale <= 3.4e38f)) DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: scale must be finite");
+  // (times log2 e and the int8 codes' 512 it has to stay within float32)
+  if (!(a.scale >= -0x1p100f && a.scale <= 0x1p100f))
+    DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: scale must be finite, at most 2^100");
   const int64_t esize = quant ? 1 : 2;
   if (a.cache.k_slot_stride * esize > 0x7fffffff || a.cache.v_slot_stride * esize > 0x7fffffff)
     DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: slots are too far apart");

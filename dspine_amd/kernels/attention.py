@@ -69,8 +69,8 @@ def tree_attention(q: torch.Tensor, cache: KVCache, *, T: int, page_table: torch
     if page_table.stride(1) != 1 and page_table.shape[1] > 1:
         raise ValueError("page_table rows must be contiguous")
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
+    if not abs(scale) <= 2.0 ** 100:
+        raise ValueError("scale must be finite, at most 2^100")
     if out is None:
         out = torch.empty((rows, heads, dim), dtype=q.dtype, device=q.device)
     if out.shape != q.shape or out.dtype != q.dtype:

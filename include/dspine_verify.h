@@ -458,7 +458,7 @@ int dsv_kv_read(const dsv_kv_cache* cache, void* k, void* v, int32_t dtype, int6
 /* row = row_offsets[b] + i, else b * T + i.  It sees the positions p < prefix_lens[b] and, of the */
 /* window p = prefix_lens[b] + j, j < n_b, those whose bit j is set in masks[b, i] (int64          */
 /* [bs, T]; NULL: j <= i).  Position p lies in slot page_table[b, p]; positions past page_cols and */
-/* slots outside [0, num_slots) hold nothing.  s = scale * q.k, out = sum softmax(s) v             */
+/* slots outside [0, num_slots) hold nothing.  s = scale * q.k (|scale| <= 2^100), out = sum softmax(s) v             */
 /* [rows, q_heads, dim] of q's type, lse = log sum e^s (float32 [rows, q_heads], may be NULL); a   */
 /* node that sees nothing: 0 and -inf.  Rows of no node are left as they were.                     */
 typedef struct dsv_tree_attention_args {
