@@ -21,14 +21,14 @@
 // Only the device knows the lengths: every wave computes the same plan from them.  A request within one range is
 // finished there; the parts of the others are left as sums and joined by k_attn_join.
 //
-// Measured, both launches of a call (8 cache heads, dim 128; the card copies at 4.8 TB/s and multiplies at 1.36 PF):
-//   64 requests, 17 nodes, 4 query heads a cache head, bf16, 1k to 8k positions   270 us   4.4 TB/s: memory
-//   8 requests, 1 node, int8, 16k to 64k positions                                175 us   3.9 TB/s: memory, and 8 to 16 bits
-//   16 requests, 64 nodes, 8 query heads a cache head, e4m3, 4k to 12k            438 us   0.61 PF: a wave's own chain of LDS
-//       reads, products, exponentials and products (matrix pipe busy a quarter of the time, VALU a third)
+// Measured, a call among others (8 cache heads, dim 128; the card copies at 4.8 TB/s and multiplies at 1.36 PF):
+//   64 requests, 17 nodes, 4 query heads a cache head, bf16, 1k to 8k positions   271 us   4.4 TB/s: memory
+//   8 requests, 1 node, int8, 16k to 64k positions                                176 us   3.8 TB/s: memory, and 8 to 16 bits
+//   16 requests, 64 nodes, 8 query heads a cache head, e4m3, 4k to 12k            425 us   0.63 PF: a wave's own chain of LDS
+//       reads, products, exponentials and products (matrix pipe busy 25 % of the time, VALU 40 %)
 //   4 requests, 25 nodes, bf16, 1.5k to 4.7k                                       35 us   1.5 TB/s: latency (the plan, the
 //       first loads, the outputs and the second launch take longer than a workgroup's six tiles)
-//   1 request, 1 node, bf16, 640                                                   17 us   latency (8 + 5 us in two launches)
+//   1 request, 1 node, bf16, 640                                                   17 us   latency (8.4 + 4.9 us in two launches)
 #pragma once
 #include "dsv_cache.h"
 #include "dsv_common.h"
@@ -277,7 +277,13 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
   const int dim = FULL ? DP : c.dim;  // (a constant for the common sizes: no test of it in the loop)
   constexpr bool QUANT = CT == DSV_E4M3 || CT == DSV_I8, STAGED = FORM != AT_DIRECT;
   constexpr int WK = FORM == AT_DIRECT ? AT_WAVES : (FORM == AT_PAIRS ? 2 : 1);  // waves of the same rows
-  constexpr int PT = CT == DSV_BF16 ? DSV_BF16 : DSV_F16;  // the weights' type
+  // The weights' type in the second product: the values' own for 16-bit caches, float16 for the 8-bit codes (exact in it).  A
+  // weight (times its value scale) is rounded to it once, by 2^-9 (bfloat16) or 2^-12 at most.  The errors are random: over n
+  // positions of like weight they leave 1 / sqrt(n) of that.  Measured against float64, the output's own rounding included:
+  // bfloat16 caches 1.7e-3 to 2.3e-3 (with float32 weights 1.7e-3), 8-bit ones 1.7e-3 (1.7e-3), float16 ones 2.5e-4
+  // (2.1e-4).  Keeping the low half would take a second product of every value.  Sums, references, partial outputs and the
+  // join are float32.
+  constexpr int PT = CT == DSV_BF16 ? DSV_BF16 : DSV_F16;
   // float16 weights are held 2^11 higher, so that what their range loses lies below 2^-35 of the row's largest
   constexpr float SHIFT = PT == DSV_F16 ? 11.f : 0.f, LIM = PT == DSV_F16 ? 4.f : 8.f;
   constexpr int ESZ = QUANT ? 1 : 2;
@@ -992,8 +998,9 @@ struct AttnShape {
   int form, R, WR, RB;
   int waves;  // of a workgroup
 };
-// Waves a SIMD the kernels' registers are held to.
-// Waves a SIMD that the registers are for: 256 of them each, 512 where the sums of a wide dim need more.
+// Waves a SIMD that the registers are for: 256 of them each, 512 where the sums of a wide dim need more.  (Two row tiles of dim
+// 128 want more than 256: 6 to 8 are spilled for 8-bit caches, up to 20 where the dim is not known; none with 16-bit caches
+// of dim 128.)
 constexpr int attn_occupancy(int form, int R, int dim) {
   return dim > 128 && form != AT_ROWS ? 1 : 2;
 }

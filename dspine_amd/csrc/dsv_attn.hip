@@ -14,8 +14,8 @@ extern template void launch_attn<DSV_F16, DSV_I8>(const AttnParams&, const AttnS
 constexpr int AJ_THREADS = 256, AJ_PARTS = 4;
 
 // The parts of a request joined: 8 elements of a row a thread, the parts in their order.  Bound by latency (the plan's
-// lengths, then the parts: 4.7 us after one request's few parts, 7 to 8 us for most batches) and, for many rows, by the
-// sums' bytes (14 us for 16 requests of 512 rows a head).  A launch of its own: a last workgroup that joins would need
+// lengths, then the parts: 4.9 us after one request's few parts, 7 to 8 us for most batches) and, for many rows, by the
+// sums' bytes (14.6 us for 16 requests of 512 rows a head).  A launch of its own: a last workgroup that joins would need
 // counters that somebody clears.
 template <int XT, int DP>
 __global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
@@ -83,13 +83,14 @@ __global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
   if (d == 0 && a.lse) a.lse[row * a.q_heads + qh] = lt == 0.f ? -INFINITY : (top + log2f(lt)) * 0.693147180559945309f;
 }
 
-// The forms by rows a cache head (times are GPU times of a call, 8 cache heads of dim 128):
-//   up to 16: direct.  8 x 64k positions, int8: 184 us, 195 staged; bf16 at the same bytes: 253 and 249.
-//   17 to 32: staged, two waves for the same rows.  32 rows, 1 x 640 positions: 18.0 us, 19.3 with one wave for them
-//     and two that only bring; 16 x 2k to 8k: 87 and 88.
-//   up to 128: staged, a wave for each 16.  With 32 a wave: 305 us for 277 (68 rows), 44.6 for 40.2 (100 rows).
-//   more: staged, 32 a wave (half the LDS reads a product).  With 16: 570 us for 421 (512 rows, e4m3, one value scale
-//     for a wave's rows; 438 with one a row), 178 for 157 (132 rows, bf16).  Dims above 128 have no registers for it.
+// The forms by rows a cache head (times are of captured calls replayed over three inputs in turn, 8 cache heads of dim 128;
+// both sides of each line on one build and one card):
+//   up to 16: direct.  8 x 1 node, 16k to 64k positions, int8: 183 us, 204 staged; 64 x 4 nodes, 1k to 8k, bf16: 253 and 249.
+//   17 to 32: staged, two waves for the same rows.  32 rows, 1 x 640 positions: 18.1 us, 19.7 with one wave for them
+//     and two that only bring; 16 x 2k to 8k: 87 and 90.
+//   up to 128: staged, a wave for each 16.  With 32 a wave: 309 us for 278 (68 rows), 44.6 for 40.6 (100 rows).
+//   more: staged, 32 a wave (half the LDS reads a product).  With 16: 558 us for 432 (512 rows, e4m3), 180 for 157
+//     (132 rows, bf16).  Dims above 128 have no registers for it.
 static AttnShape attn_shape(int T, int G, int dim) {
   const int tiles = (T * G + 15) / 16;
   AttnShape s;
@@ -167,8 +168,9 @@ extern "C" int dsv_tree_attention(const dsv_tree_attention_args* args, dsv_strea
   P.WR = s.WR;
   P.RB = s.RB;
   P.most = attn_ranges(s, a.cache.heads, a.cache.dim);
-  // A part of a request costs its start and its sums, so a range has a few tiles at least (twice and half of these:
-  // 18.2 and 18.9 us for 17.0 direct, 43.4 and 43.5 for 37.9 staged).
+  // A part of a request costs its start and its sums, so a range has a few tiles at least (twice and half of these, replayed
+  // as above: 18.5 and 19.3 us for 17.2 direct, 1 x 640; 44.0 and 43.9 for 38.3 staged, 13 x 23 nodes; 41.6 and 40.5 for
+  // 40.6, 4 x 25 nodes).
   P.least = fast_div(s.form == AT_ROWS ? 4 : 2);
   const int64_t blocks = (P.most + 7) / 8 * 8 * (int64_t)a.cache.heads * s.RB;
   const int64_t wide = a.cache.dim <= 64 ? 64 : (a.cache.dim <= 128 ? 128 : 256), per = AJ_THREADS / (wide / 8);

@@ -55,7 +55,7 @@ __device__ __forceinline__ KvRow kv_row(const KvParams& P, int u) {
 // Codes of a quantised row: a = the row's largest magnitude, scale = a * (1 / top), code = rne(x * ((1 / a) * top)).
 // The magnitudes are compared as the type's own 15 bits, which order like the values and keep a NaN or an infinity
 // on top.  Bound by memory: each activation is read once, each code and scale written once (16384 tokens of 8 heads of
-// 128 into int8: 22.6 us, 4.5 TB/s; 8 values a lane and one row a group: 34 us).  A few tokens: 3.3 us, latency.
+// 128 into int8: 22.9 us, 4.5 TB/s; 8 values a lane and one row a group: 34 us).  A few tokens: 3.2 us, latency.
 template <int XT, int CT>
 __global__ __launch_bounds__(KV_THREADS) void k_kv_write(KvParams P) {
   constexpr int EL = kv_lane<CT>(), V = EL / 8;
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(KV_THREADS) void k_kv_write(KvParams P) {
 }
 
 // The values of the slots' rows, code * scale in float32, rounded once to the output's type.  Bound by memory (50000
-// slots of 8 heads of 128, int8 to bf16: 68 us, 4.6 TB/s; 8 values a lane and one row a group: 109 us).
+// slots of 8 heads of 128, int8 to bf16: 69 us, 4.5 TB/s; 8 values a lane and one row a group: 109 us).
 template <int CT, int XT>
 __global__ __launch_bounds__(KV_THREADS) void k_kv_read(KvParams P) {
   constexpr bool QUANT = CT == DSV_E4M3 || CT == DSV_I8;
