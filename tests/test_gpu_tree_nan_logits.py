@@ -11,7 +11,8 @@ pytestmark = pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("V", [5, 23, 4099, 40003])
 @pytest.mark.parametrize("shift", [0, 1, 3])
-def test_nan_is_the_lowest(device, shift, V, dtype):
+@pytest.mark.parametrize("signalling", [False, True])
+def test_nan_is_the_lowest(device, signalling, shift, V, dtype):
     from dspine_amd.verification.tree import accept_greedy_tree
 
     bs, g = 12, torch.Generator().manual_seed(V)
@@ -33,8 +34,12 @@ def test_nan_is_the_lowest(device, shift, V, dtype):
     want = torch.stack([row.eq(row.max()).nonzero()[0, 0] for row in want])
     wide = torch.zeros(bs, V + 7)  # (rows begin anywhere)
     wide[:, shift: shift + V] = logits
+    wide = wide.to(dtype)
+    if signalling:
+        raw = torch.int16 if dtype == torch.bfloat16 else torch.int32
+        wide.view(raw)[torch.isnan(wide)] = {torch.int16: 0x7F81, torch.int32: 0x7F800001}[raw]
     outs, _ = accept_greedy_tree(candidates=torch.zeros(bs, 1, dtype=torch.int64, device=device),
                                  parents=torch.full((bs, 1), -1, dtype=torch.int32, device=device),
-                                 next_token_logits=wide.to(dtype).to(device)[:, shift: shift + V],
+                                 next_token_logits=wide.to(device)[:, shift: shift + V],
                                  prefix_lens=torch.zeros(bs, dtype=torch.int32, device=device))
     assert outs[2].tolist() == want.tolist()

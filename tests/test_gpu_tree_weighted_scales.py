@@ -49,7 +49,7 @@ def _reference(d):
 def _lower(d, positions, down, power):
     """Scores of request 0's ``positions`` about ``down`` below the others', their value scales 2^power above."""
     k, v, ks, vs = d["cache"]
-    d["q"][..., 0] = 8.0  # over sqrt(64): a key's first element adds itself to the score
+    d["q"][..., 0] = round(math.sqrt(k.shape[2]))  # a key's first element adds (about) itself to the score
     at = d["page_table"][0].long()[positions]
     k[at] = torch.zeros_like(k[at])
     k[at, :, 0] = torch.full(k[at, :, 0].shape, -R.TOP[k.dtype]).to(k.dtype)
@@ -65,6 +65,18 @@ def test_a_large_scale_without_weight(device, place, power, T, G, dtype):
     """Weights of e^-60 (2^-87): up to scales 2^80 apart those positions hardly count, at 2^100 they are the output."""
     d = _round(51, bs=2, T=T, H=2, G=G, D=64, act=BF, dtype=dtype, lens=[700, 90], tree=True)
     _lower(d, {"first": [0], "inside": [333], "last": [699], "every": list(range(5, 700, 9))}[place], 60.0, power)
+    out, lse = _call(d, device)
+    want, wl, otol, ltol = _reference(d)
+    R.close(out.cpu(), want, otol)
+    R.close(lse.cpu(), wl, ltol)
+
+
+@pytest.mark.parametrize("dtype", [E4, I8])
+@pytest.mark.parametrize("T, G", FORMS)
+@pytest.mark.parametrize("D", [96, 128, 192, 256])
+def test_a_large_scale_without_weight_at_other_dims(device, D, T, G, dtype):
+    d = _round(57, bs=2, T=T, H=1, G=G, D=D, act=BF, dtype=dtype, lens=[400, 90], tree=True)
+    _lower(d, list(range(5, 400, 9)), 60.0, 36)
     out, lse = _call(d, device)
     want, wl, otol, ltol = _reference(d)
     R.close(out.cpu(), want, otol)
