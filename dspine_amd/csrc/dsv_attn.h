@@ -55,7 +55,7 @@ struct AttnParams {
   FastDiv least;       // tiles of a range at least (a batch of fewer is one range)
   uint32_t num_slots, k_step, v_step;  // slots; bytes from slot to slot
   float* part_o;       // [2 * range + (the range's last request, not its first)][head][row][dim]
-  float4* part_ml;     // the same of [row]: reference of the scores, sum of the weights, reference of the weighted values
+  float4* part_ml;     // the same of [row]: reference of the scores, sum of the weights, reference of the weighted values less the first
 };
 
 // The request's nodes, its context and its positions (context and window) that the page table has.
@@ -374,17 +374,16 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
   // With value scales the row has two references, both powers of two that only move up: m of its scores, 2^4 at most below
   // any, for the sum l of the weights, and `mref` of weight times scale, for the float16 operands: those of the positions that
   // count lie within [2^10, 2^15] at their largest, whatever scales positions without weight have.  A score is taken against
-  // mref, and mref - m = vlog (vtop = 2^vlog) is put back into l.  -120 <= vlog, so that the weights stay within float32, and
+  // mref, and mref - m = vlog is put back into l.  -120 <= vlog, so that the weights stay within float32, and
   // vlog <= 117 for any finite scale: weights down to 2^-32 of the row's largest are then float32 numbers, subnormal ones
   // at the far end, and count in l.
-  float vlog[R], vtop[R];
+  float vlog[R];
   bool fresh = true;  // some row has no reference yet
 #pragma unroll
   for (int rt = 0; rt < R; ++rt) {
     mref[rt] = AT_LOW;
     l[rt] = 0.f;
     vlog[rt] = 0.f;
-    vtop[rt] = 1.f;
 #pragma unroll
     for (int e = 0; e < EPL; ++e) o[rt][e] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -555,34 +554,39 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
         for (int j = 0; j < 8; ++j) top = fmaxf(top, s[rt][j / 4][j & 3]);
         top = across_groups_max(top);
         const bool unset = mref[rt] == AT_LOW;
-        float move, keep_l;  // of the reference: up, or anywhere from none
+        // The reference moves up (or anywhere from none).  Where it is so large that float32 rounds it, the step's own scores still
+        // move by what was meant: nothing leaves float16's range.
+        float move;
         if constexpr (QUANT) {
+          // the scores' reference relative to the present one of the weighted values, then the new one of those relative to it
+          const bool any = top != AT_LOW;
+          const float old = unset ? 0.f : -vlog[rt], low = !any ? old : (unset ? ceilf(top) : fmaxf(old, ceilf(top)));
           float high = -INFINITY;  // weight times scale
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const float v = fabsf(vs[j]);
-            high = fmaxf(high, s[rt][j / 4][j & 3] + (v < INFINITY ? __builtin_amdgcn_logf(v) : -INFINITY));
+            high = fmaxf(high, s[rt][j / 4][j & 3] - low + (v < INFINITY ? __builtin_amdgcn_logf(v) : -INFINITY));
           }
           high = across_groups_max(high);
-          const bool any = top != AT_LOW;
-          const float old = -vlog[rt], low = !any ? old : (unset ? ceilf(top) : fmaxf(old, ceilf(top)));  // the scores'
-          move = fmaxf(ceilf(high) - SHIFT, low - 120.f);
-          if (!any || (!unset && move < 0.f)) move = 0.f;
-          keep_l = unset ? 0.f : __builtin_amdgcn_exp2f(old - low);
-          if (any) vlog[rt] = move - low;
-          vtop[rt] = __builtin_amdgcn_exp2f(vlog[rt]);
+          const float up = any ? fmaxf(fmaxf(ceilf(high) - SHIFT, -120.f), unset ? -120.f : -low) : -low;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s[rt][j / 4][j & 3] = s[rt][j / 4][j & 3] - low - up;
+          l[rt] *= unset ? 0.f : __builtin_amdgcn_exp2f(old - low);
+          vlog[rt] = up;
+          move = low + up;
         } else {
           move = top - SHIFT;
+          if (top - move > SHIFT + LIM) move = top;
           if (top == AT_LOW || (!unset && move < 0.f)) move = 0.f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) s[rt][j / 4][j & 3] -= move;
         }
         if (top != AT_LOW || !unset) mref[rt] = (unset ? 0.f : mref[rt]) + move;
         none |= mref[rt] == AT_LOW;
         const float keep = unset ? 0.f : __builtin_amdgcn_exp2f(-move);
-        l[rt] *= QUANT ? keep_l : keep;
+        if constexpr (!QUANT) l[rt] *= keep;
 #pragma unroll
         for (int e = 0; e < EPL; ++e) o[rt][e] *= keep;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[rt][j / 4][j & 3] -= move;
       }
       fresh = __any(none);
     }
@@ -604,7 +608,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
         }
         pf[rt][j / 2] = pack_act<PT>(w[0], w[1]);
       }
-      l[rt] = QUANT ? fmaf(sum, vtop[rt], l[rt]) : sum;
+      l[rt] = QUANT ? fmaf(sum, __builtin_amdgcn_exp2f(vlog[rt]), l[rt]) : sum;
     }
 #pragma unroll
     for (int e0 = 0; e0 < EPL; e0 += GRP) {
@@ -909,21 +913,29 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
   for (int rt = 0; rt < R; ++rt) {
     l[rt] = across_groups_sum(l[rt]);
     if (g == 0) {
-      s_r[wave][rt * 16 + m] = mref[rt];
       s_m[wave][rt * 16 + m] = QUANT && mref[rt] != AT_LOW ? mref[rt] - vlog[rt] : mref[rt];
+      s_r[wave][rt * 16 + m] = vlog[rt];
       s_l[wave][rt * 16 + m] = l[rt];
     }
   }
   __syncthreads();
   constexpr float unit = CT == DSV_I8 ? I8_UNIT : 1.f;
+  // the waves' common reference of the weighted values, relative to that of the scores, `top`
+  auto lifted = [&](int wr, int r, float top) {
+    float ref = AT_LOW;
+    for (int k = 0; k < WK; ++k) ref = fmaxf(ref, s_m[wr * WK + k][r] - top + s_r[wr * WK + k][r]);
+    return ref;
+  };
   // the positions whose values were set aside where they are not finite
   const int aside0 = clear / SET_ASIDE * SET_ASIDE > t0 * AT_TILE ? clear / SET_ASIDE * SET_ASIDE : t0 * AT_TILE;
   const int aside1 = t1 * AT_TILE < req.total ? t1 * AT_TILE : req.total;
 #pragma unroll
   for (int rt = 0; rt < R; ++rt) {
     float top = AT_LOW;
-    for (int k = 0; k < WK; ++k) top = fmaxf(top, s_r[wr * WK + k][rt * 16 + m]);
-    const float f = __builtin_amdgcn_exp2f(mref[rt] - top) * unit;
+    for (int k = 0; k < WK; ++k) top = fmaxf(top, s_m[wr * WK + k][rt * 16 + m]);
+    float less = s_m[wave][rt * 16 + m] - top;
+    if constexpr (QUANT) less = less + vlog[rt] - lifted(wr, rt * 16 + m, top);
+    const float f = __builtin_amdgcn_exp2f(less) * unit;
     if (rt) __syncthreads();
 #pragma unroll
     for (int r = 0; r < 4; ++r)
@@ -936,11 +948,9 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       const int rr = i / (DP / 8), d = i % (DP / 8) * 8, r = row0 + rt * 16 + rr;
       if (r >= n_rows || d >= dim) continue;
       float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      float mt = AT_LOW, lt = 0.f, ref = AT_LOW;
-      for (int k = 0; k < WK; ++k) {
-        mt = fmaxf(mt, s_m[wr * WK + k][rt * 16 + rr]);
-        ref = fmaxf(ref, s_r[wr * WK + k][rt * 16 + rr]);
-      }
+      float mt = AT_LOW, lt = 0.f;
+      for (int k = 0; k < WK; ++k) mt = fmaxf(mt, s_m[wr * WK + k][rt * 16 + rr]);
+      const float ref = QUANT ? lifted(wr, rt * 16 + rr, mt) : 0.f;
       for (int k = 0; k < WK; ++k) {
         lt += s_l[wr * WK + k][rt * 16 + rr] * __builtin_amdgcn_exp2f(s_m[wr * WK + k][rt * 16 + rr] - mt);
 #pragma unroll
@@ -972,7 +982,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
         if (row < 0) continue;
         const float inv = lt == 0.f ? 0.f : 1.f / lt;
         if constexpr (QUANT) {  // (two steps: either factor alone may leave float32 where the product does not)
-          const float up = __builtin_amdgcn_exp2f(ref - mt);
+          const float up = __builtin_amdgcn_exp2f(ref);
 #pragma unroll
           for (int u = 0; u < 8; ++u) sum[u] = sum[u] * inv * up;
         } else {

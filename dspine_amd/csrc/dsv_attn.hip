@@ -40,7 +40,7 @@ __global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
   auto part = [&](int i) {
     return ((int64_t)(2 * i + (i == i0 && plan.start(i) < before ? 1 : 0)) * c.heads + h) * rows + r;
   };
-  float top = AT_LOW, ref = AT_LOW, lt = 0.f, sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  float top = AT_LOW, ref = 0.f, lt = 0.f, sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int i = i0; i <= i1; i += AJ_PARTS) {  // (the references and the sums of a few parts are asked for at once)
     float4 ml[AJ_PARTS];
     f32x4 x[AJ_PARTS][2];
@@ -51,12 +51,14 @@ __global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
       x[j][0] = *reinterpret_cast<const f32x4*>(P.part_o + at * c.dim + d);
       x[j][1] = *reinterpret_cast<const f32x4*>(P.part_o + at * c.dim + d + 4);
     }
-    const float old = top, old_ref = ref;
+    const float old = top;
 #pragma unroll
-    for (int j = 0; j < AJ_PARTS; ++j) {  // (the last part again, where there are fewer)
-      top = fmaxf(top, ml[j].x);
-      ref = fmaxf(ref, ml[j].z);
-    }
+    for (int j = 0; j < AJ_PARTS; ++j) top = fmaxf(top, ml[j].x);  // (the last part again, where there are fewer)
+    // (the weighted values' reference is kept relative to the scores': the difference is small where both are large)
+    const float old_ref = ref + (old - top);
+    ref = old_ref;
+#pragma unroll
+    for (int j = 0; j < AJ_PARTS; ++j) ref = fmaxf(ref, ml[j].x - top + ml[j].z);
     const float keep = __builtin_amdgcn_exp2f(old_ref - ref);
     lt *= __builtin_amdgcn_exp2f(old - top);
 #pragma unroll
@@ -64,14 +66,14 @@ __global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
 #pragma unroll
     for (int j = 0; j < AJ_PARTS; ++j) {
       if (i + j > i1) break;
-      const float f = __builtin_amdgcn_exp2f(ml[j].z - ref);
+      const float f = __builtin_amdgcn_exp2f(ml[j].x - top + ml[j].z - ref);
       lt = fmaf(ml[j].y, __builtin_amdgcn_exp2f(ml[j].x - top), lt);
 #pragma unroll
       for (int u = 0; u < 8; ++u) sum[u] = fmaf(x[j][u / 4][u & 3], f, sum[u]);
     }
   }
   // (two steps: either factor alone may leave float32 where the product does not)
-  const float inv = lt == 0.f ? 0.f : 1.f / lt, up = __builtin_amdgcn_exp2f(ref - top);
+  const float inv = lt == 0.f ? 0.f : 1.f / lt, up = __builtin_amdgcn_exp2f(ref);
 #pragma unroll
   for (int u = 0; u < 8; ++u) sum[u] = sum[u] * inv * up;
   uint4 v;
