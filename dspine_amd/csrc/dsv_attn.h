@@ -22,13 +22,13 @@
 // finished there; the parts of the others are left as sums and joined by k_attn_join.
 //
 // Measured, a call among others (8 cache heads, dim 128; the card copies at 4.8 TB/s and multiplies at 1.36 PF):
-//   64 requests, 17 nodes, 4 query heads a cache head, bf16, 1k to 8k positions   271 us   4.4 TB/s: memory
-//   8 requests, 1 node, int8, 16k to 64k positions                                176 us   3.8 TB/s: memory, and 8 to 16 bits
-//   16 requests, 64 nodes, 8 query heads a cache head, e4m3, 4k to 12k            425 us   0.63 PF: a wave's own chain of LDS
+//   64 requests, 17 nodes, 4 query heads a cache head, bf16, 1k to 8k positions   268 us   4.5 TB/s: memory
+//   8 requests, 1 node, int8, 16k to 64k positions                                175 us   3.9 TB/s: memory, and 8 to 16 bits
+//   16 requests, 64 nodes, 8 query heads a cache head, e4m3, 4k to 12k            430 us   0.62 PF: a wave's own chain of LDS
 //       reads, products, exponentials and products (matrix pipe busy 25 % of the time, VALU 40 %)
-//   4 requests, 25 nodes, bf16, 1.5k to 4.7k                                       35 us   1.5 TB/s: latency (the plan, the
+//   4 requests, 25 nodes, bf16, 1.5k to 4.7k                                       36 us   1.5 TB/s: latency (the plan, the
 //       first loads, the outputs and the second launch take longer than a workgroup's six tiles)
-//   1 request, 1 node, bf16, 640                                                   17 us   latency (8.4 + 4.9 us in two launches)
+//   1 request, 1 node, bf16, 640                                                   17 us   latency (8.6 + 5.1 us in two launches)
 #pragma once
 #include "dsv_cache.h"
 #include "dsv_common.h"
@@ -1009,8 +1009,7 @@ struct AttnShape {
   int waves;  // of a workgroup
 };
 // Waves a SIMD that the registers are for: 256 of them each, 512 where the sums of a wide dim need more.  (Two row tiles of dim
-// 128 want more than 256: 6 to 8 are spilled for 8-bit caches, up to 20 where the dim is not known; none with 16-bit caches
-// of dim 128.)
+// 128 want more than 256: 8 to 10 are spilled for 8-bit caches, none for 16-bit ones; up to 24 where the dim is not known.)
 constexpr int attn_occupancy(int form, int R, int dim) {
   return dim > 128 && form != AT_ROWS ? 1 : 2;
 }

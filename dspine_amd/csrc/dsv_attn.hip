@@ -14,8 +14,8 @@ extern template void launch_attn<DSV_F16, DSV_I8>(const AttnParams&, const AttnS
 constexpr int AJ_THREADS = 256, AJ_PARTS = 4;
 
 // The parts of a request joined: 8 elements of a row a thread, the parts in their order.  Bound by latency (the plan's
-// lengths, then the parts: 4.9 us after one request's few parts, 7 to 8 us for most batches) and, for many rows, by the
-// sums' bytes (14.6 us for 16 requests of 512 rows a head).  A launch of its own: a last workgroup that joins would need
+// lengths, then the parts: 5.1 us after one request's few parts, 7 to 8 us for most batches) and, for many rows, by the
+// sums' bytes (14.3 us for 16 requests of 512 rows a head).  A launch of its own: a last workgroup that joins would need
 // counters that somebody clears.
 template <int XT, int DP>
 __global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
@@ -91,7 +91,7 @@ __global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
 //   17 to 32: staged, two waves for the same rows.  32 rows, 1 x 640 positions: 18.1 us, 19.7 with one wave for them
 //     and two that only bring; 16 x 2k to 8k: 87 and 90.
 //   up to 128: staged, a wave for each 16.  With 32 a wave: 309 us for 278 (68 rows), 44.6 for 40.6 (100 rows).
-//   more: staged, 32 a wave (half the LDS reads a product).  With 16: 558 us for 432 (512 rows, e4m3), 180 for 157
+//   more: staged, 32 a wave (half the LDS reads a product).  With 16: 559 us for 437 (512 rows, e4m3), 179 for 157
 //     (132 rows, bf16).  Dims above 128 have no registers for it.
 static AttnShape attn_shape(int T, int G, int dim) {
   const int tiles = (T * G + 15) / 16;
