@@ -55,7 +55,7 @@ struct AttnParams {
   FastDiv least;       // tiles of a range at least (a batch of fewer is one range)
   uint32_t num_slots, k_step, v_step;  // slots; bytes from slot to slot
   float* part_o;       // [2 * range + (the range's last request, not its first)][head][row][dim]
-  float4* part_ml;     // the same of [row]: reference of the scores, sum of the weights, reference of the weighted values less the first
+  float4* part_ml;     // the same of [row]: the scores' reference, the weights' sum, the weighted values' reference less the first
 };
 
 // The request's nodes, its context and its positions (context and window) that the page table has.
@@ -374,7 +374,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
   // With value scales the row has two references, both powers of two that only move up: m of its scores, 2^4 at most below
   // any, for the sum l of the weights, and `mref` of weight times scale, for the float16 operands: those of the positions that
   // count lie within [2^10, 2^15] at their largest, whatever scales positions without weight have.  A score is taken against
-  // mref, and mref - m = vlog is put back into l.  -120 <= vlog, so that the weights stay within float32, and
+  // mref, and the difference vlog = mref - m goes back into l.  -120 <= vlog, so that the weights stay within float32, and
   // vlog <= 117 for any finite scale: weights down to 2^-32 of the row's largest are then float32 numbers, subnormal ones
   // at the far end, and count in l.
   float vlog[R];
