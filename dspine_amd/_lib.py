@@ -31,6 +31,9 @@ EXPORTS = (
     "dsv_factor_gemm", "dsv_filter_probs", "dsv_filter_workspace_bytes",
     "dsv_kv_write", "dsv_kv_read", "dsv_tree_attention", "dsv_tree_attention_workspace_bytes",
     "dsv_tree_masks", "dsv_tree_verify", "dsv_tree_verify_workspace_bytes", "dsv_commit_tree",
+    "dsv_index_blocks", "dsv_score_blocks", "dsv_select_blocks", "dsv_block_attention",
+    "dsv_copy_slots", "dsv_fork_requests", "dsv_free_requests", "dsv_free_requests_workspace_bytes",
+    "dsv_compact_requests", "dsv_compact_requests_workspace_bytes",
 )
 DSV_ADJ_ADD, DSV_ADJ_SCALE = 0, 1
 
@@ -118,6 +121,35 @@ class TreeAttentionArgs(ctypes.Structure):
         ("page_table", vp), ("page_stride", i64), ("page_cols", i64),
         ("workspace", vp), ("workspace_bytes", i64),
     ]
+
+
+class BlockIndexC(ctypes.Structure):
+    """Mirror of ``dsv_block_index``."""
+
+    _fields_ = [("bounds", vp), ("dtype", i32), ("heads", i32), ("dim", i32), ("block_size", i32), ("rows", i64)]
+
+
+class ScoreBlocksArgs(ctypes.Structure):
+    """Mirror of ``dsv_score_blocks_args``."""
+
+    _fields_ = [
+        ("index", BlockIndexC), ("q", vp), ("scores", vp), ("q_heads", i32), ("pad0", i32),
+        ("rows", i64), ("q_row_stride", i64), ("q_head_stride", i64), ("bs", i32), ("T", i32),
+        ("prefix_lens", vp), ("verify_lens", vp), ("row_offsets", vp), ("row_offsets_i64", i32), ("scale", _c.c_float),
+        ("block_table", vp), ("block_stride", i64), ("block_cols", i64),
+    ]
+
+
+class BlockAttentionArgs(ctypes.Structure):
+    """Mirror of ``dsv_block_attention_args``."""
+
+    _fields_ = [("tree", TreeAttentionArgs), ("blocks", vp), ("count", i32), ("block_size", i32)]
+
+
+class SlotRows(ctypes.Structure):
+    """Mirror of ``dsv_slot_rows``."""
+
+    _fields_ = [("base", vp), ("slot_stride", i64), ("head_stride", i64), ("heads", i32), ("bytes", i32)]
 
 
 _lock = threading.Lock()
@@ -211,6 +243,28 @@ def load():
         lib.dsv_commit_tree.restype = i32
         lib.dsv_commit_tree.argtypes = [i32, i32, vp, vp, vp, vp, i32, vp, i32, vp, i64, i64, vp, vp, vp, i32, vp, vp,
                                         vp]
+        lib.dsv_index_blocks.restype = i32
+        lib.dsv_index_blocks.argtypes = [ctypes.POINTER(BlockIndexC), ctypes.POINTER(KvCache), vp, i64, i64, vp, i64, i64,
+                                         vp, vp, i32, i64, vp]
+        lib.dsv_score_blocks.restype = i32
+        lib.dsv_score_blocks.argtypes = [ctypes.POINTER(ScoreBlocksArgs), vp]
+        lib.dsv_select_blocks.restype = i32
+        lib.dsv_select_blocks.argtypes = [vp, i32, i32, i64, vp, i32, i32, i32, i32, vp, vp]
+        lib.dsv_block_attention.restype = i32
+        lib.dsv_block_attention.argtypes = [ctypes.POINTER(BlockAttentionArgs), vp]
+        lib.dsv_copy_slots.restype = i32
+        lib.dsv_copy_slots.argtypes = [ctypes.POINTER(SlotRows), i32, i64, vp, i32, vp, i32, i64, vp, vp]
+        lib.dsv_fork_requests.restype = i32
+        lib.dsv_fork_requests.argtypes = [vp, i64, i64, i64, vp, i32, vp, i64, vp, vp, i32, i64, vp]
+        lib.dsv_free_requests_workspace_bytes.restype = i64
+        lib.dsv_free_requests_workspace_bytes.argtypes = [i64]
+        lib.dsv_free_requests.restype = i32
+        lib.dsv_free_requests.argtypes = [vp, i64, i64, i64, vp, i32, vp, i64, vp, i32, i64, vp, i64, vp, vp, i64, vp]
+        lib.dsv_compact_requests_workspace_bytes.restype = i64
+        lib.dsv_compact_requests_workspace_bytes.argtypes = [i64]
+        lib.dsv_compact_requests.restype = i32
+        lib.dsv_compact_requests.argtypes = [vp, i64, i64, i64, vp, i32, vp, i64, vp, i32, i64,
+                                             ctypes.POINTER(SlotRows), i32, vp, vp, i64, vp, vp, i64, vp]
         lib.dsv_factor_workspace_doubles.restype = i64
         lib.dsv_factor_workspace_doubles.argtypes = [i64, i32, i32, i32]
         lib.dsv_factor_table.restype = i32

@@ -56,17 +56,43 @@ struct AttnParams {
   uint32_t num_slots, k_step, v_step;  // slots; bytes from slot to slot
   float* part_o;       // [2 * range + (the range's last request, not its first)][head][row][dim]
   float4* part_ml;     // the same of [row]: the scores' reference, the weights' sum, the weighted values' reference less the first
+  // (attention over selected blocks)
+  const int32_t* blocks;  // [request][cache head][count]
+  int count, shift;       // blocks of 2^shift positions
 };
 
-// The request's nodes, its context and its positions (context and window) that the page table has.
+// The request's nodes, its context and its positions (context and window) that the page table has.  BLOCKS: its positions
+// are numbered as they are read, those of the selected blocks, then those of the unfinished block and the window.
 struct Request {
   int nodes;
   int prefix, total;  // within the table
 };
-__device__ __forceinline__ Request request_of(const dsv_tree_attention_args& a, int64_t b) {
+// (so far from the largest int that a window behind it stays below)
+__device__ __forceinline__ int context_of(const dsv_tree_attention_args& a, int64_t b) {
+  const int pre = a.prefix_lens[b];
+  return pre < 0 ? 0 : (pre > 0x7fffff00 ? 0x7fffff00 : pre);
+}
+// A request's finished blocks, and how many entries of its lists are read.
+struct Finished {
+  int full, read;
+};
+__device__ __forceinline__ Finished finished_of(const AttnParams& P, int64_t b) {
+  Finished f;
+  f.full = context_of(P.a, b) >> P.shift;
+  f.read = f.full < P.count ? f.full : P.count;
+  return f;
+}
+template <bool BLOCKS>
+__device__ __forceinline__ Request request_of(const AttnParams& P, int64_t b) {
+  const dsv_tree_attention_args& a = P.a;
   Request r;
   int n = a.verify_lens ? a.verify_lens[b] : a.T;
   r.nodes = n < 0 ? 0 : (n > a.T ? a.T : n);
+  if constexpr (BLOCKS) {
+    r.prefix = (finished_of(P, b).read << P.shift) + (context_of(a, b) & ((1 << P.shift) - 1));
+    r.total = r.prefix + r.nodes;
+    return r;
+  }
   const int pre = a.prefix_lens[b];
   const int64_t from = pre < 0 ? 0 : pre, to = from + r.nodes;
   r.prefix = (int)(from < a.page_cols ? from : a.page_cols);
@@ -94,6 +120,7 @@ struct Plan {
                        : more + (int)((uint32_t)(tile - wide) / (uint32_t)(size < 1 ? 1 : size));
   }
 };
+template <bool BLOCKS>
 __device__ __forceinline__ Plan plan_of(const AttnParams& P, int lane) {
   Plan p;
   p.small = P.a.bs <= WAVE;
@@ -102,12 +129,12 @@ __device__ __forceinline__ Plan plan_of(const AttnParams& P, int lane) {
   int sum = 0;
   if (p.small) {
     if (lane < P.a.bs) {
-      p.mine = request_of(P.a, lane);
+      p.mine = request_of<BLOCKS>(P, lane);
       p.tiles = tiles_of(p.mine);
     }
     sum = p.tiles;
   } else {
-    for (int b = lane; b < P.a.bs; b += WAVE) sum += tiles_of(request_of(P.a, b));
+    for (int b = lane; b < P.a.bs; b += WAVE) sum += tiles_of(request_of<BLOCKS>(P, b));
   }
   p.total = wave_sum(sum);
   const int r = (int)P.least.div((uint32_t)p.total + P.least.d - 1);
@@ -117,25 +144,28 @@ __device__ __forceinline__ Plan plan_of(const AttnParams& P, int lane) {
   return p;
 }
 // Request b (the same in every lane).
+template <bool BLOCKS>
 __device__ __forceinline__ Request request_in(const AttnParams& P, const Plan& p, int b) {
-  if (!p.small) return request_of(P.a, b);
+  if (!p.small) return request_of<BLOCKS>(P, b);
   return Request{readlane_at(p.mine.nodes, b), readlane_at(p.mine.prefix, b), readlane_at(p.mine.total, b)};
 }
 // Tiles of the requests before b.
+template <bool BLOCKS>
 __device__ __forceinline__ int tiles_before(const AttnParams& P, const Plan& p, int b, int lane) {
   int sum = 0;
   if (p.small)
     sum = lane < b ? p.tiles : 0;
   else
-    for (int i = lane; i < b; i += WAVE) sum += tiles_of(request_of(P.a, i));
+    for (int i = lane; i < b; i += WAVE) sum += tiles_of(request_of<BLOCKS>(P, i));
   return wave_sum(sum);
 }
 // The request of a tile (tile < total) and the tiles before it; -1 if there is none (lengths that change under the call).
+template <bool BLOCKS>
 __device__ __forceinline__ int request_at(const AttnParams& P, const Plan& p, int tile, int lane, int& before) {
   before = 0;
   for (int b0 = 0; b0 < P.a.bs; b0 += WAVE) {
     const int i = b0 + lane;
-    const int n = p.small ? p.tiles : (i < P.a.bs ? tiles_of(request_of(P.a, i)) : 0);
+    const int n = p.small ? p.tiles : (i < P.a.bs ? tiles_of(request_of<BLOCKS>(P, i)) : 0);
     const int end = before + wave_incl_scan(n);
     const uint64_t past = __ballot(end > tile);
     if (past) {
@@ -270,7 +300,7 @@ enum { AT_DIRECT = 0, AT_PAIRS = 1, AT_ROWS = 2 };
 constexpr int AT_TILES(int FORM, int R) { return FORM == 2 && R == 2 ? 2 : 1; }
 constexpr int AT_DEPTH(int R, int DP) { return R == 1 && DP <= 128 ? 2 : 1; }
 
-template <int XT, int CT, int DP, bool FULL, int R, int FORM, int WAVES, int OCC>
+template <int XT, int CT, int DP, bool FULL, int R, int FORM, int WAVES, int OCC, bool BLOCKS>
 __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
   const dsv_tree_attention_args& a = P.a;
   const dsv_kv_cache& c = a.cache;
@@ -311,16 +341,16 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
   const int HB = c.heads * P.RB;
   const int inner = (int)((blockIdx.x / 8) % HB), range = (int)((blockIdx.x / 8) / HB) * 8 + (int)(blockIdx.x % 8);
   const int h = inner / P.RB, rb = inner - h * P.RB;
-  const Plan plan = plan_of(P, lane);
+  const Plan plan = plan_of<BLOCKS>(P, lane);
   if (range >= plan.ranges || plan.total == 0) return;
   const int wr = wave / WK, wk = wave - wr * WK;
   const int block0 = rb * 16 * R * P.WR, row0 = block0 + wr * 16 * R;
   int tile = plan.start(range), before;
   const int stop = plan.start(range + 1);
-  int b = __builtin_amdgcn_readfirstlane(request_at(P, plan, tile, lane, before));
+  int b = __builtin_amdgcn_readfirstlane(request_at<BLOCKS>(P, plan, tile, lane, before));
   // the range's requests, one after the other
   for (bool first = true; tile < stop && b >= 0 && b < a.bs; first = false) {
-  const Request req = request_in(P, plan, b);
+  const Request req = request_in<BLOCKS>(P, plan, b);
   const int n_rows = req.nodes * (int)P.G.d, tiles = tiles_of(req);
   const int t0 = tile - before, t1 = stop - before < tiles ? stop - before : tiles;
   const int request = b;
@@ -390,10 +420,42 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
 
   const int last = req.total - 1;
   auto good = [&](uint32_t slot) { return slot < P.num_slots; };
+  // BLOCKS: where a group of 16 positions, numbered as they are read, begins in the request, or -1 where its entry names no
+  // finished block.  The list is read through the scalar cache: the group is the same in every lane.
+  const Finished done = BLOCKS ? finished_of(P, request) : Finished{0, 0};
+  const auto* const list = reinterpret_cast<const __attribute__((address_space(4))) int32_t*>(
+      reinterpret_cast<uintptr_t>(P.blocks + (BLOCKS ? ((int64_t)request * c.heads + h) * P.count : 0)));
+  auto entry = [&](int v) {
+    const int e = v >> P.shift;
+    return list[e < P.count ? e : P.count - 1];
+  };
+  auto group_of = [&](int v, int id) {
+    if (v >> P.shift >= done.read) return ((done.full - done.read) << P.shift) + v;
+    return (uint32_t)id < (uint32_t)done.full ? (id << P.shift) + (v & ((1 << P.shift) - 1)) : -1;
+  };
+  auto group = [&](int v) { return group_of(v, entry(v)); };
+  // the slot of position i of the group that begins at `from`
+  auto slot_in = [&](int from, int i) {
+    return from >= 0 && (int64_t)from + i < a.page_cols ? (uint32_t)table[from + i] : ~0u;
+  };
+  // those of its positions g * 4 .. g * 4 + 3
+  auto four_slots = [&](int from, uint32_t* vs) {
+    if (from >= 0 && (int64_t)from + 16 <= a.page_cols) {
+      uint4 v;
+      __builtin_memcpy(&v, table + from + g * 4, 16);
+      vs[0] = v.x, vs[1] = v.y, vs[2] = v.z, vs[3] = v.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) vs[j] = slot_in(from, g * 4 + j);
+    }
+  };
   // the slots of 32 positions from `base`: of the key rows m and 16 + m, and of this lane's eight positions
   // g * 4 + j, 16 + g * 4 + j (j < 4); the others' entries are not touched
   auto key_slots = [&](int base, uint32_t& k0, uint32_t& k1) {
-    if (base + AT_STEP <= req.total) {
+    if constexpr (BLOCKS) {
+      k0 = base + m <= last ? slot_in(group(base), m) : ~0u;
+      k1 = base + 16 + m <= last ? slot_in(group(base + 16), m) : ~0u;
+    } else if (base + AT_STEP <= req.total) {
       k0 = (uint32_t)table[base + m];
       k1 = (uint32_t)table[base + 16 + m];
     } else {
@@ -402,7 +464,12 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
     }
   };
   auto value_slots = [&](auto whole_, int base, uint32_t (&vs)[8]) {
-    if (decltype(whole_)::value || base + AT_STEP <= req.total) {
+    if constexpr (BLOCKS) {
+      four_slots(group(base), vs);
+      four_slots(group(base + 16), vs + 4);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) vs[j] = base + (j / 4) * 16 + g * 4 + (j & 3) <= last ? vs[j] : ~0u;
+    } else if (decltype(whole_)::value || base + AT_STEP <= req.total) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         uint4 v;
@@ -669,7 +736,24 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
     if (t < whole) {
       uint32_t ks0[2], vs0[8], ks1[2], vs1[8], here0, here1, kw[2][KL][4], wv0[8][VW], wv1[8][VW];
       float scale;
+      // (BLOCKS: the entries of a step's groups are asked for a step before its slots)
+      int entries[2] = {0, 0}, entries_at = 0;
+      auto ask_entries = [&](int i) {
+        if constexpr (BLOCKS) {
+          entries_at = (i < whole ? i : t) * AT_STEP;
+          entries[0] = entry(entries_at);
+          entries[1] = entry(entries_at + 16);
+        }
+      };
       auto slots = [&](int i, uint32_t (&ks)[2], uint32_t (&vs)[8]) {
+        if constexpr (BLOCKS) {
+          const int from0 = group_of(entries_at, entries[0]), from1 = group_of(entries_at + 16, entries[1]);
+          ks[0] = slot_in(from0, m);
+          ks[1] = slot_in(from1, m);
+          four_slots(from0, vs);
+          four_slots(from1, vs + 4);
+          return;
+        }
         ks[0] = (uint32_t)table[i * AT_STEP + m];
         ks[1] = (uint32_t)table[i * AT_STEP + 16 + m];
         value_slots(Int<1>{}, i * AT_STEP, vs);
@@ -694,6 +778,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
              [&](int e, uint32_t (&vo)[4]) { value_operand<CT>(wv, e, vo); },
              [&]() {
                slots(t + 2 * WK < whole ? t + 2 * WK : t, then_ks, then_slot);
+               ask_entries(t + 3 * WK);
                __builtin_amdgcn_sched_barrier(0);
                load(ks, slot, then, then_here);
                __builtin_amdgcn_sched_barrier(0);
@@ -702,8 +787,11 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
              [](int) {});
         t += WK;
       };
+      ask_entries(t);
       slots(t, ks0, vs0);
+      ask_entries(t + WK);
       slots(t + WK < whole ? t + WK : t, ks1, vs1);
+      ask_entries(t + 2 * WK);
       load(ks0, vs0, wv0, here0);
       while (true) {
         go(wv0, here0, wv1, here1, ks1, vs1, ks0, vs0);
@@ -741,15 +829,29 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
     struct Brought {
       uint32_t kw[KL][4], wv[4][VW];
       uint32_t kslot, vslot[4];  // of the next tile to be loaded
+      int entry;                 // BLOCKS: of the piece of the tile whose slots are asked for next
       uint32_t have;             // bits of the 16 positions
       float scale;
     };
     Brought sets[DEPTH];
     const bool brings = wave < AT_WAVES * NT;
     const int piece = wave % AT_WAVES, ahead = NT > 1 ? wave / AT_WAVES : 0;  // what of a turn's which tile
+    auto fetch_entry = [&](Brought& f, int t) {
+      if constexpr (BLOCKS) f.entry = entry(t * AT_TILE + piece * 16);
+    };
     auto fetch_slots = [&](Brought& f, int t) {
       if (t >= t1) return;
       const int base = t * AT_TILE + piece * 16;
+      if constexpr (BLOCKS) {
+        const int from = group_of(base, f.entry);
+        f.kslot = base + m <= last ? slot_in(from, m) : ~0u;
+        four_slots(from, f.vslot);
+        if (base + 16 > req.total)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) f.vslot[j] = base + g * 4 + j <= last ? f.vslot[j] : ~0u;
+        fetch_entry(f, t + NT * DEPTH);
+        return;
+      }
       if (base + 16 <= req.total) {
         f.kslot = (uint32_t)table[base + m];
         uint4 v;
@@ -802,6 +904,8 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       }
     };
     if (brings) {
+      fetch_entry(sets[0], t0 + ahead);
+      if constexpr (DEPTH > 1) fetch_entry(sets[1], t0 + 1);
       fetch_slots(sets[0], t0 + ahead);
       if constexpr (DEPTH > 1) fetch_slots(sets[1], t0 + 1);
       ask(sets[0], t0 + ahead);
@@ -960,7 +1064,7 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
       if (CT != DSV_I8 && s_odd) {
         const uint64_t mask = mask_of(a, request, node);
         for (int p = aside0; p < aside1; ++p) {
-          const uint32_t slot = (uint32_t)table[p];
+          const uint32_t slot = BLOCKS ? slot_in(group(p & ~15), p & 15) : (uint32_t)table[p];
           const int j = p - req.prefix;
           if (!good(slot) || !(j < 0 || (j < 64 && ((mask >> (j & 63)) & 1)))) continue;
           const uint8_t* v = vhead + (uint64_t)slot * P.v_step + d * ESZ;
@@ -1014,7 +1118,7 @@ constexpr int attn_occupancy(int form, int R, int dim) {
   return dim > 128 && form != AT_ROWS ? 1 : 2;
 }
 
-template <int XT, int CT>
+template <int XT, int CT, bool BLOCKS>
 void launch_attn(const AttnParams& P, const AttnShape& s, unsigned blocks, hipStream_t stream) {
   auto go = [&](auto kern, int n) { hipLaunchKernelGGL(kern, dim3(blocks), dim3((unsigned)n * 64u), 0, stream, P); };
   const int D = P.a.cache.dim;
@@ -1022,13 +1126,13 @@ void launch_attn(const AttnParams& P, const AttnShape& s, unsigned blocks, hipSt
     constexpr int DP = decltype(dp)::value;
     constexpr bool FULL = decltype(full)::value;
     if (s.form == AT_DIRECT)
-      go(k_attn<XT, CT, DP, FULL, 1, AT_DIRECT, AT_WAVES, attn_occupancy(AT_DIRECT, 1, DP)>, s.waves);
+      go(k_attn<XT, CT, DP, FULL, 1, AT_DIRECT, AT_WAVES, attn_occupancy(AT_DIRECT, 1, DP), BLOCKS>, s.waves);
     else if (s.form == AT_PAIRS)
-      go(k_attn<XT, CT, DP, FULL, 1, AT_PAIRS, AT_WAVES, attn_occupancy(AT_PAIRS, 1, DP)>, s.waves);
+      go(k_attn<XT, CT, DP, FULL, 1, AT_PAIRS, AT_WAVES, attn_occupancy(AT_PAIRS, 1, DP), BLOCKS>, s.waves);
     else if (s.R == 1)
-      go(k_attn<XT, CT, DP, FULL, 1, AT_ROWS, AT_MOST, attn_occupancy(AT_ROWS, 1, DP)>, s.waves);
+      go(k_attn<XT, CT, DP, FULL, 1, AT_ROWS, AT_MOST, attn_occupancy(AT_ROWS, 1, DP), BLOCKS>, s.waves);
     else if constexpr (DP <= 128)
-      go(k_attn<XT, CT, DP, FULL, 2, AT_ROWS, AT_MOST, attn_occupancy(AT_ROWS, 2, DP)>, s.waves);
+      go(k_attn<XT, CT, DP, FULL, 2, AT_ROWS, AT_MOST, attn_occupancy(AT_ROWS, 2, DP), BLOCKS>, s.waves);
   };
   if (D <= 64)
     D == 64 ? width(Int<64>{}, Int<1>{}) : width(Int<64>{}, Int<0>{});

@@ -4,12 +4,18 @@
 
 namespace dsv {
 
-template void launch_attn<DSV_BF16, DSV_BF16>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
-template void launch_attn<DSV_F16, DSV_F16>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
-extern template void launch_attn<DSV_BF16, DSV_E4M3>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
-extern template void launch_attn<DSV_F16, DSV_E4M3>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
-extern template void launch_attn<DSV_BF16, DSV_I8>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
-extern template void launch_attn<DSV_F16, DSV_I8>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
+template void launch_attn<DSV_BF16, DSV_BF16, false>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
+template void launch_attn<DSV_F16, DSV_F16, false>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
+extern template void launch_attn<DSV_BF16, DSV_E4M3, false>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
+extern template void launch_attn<DSV_F16, DSV_E4M3, false>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
+extern template void launch_attn<DSV_BF16, DSV_I8, false>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
+extern template void launch_attn<DSV_F16, DSV_I8, false>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
+extern template void launch_attn<DSV_BF16, DSV_BF16, true>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
+extern template void launch_attn<DSV_F16, DSV_F16, true>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
+extern template void launch_attn<DSV_BF16, DSV_E4M3, true>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
+extern template void launch_attn<DSV_F16, DSV_E4M3, true>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
+extern template void launch_attn<DSV_BF16, DSV_I8, true>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
+extern template void launch_attn<DSV_F16, DSV_I8, true>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
 
 constexpr int AJ_THREADS = 256, AJ_PARTS = 4;
 
@@ -17,7 +23,7 @@ constexpr int AJ_THREADS = 256, AJ_PARTS = 4;
 // lengths, then the parts: 5.1 us after one request's few parts, 7 to 8 us for most batches) and, for many rows, by the
 // sums' bytes (14.3 us for 16 requests of 512 rows a head).  A launch of its own: a last workgroup that joins would need
 // counters that somebody clears.
-template <int XT, int DP>
+template <int XT, int DP, bool BLOCKS>
 __global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
   const dsv_tree_attention_args& a = P.a;
   const dsv_kv_cache& c = a.cache;
@@ -26,11 +32,11 @@ __global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
   const int rows = a.T * (int)P.G.d, blocks = (rows + ROWS - 1) / ROWS;
   const int b = (int)(blockIdx.x / (c.heads * blocks)), in = (int)(blockIdx.x - (int64_t)b * c.heads * blocks);
   const int h = in / blocks, r = (in - h * blocks) * ROWS + (int)threadIdx.x / PER, d = (int)threadIdx.x % PER * 8;
-  const Plan plan = plan_of(P, lane);
-  const Request req = request_in(P, plan, b);
+  const Plan plan = plan_of<BLOCKS>(P, lane);
+  const Request req = request_in<BLOCKS>(P, plan, b);
   const int tiles = tiles_of(req);
   if ((in - h * blocks) * ROWS >= req.nodes * (int)P.G.d) return;
-  const int before = tiles_before(P, plan, b, lane);
+  const int before = tiles_before<BLOCKS>(P, plan, b, lane);
   const int i0 = plan.range_of(before), i1 = plan.range_of(before + tiles - 1);
   if (i0 == i1 || r >= req.nodes * (int)P.G.d || d >= c.dim) return;
   const int node = (int)P.G.div((uint32_t)r), qh = h * (int)P.G.d + r - node * (int)P.G.d;
@@ -123,45 +129,40 @@ static int attn_ranges(const AttnShape& s, int heads, int dim) {
   return (int)best;
 }
 
-}  // namespace dsv
-
-using namespace dsv;
-
-extern "C" int64_t dsv_tree_attention_workspace_bytes(int32_t bs, int32_t T, int32_t heads, int32_t q_heads,
-                                                      int32_t dim) {
-  if (bs < 1 || T < 1 || heads < 1 || q_heads < heads || dim < 1) return 0;
-  const AttnShape s = attn_shape(T, q_heads / heads, dim);
-  const int64_t rows = 2 * (int64_t)attn_ranges(s, heads, dim) * q_heads * T;
-  return rows * (dim * (int64_t)sizeof(float) + (int64_t)sizeof(float4));
-}
-
-extern "C" int dsv_tree_attention(const dsv_tree_attention_args* args, dsv_stream_t stream_) {
-  hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
-  if (!args) DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: no arguments");
-  const dsv_tree_attention_args& a = *args;
-  const int rc = check_cache("dsv_tree_attention", &a.cache);
+// Both attentions' call: over all of a request's positions, or (`lists`) over selected blocks.
+static int attention(const char* what, const dsv_tree_attention_args& a, const dsv_block_attention_args* lists,
+                     hipStream_t stream) {
+  const int rc = check_cache(what, &a.cache);
   if (rc != DSV_OK) return rc;
   if (a.dtype != DSV_BF16 && a.dtype != DSV_F16)
-    DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: unknown activation type %d", a.dtype);
+    DSV_FAIL(DSV_ERR_INVALID, "%s: unknown activation type %d", what, a.dtype);
   const bool quant = a.cache.dtype == DSV_E4M3 || a.cache.dtype == DSV_I8;
   if (!quant && a.cache.dtype != a.dtype)
-    DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: queries and an unquantised cache must be of one type");
+    DSV_FAIL(DSV_ERR_INVALID, "%s: queries and an unquantised cache must be of one type", what);
   if (a.bs < 1 || a.T < 1 || a.T > AT_NODES || a.rows < 0 || (!a.row_offsets && a.rows != (int64_t)a.bs * a.T))
-    DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: invalid layout (bs %d, T %d, rows %lld)", a.bs, a.T, (long long)a.rows);
+    DSV_FAIL(DSV_ERR_INVALID, "%s: invalid layout (bs %d, T %d, rows %lld)", what, a.bs, a.T, (long long)a.rows);
   if (a.q_heads < 1 || a.q_heads % a.cache.heads || a.q_heads > 65535)
-    DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: %d query heads over %d cache heads", a.q_heads, a.cache.heads);
+    DSV_FAIL(DSV_ERR_INVALID, "%s: %d query heads over %d cache heads", what, a.q_heads, a.cache.heads);
+  if (lists) {
+    const int size = lists->block_size;
+    if (size != 16 && size != 32 && size != 64 && size != 128)
+      DSV_FAIL(DSV_ERR_INVALID, "%s: a block has 16, 32, 64 or 128 positions (got %d)", what, size);
+    if (lists->count < 1 || (int64_t)lists->count * size > 0x7fff0000ll)
+      DSV_FAIL(DSV_ERR_INVALID, "%s: %d blocks of %d positions", what, lists->count, size);
+  }
   if (a.rows == 0) return DSV_OK;
+  if (lists && !lists->blocks) DSV_FAIL(DSV_ERR_INVALID, "%s: the lists of blocks are required", what);
   if (!a.q || !a.out || !a.prefix_lens || !a.page_table || a.page_cols < 1 || a.page_cols > 0x7fffffc0)
-    DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: q, out, prefix_lens and a page table are required");
+    DSV_FAIL(DSV_ERR_INVALID, "%s: q, out, prefix_lens and a page table are required", what);
   if ((uintptr_t)a.q % 16 || (uintptr_t)a.out % 16 || a.q_row_stride % 8 || a.q_head_stride % 8 ||
       a.out_row_stride % 8 || a.out_head_stride % 8)
-    DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: rows of q and out must start on 16-byte boundaries");
+    DSV_FAIL(DSV_ERR_INVALID, "%s: rows of q and out must start on 16-byte boundaries", what);
   // (times log2 e and the int8 codes' 512 it has to stay within float32)
   if (!(a.scale >= -0x1p100f && a.scale <= 0x1p100f))
-    DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: scale must be finite, at most 2^100");
+    DSV_FAIL(DSV_ERR_INVALID, "%s: scale must be finite, at most 2^100", what);
   const int64_t esize = quant ? 1 : 2;
   if (a.cache.k_slot_stride * esize > 0x7fffffff || a.cache.v_slot_stride * esize > 0x7fffffff)
-    DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: slots are too far apart");
+    DSV_FAIL(DSV_ERR_INVALID, "%s: slots are too far apart", what);
   AttnParams P;
   P.a = a;
   const int G = a.q_heads / a.cache.heads;
@@ -177,36 +178,69 @@ extern "C" int dsv_tree_attention(const dsv_tree_attention_args* args, dsv_strea
   const int64_t blocks = (P.most + 7) / 8 * 8 * (int64_t)a.cache.heads * s.RB;
   const int64_t wide = a.cache.dim <= 64 ? 64 : (a.cache.dim <= 128 ? 128 : 256), per = AJ_THREADS / (wide / 8);
   const int64_t joins = (a.T * (int64_t)G + per - 1) / per * a.cache.heads * a.bs;
-  const int64_t tiles = ((a.page_cols + AT_TILE - 1) / AT_TILE + 1) * a.bs;  // at most
+  const int64_t most = lists ? ((int64_t)lists->count + 1) * lists->block_size : a.page_cols;
+  const int64_t tiles = ((most + AT_TILE - 1) / AT_TILE + 1) * a.bs;  // at most
   if (blocks > 0x7fffffffll || joins > 0x7fffffffll || tiles > 0x7fffff00ll)
-    DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: too many nodes or positions for one call");
+    DSV_FAIL(DSV_ERR_INVALID, "%s: too many nodes or positions for one call", what);
   const int64_t need = dsv_tree_attention_workspace_bytes(a.bs, a.T, a.cache.heads, a.q_heads, a.cache.dim);
   if (!a.workspace || (uintptr_t)a.workspace % 16)
-    DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: a 16-byte-aligned workspace is required");
+    DSV_FAIL(DSV_ERR_INVALID, "%s: a 16-byte-aligned workspace is required", what);
   if (a.workspace_bytes < need)
-    DSV_FAIL(DSV_ERR_WORKSPACE, "dsv_tree_attention: workspace %lld < %lld", (long long)a.workspace_bytes, (long long)need);
+    DSV_FAIL(DSV_ERR_WORKSPACE, "%s: workspace %lld < %lld", what, (long long)a.workspace_bytes, (long long)need);
   P.num_slots = (uint32_t)(a.cache.num_slots < 0x7fffffff ? a.cache.num_slots : 0x7fffffff);
   P.k_step = (uint32_t)(a.cache.k_slot_stride * esize);
   P.v_step = (uint32_t)(a.cache.v_slot_stride * esize);
   P.part_o = reinterpret_cast<float*>(a.workspace);
   P.part_ml = reinterpret_cast<float4*>(P.part_o + 2 * (int64_t)P.most * a.q_heads * a.T * a.cache.dim);
-  const bool bf = a.dtype == DSV_BF16;
-  if (a.cache.dtype == DSV_E4M3)
-    bf ? launch_attn<DSV_BF16, DSV_E4M3>(P, s, (unsigned)blocks, stream) : launch_attn<DSV_F16, DSV_E4M3>(P, s, (unsigned)blocks, stream);
-  else if (a.cache.dtype == DSV_I8)
-    bf ? launch_attn<DSV_BF16, DSV_I8>(P, s, (unsigned)blocks, stream) : launch_attn<DSV_F16, DSV_I8>(P, s, (unsigned)blocks, stream);
-  else
-    bf ? launch_attn<DSV_BF16, DSV_BF16>(P, s, (unsigned)blocks, stream) : launch_attn<DSV_F16, DSV_F16>(P, s, (unsigned)blocks, stream);
-  DSV_CHECK_LAUNCH("k_attn");
-  if (P.most > 1) {
-    auto join = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)joins), dim3(AJ_THREADS), 0, stream, P); };
-    if (wide == 64)
-      bf ? join(k_attn_join<DSV_BF16, 64>) : join(k_attn_join<DSV_F16, 64>);
-    else if (wide == 128)
-      bf ? join(k_attn_join<DSV_BF16, 128>) : join(k_attn_join<DSV_F16, 128>);
+  P.blocks = lists ? lists->blocks : nullptr;
+  P.count = lists ? lists->count : 0;
+  P.shift = lists ? __builtin_ctz((unsigned)lists->block_size) : 0;
+  auto go = [&](auto selected) -> int {
+    constexpr bool BLOCKS = decltype(selected)::value;
+    const bool bf = a.dtype == DSV_BF16;
+    if (a.cache.dtype == DSV_E4M3)
+      bf ? launch_attn<DSV_BF16, DSV_E4M3, BLOCKS>(P, s, (unsigned)blocks, stream)
+         : launch_attn<DSV_F16, DSV_E4M3, BLOCKS>(P, s, (unsigned)blocks, stream);
+    else if (a.cache.dtype == DSV_I8)
+      bf ? launch_attn<DSV_BF16, DSV_I8, BLOCKS>(P, s, (unsigned)blocks, stream)
+         : launch_attn<DSV_F16, DSV_I8, BLOCKS>(P, s, (unsigned)blocks, stream);
     else
-      bf ? join(k_attn_join<DSV_BF16, 256>) : join(k_attn_join<DSV_F16, 256>);
-    DSV_CHECK_LAUNCH("k_attn_join");
-  }
-  return DSV_OK;
+      bf ? launch_attn<DSV_BF16, DSV_BF16, BLOCKS>(P, s, (unsigned)blocks, stream)
+         : launch_attn<DSV_F16, DSV_F16, BLOCKS>(P, s, (unsigned)blocks, stream);
+    DSV_CHECK_LAUNCH("k_attn");
+    if (P.most > 1) {
+      auto join = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)joins), dim3(AJ_THREADS), 0, stream, P); };
+      if (wide == 64)
+        bf ? join(k_attn_join<DSV_BF16, 64, BLOCKS>) : join(k_attn_join<DSV_F16, 64, BLOCKS>);
+      else if (wide == 128)
+        bf ? join(k_attn_join<DSV_BF16, 128, BLOCKS>) : join(k_attn_join<DSV_F16, 128, BLOCKS>);
+      else
+        bf ? join(k_attn_join<DSV_BF16, 256, BLOCKS>) : join(k_attn_join<DSV_F16, 256, BLOCKS>);
+      DSV_CHECK_LAUNCH("k_attn_join");
+    }
+    return DSV_OK;
+  };
+  return lists ? go(Int<1>{}) : go(Int<0>{});
+}
+
+}  // namespace dsv
+
+using namespace dsv;
+
+extern "C" int64_t dsv_tree_attention_workspace_bytes(int32_t bs, int32_t T, int32_t heads, int32_t q_heads,
+                                                      int32_t dim) {
+  if (bs < 1 || T < 1 || heads < 1 || q_heads < heads || dim < 1) return 0;
+  const AttnShape s = attn_shape(T, q_heads / heads, dim);
+  const int64_t rows = 2 * (int64_t)attn_ranges(s, heads, dim) * q_heads * T;
+  return rows * (dim * (int64_t)sizeof(float) + (int64_t)sizeof(float4));
+}
+
+extern "C" int dsv_tree_attention(const dsv_tree_attention_args* args, dsv_stream_t stream) {
+  if (!args) DSV_FAIL(DSV_ERR_INVALID, "dsv_tree_attention: no arguments");
+  return attention("dsv_tree_attention", *args, nullptr, reinterpret_cast<hipStream_t>(stream));
+}
+
+extern "C" int dsv_block_attention(const dsv_block_attention_args* args, dsv_stream_t stream) {
+  if (!args) DSV_FAIL(DSV_ERR_INVALID, "dsv_block_attention: no arguments");
+  return attention("dsv_block_attention", args->tree, args, reinterpret_cast<hipStream_t>(stream));
 }

@@ -1,0 +1,9 @@
+// The kernels of attention over selected blocks of the 16-bit caches.
+#include "dsv_attn.h"
+
+namespace dsv {
+
+template void launch_attn<DSV_BF16, DSV_BF16, true>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
+template void launch_attn<DSV_F16, DSV_F16, true>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
+
+}  // namespace dsv

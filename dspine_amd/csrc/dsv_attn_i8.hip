@@ -3,7 +3,7 @@
 
 namespace dsv {
 
-template void launch_attn<DSV_BF16, DSV_I8>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
-template void launch_attn<DSV_F16, DSV_I8>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
+template void launch_attn<DSV_BF16, DSV_I8, false>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
+template void launch_attn<DSV_F16, DSV_I8, false>(const AttnParams&, const AttnShape&, unsigned, hipStream_t);
 
 }  // namespace dsv

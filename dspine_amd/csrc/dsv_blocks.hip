@@ -1,0 +1,557 @@
+// Blocks of a cache and what selects among them, for gfx950: the least and largest key elements of finished blocks, the
+// bound of every block's attention scores that follows from them, and the best blocks of each (request, cache head).
+#include "dsv_cache.h"
+#include "dsv_common.h"
+
+namespace dsv {
+
+constexpr int BI_THREADS = 256;
+
+struct IndexParams {
+  dsv_block_index x;
+  dsv_kv_cache c;
+  const int32_t *page_table, *block_table, *from_lens, *to_lens;
+  int64_t page_stride, page_cols, block_stride, block_cols;
+  int shift, G, most;  // block of 2^shift positions; lanes of a row; blocks a request may have finished
+};
+
+// Bounds of a finished block, a workgroup a (block, head): groups of G lanes hold a position's row, 16 bytes a lane, and
+// run over the block's positions; the groups' results join within a wave by lane moves, the waves' through LDS.  NaN
+// counts as the least and the largest.
+template <int CT, int IT>
+__global__ __launch_bounds__(BI_THREADS) void k_index_blocks(IndexParams P) {
+  constexpr bool QUANT = CT == DSV_E4M3 || CT == DSV_I8;
+  constexpr int EL = QUANT ? 16 : 8, ROWS = 4, NW = BI_THREADS / WAVE;
+  __shared__ float s_lo[NW][256], s_hi[NW][256];
+  const dsv_kv_cache& c = P.c;
+  const int h = (int)(blockIdx.x % (uint32_t)c.heads);
+  const uint32_t at = blockIdx.x / (uint32_t)c.heads;
+  const int b = (int)(at / (uint32_t)P.most);
+  const int from = P.from_lens[b], to = P.to_lens[b];
+  const int64_t j = (int64_t)((from < 0 ? 0 : from) >> P.shift) + at % (uint32_t)P.most;
+  if (to < 0 || j >= to >> P.shift || j >= P.block_cols) return;
+  const int32_t row = P.block_table[b * P.block_stride + j];
+  if (row < 0 || row >= P.x.rows) return;
+  const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
+  const int l = tid & (P.G - 1), group = tid / P.G, groups = BI_THREADS / P.G, B = 1 << P.shift;
+  const bool in = l * EL < c.dim;
+  const int64_t p0 = j << P.shift;
+  const int32_t* table = P.page_table + b * P.page_stride + p0;
+  float lo[EL], hi[EL];
+#pragma unroll
+  for (int e = 0; e < EL; ++e) lo[e] = INFINITY, hi[e] = -INFINITY;
+  bool some = false;
+  for (int i0 = group; i0 < B; i0 += groups * ROWS) {
+    uint4 x[ROWS];
+    float scale[ROWS];
+    bool has[ROWS];
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+      const int i = i0 + u * groups;
+      const int64_t slot = i < B && p0 + i < P.page_cols ? table[i] : -1;
+      has[u] = slot >= 0 && slot < c.num_slots;
+      const int64_t s = has[u] ? slot : 0;
+      x[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(c.k) +
+                                             (s * c.k_slot_stride + h * c.k_head_stride + (in ? l * EL : 0)) * (QUANT ? 1 : 2));
+      if constexpr (QUANT) scale[u] = c.k_scale[s * c.ks_slot_stride + h * c.ks_head_stride];
+    }
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) {
+      if (!has[u]) continue;
+      some = true;
+      const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+      float f[EL];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (QUANT) {
+          unpack_codes<CT>(w[i], f + 4 * i);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) f[4 * i + k] *= scale[u];
+        } else {
+          f[2 * i] = act_to_f32<CT>(w[i] & 0xffffu);
+          f[2 * i + 1] = act_to_f32<CT>(w[i] >> 16);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < EL; ++e) {
+        lo[e] = __builtin_elementwise_minimum(lo[e], f[e]);
+        hi[e] = __builtin_elementwise_maximum(hi[e], f[e]);
+      }
+    }
+  }
+  for (int o = P.G; o < WAVE; o *= 2) {
+#pragma unroll
+    for (int e = 0; e < EL; ++e) {
+      lo[e] = __builtin_elementwise_minimum(lo[e], __shfl_xor(lo[e], o, WAVE));
+      hi[e] = __builtin_elementwise_maximum(hi[e], __shfl_xor(hi[e], o, WAVE));
+    }
+  }
+  if (in && lane < P.G) {
+#pragma unroll
+    for (int e = 0; e < EL; ++e) s_lo[wave][l * EL + e] = lo[e], s_hi[wave][l * EL + e] = hi[e];
+  }
+  const bool any = __syncthreads_or(some);
+  // element pairs: the least ones, then the largest
+  for (int i = tid; i < c.dim; i += BI_THREADS) {
+    const bool high = i >= c.dim / 2;
+    const int d = (high ? i - c.dim / 2 : i) * 2;
+    float v[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float a = high ? s_hi[0][d + k] : s_lo[0][d + k];
+#pragma unroll
+      for (int w = 1; w < NW; ++w)
+        a = high ? __builtin_elementwise_maximum(a, s_hi[w][d + k]) : __builtin_elementwise_minimum(a, s_lo[w][d + k]);
+      v[k] = any ? a : 0.f;
+    }
+    uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(P.x.bounds) + ((int64_t)row * c.heads + h) * 2 * c.dim);
+    out[i] = pack_act<IT>(v[0], v[1]);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Scores: with q+ and q- a query's positive and negative elements, sum_d max(q lo, q hi) = q- . lo + q+ . hi, a product
+// over 2 * dim elements of an index row as it lies in memory.  The matrix cores take 16 blocks as rows and 16 queries as
+// columns; a block's score is the largest of its columns'.
+// ---------------------------------------------------------------------------------------
+constexpr int SB_THREADS = 256, SB_WAVES = SB_THREADS / WAVE;
+constexpr int SB_STAGE = 64 * 1024 / 1024;  // query operands of 1 KB in LDS
+constexpr int SB_STEPS = 4;                 // steps of a workgroup at most
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+struct ScoreParams {
+  dsv_score_blocks_args a;
+  FastDiv G;
+  int shift, steps, chunks;  // steps of a workgroup, workgroups of a (request, head)
+};
+
+template <int IT>
+__device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
+  if constexpr (IT == DSV_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bhalf8, a), __builtin_bit_cast(bhalf8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+
+// The positive (or negative) elements of a pair, zeros in place of the others; NaN stays.
+template <int IT>
+__device__ __forceinline__ uint32_t half_of(uint32_t w, bool positive) {
+  constexpr uint32_t INF = IT == DSV_BF16 ? 0x7f80u : 0x7c00u;
+  uint32_t keep = 0;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t x = (w >> (16 * i)) & 0xffffu;
+    if ((x >> 15 != 0) != positive || (x & 0x7fffu) > INF) keep |= 0xffffu << (16 * i);
+  }
+  return w & keep;
+}
+
+template <int IT, int NK, bool FULL>
+__global__ __launch_bounds__(SB_THREADS, 2) void k_score_blocks(ScoreParams P) {
+  const dsv_score_blocks_args& a = P.a;
+  const dsv_block_index& x = a.index;
+  const int nk = FULL ? NK : x.dim / 16;        // products of 32 of the row's 2 * dim elements
+  constexpr int TB = NK > 8 ? 1 : 2;            // tiles of 16 blocks a wave
+  constexpr int STEP = SB_WAVES * TB * 16;
+  constexpr int TILES = SB_STAGE / NK;          // query tiles staged at once
+  __shared__ uint4 s_q[TILES * NK][WAVE];
+  __shared__ float s_best[SB_STEPS * STEP];
+  const int tid = threadIdx.x, lane = tid & (WAVE - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
+  const int m = lane & 15, g = lane >> 4;
+  const int chunk = (int)(blockIdx.x % (uint32_t)P.chunks);
+  const uint32_t bh = blockIdx.x / (uint32_t)P.chunks;
+  const int b = (int)(bh / (uint32_t)x.heads), h = (int)(bh - (uint32_t)b * x.heads);
+  const int pre = a.prefix_lens[b];
+  const int64_t full = pre < 0 ? 0 : pre >> P.shift;
+  int n = a.verify_lens ? a.verify_lens[b] : a.T;
+  n = n < 0 ? 0 : (n > a.T ? a.T : n);
+  const int rows = n * (int)P.G.d, tiles = (rows + 15) / 16;
+  const int64_t cols = a.block_cols, first = (int64_t)chunk * P.steps * STEP;
+  const int64_t past = first + P.steps * STEP < cols ? first + P.steps * STEP : cols;  // of the table
+  const int64_t end = rows == 0 ? first : (past < full ? past : full);               // of the blocks that have a score
+  float* const out = a.scores + (int64_t)bh * cols;
+  const int32_t* const table = a.block_table + b * a.block_stride;
+  const int64_t row0 = a.row_offsets ? load_index(a.row_offsets, a.row_offsets_i64, b) : (int64_t)b * a.T;
+  for (int64_t i = (end > first ? end : first) + tid; i < past; i += SB_THREADS) out[i] = -INFINITY;
+  if (end <= first) return;
+  for (int t0 = 0; t0 < tiles; t0 += TILES) {
+    const int here = tiles - t0 < TILES ? tiles - t0 : TILES;
+    if (t0) __syncthreads();
+    for (int i = wave; i < here * nk; i += SB_WAVES) {
+      const int t = i / nk, kk = i - t * nk;
+      int r = (t0 + t) * 16 + m;
+      r = r < rows ? r : rows - 1;  // (a row again: the largest stays the largest)
+      const int node = (int)P.G.div((uint32_t)r), head = h * (int)P.G.d + r - node * (int)P.G.d;
+      const int64_t row = row0 + node;
+      const int e = kk * 32 + g * 8;
+      const bool positive = e >= x.dim;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (row >= 0 && row < a.rows)
+        w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + row * a.q_row_stride +
+                                            head * a.q_head_stride + (positive ? e - x.dim : e));
+      s_q[t * NK + kk][lane] = make_uint4(half_of<IT>(w.x, positive), half_of<IT>(w.y, positive),
+                                          half_of<IT>(w.z, positive), half_of<IT>(w.w, positive));
+    }
+    __syncthreads();
+    for (int step = 0; step < P.steps; ++step) {
+      const int64_t j0 = first + step * STEP + wave * TB * 16;
+      if (j0 >= end) break;
+      uint4 k[TB][NK];
+      bool there[TB];
+#pragma unroll
+      for (int t = 0; t < TB; ++t) {
+        const int64_t j = j0 + t * 16 + m;
+        const int32_t row = j < end ? table[j] : -1;
+        there[t] = row >= 0 && row < x.rows;
+        const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(x.bounds) +
+                                                           ((int64_t)(there[t] ? row : 0) * x.heads + h) * 2 * x.dim) + g;
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk)
+          if (FULL || kk < nk) k[t][kk] = from[kk * 4];
+      }
+      f32x4 best[TB];
+#pragma unroll
+      for (int t = 0; t < TB; ++t) best[t] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      for (int rt = 0; rt < here; ++rt) {
+        f32x4 s[TB];
+#pragma unroll
+        for (int t = 0; t < TB; ++t) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) {
+          if (FULL || kk < nk) {
+            const uint4 q = s_q[rt * NK + kk][lane];
+#pragma unroll
+            for (int t = 0; t < TB; ++t) s[t] = mfma16<IT>(k[t][kk], q, s[t]);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < TB; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) best[t][r] = __builtin_elementwise_maximum(best[t][r], s[t][r]);
+      }
+#pragma unroll
+      for (int t = 0; t < TB; ++t) {
+        // the 16 columns of a row lie in 16 neighbouring lanes; lane (r, g) keeps row g * 4 + r
+        float mine = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float v = best[t][r];
+          v = __builtin_elementwise_maximum(v, dpp<DPP_QUAD_XOR1>(v, v));
+          v = __builtin_elementwise_maximum(v, dpp<DPP_QUAD_XOR2>(v, v));
+          v = __builtin_elementwise_maximum(v, dpp<DPP_ROW_HALF_MIRROR>(v, v));
+          v = __builtin_elementwise_maximum(v, dpp<DPP_ROW_MIRROR>(v, v));
+          mine = m == r ? v : mine;
+        }
+        // (lane i of the tile knows whether block i is there)
+        const bool has = __shfl((int)there[t], g * 4 + (m & 3), WAVE) != 0;
+        const int64_t j = j0 + t * 16 + g * 4 + m;
+        if (m < 4 && j < end) {
+          const int at = (int)(j - first);
+          if (t0) mine = __builtin_elementwise_maximum(mine, s_best[at]);
+          if (t0 + here < tiles)
+            s_best[at] = mine;  // (read by the same lane)
+          else
+            out[j] = has ? mine * a.scale : -INFINITY;
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// The best blocks.
+// ---------------------------------------------------------------------------------------
+struct SelectParams {
+  const float* scores;
+  const int32_t* prefix_lens;
+  int32_t* blocks;
+  int64_t cols;
+  int heads, shift, count, first, last;
+};
+
+// A workgroup a (request, head), its scores in registers as keys that order like them.  The `need`-th largest key is
+// found in 256 equal bins of the range that holds it, again within that bin until at most 64 keys are left, which one
+// wave ranks by counting; equal keys count by their index, the lowest first.  The chosen ones are written in order.
+template <int NW, int PER>
+__global__ __launch_bounds__(NW * WAVE) void k_select_blocks(SelectParams P) {
+  constexpr int NT = NW * WAVE;
+  __shared__ uint32_t s_hist[256], s_val[WAVE], s_red[2][NW], s_found[4];
+  __shared__ int s_idx[WAVE], s_count[PER * NW + WAVE], s_n;
+  const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
+  const int64_t row = blockIdx.x;
+  const int pre = P.prefix_lens[row / P.heads];
+  const int64_t full = pre < 0 ? 0 : pre >> P.shift;
+  const int n = (int)(full < P.cols ? full : P.cols);
+  int32_t* const out = P.blocks + row * P.count;
+  if (n <= P.count) {
+    for (int i = tid; i < P.count; i += NT) out[i] = i < n ? i : -1;
+    return;
+  }
+  const float* scores = P.scores + row * P.cols;
+  const int c0 = P.first, c1 = n - P.last;  // the candidates
+  uint32_t key[PER];
+  uint32_t lo = ~0u, hi = 0u;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int j = i * NT + tid;
+    key[i] = 0;
+    if (j >= c0 && j < c1) {
+      const float v = scores[j];
+      key[i] = f32_key(v == v ? v : -INFINITY);
+      lo = key[i] < lo ? key[i] : lo;
+      hi = key[i] > hi ? key[i] : hi;
+    }
+  }
+  uint32_t need = (uint32_t)(P.count - P.first - P.last), left = (uint32_t)(c1 - c0);
+  // chosen: above `tkey`, or equal to it at an index up to `tidx`
+  uint32_t tkey = ~0u;
+  int tidx = -1;
+  if (need) {
+    lo = ~wave_max_u32(~lo);
+    hi = wave_max_u32(hi);
+    if (lane == 0) s_red[0][wave] = lo, s_red[1][wave] = hi;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      lo = s_red[0][w] < lo ? s_red[0][w] : lo;
+      hi = s_red[1][w] > hi ? s_red[1][w] : hi;
+    }
+    bool ties = false;  // the values are now the indices, turned round, of the keys that equal tkey
+    auto value = [&](int i) { return ties ? (key[i] == tkey ? ~(uint32_t)(i * NT + tid) : 0u) : key[i]; };
+    while (true) {
+      if (left == need) {  // all that is left
+        if (ties)
+          tidx = (int)~lo;
+        else
+          tkey = lo, tidx = 0x7fffffff;
+        break;
+      }
+      if (left <= WAVE) {
+        if (tid == 0) s_n = 0;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const uint32_t v = value(i);
+          if (v >= lo && v <= hi && v) {
+            const int at = atomicAdd(&s_n, 1);
+            if (at < WAVE) s_val[at] = v, s_idx[at] = i * NT + tid;
+          }
+        }
+        __syncthreads();
+        if (wave == 0) {
+          const int held = s_n < WAVE ? s_n : WAVE;
+          const uint32_t v = lane < held ? s_val[lane] : 0u;
+          const int idx = lane < held ? s_idx[lane] : 0x7fffffff;
+          uint32_t before = 0;
+          for (int k = 0; k < held; ++k) {
+            const uint32_t u = s_val[k];
+            before += u > v || (u == v && s_idx[k] < idx);
+          }
+          if (lane < held && before == need - 1) s_found[0] = v, s_found[1] = (uint32_t)idx;
+        }
+        __syncthreads();
+        if (!ties) tkey = s_found[0];
+        tidx = (int)s_found[1];
+        break;
+      }
+      if (lo == hi) {  // (more equal keys than a wave ranks)
+        ties = true;
+        tkey = lo;
+        lo = ~(uint32_t)(n - 1);
+        hi = ~0u;
+      }
+      const uint32_t range = hi - lo;
+      const int bits = 32 - __builtin_clz(range), s = bits > 8 ? bits - 8 : 0;
+      for (int i = tid; i < 256; i += NT) s_hist[i] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const uint32_t v = value(i);
+        if (v >= lo && v <= hi && v) atomicAdd(&s_hist[(v - lo) >> s], 1u);
+      }
+      __syncthreads();
+      if (wave == 0) {  // from the top: lane l has the bins 255 - 4 l and the three below
+        uint32_t bin[4], sum = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) bin[k] = s_hist[255 - 4 * lane - k], sum += bin[k];
+        const uint32_t upto = wave_incl_scan(sum);
+        uint32_t above = upto - sum;
+        if (above < need && upto >= need) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (above < need && above + bin[k] >= need) s_found[0] = (uint32_t)(255 - 4 * lane - k), s_found[1] = above, s_found[2] = bin[k];
+            above += bin[k];
+          }
+        }
+      }
+      __syncthreads();
+      const uint32_t from = lo + (s_found[0] << s), most = from + ((1u << s) - 1u);
+      need -= s_found[1];
+      left = s_found[2];
+      hi = most < hi && most >= from ? most : hi;
+      lo = from;
+      __syncthreads();  // (before s_found and s_hist are written again)
+    }
+  }
+  uint32_t chosen = 0;  // bit i: this thread's index i
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int j = i * NT + tid;
+    const bool yes = j < n && (j < c0 || j >= c1 || key[i] > tkey || (key[i] == tkey && j <= tidx));
+    chosen |= (yes ? 1u : 0u) << i;
+    const uint64_t all = __ballot(yes);
+    if (lane == 0) s_count[i * NW + wave] = __popcll(all);
+  }
+  __syncthreads();
+  if (wave == 0) {
+    int before = 0;
+    for (int k = 0; k < PER * NW; k += WAVE) {
+      const int v = k + lane < PER * NW ? s_count[k + lane] : 0;
+      const int upto = wave_incl_scan(v);
+      if (k + lane < PER * NW) s_count[k + lane] = before + upto - v;
+      before += readlane<WAVE - 1>(upto);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const bool yes = (chosen >> i) & 1;
+    const uint64_t all = __ballot(yes);
+    if (yes) {
+      const int at = s_count[i * NW + wave] + __popcll(all & ((1ull << lane) - 1));
+      if (at < P.count) out[at] = i * NT + tid;
+    }
+  }
+}
+
+static int check_index(const char* what, const dsv_block_index& x) {
+  if (!x.bounds || (uintptr_t)x.bounds % 16) DSV_FAIL(DSV_ERR_INVALID, "%s: the index's bounds are required, 16-byte aligned", what);
+  if (x.dtype != DSV_BF16 && x.dtype != DSV_F16) DSV_FAIL(DSV_ERR_INVALID, "%s: unknown index type %d", what, x.dtype);
+  if (x.heads < 1 || x.heads > 65535 || x.rows < 1 || x.dim < 16 || x.dim > 256 || x.dim % 16)
+    DSV_FAIL(DSV_ERR_INVALID, "%s: an index needs rows, heads and a dim that is a multiple of 16 up to 256 (got %lld, %d, %d)",
+             what, (long long)x.rows, x.heads, x.dim);
+  if (x.block_size != 16 && x.block_size != 32 && x.block_size != 64 && x.block_size != 128)
+    DSV_FAIL(DSV_ERR_INVALID, "%s: a block has 16, 32, 64 or 128 positions (got %d)", what, x.block_size);
+  return DSV_OK;
+}
+
+}  // namespace dsv
+
+using namespace dsv;
+
+extern "C" int dsv_index_blocks(const dsv_block_index* index, const dsv_kv_cache* cache, const int32_t* page_table,
+                                int64_t page_stride, int64_t page_cols, const int32_t* block_table, int64_t block_stride,
+                                int64_t block_cols, const int32_t* from_lens, const int32_t* to_lens, int32_t bs,
+                                int64_t longest, dsv_stream_t stream_) {
+  hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+  if (!index) DSV_FAIL(DSV_ERR_INVALID, "dsv_index_blocks: no index");
+  int rc = check_index("dsv_index_blocks", *index);
+  if (rc == DSV_OK) rc = check_cache("dsv_index_blocks", cache);
+  if (rc != DSV_OK) return rc;
+  if (index->heads != cache->heads || index->dim != cache->dim)
+    DSV_FAIL(DSV_ERR_INVALID, "dsv_index_blocks: the index and the cache must have the same heads and dim");
+  if (bs < 0 || longest < 0) DSV_FAIL(DSV_ERR_INVALID, "dsv_index_blocks: invalid layout (bs %d, longest %lld)", bs, (long long)longest);
+  if (bs == 0 || longest == 0) return DSV_OK;
+  if (!page_table || !block_table || !from_lens || !to_lens || page_cols < 1 || block_cols < 1)
+    DSV_FAIL(DSV_ERR_INVALID, "dsv_index_blocks: tables and lengths are required");
+  IndexParams P{*index, *cache, page_table, block_table, from_lens, to_lens, page_stride, page_cols, block_stride, block_cols, 0, 0, 0};
+  P.shift = __builtin_ctz((unsigned)index->block_size);
+  int64_t most = longest > 0x7fffffff ? 0x7fffffff : longest;
+  most = (most + index->block_size - 1) >> P.shift;  // (a growth of n positions finishes ceil(n / size) blocks at most)
+  if (most > block_cols) most = block_cols;
+  const int64_t grid = most * bs * cache->heads;
+  if (grid > 0x7fffffffll) DSV_FAIL(DSV_ERR_INVALID, "dsv_index_blocks: too many blocks for one call");
+  P.most = (int)most;
+  const bool quant = cache->dtype == DSV_E4M3 || cache->dtype == DSV_I8;
+  P.G = 1;
+  while (P.G * (quant ? 16 : 8) < cache->dim) P.G *= 2;
+  auto launch = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(BI_THREADS), 0, stream, P); };
+  const bool bf = index->dtype == DSV_BF16;
+  auto to = [&](auto ct) {
+    constexpr int CT = decltype(ct)::value;
+    bf ? launch(k_index_blocks<CT, DSV_BF16>) : launch(k_index_blocks<CT, DSV_F16>);
+  };
+  if (cache->dtype == DSV_BF16)
+    to(Int<DSV_BF16>{});
+  else if (cache->dtype == DSV_F16)
+    to(Int<DSV_F16>{});
+  else if (cache->dtype == DSV_E4M3)
+    to(Int<DSV_E4M3>{});
+  else
+    to(Int<DSV_I8>{});
+  DSV_CHECK_LAUNCH("k_index_blocks");
+  return DSV_OK;
+}
+
+extern "C" int dsv_score_blocks(const dsv_score_blocks_args* args, dsv_stream_t stream_) {
+  hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+  if (!args) DSV_FAIL(DSV_ERR_INVALID, "dsv_score_blocks: no arguments");
+  const dsv_score_blocks_args& a = *args;
+  const int rc = check_index("dsv_score_blocks", a.index);
+  if (rc != DSV_OK) return rc;
+  if (a.bs < 1 || a.T < 1 || a.T > 64 || a.rows < 0 || (!a.row_offsets && a.rows != (int64_t)a.bs * a.T))
+    DSV_FAIL(DSV_ERR_INVALID, "dsv_score_blocks: invalid layout (bs %d, T %d, rows %lld)", a.bs, a.T, (long long)a.rows);
+  if (a.q_heads < 1 || a.q_heads % a.index.heads || a.q_heads > 65535)
+    DSV_FAIL(DSV_ERR_INVALID, "dsv_score_blocks: %d query heads over %d index heads", a.q_heads, a.index.heads);
+  if (!(a.scale > 0.f && a.scale <= 0x1p100f)) DSV_FAIL(DSV_ERR_INVALID, "dsv_score_blocks: scale must be positive, at most 2^100");
+  if (!a.scores || !a.prefix_lens || !a.block_table || a.block_cols < 1 || a.block_cols > 0x7ffffff || (a.rows && !a.q))
+    DSV_FAIL(DSV_ERR_INVALID, "dsv_score_blocks: q, scores, prefix_lens and a block table are required");
+  if ((uintptr_t)a.q % 16 || a.q_row_stride % 8 || a.q_head_stride % 8)
+    DSV_FAIL(DSV_ERR_INVALID, "dsv_score_blocks: rows of q must start on 16-byte boundaries");
+  ScoreParams P;
+  P.a = a;
+  P.G = fast_div((uint32_t)(a.q_heads / a.index.heads));
+  P.shift = __builtin_ctz((unsigned)a.index.block_size);
+  const int step = SB_WAVES * 16 * (a.index.dim > 128 ? 1 : 2);
+  const int64_t steps = (a.block_cols + step - 1) / step, bh = (int64_t)a.bs * a.index.heads;
+  const int64_t per = steps * bh / 2048;
+  P.steps = (int)(per < 1 ? 1 : (per > SB_STEPS ? SB_STEPS : per));
+  P.chunks = (int)((steps + P.steps - 1) / P.steps);
+  if (bh * P.chunks > 0x7fffffffll) DSV_FAIL(DSV_ERR_INVALID, "dsv_score_blocks: too many blocks for one call");
+  auto launch = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)(bh * P.chunks)), dim3(SB_THREADS), 0, stream, P); };
+  auto type = [&](auto it) {
+    constexpr int IT = decltype(it)::value;
+    const int D = a.index.dim;
+    if (D <= 64)
+      D == 64 ? launch(k_score_blocks<IT, 4, true>) : launch(k_score_blocks<IT, 4, false>);
+    else if (D <= 128)
+      D == 128 ? launch(k_score_blocks<IT, 8, true>) : launch(k_score_blocks<IT, 8, false>);
+    else
+      D == 256 ? launch(k_score_blocks<IT, 16, true>) : launch(k_score_blocks<IT, 16, false>);
+  };
+  a.index.dtype == DSV_BF16 ? type(Int<DSV_BF16>{}) : type(Int<DSV_F16>{});
+  DSV_CHECK_LAUNCH("k_score_blocks");
+  return DSV_OK;
+}
+
+extern "C" int dsv_select_blocks(const float* scores, int32_t bs, int32_t heads, int64_t cols, const int32_t* prefix_lens,
+                                 int32_t block_size, int32_t count, int32_t first, int32_t last, int32_t* blocks,
+                                 dsv_stream_t stream_) {
+  hipStream_t stream = reinterpret_cast<hipStream_t>(stream_);
+  if (bs < 1 || heads < 1 || heads > 65535 || cols < 1 || cols > 32768)
+    DSV_FAIL(DSV_ERR_INVALID, "dsv_select_blocks: 1 to 32768 blocks of a request are ranked (bs %d, heads %d, blocks %lld)", bs,
+             heads, (long long)cols);
+  if (block_size != 16 && block_size != 32 && block_size != 64 && block_size != 128)
+    DSV_FAIL(DSV_ERR_INVALID, "dsv_select_blocks: a block has 16, 32, 64 or 128 positions (got %d)", block_size);
+  if (count < 1 || first < 0 || last < 0 || (int64_t)first + last > count)
+    DSV_FAIL(DSV_ERR_INVALID, "dsv_select_blocks: count %d has to hold the first %d and the last %d", count, first, last);
+  if (!scores || !prefix_lens || !blocks) DSV_FAIL(DSV_ERR_INVALID, "dsv_select_blocks: null pointer");
+  const int64_t rows = (int64_t)bs * heads;
+  if (rows > 0x7fffffffll || rows * count > (1ll << 40)) DSV_FAIL(DSV_ERR_INVALID, "dsv_select_blocks: too many rows for one call");
+  SelectParams P{scores, prefix_lens, blocks, cols, heads, __builtin_ctz((unsigned)block_size), count, first, last};
+  auto launch = [&](auto kern, int waves) { hipLaunchKernelGGL(kern, dim3((unsigned)rows), dim3((unsigned)(waves * WAVE)), 0, stream, P); };
+  if (cols <= 512)
+    launch(k_select_blocks<1, 8>, 1);
+  else if (cols <= 2048)
+    launch(k_select_blocks<4, 8>, 4);
+  else if (cols <= 8192)
+    launch(k_select_blocks<16, 8>, 16);
+  else
+    launch(k_select_blocks<16, 32>, 16);
+  DSV_CHECK_LAUNCH("k_select_blocks");
+  return DSV_OK;
+}

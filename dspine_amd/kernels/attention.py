@@ -38,6 +38,18 @@ def tree_attention(q: torch.Tensor, cache: KVCache, *, T: int, page_table: torch
     current stream (in a captured graph: in the graph's own pool) or takes from ``workspace``; two calls
     that may run at once must not be given one workspace, and one whose buffer a captured graph uses must live as
     long as the graph."""
+    a, dev, out = attention_args(q, cache, T=T, page_table=page_table, prefix_lens=prefix_lens, verify_lens=verify_lens,
+                                 row_offsets=row_offsets, masks=masks, scale=scale, out=out, lse=lse)
+    if a is not None:
+        scratch = with_workspace(a, dev, workspace)  # (held until the launch)
+        _lib.launch("dsv_tree_attention", dev, _lib.load().dsv_tree_attention, a)
+        del scratch
+    return out
+
+
+def attention_args(q, cache, *, T, page_table, prefix_lens, verify_lens, row_offsets, masks, scale, out, lse, also=()):
+    """(the ``dsv_tree_attention_args`` but for the workspace, or None without rows; the device; out), checked;
+    ``also``: tensors that have to be on the same device."""
     if q.ndim != 3 or q.dtype not in _ACT:
         raise ValueError("q must be bfloat16 or float16 [rows, q_heads, dim]")
     c = cache_fields(cache)
@@ -81,16 +93,21 @@ def tree_attention(q: torch.Tensor, cache: KVCache, *, T: int, page_table: torch
         q_at, q_row, q_head = _rows(q, "q")
         out_at, out_row, out_head = _rows(out, "out")
         _distinct(out, "out")
-    dev = _lib.require_cuda(q, *tensors_of(cache), page_table, prefix_lens, verify_lens, row_offsets, masks, out, lse)
+    dev = _lib.require_cuda(q, *tensors_of(cache), page_table, prefix_lens, verify_lens, row_offsets, masks, out, lse,
+                            *also)
     if rows == 0:
-        return out
-    lib = _lib.load()
+        return None, dev, out
     ptr = _lib.ptr
-    wbuf = (workspace or Workspace()).get(lib.dsv_tree_attention_workspace_bytes(bs, T, c.heads, heads, dim), dev)
-    a = _lib.TreeAttentionArgs(
+    return _lib.TreeAttentionArgs(
         c, q_at, out_at, ptr(lse), _ACT[q.dtype], heads, rows, q_row, q_head, out_row, out_head, bs, T,
         prefix_lens.data_ptr(), ptr(verify_lens), ptr(row_offsets),
         int(row_offsets is not None and row_offsets.dtype == torch.int64), scale, ptr(masks), page_table.data_ptr(),
-        page_table.stride(0), page_table.shape[1], wbuf.data_ptr(), wbuf.numel())
-    _lib.launch("dsv_tree_attention", dev, lib.dsv_tree_attention, a)
-    return out
+        page_table.stride(0), page_table.shape[1], None, 0), dev, out
+
+
+def with_workspace(a, dev, workspace):
+    """Give a call its scratch memory; returns what holds it."""
+    nbytes = _lib.load().dsv_tree_attention_workspace_bytes(a.bs, a.T, a.cache.heads, a.q_heads, a.cache.dim)
+    buf = (workspace or Workspace()).get(nbytes, dev)
+    a.workspace, a.workspace_bytes = buf.data_ptr(), buf.numel()
+    return buf

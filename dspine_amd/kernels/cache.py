@@ -156,3 +156,44 @@ def read_kv(cache: KVCache, slots: torch.Tensor, *, dtype: torch.dtype = torch.b
     _lib.launch("dsv_kv_read", dev, _lib.load().dsv_kv_read, c, k.data_ptr(), v.data_ptr(), _OUT[k.dtype], shape[0],
                 slots.data_ptr(), i64)
     return k, v
+
+
+def slot_rows(caches):
+    """(the ``dsv_slot_rows`` of every tensor of the caches, an array of them; the tensors; the slots, which all
+    must have alike).  A cache is a ``KVCache`` or a ``BlockIndex``; one alone or a list of them."""
+    rows, tensors, slots = [], [], set()
+    for cache in caches if isinstance(caches, (list, tuple)) else [caches]:
+        if isinstance(cache, KVCache):
+            cache_fields(cache, write=True)
+            own = [t for t in tensors_of(cache) if t is not None]
+        elif getattr(cache, "bounds", None) is not None:
+            own = [cache.bounds]
+            if not cache.bounds.is_contiguous() or cache.bounds.ndim != 4:
+                raise ValueError("an index's bounds must be contiguous [rows, heads, 2, dim]")
+        else:
+            raise ValueError("caches must be KVCache or BlockIndex objects")
+        for t in own:
+            size, heads = t.element_size(), 1 if t.ndim == 4 else t.shape[1]
+            each = t[0].numel() // heads * size
+            rows.append(_lib.SlotRows(t.data_ptr(), t.stride(0) * size, t.stride(1) * size if t.ndim < 4 else 0, heads, each))
+            tensors.append(t)
+            slots.add(t.shape[0])
+    if len(slots) != 1:
+        raise ValueError("caches must have one number of slots, and there must be one")
+    return (_lib.SlotRows * len(rows))(*rows), tensors, slots.pop()
+
+
+def copy_kv(caches, src: torch.Tensor, dst: torch.Tensor, *, count: torch.Tensor | None = None) -> None:
+    """Everything that slot ``src[i]`` holds into slot ``dst[i]`` (int32 or int64 [n] each), in every one of ``caches`` (a
+    ``KVCache``, a ``BlockIndex`` or a list of them with one number of slots: a model's layers), on the current stream.
+    Pairs with a slot outside the pool are skipped; the dst must be distinct and none of them a src, or what they
+    hold is undefined.  ``count`` (int32 [1], on the device): only its first so many pairs."""
+    i64 = _check_slots(src), _check_slots(dst)
+    if src.numel() != dst.numel():
+        raise ValueError("src and dst must have one length")
+    if count is not None and (count.dtype != torch.int32 or count.numel() < 1):
+        raise ValueError("count must be int32 [1]")
+    rows, tensors, slots = slot_rows(caches)
+    dev = _lib.require_cuda(*tensors, src, dst, count)
+    _lib.launch("dsv_copy_slots", dev, _lib.load().dsv_copy_slots, rows, len(rows), slots, src.data_ptr(), i64[0],
+                dst.data_ptr(), i64[1], src.numel(), _lib.ptr(count))

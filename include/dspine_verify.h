@@ -52,6 +52,16 @@
  *   dsv_tree_masks        a drafted tree's ancestor masks and depths from its parents
  *   dsv_tree_verify       greedy acceptance of a drafted tree
  *   dsv_commit_tree       dsv_commit_accept for an accepted path of a tree
+ *
+ * Operators for long contexts and for the cache's pages around the rounds (no counterpart either):
+ *   dsv_index_blocks      the least and largest key elements of a request's finished blocks
+ *   dsv_score_blocks      a bound of every block's attention scores, from its index and the queries
+ *   dsv_select_blocks     the best blocks of each (request, cache head)
+ *   dsv_block_attention   dsv_tree_attention over selected blocks instead of the whole context
+ *   dsv_copy_slots        rows of cache slots to other slots, all layers at once
+ *   dsv_fork_requests     requests forked from others, whose slots they then share
+ *   dsv_free_requests     requests that end: the slots that nobody else holds
+ *   dsv_compact_requests  the used slots of a pool moved to its front
  */
 #ifndef DSPINE_VERIFY_H
 #define DSPINE_VERIFY_H
@@ -515,6 +525,117 @@ int dsv_commit_tree(int32_t bs, int32_t T, const int32_t* accept, const int32_t*
                     int32_t req_pool_i64, int32_t* req_to_token, int64_t rt_stride, int64_t rt_cols,
                     const int64_t* out_cache_loc, const int64_t* slot_offsets, void* seq_lens,
                     int32_t seq_lens_i64, int64_t* free_slots, int32_t* free_count, dsv_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------- */
+/* Long contexts: attention over selected blocks.                                            */
+/* ---------------------------------------------------------------------------------------- */
+/* A block is block_size (16, 32, 64 or 128) consecutive positions of a request that begin at a     */
+/* multiple of it; request b has prefix_lens[b] / block_size finished ones.  The index holds, in row */
+/* block_table[b, j] for block j, each cache head's least and largest key elements.                 */
+typedef struct dsv_block_index {
+  void* bounds;                /* [rows, heads, 2, dim] contiguous, 16-byte aligned: least, largest */
+  int32_t dtype;               /* DSV_BF16 / DSV_F16 */
+  int32_t heads, dim, block_size;
+  int64_t rows;
+} dsv_block_index;
+
+/* The bounds of the blocks that request b finished as it grew from from_lens[b] to to_lens[b]         */
+/* positions (by `longest` at most): j with from / block_size <= j < to / block_size.  Keys as          */
+/* dsv_kv_read gives them, rounded once; a NaN makes both of its element's bounds NaN.  Positions      */
+/* that hold nothing (past page_cols, slots outside the cache) do not count, a block without any      */
+/* other has zeros.  Blocks past block_cols and rows outside the index are skipped.                   */
+int dsv_index_blocks(const dsv_block_index* index, const dsv_kv_cache* cache, const int32_t* page_table,
+                     int64_t page_stride, int64_t page_cols, const int32_t* block_table, int64_t block_stride,
+                     int64_t block_cols, const int32_t* from_lens, const int32_t* to_lens, int32_t bs,
+                     int64_t longest, dsv_stream_t stream);
+
+/* scores[b, h, j] (float32 [bs, heads, block_cols], contiguous): the largest, over request b's nodes   */
+/* and the query heads of cache head h, of scale * sum_d (min(q_d, 0) least_d + max(q_d, 0) largest_d), */
+/* which no scaled score of the block's keys exceeds but for rounding; float32 sums.  -inf for blocks   */
+/* that are not finished, rows outside the index and requests without nodes; NaN where a query, a bound */
+/* or their product is.  Nodes and rows as in dsv_tree_attention; 0 < scale <= 2^100.                  */
+typedef struct dsv_score_blocks_args {
+  dsv_block_index index;
+  const void* q;               /* [rows, q_heads, dim] of the index's type, 16-byte-aligned rows */
+  float* scores;
+  int32_t q_heads, pad0;
+  int64_t rows, q_row_stride, q_head_stride;
+  int32_t bs, T;
+  const int32_t* prefix_lens;  /* [bs] */
+  const int32_t* verify_lens;  /* [bs] or NULL */
+  const void* row_offsets;     /* [bs] int32 / int64, or NULL (then rows == bs * T) */
+  int32_t row_offsets_i64;
+  float scale;
+  const int32_t* block_table;  /* [bs, block_cols] */
+  int64_t block_stride, block_cols;
+} dsv_score_blocks_args;
+int dsv_score_blocks(const dsv_score_blocks_args* args, dsv_stream_t stream);
+
+/* blocks[b, h] (int32 [count]): of the n = min(prefix_lens[b] / block_size, cols) finished blocks the   */
+/* first `first`, the last `last` and, to make `count` of them, those of the largest scores[b, h]      */
+/* (float32 [bs, heads, cols], contiguous, cols <= 32768; ties to the lowest block, NaN as -inf), in     */
+/* ascending order; -1 behind them where n < count.  first + last <= count.                           */
+int dsv_select_blocks(const float* scores, int32_t bs, int32_t heads, int64_t cols, const int32_t* prefix_lens,
+                      int32_t block_size, int32_t count, int32_t first, int32_t last, int32_t* blocks,
+                      dsv_stream_t stream);
+
+/* dsv_tree_attention where the nodes see, for cache head h, only the positions of the finished blocks  */
+/* blocks[b, h, i], i < min(count, prefix_lens[b] / block_size) (int32 [bs, heads, count]; an entry that */
+/* names no finished block holds nothing, one that names a block again counts it again), the positions  */
+/* from the last finished block's end on, and the window under its masks.  Workspace as there.          */
+typedef struct dsv_block_attention_args {
+  dsv_tree_attention_args tree;
+  const int32_t* blocks;
+  int32_t count, block_size;
+} dsv_block_attention_args;
+int dsv_block_attention(const dsv_block_attention_args* args, dsv_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------- */
+/* The life of the cache's pages (a page is a slot).                                          */
+/* ---------------------------------------------------------------------------------------- */
+/* One tensor's rows of a slot: heads rows of `bytes` bytes (whole 4-byte words), strides in bytes. */
+typedef struct dsv_slot_rows {
+  void* base;
+  int64_t slot_stride, head_stride;
+  int32_t heads, bytes;
+} dsv_slot_rows;
+
+/* Every tensor's rows of slot src[i] into slot dst[i] (int32 / int64), i < n, or i < min(n, count[0])  */
+/* (int32 on the device, may be NULL); pairs with a slot outside [0, num_slots) are skipped.  The dst    */
+/* are distinct and no dst is a src.                                                                  */
+int dsv_copy_slots(const dsv_slot_rows* rows, int32_t n_rows, int64_t num_slots, const void* src, int32_t src_i64,
+                   const void* dst, int32_t dst_i64, int64_t n, const int32_t* count, dsv_stream_t stream);
+
+/* In what follows row r of req_to_token [rows, rt_cols] holds seq_lens[r] (int32 / int64, clamped into  */
+/* [0, rt_cols]) slots, and shared[slot] (int32 [num_slots]) counts the rows beyond the first that hold */
+/* a slot.  Rows of a call outside the table are skipped, and so are slots outside the pool.            */
+/*                                                                                                   */
+/* Row children[i] becomes row parents[i]: its entries, its length, one holder more of each slot (the  */
+/* child's former entries are not released).  Children are distinct and not among the parents; a pair    */
+/* of equal rows is skipped.                                                                          */
+int dsv_fork_requests(int32_t* req_to_token, int64_t rows, int64_t rt_stride, int64_t rt_cols, void* seq_lens,
+                      int32_t seq_lens_i64, int32_t* shared, int64_t num_slots, const void* parents,
+                      const void* children, int32_t rows_i64, int64_t n, dsv_stream_t stream);
+
+/* The rows at[i] (i < n; one named again counts once) end: their lengths become 0, each slot loses a    */
+/* holder, and the slots that had no other go to free_slots (int64, ascending, `capacity` of them at   */
+/* most) and their number to free_count[0].  A negative count in shared counts as freed.               */
+int dsv_free_requests(int32_t* req_to_token, int64_t rows, int64_t rt_stride, int64_t rt_cols, void* seq_lens,
+                      int32_t seq_lens_i64, int32_t* shared, int64_t num_slots, const void* at, int32_t rows_i64,
+                      int64_t n, int64_t* free_slots, int64_t capacity, int32_t* free_count, void* workspace,
+                      int64_t workspace_bytes, dsv_stream_t stream);
+int64_t dsv_free_requests_workspace_bytes(int64_t num_slots);
+
+/* With U distinct slots in the rows at[i], i < n, which are all the rows that hold any: the used slots  */
+/* at or above U move, in ascending order, into the unused ones below U, in ascending order.  The rows' */
+/* entries, shared (may be NULL) and the tensors of slot_rows follow.  src, dst [capacity >= num_slots  */
+/* / 2]: the moves; counts [2]: U and the number of moves.                                             */
+int dsv_compact_requests(int32_t* req_to_token, int64_t rows, int64_t rt_stride, int64_t rt_cols,
+                         const void* seq_lens, int32_t seq_lens_i64, int32_t* shared, int64_t num_slots,
+                         const void* at, int32_t rows_i64, int64_t n, const dsv_slot_rows* slot_rows,
+                         int32_t n_slot_rows, int64_t* src, int64_t* dst, int64_t capacity, int32_t* counts,
+                         void* workspace, int64_t workspace_bytes, dsv_stream_t stream);
+int64_t dsv_compact_requests_workspace_bytes(int64_t num_slots);
 
 #ifdef __cplusplus
 }
