@@ -305,7 +305,7 @@ def stream_of(device: torch.device) -> int:
 def launch(what: str, device: torch.device, call, *args) -> None:
     """``call(*args, stream)`` on the device's current stream, that device being the current one
     during the call."""
-    if torch.cuda.current_device() == device.index:
+    if torch._C._cuda_getDevice() == device.index:  # (there are device tensors: torch's runtime is up)
         rc = call(*args, torch._C._cuda_getCurrentRawStream(device.index))
     else:
         with torch.cuda.device(device):
@@ -323,16 +323,17 @@ def dtype_code(t: torch.Tensor) -> int:
 
 
 def require_cuda(*tensors) -> torch.device:
-    dev = None
+    dev, index = None, -1
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
-            raise ValueError("the HIP verification path requires device (cuda) tensors")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError("all tensors must be on one device")
+        at = t.get_device()  # (-1: not on a device)
+        if at != index or at < 0:
+            if not t.is_cuda:
+                raise ValueError("the HIP verification path requires device (cuda) tensors")
+            if dev is not None:
+                raise ValueError("all tensors must be on one device")
+            dev, index = t.device, at
     if dev is None:
         raise ValueError("no device tensor given")
     return dev

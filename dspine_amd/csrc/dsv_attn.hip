@@ -47,16 +47,25 @@ __global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
     return ((int64_t)(2 * i + (i == i0 && plan.start(i) < before ? 1 : 0)) * c.heads + h) * rows + r;
   };
   float top = AT_LOW, ref = 0.f, lt = 0.f, sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (int i = i0; i <= i1; i += AJ_PARTS) {  // (the references and the sums of a few parts are asked for at once)
-    float4 ml[AJ_PARTS];
-    f32x4 x[AJ_PARTS][2];
+  // (the references and the sums of a few parts are asked for at once, those of the next few while these are added)
+  float4 next_ml[AJ_PARTS];
+  f32x4 next_x[AJ_PARTS][2];
+  auto ask = [&](int i) {
 #pragma unroll
     for (int j = 0; j < AJ_PARTS; ++j) {
       const int64_t at = part(i + j <= i1 ? i + j : i1);
-      ml[j] = P.part_ml[at];
-      x[j][0] = *reinterpret_cast<const f32x4*>(P.part_o + at * c.dim + d);
-      x[j][1] = *reinterpret_cast<const f32x4*>(P.part_o + at * c.dim + d + 4);
+      next_ml[j] = P.part_ml[at];
+      next_x[j][0] = *reinterpret_cast<const f32x4*>(P.part_o + at * c.dim + d);
+      next_x[j][1] = *reinterpret_cast<const f32x4*>(P.part_o + at * c.dim + d + 4);
     }
+  };
+  ask(i0);
+  for (int i = i0; i <= i1; i += AJ_PARTS) {
+    float4 ml[AJ_PARTS];
+    f32x4 x[AJ_PARTS][2];
+#pragma unroll
+    for (int j = 0; j < AJ_PARTS; ++j) ml[j] = next_ml[j], x[j][0] = next_x[j][0], x[j][1] = next_x[j][1];
+    if (i + AJ_PARTS <= i1) ask(i + AJ_PARTS);
     const float old = top;
 #pragma unroll
     for (int j = 0; j < AJ_PARTS; ++j) top = fmaxf(top, ml[j].x);  // (the last part again, where there are fewer)

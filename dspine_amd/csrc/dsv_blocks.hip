@@ -12,53 +12,80 @@ struct IndexParams {
   dsv_kv_cache c;
   const int32_t *page_table, *block_table, *from_lens, *to_lens;
   int64_t page_stride, page_cols, block_stride, block_cols;
-  int shift, G, most;  // block of 2^shift positions; lanes of a row; blocks a request may have finished
+  int bs, shift, most;  // block of 2^shift positions; blocks a request may have finished
 };
 
-// Bounds of a finished block, a workgroup a (block, head): groups of G lanes hold a position's row, 16 bytes a lane, and
-// run over the block's positions; the groups' results join within a wave by lane moves, the waves' through LDS.  NaN
-// counts as the least and the largest.
-template <int CT, int IT>
+// The least and largest of N elements over the lanes that differ in the bits from O down to G.  A step halves the elements
+// that a lane is left with, as long as there are any to halve: 2 N exchanges in all in place of 2 N a step.
+template <int N, int O, int G>
+__device__ __forceinline__ void join_bounds(float* lo, float* hi, int lane) {
+  if constexpr (O >= G) {
+    if constexpr (N > 1) {
+      const bool up = lane & O;
+#pragma unroll
+      for (int e = 0; e < N / 2; ++e) {
+        const float l = __shfl_xor(up ? lo[e] : lo[e + N / 2], O, WAVE), h = __shfl_xor(up ? hi[e] : hi[e + N / 2], O, WAVE);
+        lo[e] = __builtin_elementwise_minimum(up ? lo[e + N / 2] : lo[e], l);
+        hi[e] = __builtin_elementwise_maximum(up ? hi[e + N / 2] : hi[e], h);
+      }
+      join_bounds<N / 2, O / 2, G>(lo, hi, lane);
+    } else {
+      lo[0] = __builtin_elementwise_minimum(lo[0], __shfl_xor(lo[0], O, WAVE));
+      hi[0] = __builtin_elementwise_maximum(hi[0], __shfl_xor(hi[0], O, WAVE));
+      join_bounds<1, O / 2, G>(lo, hi, lane);
+    }
+  }
+}
+
+// Bounds of a finished block, a wave a (block, head): its lanes hold the block's slots, groups of G lanes take a position's
+// row, 16 bytes a lane, BI_ROWS rows in flight together.  NaN counts as the least and the largest.
+constexpr int BI_ROWS = 8;
+template <int CT, int IT, int G>
 __global__ __launch_bounds__(BI_THREADS) void k_index_blocks(IndexParams P) {
   constexpr bool QUANT = CT == DSV_E4M3 || CT == DSV_I8;
-  constexpr int EL = QUANT ? 16 : 8, ROWS = 4, NW = BI_THREADS / WAVE;
-  __shared__ float s_lo[NW][256], s_hi[NW][256];
+  constexpr int EL = QUANT ? 16 : 8, GROUPS = WAVE / G;
   const dsv_kv_cache& c = P.c;
-  const int h = (int)(blockIdx.x % (uint32_t)c.heads);
-  const uint32_t at = blockIdx.x / (uint32_t)c.heads;
-  const int b = (int)(at / (uint32_t)P.most);
+  const int lane = threadIdx.x & (WAVE - 1), l = lane & (G - 1), group = lane / G;
+  const uint32_t unit = blockIdx.x * (BI_THREADS / WAVE) + __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const uint32_t at = unit / (uint32_t)c.heads, b = at / (uint32_t)P.most;
+  const int h = (int)(unit - at * (uint32_t)c.heads);
+  if (b >= (uint32_t)P.bs) return;
   const int from = P.from_lens[b], to = P.to_lens[b];
-  const int64_t j = (int64_t)((from < 0 ? 0 : from) >> P.shift) + at % (uint32_t)P.most;
+  const int64_t j = (int64_t)((from < 0 ? 0 : from) >> P.shift) + (at - b * (uint32_t)P.most);
   if (to < 0 || j >= to >> P.shift || j >= P.block_cols) return;
   const int32_t row = P.block_table[b * P.block_stride + j];
-  if (row < 0 || row >= P.x.rows) return;
-  const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
-  const int l = tid & (P.G - 1), group = tid / P.G, groups = BI_THREADS / P.G, B = 1 << P.shift;
-  const bool in = l * EL < c.dim;
+  const int B = 1 << P.shift;
   const int64_t p0 = j << P.shift;
   const int32_t* table = P.page_table + b * P.page_stride + p0;
+  int32_t slots[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int i = k * WAVE + lane;
+    slots[k] = i < B && p0 + i < P.page_cols ? table[i] : -1;
+    if (slots[k] >= c.num_slots) slots[k] = -1;
+  }
+  if (row < 0 || row >= P.x.rows) return;
+  const bool any = __any(slots[0] >= 0 || slots[1] >= 0);
+  const bool in = l * EL < c.dim;
+  const uint8_t* base = reinterpret_cast<const uint8_t*>(c.k) + (h * c.k_head_stride + (in ? l * EL : 0)) * (QUANT ? 1 : 2);
   float lo[EL], hi[EL];
 #pragma unroll
   for (int e = 0; e < EL; ++e) lo[e] = INFINITY, hi[e] = -INFINITY;
-  bool some = false;
-  for (int i0 = group; i0 < B; i0 += groups * ROWS) {
-    uint4 x[ROWS];
-    float scale[ROWS];
-    bool has[ROWS];
+  for (int i0 = 0; i0 < B; i0 += GROUPS * BI_ROWS) {
+    uint4 x[BI_ROWS];
+    float scale[BI_ROWS];
+    bool has[BI_ROWS];
 #pragma unroll
-    for (int u = 0; u < ROWS; ++u) {
-      const int i = i0 + u * groups;
-      const int64_t slot = i < B && p0 + i < P.page_cols ? table[i] : -1;
-      has[u] = slot >= 0 && slot < c.num_slots;
+    for (int u = 0; u < BI_ROWS; ++u) {
+      const int i = i0 + u * GROUPS + group;
+      const int32_t slot = i < B ? __shfl(i < WAVE ? slots[0] : slots[1], i & (WAVE - 1), WAVE) : -1;
+      has[u] = slot >= 0;
       const int64_t s = has[u] ? slot : 0;
-      x[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(c.k) +
-                                             (s * c.k_slot_stride + h * c.k_head_stride + (in ? l * EL : 0)) * (QUANT ? 1 : 2));
+      x[u] = *reinterpret_cast<const uint4*>(base + s * c.k_slot_stride * (QUANT ? 1 : 2));
       if constexpr (QUANT) scale[u] = c.k_scale[s * c.ks_slot_stride + h * c.ks_head_stride];
     }
 #pragma unroll
-    for (int u = 0; u < ROWS; ++u) {
-      if (!has[u]) continue;
-      some = true;
+    for (int u = 0; u < BI_ROWS; ++u) {
       const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
       float f[EL];
 #pragma unroll
@@ -72,40 +99,34 @@ __global__ __launch_bounds__(BI_THREADS) void k_index_blocks(IndexParams P) {
           f[2 * i + 1] = act_to_f32<CT>(w[i] >> 16);
         }
       }
+      if (has[u])
 #pragma unroll
-      for (int e = 0; e < EL; ++e) {
-        lo[e] = __builtin_elementwise_minimum(lo[e], f[e]);
-        hi[e] = __builtin_elementwise_maximum(hi[e], f[e]);
-      }
+        for (int e = 0; e < EL; ++e) {
+          lo[e] = __builtin_elementwise_minimum(lo[e], f[e]);
+          hi[e] = __builtin_elementwise_maximum(hi[e], f[e]);
+        }
     }
   }
-  for (int o = P.G; o < WAVE; o *= 2) {
+  join_bounds<EL, WAVE / 2, G>(lo, hi, lane);
+  // what is left of the lane's elements, and where: the highest lane bits chose the halves
+  constexpr int STEPS = G == 32 ? 1 : (G == 16 ? 2 : (G == 8 ? 3 : 4)), HALVED = EL == 8 && STEPS > 3 ? 3 : STEPS;
+  constexpr int LEFT = EL >> HALVED;
+  int d = l * EL;
 #pragma unroll
-    for (int e = 0; e < EL; ++e) {
-      lo[e] = __builtin_elementwise_minimum(lo[e], __shfl_xor(lo[e], o, WAVE));
-      hi[e] = __builtin_elementwise_maximum(hi[e], __shfl_xor(hi[e], o, WAVE));
+  for (int k = 0; k < HALVED; ++k) d += lane & (WAVE / 2 >> k) ? EL >> (k + 1) : 0;
+  const bool first = (lane & (WAVE / (1 << HALVED) - 1) & ~(G - 1)) == 0;  // (of the lanes that hold the same)
+  if (!in || !first) return;
+  uint16_t* out = reinterpret_cast<uint16_t*>(P.x.bounds) + ((int64_t)row * c.heads + h) * 2 * c.dim + d;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const float* v = k ? hi : lo;
+    if constexpr (LEFT >= 2) {
+#pragma unroll
+      for (int e = 0; e < LEFT; e += 2)
+        *reinterpret_cast<uint32_t*>(out + k * c.dim + e) = any ? pack_act<IT>(v[e], v[e + 1]) : 0u;
+    } else {
+      out[k * c.dim] = any ? (uint16_t)pack_act<IT>(v[0], 0.f) : (uint16_t)0;
     }
-  }
-  if (in && lane < P.G) {
-#pragma unroll
-    for (int e = 0; e < EL; ++e) s_lo[wave][l * EL + e] = lo[e], s_hi[wave][l * EL + e] = hi[e];
-  }
-  const bool any = __syncthreads_or(some);
-  // element pairs: the least ones, then the largest
-  for (int i = tid; i < c.dim; i += BI_THREADS) {
-    const bool high = i >= c.dim / 2;
-    const int d = (high ? i - c.dim / 2 : i) * 2;
-    float v[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float a = high ? s_hi[0][d + k] : s_lo[0][d + k];
-#pragma unroll
-      for (int w = 1; w < NW; ++w)
-        a = high ? __builtin_elementwise_maximum(a, s_hi[w][d + k]) : __builtin_elementwise_minimum(a, s_lo[w][d + k]);
-      v[k] = any ? a : 0.f;
-    }
-    uint32_t* out = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(P.x.bounds) + ((int64_t)row * c.heads + h) * 2 * c.dim);
-    out[i] = pack_act<IT>(v[0], v[1]);
   }
 }
 
@@ -115,8 +136,9 @@ __global__ __launch_bounds__(BI_THREADS) void k_index_blocks(IndexParams P) {
 // columns; a block's score is the largest of its columns'.
 // ---------------------------------------------------------------------------------------
 constexpr int SB_THREADS = 256, SB_WAVES = SB_THREADS / WAVE;
-constexpr int SB_STAGE = 64 * 1024 / 1024;  // query operands of 1 KB in LDS
-constexpr int SB_STEPS = 4;                 // steps of a workgroup at most
+constexpr int SB_STAGE = 60;  // pieces of 16 queries' 32 elements (1 KB) in LDS at most
+constexpr int SB_STEP = SB_WAVES * 16;  // blocks of a step: 16 a wave (32, with fewer steps: 43 us for 41)
+constexpr int SB_STEPS = 8;             // steps of a workgroup at most
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
@@ -126,6 +148,7 @@ struct ScoreParams {
   dsv_score_blocks_args a;
   FastDiv G;
   int shift, steps, chunks;  // steps of a workgroup, workgroups of a (request, head)
+  int staged;                // query tiles in LDS at once
 };
 
 template <int IT>
@@ -136,127 +159,129 @@ __device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
 }
 
-// The positive (or negative) elements of a pair, zeros in place of the others; NaN stays.
-template <int IT>
-__device__ __forceinline__ uint32_t half_of(uint32_t w, bool positive) {
-  constexpr uint32_t INF = IT == DSV_BF16 ? 0x7f80u : 0x7c00u;
-  uint32_t keep = 0;
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t x = (w >> (16 * i)) & 0xffffu;
-    if ((x >> 15 != 0) != positive || (x & 0x7fffu) > INF) keep |= 0xffffu << (16 * i);
-  }
-  return w & keep;
+// A pair's negative and positive elements, zeros in place of the others (a NaN stays in one of them).
+__device__ __forceinline__ void split_signs(uint32_t w, uint32_t& negative, uint32_t& positive) {
+  typedef short short2v __attribute__((ext_vector_type(2)));
+  const uint32_t sign = __builtin_bit_cast(uint32_t, __builtin_bit_cast(short2v, w) >> 15);
+  negative = w & sign;
+  positive = w & ~sign;
 }
 
-template <int IT, int NK, bool FULL>
-__global__ __launch_bounds__(SB_THREADS, 2) void k_score_blocks(ScoreParams P) {
+// A workgroup some steps of a (request, head)'s blocks, its queries as operands in LDS; a wave 16 blocks a step, their
+// bounds in registers for all of the queries.
+template <int IT, int NC, bool FULL>
+__global__ __launch_bounds__(SB_THREADS) void k_score_blocks(ScoreParams P) {
   const dsv_score_blocks_args& a = P.a;
   const dsv_block_index& x = a.index;
-  const int nk = FULL ? NK : x.dim / 16;        // products of 32 of the row's 2 * dim elements
-  constexpr int TB = NK > 8 ? 1 : 2;            // tiles of 16 blocks a wave
-  constexpr int STEP = SB_WAVES * TB * 16;
-  constexpr int TILES = SB_STAGE / NK;          // query tiles staged at once
-  __shared__ uint4 s_q[TILES * NK][WAVE];
-  __shared__ float s_best[SB_STEPS * STEP];
+  const int dim = FULL ? NC * 32 : x.dim;
+  constexpr int AHEAD = 8;            // pieces of queries in flight
+  extern __shared__ uint4 s_q[];      // [staged * NC][WAVE]
+  __shared__ float s_best[SB_STEPS * SB_STEP];
   const int tid = threadIdx.x, lane = tid & (WAVE - 1);
   const int wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
   const int m = lane & 15, g = lane >> 4;
-  const int chunk = (int)(blockIdx.x % (uint32_t)P.chunks);
-  const uint32_t bh = blockIdx.x / (uint32_t)P.chunks;
+  // (the first chunks of all, then the second ones: neighbouring workgroups go to different XCDs, and chunk by chunk the XCDs
+  // with the last ones of every request had least to do: 52 us for 43)
+  const uint32_t bhs = (uint32_t)a.bs * (uint32_t)x.heads, bh = blockIdx.x % bhs;
+  const int chunk = (int)(blockIdx.x / bhs);
   const int b = (int)(bh / (uint32_t)x.heads), h = (int)(bh - (uint32_t)b * x.heads);
   const int pre = a.prefix_lens[b];
   const int64_t full = pre < 0 ? 0 : pre >> P.shift;
   int n = a.verify_lens ? a.verify_lens[b] : a.T;
   n = n < 0 ? 0 : (n > a.T ? a.T : n);
   const int rows = n * (int)P.G.d, tiles = (rows + 15) / 16;
-  const int64_t cols = a.block_cols, first = (int64_t)chunk * P.steps * STEP;
-  const int64_t past = first + P.steps * STEP < cols ? first + P.steps * STEP : cols;  // of the table
+  const int64_t cols = a.block_cols, first = (int64_t)chunk * P.steps * SB_STEP;
+  const int64_t past = first + P.steps * SB_STEP < cols ? first + P.steps * SB_STEP : cols;  // of the table
   const int64_t end = rows == 0 ? first : (past < full ? past : full);               // of the blocks that have a score
   float* const out = a.scores + (int64_t)bh * cols;
   const int32_t* const table = a.block_table + b * a.block_stride;
   const int64_t row0 = a.row_offsets ? load_index(a.row_offsets, a.row_offsets_i64, b) : (int64_t)b * a.T;
   for (int64_t i = (end > first ? end : first) + tid; i < past; i += SB_THREADS) out[i] = -INFINITY;
   if (end <= first) return;
-  for (int t0 = 0; t0 < tiles; t0 += TILES) {
-    const int here = tiles - t0 < TILES ? tiles - t0 : TILES;
+  uint4 k[NC][2];
+  bool there = false;
+  // a step's bounds: lane (m, g) elements g * 8 .. of each 32 of block m's
+  auto load = [&](int64_t j0) {
+    const int64_t j = j0 + m;
+    const int32_t row = j < end ? table[j] : -1;
+    there = row >= 0 && row < x.rows;
+    const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(x.bounds) +
+                                                       ((int64_t)(there ? row : 0) * x.heads + h) * 2 * dim);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const bool in = FULL || c * 32 + g * 8 < dim;
+      const int at = in ? c * 4 + g : 0;
+      k[c][0] = from[at];
+      k[c][1] = from[dim / 8 + at];
+      if (!in) k[c][0] = k[c][1] = make_uint4(0, 0, 0, 0);
+    }
+  };
+  for (int t0 = 0; t0 < tiles; t0 += P.staged) {
+    const int here = tiles - t0 < P.staged ? tiles - t0 : P.staged;
     if (t0) __syncthreads();
-    for (int i = wave; i < here * nk; i += SB_WAVES) {
-      const int t = i / nk, kk = i - t * nk;
-      int r = (t0 + t) * 16 + m;
-      r = r < rows ? r : rows - 1;  // (a row again: the largest stays the largest)
-      const int node = (int)P.G.div((uint32_t)r), head = h * (int)P.G.d + r - node * (int)P.G.d;
-      const int64_t row = row0 + node;
-      const int e = kk * 32 + g * 8;
-      const bool positive = e >= x.dim;
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (row >= 0 && row < a.rows)
-        w = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + row * a.q_row_stride +
-                                            head * a.q_head_stride + (positive ? e - x.dim : e));
-      s_q[t * NK + kk][lane] = make_uint4(half_of<IT>(w.x, positive), half_of<IT>(w.y, positive),
-                                          half_of<IT>(w.z, positive), half_of<IT>(w.w, positive));
+    // (the first step's bounds are asked for behind the first queries)
+    for (int i0 = wave; i0 < here * NC || i0 == wave; i0 += SB_WAVES * AHEAD) {
+      uint4 w[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int i = i0 + u * SB_WAVES, t = i / NC, c = i - t * NC;
+        int r = (t0 + t) * 16 + m;
+        r = r < rows ? r : rows - 1;  // (a row again: the largest stays the largest)
+        const int node = (int)P.G.div((uint32_t)r), head = h * (int)P.G.d + r - node * (int)P.G.d;
+        const int64_t row = row0 + node;
+        const int d = c * 32 + g * 8;
+        w[u] = make_uint4(0, 0, 0, 0);
+        if (i < here * NC && row >= 0 && row < a.rows && (FULL || d < dim))
+          w[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + row * a.q_row_stride +
+                                                 head * a.q_head_stride + d);
+      }
+      if (i0 == wave) load(first + wave * 16);
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u)
+        if (i0 + u * SB_WAVES < here * NC) s_q[(i0 + u * SB_WAVES) * WAVE + lane] = w[u];
     }
     __syncthreads();
     for (int step = 0; step < P.steps; ++step) {
-      const int64_t j0 = first + step * STEP + wave * TB * 16;
+      const int64_t j0 = first + step * SB_STEP + wave * 16;
       if (j0 >= end) break;
-      uint4 k[TB][NK];
-      bool there[TB];
-#pragma unroll
-      for (int t = 0; t < TB; ++t) {
-        const int64_t j = j0 + t * 16 + m;
-        const int32_t row = j < end ? table[j] : -1;
-        there[t] = row >= 0 && row < x.rows;
-        const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(x.bounds) +
-                                                           ((int64_t)(there[t] ? row : 0) * x.heads + h) * 2 * x.dim) + g;
-#pragma unroll
-        for (int kk = 0; kk < NK; ++kk)
-          if (FULL || kk < nk) k[t][kk] = from[kk * 4];
-      }
-      f32x4 best[TB];
-#pragma unroll
-      for (int t = 0; t < TB; ++t) best[t] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      f32x4 best = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       for (int rt = 0; rt < here; ++rt) {
-        f32x4 s[TB];
+        f32x4 s = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int t = 0; t < TB; ++t) s[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kk = 0; kk < NK; ++kk) {
-          if (FULL || kk < nk) {
-            const uint4 q = s_q[rt * NK + kk][lane];
-#pragma unroll
-            for (int t = 0; t < TB; ++t) s[t] = mfma16<IT>(k[t][kk], q, s[t]);
-          }
+        for (int c = 0; c < NC; ++c) {
+          const uint4 q = s_q[(rt * NC + c) * WAVE + lane];
+          uint4 low, high;
+          split_signs(q.x, low.x, high.x);
+          split_signs(q.y, low.y, high.y);
+          split_signs(q.z, low.z, high.z);
+          split_signs(q.w, low.w, high.w);
+          s = mfma16<IT>(k[c][0], low, s);
+          s = mfma16<IT>(k[c][1], high, s);
         }
 #pragma unroll
-        for (int t = 0; t < TB; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) best[t][r] = __builtin_elementwise_maximum(best[t][r], s[t][r]);
+        for (int r = 0; r < 4; ++r) best[r] = __builtin_elementwise_maximum(best[r], s[r]);
       }
+      const bool has = __shfl((int)there, g * 4 + (m & 3), WAVE) != 0;  // (lane i knows block i)
+      if (step + 1 < P.steps && j0 + SB_STEP < end) load(j0 + SB_STEP);
+      // the 16 columns of a row lie in 16 neighbouring lanes; lane (r, g) keeps row g * 4 + r
+      float mine = 0.f;
 #pragma unroll
-      for (int t = 0; t < TB; ++t) {
-        // the 16 columns of a row lie in 16 neighbouring lanes; lane (r, g) keeps row g * 4 + r
-        float mine = 0.f;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float v = best[t][r];
-          v = __builtin_elementwise_maximum(v, dpp<DPP_QUAD_XOR1>(v, v));
-          v = __builtin_elementwise_maximum(v, dpp<DPP_QUAD_XOR2>(v, v));
-          v = __builtin_elementwise_maximum(v, dpp<DPP_ROW_HALF_MIRROR>(v, v));
-          v = __builtin_elementwise_maximum(v, dpp<DPP_ROW_MIRROR>(v, v));
-          mine = m == r ? v : mine;
-        }
-        // (lane i of the tile knows whether block i is there)
-        const bool has = __shfl((int)there[t], g * 4 + (m & 3), WAVE) != 0;
-        const int64_t j = j0 + t * 16 + g * 4 + m;
-        if (m < 4 && j < end) {
-          const int at = (int)(j - first);
-          if (t0) mine = __builtin_elementwise_maximum(mine, s_best[at]);
-          if (t0 + here < tiles)
-            s_best[at] = mine;  // (read by the same lane)
-          else
-            out[j] = has ? mine * a.scale : -INFINITY;
-        }
+      for (int r = 0; r < 4; ++r) {
+        float v = best[r];
+        v = __builtin_elementwise_maximum(v, dpp<DPP_QUAD_XOR1>(v, v));
+        v = __builtin_elementwise_maximum(v, dpp<DPP_QUAD_XOR2>(v, v));
+        v = __builtin_elementwise_maximum(v, dpp<DPP_ROW_HALF_MIRROR>(v, v));
+        v = __builtin_elementwise_maximum(v, dpp<DPP_ROW_MIRROR>(v, v));
+        mine = m == r ? v : mine;
+      }
+      const int64_t j = j0 + g * 4 + m;
+      if (m < 4 && j < end) {
+        const int at = (int)(j - first);
+        if (t0) mine = __builtin_elementwise_maximum(mine, s_best[at]);
+        if (t0 + here < tiles)
+          s_best[at] = mine;  // (read by the same lane)
+        else
+          out[j] = has ? mine * a.scale : -INFINITY;
       }
     }
   }
@@ -458,31 +483,36 @@ extern "C" int dsv_index_blocks(const dsv_block_index* index, const dsv_kv_cache
   if (bs == 0 || longest == 0) return DSV_OK;
   if (!page_table || !block_table || !from_lens || !to_lens || page_cols < 1 || block_cols < 1)
     DSV_FAIL(DSV_ERR_INVALID, "dsv_index_blocks: tables and lengths are required");
-  IndexParams P{*index, *cache, page_table, block_table, from_lens, to_lens, page_stride, page_cols, block_stride, block_cols, 0, 0, 0};
+  IndexParams P{*index, *cache, page_table, block_table, from_lens, to_lens, page_stride, page_cols, block_stride, block_cols, bs, 0, 0};
   P.shift = __builtin_ctz((unsigned)index->block_size);
   int64_t most = longest > 0x7fffffff ? 0x7fffffff : longest;
   most = (most + index->block_size - 1) >> P.shift;  // (a growth of n positions finishes ceil(n / size) blocks at most)
   if (most > block_cols) most = block_cols;
-  const int64_t grid = most * bs * cache->heads;
-  if (grid > 0x7fffffffll) DSV_FAIL(DSV_ERR_INVALID, "dsv_index_blocks: too many blocks for one call");
+  const int64_t units = most * bs * cache->heads, grid = (units + BI_THREADS / WAVE - 1) / (BI_THREADS / WAVE);
+  if (units > 0x7fffffffll) DSV_FAIL(DSV_ERR_INVALID, "dsv_index_blocks: too many blocks for one call");
   P.most = (int)most;
-  const bool quant = cache->dtype == DSV_E4M3 || cache->dtype == DSV_I8;
-  P.G = 1;
-  while (P.G * (quant ? 16 : 8) < cache->dim) P.G *= 2;
-  auto launch = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(BI_THREADS), 0, stream, P); };
   const bool bf = index->dtype == DSV_BF16;
-  auto to = [&](auto ct) {
-    constexpr int CT = decltype(ct)::value;
-    bf ? launch(k_index_blocks<CT, DSV_BF16>) : launch(k_index_blocks<CT, DSV_F16>);
+  auto to = [&](auto ct, auto g) {
+    auto launch = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(BI_THREADS), 0, stream, P); };
+    constexpr int CT = decltype(ct)::value, G = decltype(g)::value;
+    bf ? launch(k_index_blocks<CT, DSV_BF16, G>) : launch(k_index_blocks<CT, DSV_F16, G>);
+  };
+  // (lanes of a row)
+  auto width = [&](auto ct) {
+    constexpr int CT = decltype(ct)::value, EL = CT == DSV_E4M3 || CT == DSV_I8 ? 16 : 8;
+    const int lanes = (cache->dim + EL - 1) / EL;
+    if constexpr (EL == 8)
+      if (lanes > 16) return to(ct, Int<32>{});
+    lanes > 8 ? to(ct, Int<16>{}) : (lanes > 4 ? to(ct, Int<8>{}) : to(ct, Int<4>{}));
   };
   if (cache->dtype == DSV_BF16)
-    to(Int<DSV_BF16>{});
+    width(Int<DSV_BF16>{});
   else if (cache->dtype == DSV_F16)
-    to(Int<DSV_F16>{});
+    width(Int<DSV_F16>{});
   else if (cache->dtype == DSV_E4M3)
-    to(Int<DSV_E4M3>{});
+    width(Int<DSV_E4M3>{});
   else
-    to(Int<DSV_I8>{});
+    width(Int<DSV_I8>{});
   DSV_CHECK_LAUNCH("k_index_blocks");
   return DSV_OK;
 }
@@ -506,22 +536,25 @@ extern "C" int dsv_score_blocks(const dsv_score_blocks_args* args, dsv_stream_t 
   P.a = a;
   P.G = fast_div((uint32_t)(a.q_heads / a.index.heads));
   P.shift = __builtin_ctz((unsigned)a.index.block_size);
-  const int step = SB_WAVES * 16 * (a.index.dim > 128 ? 1 : 2);
-  const int64_t steps = (a.block_cols + step - 1) / step, bh = (int64_t)a.bs * a.index.heads;
-  const int64_t per = steps * bh / 2048;
+  const int64_t steps = (a.block_cols + SB_STEP - 1) / SB_STEP, bh = (int64_t)a.bs * a.index.heads;
+  const int64_t per = steps * bh / 4096;  // (half and twice as many workgroups: 44 and 42 us for 41)
   P.steps = (int)(per < 1 ? 1 : (per > SB_STEPS ? SB_STEPS : per));
   P.chunks = (int)((steps + P.steps - 1) / P.steps);
   if (bh * P.chunks > 0x7fffffffll) DSV_FAIL(DSV_ERR_INVALID, "dsv_score_blocks: too many blocks for one call");
-  auto launch = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)(bh * P.chunks)), dim3(SB_THREADS), 0, stream, P); };
+  const int tiles = (a.T * (int)P.G.d + 15) / 16;
+  auto launch = [&](auto kern, int pieces) {
+    P.staged = tiles < SB_STAGE / pieces ? tiles : SB_STAGE / pieces;
+    hipLaunchKernelGGL(kern, dim3((unsigned)(bh * P.chunks)), dim3(SB_THREADS), (unsigned)(P.staged * pieces) * 1024u, stream, P);
+  };
   auto type = [&](auto it) {
     constexpr int IT = decltype(it)::value;
     const int D = a.index.dim;
     if (D <= 64)
-      D == 64 ? launch(k_score_blocks<IT, 4, true>) : launch(k_score_blocks<IT, 4, false>);
+      D == 64 ? launch(k_score_blocks<IT, 2, true>, 2) : launch(k_score_blocks<IT, 2, false>, 2);
     else if (D <= 128)
-      D == 128 ? launch(k_score_blocks<IT, 8, true>) : launch(k_score_blocks<IT, 8, false>);
+      D == 128 ? launch(k_score_blocks<IT, 4, true>, 4) : launch(k_score_blocks<IT, 4, false>, 4);
     else
-      D == 256 ? launch(k_score_blocks<IT, 16, true>) : launch(k_score_blocks<IT, 16, false>);
+      D == 256 ? launch(k_score_blocks<IT, 8, true>, 8) : launch(k_score_blocks<IT, 8, false>, 8);
   };
   a.index.dtype == DSV_BF16 ? type(Int<DSV_BF16>{}) : type(Int<DSV_F16>{});
   DSV_CHECK_LAUNCH("k_score_blocks");

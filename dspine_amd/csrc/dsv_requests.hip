@@ -32,42 +32,93 @@ struct TableParams {
   int64_t chunks;
 };
 
-// A workgroup a (pair, 256 columns).  Pairs of one parent in a row count its slots together, the first for all.
-__global__ __launch_bounds__(RQ_THREADS) void k_fork(TableParams P, const void* children) {
-  const int64_t i = blockIdx.x / P.chunks, chunk = blockIdx.x - i * P.chunks;
-  auto pair = [&](int64_t k, int64_t& parent, int64_t& child) {
-    parent = load_index(P.at, P.rows_i64, k);
-    child = load_index(children, P.rows_i64, k);
-    return parent >= 0 && parent < P.rows && child >= 0 && child < P.rows && child != parent;
-  };
-  int64_t parent, child, other, unused;
-  if (!pair(i, parent, child)) return;
-  const int64_t len = held(P.lens, P.lens_i64, parent, P.cols), p = chunk * RQ_THREADS + threadIdx.x;
-  if (p == 0) set_len(P.lens, P.lens_i64, child, len);
-  if (chunk * RQ_THREADS >= len) return;
-  int times = 1;
-  if (i > 0 && pair(i - 1, other, unused) && other == parent)
-    times = 0;
-  else
-    while (i + times < P.n && pair(i + times, other, unused) && other == parent) ++times;
-  if (p >= len) return;
-  const int32_t slot = P.table[parent * P.stride + p];
-  P.table[child * P.stride + p] = slot;
-  if (times && slot >= 0 && slot < P.num_slots) atomicAdd(&P.shared[slot], times);
+// Samples of one prompt hold its slots at the same positions, so a thread takes its column's entries of RQ_ROWS rows and
+// counts equal ones together: what bounds a fork or a release of long prompts is the atomics on scattered slots (27 G/s;
+// 128 rows of 20000 positions, two of each prompt: 96 us with one for every entry, MEASURE us so).
+constexpr int RQ_ROWS = 8;
+__device__ __forceinline__ void add_holders(const TableParams& P, int32_t (&slot)[RQ_ROWS], int sign) {
+  int times[RQ_ROWS];
+#pragma unroll
+  for (int r = 0; r < RQ_ROWS; ++r) {
+    times[r] = slot[r] >= 0 && slot[r] < P.num_slots;
+#pragma unroll
+    for (int k = 0; k < r; ++k) {
+      const bool same = times[r] && times[k] && slot[k] == slot[r];
+      times[k] += same;
+      times[r] = same ? 0 : times[r];
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < RQ_ROWS; ++r)
+    if (times[r]) atomicAdd(&P.shared[slot[r]], sign * times[r]);
 }
 
-// A workgroup a (row, 256 columns); a row named before is left out.
+// A workgroup RQ_ROWS pairs' 256 columns.
+__global__ __launch_bounds__(RQ_THREADS) void k_fork(TableParams P, const void* children) {
+  const int64_t group = blockIdx.x / P.chunks, chunk = blockIdx.x - group * P.chunks;
+  const int64_t p = chunk * RQ_THREADS + threadIdx.x;
+  int32_t slot[RQ_ROWS];
+  int64_t child[RQ_ROWS];
+#pragma unroll
+  for (int r = 0; r < RQ_ROWS; ++r) {
+    const int64_t i = group * RQ_ROWS + r;
+    const int64_t parent = i < P.n ? load_index(P.at, P.rows_i64, i) : -1;
+    child[r] = i < P.n ? load_index(children, P.rows_i64, i) : -1;
+    if (parent < 0 || parent >= P.rows || child[r] < 0 || child[r] >= P.rows || child[r] == parent) child[r] = -1;
+    const int64_t len = child[r] < 0 ? 0 : held(P.lens, P.lens_i64, parent, P.cols);
+    if (p == 0 && child[r] >= 0) set_len(P.lens, P.lens_i64, child[r], len);
+    if (p >= len) child[r] = -1;
+    slot[r] = child[r] < 0 ? -1 : P.table[parent * P.stride + p];
+  }
+#pragma unroll
+  for (int r = 0; r < RQ_ROWS; ++r)
+    if (child[r] >= 0) P.table[child[r] * P.stride + p] = slot[r];
+  add_holders(P, slot, 1);
+}
+
+// The rows of a group that are named before, as bits (every thread of the workgroup).
+__device__ __forceinline__ uint32_t named_before(const TableParams& P, int64_t first, uint32_t* scratch) {
+  int64_t row[RQ_ROWS];
+#pragma unroll
+  for (int r = 0; r < RQ_ROWS; ++r) row[r] = first + r < P.n ? load_index(P.at, P.rows_i64, first + r) : -1;
+  uint32_t again = 0;
+#pragma unroll
+  for (int r = 1; r < RQ_ROWS; ++r)
+#pragma unroll
+    for (int k = 0; k < r; ++k) again |= (row[k] == row[r] ? 1u : 0u) << r;
+  uint32_t mine = 0;
+  for (int64_t k = threadIdx.x; k < first; k += blockDim.x) {
+    const int64_t other = load_index(P.at, P.rows_i64, k);
+#pragma unroll
+    for (int r = 0; r < RQ_ROWS; ++r) mine |= (other == row[r] ? 1u : 0u) << r;
+  }
+  if (first == 0) return again;
+  if (threadIdx.x == 0) *scratch = 0;
+  __syncthreads();
+  if (mine) atomicOr(scratch, mine);
+  __syncthreads();
+  again |= *scratch;
+  __syncthreads();
+  return again;
+}
+
+// A column's entries of a group of rows, those named before left out.
+__device__ __forceinline__ void release_column(const TableParams& P, int64_t first, uint32_t again, int64_t p) {
+  int32_t slot[RQ_ROWS];
+#pragma unroll
+  for (int r = 0; r < RQ_ROWS; ++r) {
+    const int64_t row = first + r < P.n && !((again >> r) & 1) ? load_index(P.at, P.rows_i64, first + r) : -1;
+    const int64_t len = row < 0 || row >= P.rows ? 0 : held(P.lens, P.lens_i64, row, P.cols);
+    slot[r] = p < len ? P.table[row * P.stride + p] : -1;
+  }
+  add_holders(P, slot, -1);
+}
+
 __global__ __launch_bounds__(RQ_THREADS) void k_release(TableParams P) {
-  const int64_t i = blockIdx.x / P.chunks, chunk = blockIdx.x - i * P.chunks;
-  const int64_t row = load_index(P.at, P.rows_i64, i);
-  if (row < 0 || row >= P.rows) return;
-  const int64_t len = held(P.lens, P.lens_i64, row, P.cols), p = chunk * RQ_THREADS + threadIdx.x;
-  if (chunk * RQ_THREADS >= len) return;
-  bool again = false;
-  for (int64_t k = threadIdx.x; k < i; k += RQ_THREADS) again |= load_index(P.at, P.rows_i64, k) == row;
-  if (__syncthreads_or(again) || p >= len) return;
-  const int32_t slot = P.table[row * P.stride + p];
-  if (slot >= 0 && slot < P.num_slots) atomicSub(&P.shared[slot], 1);
+  __shared__ uint32_t s_again;
+  const int64_t group = blockIdx.x / P.chunks, chunk = blockIdx.x - group * P.chunks;
+  const uint32_t again = named_before(P, group * RQ_ROWS, &s_again);
+  release_column(P, group * RQ_ROWS, again, chunk * RQ_THREADS + threadIdx.x);
 }
 
 // Slots below zero in each chunk of the pool; the rows' lengths become zero.
@@ -110,6 +161,36 @@ __global__ __launch_bounds__(RQ_THREADS) void k_emit_freed(TableParams P, const 
   for (int k = 0; k < 16; ++k) freed |= (s0 + k < P.num_slots && P.shared[s0 + k] < 0 ? 1u : 0u) << k;
   int64_t at = before + block_excl_scan<RQ_THREADS / WAVE>((int)__popc(freed), s_red, (int*)nullptr);
   for (int k = 0; k < 16; ++k) {
+    if (!((freed >> k) & 1)) continue;
+    P.shared[s0 + k] = 0;
+    if (at < capacity) free_slots[at] = s0 + k;
+    ++at;
+  }
+}
+
+// A few rows of a small pool, all of it in one workgroup (RQ_SMALL_ENTRIES columns of rows, RQ_SMALL_SLOTS slots at most): a
+// launch in place of three.
+constexpr int RQ_WIDE = 1024, RQ_SMALL_ENTRIES = 8 * RQ_WIDE, RQ_SMALL_SLOTS = 16 * RQ_WIDE;
+__global__ __launch_bounds__(RQ_WIDE) void k_free_small(TableParams P, int64_t* free_slots, int64_t capacity, int32_t* free_count) {
+  __shared__ int s_red[RQ_WIDE / WAVE];
+  __shared__ uint32_t s_again;
+  for (int64_t first = 0; first < P.n; first += RQ_ROWS) {
+    const uint32_t again = named_before(P, first, &s_again);
+    for (int64_t p = threadIdx.x; p < P.cols; p += RQ_WIDE) release_column(P, first, again, p);
+  }
+  publish_wait();  // (the counts have reached what the loads below read)
+  __syncthreads();
+  for (int64_t k = threadIdx.x; k < P.n; k += RQ_WIDE) {
+    const int64_t row = load_index(P.at, P.rows_i64, k);
+    if (row >= 0 && row < P.rows) set_len(P.lens, P.lens_i64, row, 0);
+  }
+  const int per = (int)((P.num_slots + RQ_WIDE - 1) / RQ_WIDE), s0 = (int)threadIdx.x * per;
+  uint32_t freed = 0;
+  for (int k = 0; k < per; ++k) freed |= (s0 + k < P.num_slots && ld_dev(P.shared + s0 + k) < 0 ? 1u : 0u) << k;
+  int total;
+  int64_t at = block_excl_scan<RQ_WIDE / WAVE>((int)__popc(freed), s_red, &total);
+  if (threadIdx.x == 0) *free_count = total;
+  for (int k = 0; k < per; ++k) {
     if (!((freed >> k) & 1)) continue;
     P.shared[s0 + k] = 0;
     if (at < capacity) free_slots[at] = s0 + k;
@@ -192,27 +273,55 @@ __global__ __launch_bounds__(RQ_THREADS) void k_plan_moves(CompactParams P) {
   }
 }
 
-// The rows' entries follow the moves, and so do the counts of holders (the grid's last rows).
-__global__ __launch_bounds__(RQ_THREADS) void k_follow_moves(CompactParams P) {
-  const int64_t i = blockIdx.x / P.t.chunks, chunk = blockIdx.x - i * P.t.chunks;
-  const int64_t p = chunk * RQ_THREADS + threadIdx.x;
-  const int32_t U = P.out[0], moved = P.out[1];
-  if (i >= P.t.n) {  // (one row of workgroups more)
-    if (P.t.shared)
-      for (int64_t k = p; k < moved; k += P.t.chunks * RQ_THREADS) {
-        const int64_t from = P.src[k];
-        P.t.shared[P.dst[k]] = P.t.shared[from];
-        P.t.shared[from] = 0;
-      }
-    return;
+// The same for a small pool and few rows, in one workgroup, the used slots as bits in its LDS: a launch in place of four.
+constexpr int RQ_BITS = 2 * 16 * RQ_WIDE;  // slots at most
+__global__ __launch_bounds__(RQ_WIDE) void k_plan_small(CompactParams P) {
+  __shared__ uint32_t s_bits[RQ_BITS / 32];
+  __shared__ int s_red[RQ_WIDE / WAVE];
+  const TableParams& t = P.t;
+  const int tid = threadIdx.x;
+  static_assert(RQ_BITS / 32 == RQ_WIDE, "a word a thread");
+  s_bits[tid] = 0;
+  __syncthreads();
+  for (int64_t first = 0; first < t.n; first += RQ_ROWS) {
+    int64_t row[RQ_ROWS], len[RQ_ROWS];
+#pragma unroll
+    for (int r = 0; r < RQ_ROWS; ++r) row[r] = first + r < t.n ? load_index(t.at, t.rows_i64, first + r) : -1;
+#pragma unroll
+    for (int r = 0; r < RQ_ROWS; ++r) len[r] = row[r] < 0 || row[r] >= t.rows ? 0 : held(t.lens, t.lens_i64, row[r], t.cols);
+    for (int64_t p = tid; p < t.cols; p += RQ_WIDE) {
+      int32_t slot[RQ_ROWS];
+#pragma unroll
+      for (int r = 0; r < RQ_ROWS; ++r) slot[r] = p < len[r] ? t.table[row[r] * t.stride + p] : -1;
+#pragma unroll
+      for (int r = 0; r < RQ_ROWS; ++r)
+        if (slot[r] >= 0 && slot[r] < t.num_slots) atomicOr(&s_bits[slot[r] / 32], 1u << (slot[r] % 32));
+    }
   }
-  const int64_t row = load_index(P.t.at, P.t.rows_i64, i);
-  if (moved == 0 || row < 0 || row >= P.t.rows || p >= held(P.t.lens, P.t.lens_i64, row, P.t.cols)) return;
-  int32_t* entry = P.t.table + row * P.t.stride + p;
-  const int32_t slot = *entry;
-  if (slot < U || slot >= P.t.num_slots) return;
-  const int32_t rank = P.place[slot];
-  if (rank >= 0 && rank < moved) *entry = (int32_t)P.dst[rank];
+  __syncthreads();
+  const uint32_t word = s_bits[tid];
+  const int U = block_sum<RQ_WIDE / WAVE>((int)__popc(word), s_red);
+  // the used slots below U: what moves is what is used above it
+  const int take = U - tid * 32;
+  const int low = block_sum<RQ_WIDE / WAVE>(take <= 0 ? 0 : (int)__popc(take >= 32 ? word : word & ((1u << take) - 1u)), s_red);
+  if (tid == 0) P.out[0] = U, P.out[1] = U - low;
+  int before = 0;
+  for (int s0 = tid * 16; s0 - tid * 16 < t.num_slots; s0 += 16 * RQ_WIDE) {
+    const uint32_t bits = (s_bits[s0 / 32] >> (s0 % 32)) & 0xffffu;
+    int total;
+    int at = before + block_excl_scan<RQ_WIDE / WAVE>((int)__popc(bits), s_red, &total);  // used slots below s0
+    before += total;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int s = s0 + k;
+      if ((bits >> k) & 1) {
+        if (s >= U) P.src[at - low] = s, P.place[s] = at - low;
+        ++at;
+      } else if (s < U) {
+        P.dst[s - at] = s;
+      }
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -232,7 +341,10 @@ struct CopyParams {
   const int32_t* count;
   int64_t n, num_slots;
   int32_t src_i64, dst_i64;
+  int32_t parts;
 };
+
+typedef uint32_t uint32x4 __attribute__((ext_vector_type(4)));
 
 // Groups of G lanes take CS_ROWS moves at once, all loaded before the first is stored.
 template <class V>
@@ -249,12 +361,12 @@ __device__ __forceinline__ void copy_rows(const CopyParams& P, const CopyPart& p
       if (from[u] < 0 || from[u] >= P.num_slots || to[u] < 0 || to[u] >= P.num_slots) from[u] = to[u] = -1;
     }
     for (int k = l; k < part.pieces; k += part.G) {
-      const int head = k / part.per;
+      const int head = part.per == part.pieces ? 0 : k / part.per;
       const int64_t at = head * part.head_stride + (int64_t)(k - head * part.per) * sizeof(V);
       V x[CS_ROWS];
 #pragma unroll
       for (int u = 0; u < CS_ROWS; ++u)
-        if (from[u] >= 0) x[u] = *reinterpret_cast<const V*>(part.base + from[u] * part.slot_stride + at);
+        x[u] = *reinterpret_cast<const V*>(part.base + (from[u] < 0 ? 0 : from[u]) * part.slot_stride + at);
 #pragma unroll
       for (int u = 0; u < CS_ROWS; ++u)
         if (from[u] >= 0) *reinterpret_cast<V*>(part.base + to[u] * part.slot_stride + at) = x[u];
@@ -262,23 +374,51 @@ __device__ __forceinline__ void copy_rows(const CopyParams& P, const CopyPart& p
   }
 }
 
-__global__ __launch_bounds__(RQ_THREADS) void k_copy_slots(CopyParams P) {
-  const CopyPart& part = P.part[blockIdx.y];
+// The tensors' rows; after a plan (`follow`) the rows' entries and the counts of holders too, as two rows of workgroups more.
+__global__ __launch_bounds__(RQ_THREADS) void k_copy_slots(CopyParams P, CompactParams M) {
   int64_t n = P.n;
   if (P.count) {
     const int32_t c = *P.count;
     n = c < 0 ? 0 : (c < n ? c : n);
   }
-  if (part.wide == 16)
-    copy_rows<uint4>(P, part, n);
-  else
-    copy_rows<uint32_t>(P, part, n);
+  if ((int)blockIdx.y < P.parts) {
+    const CopyPart part = P.part[blockIdx.y];
+    if (part.wide == 16)
+      copy_rows<uint32x4>(P, part, n);
+    else
+      copy_rows<uint32_t>(P, part, n);
+    return;
+  }
+  const TableParams& t = M.t;
+  const int64_t step = (int64_t)gridDim.x * RQ_THREADS, first = (int64_t)blockIdx.x * RQ_THREADS + threadIdx.x;
+  if (n == 0) return;
+  if ((int)blockIdx.y == P.parts) {
+    if (t.shared)
+      for (int64_t k = first; k < n; k += step) {
+        const int64_t from = M.src[k];
+        t.shared[M.dst[k]] = t.shared[from];
+        t.shared[from] = 0;
+      }
+    return;
+  }
+  const int32_t U = M.out[0];
+  const int64_t units = t.n * t.chunks;
+  for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+    const int64_t i = u / t.chunks, p = (u - i * t.chunks) * RQ_THREADS + threadIdx.x;
+    const int64_t row = load_index(t.at, t.rows_i64, i);
+    if (row < 0 || row >= t.rows || p >= held(t.lens, t.lens_i64, row, t.cols)) continue;
+    int32_t* entry = t.table + row * t.stride + p;
+    const int32_t slot = *entry;
+    if (slot < U || slot >= t.num_slots) continue;
+    const int32_t rank = M.place[slot];
+    if (rank >= 0 && rank < n) *entry = (int32_t)M.dst[rank];
+  }
 }
 
 static int launch_copy(const char* what, const dsv_slot_rows* rows, int32_t n_rows, const void* src, int32_t src_i64,
                        const void* dst, int32_t dst_i64, int64_t n, const int32_t* count, int64_t num_slots,
-                       hipStream_t stream) {
-  for (int32_t at = 0; at < n_rows; at += CS_PARTS) {
+                       const CompactParams* follow, hipStream_t stream) {
+  for (int32_t at = 0; at < n_rows || (follow && at == 0); at += CS_PARTS) {
     CopyParams P;
     const int parts = n_rows - at < CS_PARTS ? n_rows - at : CS_PARTS;
     int64_t most = 1;
@@ -306,8 +446,17 @@ static int launch_copy(const char* what, const dsv_slot_rows* rows, int32_t n_ro
     P.num_slots = num_slots;
     P.src_i64 = src_i64;
     P.dst_i64 = dst_i64;
+    P.parts = parts;
+    CompactParams M{};
+    unsigned more = 0;
+    if (follow && at == 0) {
+      M = *follow;
+      more = 2;
+      const int64_t units = M.t.n * M.t.chunks;
+      most = units > most ? units : most;
+    }
     if (most > 1024) most = 1024;
-    hipLaunchKernelGGL(k_copy_slots, dim3((unsigned)most, (unsigned)parts), dim3(RQ_THREADS), 0, stream, P);
+    hipLaunchKernelGGL(k_copy_slots, dim3((unsigned)most, (unsigned)parts + more), dim3(RQ_THREADS), 0, stream, P, M);
     DSV_CHECK_LAUNCH(what);
   }
   return DSV_OK;
@@ -349,7 +498,7 @@ extern "C" int dsv_copy_slots(const dsv_slot_rows* rows, int32_t n_rows, int64_t
   if (n < 0 || n > 0x7fffffff) DSV_FAIL(DSV_ERR_INVALID, "dsv_copy_slots: n %lld", (long long)n);
   if (n == 0 || n_rows == 0) return DSV_OK;
   if (!src || !dst) DSV_FAIL(DSV_ERR_INVALID, "dsv_copy_slots: null pointer");
-  return launch_copy("k_copy_slots", rows, n_rows, src, src_i64, dst, dst_i64, n, count, num_slots,
+  return launch_copy("k_copy_slots", rows, n_rows, src, src_i64, dst, dst_i64, n, count, num_slots, nullptr,
                      reinterpret_cast<hipStream_t>(stream));
 }
 
@@ -362,7 +511,8 @@ extern "C" int dsv_fork_requests(int32_t* req_to_token, int64_t rows, int64_t rt
   if (n == 0) return DSV_OK;
   TableParams P{req_to_token, rows, rt_stride, rt_cols, seq_lens, seq_lens_i64, rows_i64, parents, n, num_slots, shared,
                 (rt_cols + RQ_THREADS - 1) / RQ_THREADS};
-  hipLaunchKernelGGL(k_fork, dim3((unsigned)(P.chunks * n)), dim3(RQ_THREADS), 0, reinterpret_cast<hipStream_t>(stream), P, children);
+  hipLaunchKernelGGL(k_fork, dim3((unsigned)(P.chunks * ((n + RQ_ROWS - 1) / RQ_ROWS))), dim3(RQ_THREADS), 0,
+                     reinterpret_cast<hipStream_t>(stream), P, children);
   DSV_CHECK_LAUNCH("k_fork");
   return DSV_OK;
 }
@@ -387,8 +537,13 @@ extern "C" int dsv_free_requests(int32_t* req_to_token, int64_t rows, int64_t rt
   TableParams P{req_to_token, rows, rt_stride, rt_cols, seq_lens, seq_lens_i64, rows_i64, at, n, num_slots, shared,
                 (rt_cols + RQ_THREADS - 1) / RQ_THREADS};
   int32_t* counts = reinterpret_cast<int32_t*>(workspace);
+  if (num_slots <= RQ_SMALL_SLOTS && (n + RQ_ROWS - 1) / RQ_ROWS * rt_cols <= RQ_SMALL_ENTRIES) {
+    hipLaunchKernelGGL(k_free_small, dim3(1), dim3(RQ_WIDE), 0, stream, P, free_slots, capacity, free_count);
+    DSV_CHECK_LAUNCH("k_free_small");
+    return DSV_OK;
+  }
   if (n) {
-    hipLaunchKernelGGL(k_release, dim3((unsigned)(P.chunks * n)), dim3(RQ_THREADS), 0, stream, P);
+    hipLaunchKernelGGL(k_release, dim3((unsigned)(P.chunks * ((n + RQ_ROWS - 1) / RQ_ROWS))), dim3(RQ_THREADS), 0, stream, P);
     DSV_CHECK_LAUNCH("k_release");
   }
   const dim3 pool((unsigned)pool_chunks(num_slots));
@@ -432,20 +587,21 @@ extern "C" int dsv_compact_requests(int32_t* req_to_token, int64_t rows, int64_t
   P.dst = dst;
   P.out = counts;
   P.pool = (int)pool;
-  const dim3 over_pool((unsigned)pool), threads(RQ_THREADS);
-  hipLaunchKernelGGL(k_clear_used, over_pool, threads, 0, stream, P);
-  DSV_CHECK_LAUNCH("k_clear_used");
-  if (n) {
-    hipLaunchKernelGGL(k_mark_used, dim3((unsigned)(P.t.chunks * n)), threads, 0, stream, P);
-    DSV_CHECK_LAUNCH("k_mark_used");
+  if (num_slots <= RQ_BITS && (n + RQ_ROWS - 1) / RQ_ROWS * rt_cols <= RQ_SMALL_ENTRIES) {
+    hipLaunchKernelGGL(k_plan_small, dim3(1), dim3(RQ_WIDE), 0, stream, P);
+    DSV_CHECK_LAUNCH("k_plan_small");
+  } else {
+    const dim3 over_pool((unsigned)pool), threads(RQ_THREADS);
+    hipLaunchKernelGGL(k_clear_used, over_pool, threads, 0, stream, P);
+    DSV_CHECK_LAUNCH("k_clear_used");
+    if (n) {
+      hipLaunchKernelGGL(k_mark_used, dim3((unsigned)(P.t.chunks * n)), threads, 0, stream, P);
+      DSV_CHECK_LAUNCH("k_mark_used");
+    }
+    hipLaunchKernelGGL(k_count_used, over_pool, threads, 0, stream, P);
+    DSV_CHECK_LAUNCH("k_count_used");
+    hipLaunchKernelGGL(k_plan_moves, over_pool, threads, 0, stream, P);
+    DSV_CHECK_LAUNCH("k_plan_moves");
   }
-  hipLaunchKernelGGL(k_count_used, over_pool, threads, 0, stream, P);
-  DSV_CHECK_LAUNCH("k_count_used");
-  hipLaunchKernelGGL(k_plan_moves, over_pool, threads, 0, stream, P);
-  DSV_CHECK_LAUNCH("k_plan_moves");
-  hipLaunchKernelGGL(k_follow_moves, dim3((unsigned)(P.t.chunks * (n + 1))), threads, 0, stream, P);
-  DSV_CHECK_LAUNCH("k_follow_moves");
-  if (n_slot_rows && num_slots > 1)
-    return launch_copy("k_copy_slots", slot_rows, n_slot_rows, src, 1, dst, 1, num_slots / 2, counts + 1, num_slots, stream);
-  return DSV_OK;
+  return launch_copy("k_copy_slots", slot_rows, n_slot_rows, src, 1, dst, 1, num_slots / 2, counts + 1, num_slots, &P, stream);
 }

@@ -161,26 +161,34 @@ def read_kv(cache: KVCache, slots: torch.Tensor, *, dtype: torch.dtype = torch.b
 def slot_rows(caches):
     """(the ``dsv_slot_rows`` of every tensor of the caches, an array of them; the tensors; the slots, which all
     must have alike).  A cache is a ``KVCache`` or a ``BlockIndex``; one alone or a list of them."""
-    rows, tensors, slots = [], [], set()
-    for cache in caches if isinstance(caches, (list, tuple)) else [caches]:
+    rows, tensors, slots = [], [], None
+    for cache in caches if isinstance(caches, (list, tuple)) else (caches,):
         if isinstance(cache, KVCache):
-            cache_fields(cache, write=True)
-            own = [t for t in tensors_of(cache) if t is not None]
-        elif getattr(cache, "bounds", None) is not None:
-            own = [cache.bounds]
-            if not cache.bounds.is_contiguous() or cache.bounds.ndim != 4:
-                raise ValueError("an index's bounds must be contiguous [rows, heads, 2, dim]")
+            c = cache_fields(cache, write=True)
+            size = 1 if c.k_scale else 2
+            rows.append((c.k, c.k_slot_stride * size, c.k_head_stride * size, c.heads, c.dim * size))
+            rows.append((c.v, c.v_slot_stride * size, c.v_head_stride * size, c.heads, c.dim * size))
+            tensors += (cache.k, cache.v)
+            if c.k_scale:
+                rows.append((c.k_scale, c.ks_slot_stride * 4, c.ks_head_stride * 4, c.heads, 4))
+                rows.append((c.v_scale, c.vs_slot_stride * 4, c.vs_head_stride * 4, c.heads, 4))
+                tensors += (cache.k_scale, cache.v_scale)
+            here = c.num_slots
         else:
-            raise ValueError("caches must be KVCache or BlockIndex objects")
-        for t in own:
-            size, heads = t.element_size(), 1 if t.ndim == 4 else t.shape[1]
-            each = t[0].numel() // heads * size
-            rows.append(_lib.SlotRows(t.data_ptr(), t.stride(0) * size, t.stride(1) * size if t.ndim < 4 else 0, heads, each))
-            tensors.append(t)
-            slots.add(t.shape[0])
-    if len(slots) != 1:
-        raise ValueError("caches must have one number of slots, and there must be one")
-    return (_lib.SlotRows * len(rows))(*rows), tensors, slots.pop()
+            x = getattr(cache, "bounds", None)
+            if x is None:
+                raise ValueError("caches must be KVCache or BlockIndex objects")
+            if x.ndim != 4 or not x.is_contiguous() or x.dtype not in _ACT or x.shape[2] != 2 or x.numel() < 1:
+                raise ValueError("an index's bounds must be contiguous bfloat16 or float16 [rows, heads, 2, dim]")
+            here, each = x.shape[0], x.numel() // x.shape[0] * 2
+            rows.append((x.data_ptr(), each, 0, 1, each))
+            tensors.append(x)
+        if slots not in (None, here):
+            raise ValueError("caches must have one number of slots")
+        slots = here
+    if slots is None:
+        raise ValueError("there must be a cache")
+    return (_lib.SlotRows * len(rows))(*rows), tensors, slots
 
 
 def copy_kv(caches, src: torch.Tensor, dst: torch.Tensor, *, count: torch.Tensor | None = None) -> None:
