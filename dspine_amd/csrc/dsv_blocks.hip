@@ -308,6 +308,10 @@ __global__ __launch_bounds__(NW * WAVE) void k_select_blocks(SelectParams P) {
   __shared__ int s_idx[WAVE], s_count[PER * NW + WAVE], s_n;
   const int tid = threadIdx.x, lane = tid & (WAVE - 1), wave = tid / WAVE;
   const int64_t row = blockIdx.x;
+  const float* scores = P.scores + row * P.cols;
+  float score[PER];  // (asked for before it is known how many of them count)
+#pragma unroll
+  for (int i = 0; i < PER; ++i) score[i] = i * NT + tid < P.cols ? scores[i * NT + tid] : 0.f;
   const int pre = P.prefix_lens[row / P.heads];
   const int64_t full = pre < 0 ? 0 : pre >> P.shift;
   const int n = (int)(full < P.cols ? full : P.cols);
@@ -316,7 +320,6 @@ __global__ __launch_bounds__(NW * WAVE) void k_select_blocks(SelectParams P) {
     for (int i = tid; i < P.count; i += NT) out[i] = i < n ? i : -1;
     return;
   }
-  const float* scores = P.scores + row * P.cols;
   const int c0 = P.first, c1 = n - P.last;  // the candidates
   uint32_t key[PER];
   uint32_t lo = ~0u, hi = 0u;
@@ -325,7 +328,7 @@ __global__ __launch_bounds__(NW * WAVE) void k_select_blocks(SelectParams P) {
     const int j = i * NT + tid;
     key[i] = 0;
     if (j >= c0 && j < c1) {
-      const float v = scores[j];
+      const float v = score[i];
       key[i] = f32_key(v == v ? v : -INFINITY);
       lo = key[i] < lo ? key[i] : lo;
       hi = key[i] > hi ? key[i] : hi;

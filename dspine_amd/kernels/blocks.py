@@ -195,12 +195,11 @@ def block_attention(q: torch.Tensor, cache: KVCache, *, T: int, blocks: torch.Te
     contiguous; ``select_blocks``), and the positions from the last finished block's end on.  An entry that names no
     finished block (-1 among them) holds nothing; one that names a block again counts it again."""
     block_size = _check_size(block_size)
+    if (blocks.ndim != 3 or blocks.shape[:1] != prefix_lens.shape[:1] or cache.k.ndim != 3 or blocks.shape[1] != cache.k.shape[1]
+            or blocks.shape[2] < 1 or blocks.dtype != torch.int32 or not blocks.is_contiguous()):
+        raise ValueError("blocks must be contiguous int32 [bs, heads, count]")
     a, dev, out = attention_args(q, cache, T=T, page_table=page_table, prefix_lens=prefix_lens, verify_lens=verify_lens,
                                  row_offsets=row_offsets, masks=masks, scale=scale, out=out, lse=lse, also=(blocks,))
-    heads = cache.k.shape[1]
-    if (blocks.ndim != 3 or blocks.shape[:2] != (prefix_lens.shape[0], heads) or blocks.shape[2] < 1
-            or blocks.dtype != torch.int32 or not blocks.is_contiguous()):
-        raise ValueError("blocks must be contiguous int32 [bs, heads, count]")
     if a is not None:
         scratch = with_workspace(a, dev, workspace)  # (held until the launch)
         _lib.launch("dsv_block_attention", dev, _lib.load().dsv_block_attention,

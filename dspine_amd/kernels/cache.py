@@ -9,6 +9,7 @@ for each (slot, head): value = code * scale.
 
 from __future__ import annotations
 
+import struct
 from dataclasses import dataclass
 
 import torch
@@ -164,16 +165,14 @@ def slot_rows(caches):
     rows, tensors, slots = [], [], None
     for cache in caches if isinstance(caches, (list, tuple)) else (caches,):
         if isinstance(cache, KVCache):
-            c = cache_fields(cache, write=True)
-            size = 1 if c.k_scale else 2
-            rows.append((c.k, c.k_slot_stride * size, c.k_head_stride * size, c.heads, c.dim * size))
-            rows.append((c.v, c.v_slot_stride * size, c.v_head_stride * size, c.heads, c.dim * size))
-            tensors += (cache.k, cache.v)
-            if c.k_scale:
-                rows.append((c.k_scale, c.ks_slot_stride * 4, c.ks_head_stride * 4, c.heads, 4))
-                rows.append((c.v_scale, c.vs_slot_stride * 4, c.vs_head_stride * 4, c.heads, 4))
-                tensors += (cache.k_scale, cache.v_scale)
-            here = c.num_slots
+            cache_fields(cache, write=True)
+            here, heads, dim = cache.k.shape
+            for t, size, each in ((cache.k, None, dim), (cache.v, None, dim), (cache.k_scale, 4, 1), (cache.v_scale, 4, 1)):
+                if t is not None:
+                    size = size or t.element_size()
+                    slot, head = t.stride()[:2]
+                    rows += (t.data_ptr(), slot * size if here > 1 else 0, head * size if heads > 1 else 0, heads, each * size)
+                    tensors.append(t)
         else:
             x = getattr(cache, "bounds", None)
             if x is None:
@@ -181,14 +180,15 @@ def slot_rows(caches):
             if x.ndim != 4 or not x.is_contiguous() or x.dtype not in _ACT or x.shape[2] != 2 or x.numel() < 1:
                 raise ValueError("an index's bounds must be contiguous bfloat16 or float16 [rows, heads, 2, dim]")
             here, each = x.shape[0], x.numel() // x.shape[0] * 2
-            rows.append((x.data_ptr(), each, 0, 1, each))
+            rows += (x.data_ptr(), each, 0, 1, each)
             tensors.append(x)
         if slots not in (None, here):
             raise ValueError("caches must have one number of slots")
         slots = here
     if slots is None:
         raise ValueError("there must be a cache")
-    return (_lib.SlotRows * len(rows))(*rows), tensors, slots
+    n = len(tensors)
+    return (_lib.SlotRows * n).from_buffer_copy(struct.pack("=" + n * "QqqiI", *rows)), tensors, slots
 
 
 def copy_kv(caches, src: torch.Tensor, dst: torch.Tensor, *, count: torch.Tensor | None = None) -> None:
