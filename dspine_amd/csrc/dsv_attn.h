@@ -29,6 +29,14 @@
 //   4 requests, 25 nodes, bf16, 1.5k to 4.7k                                       36 us   1.5 TB/s: latency (the plan, the
 //       first loads, the outputs and the second launch take longer than a workgroup's six tiles)
 //   1 request, 1 node, bf16, 640                                                   17 us   latency (8.6 + 5.1 us in two launches)
+//
+// BLOCKS: the same over a list of blocks for each (request, cache head).  The positions are numbered as they are read, so only
+// the way to a slot differs: a group of 16 positions lies in one block, and its list entry is asked for a step (a tile, where
+// tiles are staged) before its slots.
+//   64 requests, up to 17 nodes, 4 query heads a cache head, bf16, 64 blocks of 64  260 us   4.2 TB/s: memory, 256 bytes at a time
+//   16 requests, 1 node, 8192 positions in blocks of 16, 64, 128     bf16 130 to 135, int8 101 to 104: memory (int8: 282 MB, and a
+//       third more for scales whose neighbours are other heads'; heads as the caches' outer dimension: 123 and 95)
+//   1 request, 1 node, 32 blocks of 64                                              15 us   latency (9.4 + 5.3 in two launches)
 #pragma once
 #include "dsv_cache.h"
 #include "dsv_common.h"

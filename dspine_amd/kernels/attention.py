@@ -12,7 +12,7 @@ import torch
 
 from dspine_amd import _lib
 from dspine_amd.kernels.cache import _ACT, QUANTISED, KVCache, _distinct, _rows, cache_fields, tensors_of
-from dspine_amd.verify import Workspace
+from dspine_amd.verify import Workspace, scratch
 
 MAX_NODES = 64
 
@@ -41,9 +41,9 @@ def tree_attention(q: torch.Tensor, cache: KVCache, *, T: int, page_table: torch
     a, dev, out = attention_args(q, cache, T=T, page_table=page_table, prefix_lens=prefix_lens, verify_lens=verify_lens,
                                  row_offsets=row_offsets, masks=masks, scale=scale, out=out, lse=lse)
     if a is not None:
-        scratch = with_workspace(a, dev, workspace)  # (held until the launch)
+        held = with_workspace(a, dev, workspace)  # (until the launch)
         _lib.launch("dsv_tree_attention", dev, _lib.load().dsv_tree_attention, a)
-        del scratch
+        del held
     return out
 
 
@@ -107,7 +107,6 @@ def attention_args(q, cache, *, T, page_table, prefix_lens, verify_lens, row_off
 
 def with_workspace(a, dev, workspace):
     """Give a call its scratch memory; returns what holds it."""
-    nbytes = _lib.load().dsv_tree_attention_workspace_bytes(a.bs, a.T, a.cache.heads, a.q_heads, a.cache.dim)
-    buf = (workspace or Workspace()).get(nbytes, dev)
+    buf = scratch(workspace, _lib.load().dsv_tree_attention_workspace_bytes(a.bs, a.T, a.cache.heads, a.q_heads, a.cache.dim), dev)
     a.workspace, a.workspace_bytes = buf.data_ptr(), buf.numel()
     return buf

@@ -201,8 +201,8 @@ def block_attention(q: torch.Tensor, cache: KVCache, *, T: int, blocks: torch.Te
     a, dev, out = attention_args(q, cache, T=T, page_table=page_table, prefix_lens=prefix_lens, verify_lens=verify_lens,
                                  row_offsets=row_offsets, masks=masks, scale=scale, out=out, lse=lse, also=(blocks,))
     if a is not None:
-        scratch = with_workspace(a, dev, workspace)  # (held until the launch)
+        held = with_workspace(a, dev, workspace)  # (until the launch)
         _lib.launch("dsv_block_attention", dev, _lib.load().dsv_block_attention,
                     _lib.BlockAttentionArgs(a, blocks.data_ptr(), blocks.shape[2], block_size))
-        del scratch
+        del held
     return out

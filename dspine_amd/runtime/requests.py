@@ -14,7 +14,7 @@ import torch
 
 from dspine_amd import _lib
 from dspine_amd.kernels.cache import _distinct, slot_rows
-from dspine_amd.verify import Workspace
+from dspine_amd.verify import Workspace, scratch
 
 _INT = (torch.int32, torch.int64)
 
@@ -80,10 +80,10 @@ def free_requests(req_to_token: torch.Tensor, seq_lens: torch.Tensor, shared: to
         raise ValueError("free_count must be int32 [1]")
     dev = _lib.require_cuda(req_to_token, seq_lens, shared, rows, free_slots, free_count)
     lib = _lib.load()
-    scratch = (workspace or Workspace()).get(lib.dsv_free_requests_workspace_bytes(shared.numel()), dev)
+    buf = scratch(workspace, lib.dsv_free_requests_workspace_bytes(shared.numel()), dev)
     _lib.launch("dsv_free_requests", dev, lib.dsv_free_requests, *table, shared.data_ptr(), shared.numel(),
                 rows.data_ptr(), i64, rows.numel(), free_slots.data_ptr(), free_slots.numel(), free_count.data_ptr(),
-                scratch.data_ptr(), scratch.numel())
+                buf.data_ptr(), buf.numel())
     return free_slots, free_count
 
 
@@ -114,9 +114,9 @@ def compact_requests(req_to_token: torch.Tensor, seq_lens: torch.Tensor, rows: t
         raise ValueError("counts must be contiguous int32 [2]")
     dev = _lib.require_cuda(req_to_token, seq_lens, rows, *tensors, shared, moves, counts)
     lib = _lib.load()
-    scratch = (workspace or Workspace()).get(lib.dsv_compact_requests_workspace_bytes(slots), dev)
+    buf = scratch(workspace, lib.dsv_compact_requests_workspace_bytes(slots), dev)
     room = moves.shape[1]
     _lib.launch("dsv_compact_requests", dev, lib.dsv_compact_requests, *table, _lib.ptr(shared), slots, rows.data_ptr(), i64,
                 rows.numel(), parts, len(parts), moves.data_ptr(), moves.data_ptr() + 8 * room, room, counts.data_ptr(),
-                scratch.data_ptr(), scratch.numel())
+                buf.data_ptr(), buf.numel())
     return moves, counts

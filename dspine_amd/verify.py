@@ -71,6 +71,13 @@ class Workspace:
         return own[-1]
 
 
+def scratch(workspace, nbytes: int, device) -> torch.Tensor:
+    """A call's scratch memory: the caller's workspace, or memory of its own."""
+    if workspace is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return workspace.get(nbytes, device)
+
+
 _default_ws: dict = {}
 
 
