@@ -60,7 +60,7 @@ struct AttnParams {
   FastDiv G;           // query heads a cache head
   int WR, RB;          // groups of rows a workgroup, row blocks of a request
   int most;            // ranges at most
-  FastDiv least;       // tiles of a range at least (a batch of fewer is one range)
+  FastDiv least;       // tiles of a range at least (a batch of fewer is one range); not for BLOCKS
   uint32_t num_slots, k_step, v_step;  // slots; bytes from slot to slot
   float* part_o;       // [2 * range + (the range's last request, not its first)][head][row][dim]
   float4* part_ml;     // the same of [row]: the scores' reference, the weights' sum, the weighted values' reference less the first
@@ -145,7 +145,17 @@ __device__ __forceinline__ Plan plan_of(const AttnParams& P, int lane) {
     for (int b = lane; b < P.a.bs; b += WAVE) sum += tiles_of(request_of<BLOCKS>(P, b));
   }
   p.total = wave_sum(sum);
-  const int r = (int)P.least.div((uint32_t)p.total + P.least.d - 1);
+  int r;
+  if constexpr (BLOCKS) {
+    // About 16 parts of a request at most: a part costs the join 0.2 us, a tile more in a range 1 to 2 us, and a range that
+    // holds two requests 4 us, so short lists get a tile a range.  Replayed, 8 cache heads, against two tiles a range (four
+    // where tiles are staged): 1 node, 2 x 5 tiles 12.3 us for 16.5, 1 x 129 22.1 for 27.3, 1 x 257 27.0 for 34.6; 17 nodes, group 4,
+    // 4 x 5 tiles 17.3 for 25.3, 2 x 17 22.0 for 25.4; 40 nodes, group 8, 2 x 17 30.4 for 37.8, 1 x 17 29.5 for 27.9.
+    const uint32_t least = ((uint32_t)p.total / (uint32_t)P.a.bs + 8) / 16;
+    r = (int)(least < 2 ? (uint32_t)p.total : ((uint32_t)p.total + least - 1) / least);
+  } else {
+    r = (int)P.least.div((uint32_t)p.total + P.least.d - 1);
+  }
   p.ranges = r < 1 ? 1 : (r > P.most ? P.most : r);
   p.size = (int)((uint32_t)p.total / (uint32_t)p.ranges);
   p.more = p.total - p.size * p.ranges;

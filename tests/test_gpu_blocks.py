@@ -306,16 +306,23 @@ def test_attention_of_many_requests(device, dtype):
 @pytest.mark.parametrize("dtype", [BF, E4])
 @pytest.mark.parametrize("T, G", ROWS)
 def test_all_blocks_is_the_whole_context(device, T, G, dtype):
-    """Every finished block selected: tree_attention's result, and the same bits where all heads read alike."""
+    """Every finished block selected: tree_attention's result, the same bits where neither call cuts a request into parts."""
     from dspine_amd.kernels.attention import tree_attention
 
-    d = _block_round(94, count=12, size=64, bs=3, T=T, H=2, G=G, D=128, act=BF, dtype=dtype, lens=[64 * 12, 301, 0], tree=True)
-    out, lse = _call(d, device)
-    args = {k: (x.to(device) if isinstance(x, torch.Tensor) else x) for k, x in d.items()
-            if k not in ("q", "cache", "blocks", "block_size")}
-    lse2 = torch.full_like(lse, 7.0)
-    want = tree_attention(d["q"].to(device), _to(d["cache"], device), lse=lse2, **args)
-    assert torch.equal(out, want) and torch.equal(lse, lse2)
+    for lens in ([64 * 12, 301, 0], [63 - T]):
+        if min(lens) < 0:
+            continue
+        d = _block_round(94, count=12, size=16, bs=len(lens), T=T, H=2, G=G, D=128, act=BF, dtype=dtype, lens=lens, tree=True)
+        d["blocks"] = torch.arange(48, dtype=torch.int32).expand(len(lens), 2, -1).contiguous()
+        out, lse = _call(d, device)
+        args = {k: (x.to(device) if isinstance(x, torch.Tensor) else x) for k, x in d.items()
+                if k not in ("q", "cache", "blocks", "block_size")}
+        lse2 = torch.full_like(lse, 7.0)
+        want = tree_attention(d["q"].to(device), _to(d["cache"], device), lse=lse2, **args)
+        _check(d, out, lse)
+        _check(d, want, lse2)
+        if len(lens) == 1:  # (one tile)
+            assert torch.equal(out, want) and torch.equal(lse, lse2)
 
 
 def test_a_long_context_of_slots_past_32_bits_of_bytes(device):
