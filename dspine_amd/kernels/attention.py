@@ -50,13 +50,14 @@ def tree_attention(q: torch.Tensor, cache: KVCache, *, T: int, page_table: torch
 def attention_args(q, cache, *, T, page_table, prefix_lens, verify_lens, row_offsets, masks, scale, out, lse, also=()):
     """(the ``dsv_tree_attention_args`` but for the workspace, or None without rows; the device; out), checked;
     ``also``: tensors that have to be on the same device."""
-    if q.ndim != 3 or q.dtype not in _ACT:
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 3 or dtype not in _ACT:
         raise ValueError("q must be bfloat16 or float16 [rows, q_heads, dim]")
     c = cache_fields(cache)
-    rows, heads, dim = q.shape
+    rows, heads, dim = shape
     if dim != c.dim or heads < 1 or heads % c.heads:
         raise ValueError("q must have the cache's dim and a multiple of its heads")
-    if cache.k.dtype not in QUANTISED and cache.k.dtype != q.dtype:
+    if cache.k.dtype not in QUANTISED and cache.k.dtype != dtype:
         raise ValueError("queries and a 16-bit cache must be of one dtype")
     T = int(T)
     if not 1 <= T <= MAX_NODES:
@@ -76,33 +77,39 @@ def attention_args(q, cache, *, T, page_table, prefix_lens, verify_lens, row_off
         raise ValueError("verify_lens must be contiguous int32 [bs]")
     if masks is not None and (masks.shape != (bs, T) or masks.dtype != torch.int64 or not masks.is_contiguous()):
         raise ValueError("masks must be contiguous int64 [bs, T]")
-    if page_table.ndim != 2 or page_table.shape[0] != bs or page_table.dtype != torch.int32 or page_table.shape[1] < 1:
+    pages = page_table.shape
+    if len(pages) != 2 or pages[0] != bs or page_table.dtype != torch.int32 or pages[1] < 1:
         raise ValueError("page_table must be int32 [bs, L]")
-    if page_table.stride(1) != 1 and page_table.shape[1] > 1:
+    page_stride, last = page_table.stride()
+    if last != 1 and pages[1] > 1:
         raise ValueError("page_table rows must be contiguous")
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
     if not abs(scale) <= 2.0 ** 100:
         raise ValueError("scale must be finite, at most 2^100")
-    if out is None:
-        out = torch.empty((rows, heads, dim), dtype=q.dtype, device=q.device)
-    if out.shape != q.shape or out.dtype != q.dtype:
+    own = out is None
+    if own:
+        out = q.new_empty(shape)
+    elif out.shape != shape or out.dtype != dtype:
         raise ValueError("out must have q's shape and dtype")
     if lse is not None and (lse.shape != (rows, heads) or lse.dtype != torch.float32 or not lse.is_contiguous()):
         raise ValueError("lse must be contiguous float32 [rows, q_heads]")
     if rows:
         q_at, q_row, q_head = _rows(q, "q")
-        out_at, out_row, out_head = _rows(out, "out")
-        _distinct(out, "out")
+        if own:
+            out_at, out_row, out_head = out.data_ptr(), heads * dim, dim
+        else:
+            out_at, out_row, out_head = _rows(out, "out")
+            _distinct(out, "out")
     dev = _lib.require_cuda(q, *tensors_of(cache), page_table, prefix_lens, verify_lens, row_offsets, masks, out, lse,
                             *also)
     if rows == 0:
         return None, dev, out
     ptr = _lib.ptr
     return _lib.TreeAttentionArgs(
-        c, q_at, out_at, ptr(lse), _ACT[q.dtype], heads, rows, q_row, q_head, out_row, out_head, bs, T,
+        c, q_at, out_at, ptr(lse), _ACT[dtype], heads, rows, q_row, q_head, out_row, out_head, bs, T,
         prefix_lens.data_ptr(), ptr(verify_lens), ptr(row_offsets),
         int(row_offsets is not None and row_offsets.dtype == torch.int64), scale, ptr(masks), page_table.data_ptr(),
-        page_table.stride(0), page_table.shape[1], None, 0), dev, out
+        page_stride, pages[1], None, 0), dev, out
 
 
 def with_workspace(a, dev, workspace):

@@ -56,21 +56,27 @@ def _check_size(block_size):
 def index_fields(index: BlockIndex) -> _lib.BlockIndexC:
     """The ``dsv_block_index`` of an index, checked but for its device."""
     x = index.bounds
-    if x.ndim != 4 or x.shape[2] != 2 or x.dtype not in _ACT or not x.is_contiguous():
+    shape, code = x.shape, _ACT.get(x.dtype)
+    if len(shape) != 4 or shape[2] != 2 or code is None or not x.is_contiguous():
         raise ValueError("an index's bounds must be contiguous bfloat16 or float16 [rows, heads, 2, dim]")
-    rows, heads, _, dim = x.shape
+    rows, heads, _, dim = shape
     if dim % 16 or not 16 <= dim <= 256 or rows < 1 or heads < 1:
         raise ValueError("an index needs rows, heads and a dim that is a multiple of 16 up to 256")
-    if x.data_ptr() % 16:
+    at = x.data_ptr()
+    if at % 16:
         raise ValueError("an index's bounds must start on a 16-byte boundary")
-    return _lib.BlockIndexC(x.data_ptr(), _ACT[x.dtype], heads, dim, _check_size(index.block_size), rows)
+    return _lib.BlockIndexC(at, code, heads, dim, _check_size(index.block_size), rows)
 
 
 def _check_table(t, name, bs):
-    if t.ndim != 2 or t.shape[0] != bs or t.dtype != torch.int32 or t.shape[1] < 1:
+    """(address, row stride, columns)"""
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != bs or t.dtype != torch.int32 or shape[1] < 1:
         raise ValueError(f"{name} must be int32 [bs, L]")
-    if t.stride(1) != 1 and t.shape[1] > 1:
+    row, last = t.stride()
+    if last != 1 and shape[1] > 1:
         raise ValueError(f"{name} rows must be contiguous")
+    return t.data_ptr(), row, shape[1]
 
 
 def _check_lens(t, name, bs=None):
@@ -95,15 +101,13 @@ def index_blocks(index: BlockIndex, cache: KVCache, *, page_table: torch.Tensor,
         raise ValueError("the index and the cache must have the same heads and dim")
     bs = _check_lens(from_lens, "from_lens")
     _check_lens(to_lens, "to_lens", bs)
-    _check_table(page_table, "page_table", bs)
-    _check_table(block_table, "block_table", bs)
-    longest = page_table.shape[1] if longest is None else int(longest)
+    pages, table = _check_table(page_table, "page_table", bs), _check_table(block_table, "block_table", bs)
+    longest = pages[2] if longest is None else int(longest)
     if longest < 0:
         raise ValueError(f"longest {longest} is negative")
     dev = _lib.require_cuda(index.bounds, *tensors_of(cache), page_table, block_table, from_lens, to_lens)
-    _lib.launch("dsv_index_blocks", dev, _lib.load().dsv_index_blocks, x, c, page_table.data_ptr(), page_table.stride(0),
-                page_table.shape[1], block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
-                from_lens.data_ptr(), to_lens.data_ptr(), bs, longest)
+    _lib.launch("dsv_index_blocks", dev, _lib.load().dsv_index_blocks, x, c, *pages, *table, from_lens.data_ptr(),
+                to_lens.data_ptr(), bs, longest)
 
 
 def score_blocks(q: torch.Tensor, index: BlockIndex, *, T: int, block_table: torch.Tensor, prefix_lens: torch.Tensor,
@@ -138,21 +142,20 @@ def score_blocks(q: torch.Tensor, index: BlockIndex, *, T: int, block_table: tor
         raise ValueError("row_offsets must be a contiguous int32/int64 vector of batch size")
     if verify_lens is not None:
         _check_lens(verify_lens, "verify_lens", bs)
-    _check_table(block_table, "block_table", bs)
+    table = _check_table(block_table, "block_table", bs)
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
     if not 0.0 < scale <= 2.0 ** 100:
         raise ValueError("scale must be positive, at most 2^100")
-    shape = (bs, x.heads, block_table.shape[1])
+    shape = (bs, x.heads, table[2])
     if out is None:
         out = torch.empty(shape, dtype=torch.float32, device=q.device)
-    if out.shape != shape or out.dtype != torch.float32 or not out.is_contiguous():
+    elif out.shape != shape or out.dtype != torch.float32 or not out.is_contiguous():
         raise ValueError("out must be contiguous float32 [bs, heads, L]")
     q_at, q_row, q_head = _rows(q, "q") if rows else (None, 0, 0)
     dev = _lib.require_cuda(q, index.bounds, block_table, prefix_lens, verify_lens, row_offsets, out)
     a = _lib.ScoreBlocksArgs(x, q_at, out.data_ptr(), heads, 0, rows, q_row, q_head, bs, T, prefix_lens.data_ptr(),
                              _lib.ptr(verify_lens), _lib.ptr(row_offsets),
-                             int(row_offsets is not None and row_offsets.dtype == torch.int64), scale,
-                             block_table.data_ptr(), block_table.stride(0), block_table.shape[1])
+                             int(row_offsets is not None and row_offsets.dtype == torch.int64), scale, *table)
     _lib.launch("dsv_score_blocks", dev, _lib.load().dsv_score_blocks, a)
     return out
 
@@ -163,9 +166,10 @@ def select_blocks(scores: torch.Tensor, count: int, *, prefix_lens: torch.Tensor
     the ``first`` first, the ``last`` last and, to make ``count``, those of the largest ``scores`` (float32 [bs, heads, L],
     contiguous, L <= 32768; ties to the lowest block, NaN as -inf), in ascending order, then -1 where n < count.
     first + last <= count."""
-    if scores.ndim != 3 or scores.dtype != torch.float32 or not scores.is_contiguous():
+    shape = scores.shape
+    if len(shape) != 3 or scores.dtype != torch.float32 or not scores.is_contiguous():
         raise ValueError("scores must be contiguous float32 [bs, heads, L]")
-    bs, heads, cols = scores.shape
+    bs, heads, cols = shape
     if not 1 <= cols <= MAX_BLOCKS:
         raise ValueError(f"1 to {MAX_BLOCKS} blocks of a request are ranked, got {cols}")
     if bs < 1 or heads < 1:
@@ -177,7 +181,7 @@ def select_blocks(scores: torch.Tensor, count: int, *, prefix_lens: torch.Tensor
     shape = (bs, heads, count)
     if out is None:
         out = torch.empty(shape, dtype=torch.int32, device=scores.device)
-    if out.shape != shape or out.dtype != torch.int32 or not out.is_contiguous():
+    elif out.shape != shape or out.dtype != torch.int32 or not out.is_contiguous():
         raise ValueError("out must be contiguous int32 [bs, heads, count]")
     dev = _lib.require_cuda(scores, prefix_lens, out)
     _lib.launch("dsv_select_blocks", dev, _lib.load().dsv_select_blocks, scores.data_ptr(), bs, heads, cols,
@@ -195,14 +199,15 @@ def block_attention(q: torch.Tensor, cache: KVCache, *, T: int, blocks: torch.Te
     contiguous; ``select_blocks``), and the positions from the last finished block's end on.  An entry that names no
     finished block (-1 among them) holds nothing; one that names a block again counts it again."""
     block_size = _check_size(block_size)
-    if (blocks.ndim != 3 or blocks.shape[:1] != prefix_lens.shape[:1] or cache.k.ndim != 3 or blocks.shape[1] != cache.k.shape[1]
-            or blocks.shape[2] < 1 or blocks.dtype != torch.int32 or not blocks.is_contiguous()):
+    lists, k = blocks.shape, cache.k.shape
+    if (len(lists) != 3 or lists[:1] != prefix_lens.shape[:1] or len(k) != 3 or lists[1] != k[1] or lists[2] < 1
+            or blocks.dtype != torch.int32 or not blocks.is_contiguous()):
         raise ValueError("blocks must be contiguous int32 [bs, heads, count]")
     a, dev, out = attention_args(q, cache, T=T, page_table=page_table, prefix_lens=prefix_lens, verify_lens=verify_lens,
                                  row_offsets=row_offsets, masks=masks, scale=scale, out=out, lse=lse, also=(blocks,))
     if a is not None:
         held = with_workspace(a, dev, workspace)  # (until the launch)
         _lib.launch("dsv_block_attention", dev, _lib.load().dsv_block_attention,
-                    _lib.BlockAttentionArgs(a, blocks.data_ptr(), blocks.shape[2], block_size))
+                    _lib.BlockAttentionArgs(a, blocks.data_ptr(), lists[2], block_size))
         del held
     return out

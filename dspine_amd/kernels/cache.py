@@ -77,8 +77,8 @@ def tensors_of(cache: KVCache):
     return cache.k, cache.v, cache.k_scale, cache.v_scale
 
 
-def cache_fields(cache: KVCache, *, write: bool = False) -> _lib.KvCache:
-    """The ``dsv_kv_cache`` of a cache, checked but for its device."""
+def _cache_values(cache: KVCache, write: bool = False):
+    """The fields of a cache's ``dsv_kv_cache``, checked but for its device."""
     k, v, ks, vs = cache.k, cache.v, cache.k_scale, cache.v_scale
     shape, dtype = k.shape, k.dtype
     code = _CACHE.get(dtype)
@@ -102,7 +102,12 @@ def cache_fields(cache: KVCache, *, write: bool = False) -> _lib.KvCache:
         for name, t in (("cache k", k), ("cache v", v), ("k_scale", ks), ("v_scale", vs)):
             if t is not None:
                 _distinct(t, name)
-    return _lib.KvCache(k_at, v_at, code, heads, dim, 0, slots, k_slot, k_head, v_slot, v_head, *scales)
+    return k_at, v_at, code, heads, dim, 0, slots, k_slot, k_head, v_slot, v_head, *scales
+
+
+def cache_fields(cache: KVCache, *, write: bool = False) -> _lib.KvCache:
+    """The ``dsv_kv_cache`` of a cache, checked but for its device."""
+    return _lib.KvCache(*_cache_values(cache, write))
 
 
 def _check_slots(slots):
@@ -165,14 +170,14 @@ def slot_rows(caches):
     rows, tensors, slots = [], [], None
     for cache in caches if isinstance(caches, (list, tuple)) else (caches,):
         if isinstance(cache, KVCache):
-            cache_fields(cache, write=True)
-            here, heads, dim = cache.k.shape
-            for t, size, each in ((cache.k, None, dim), (cache.v, None, dim), (cache.k_scale, 4, 1), (cache.v_scale, 4, 1)):
-                if t is not None:
-                    size = size or t.element_size()
-                    slot, head = t.stride()[:2]
-                    rows += (t.data_ptr(), slot * size if here > 1 else 0, head * size if heads > 1 else 0, heads, each * size)
-                    tensors.append(t)
+            (k_at, v_at, code, heads, dim, _, here, k_slot, k_head, v_slot, v_head, ks_at, vs_at, ks_slot, ks_head, vs_slot,
+             vs_head) = _cache_values(cache, True)
+            size = 2 if ks_at is None else 1
+            rows += (k_at, k_slot * size, k_head * size, heads, dim * size, v_at, v_slot * size, v_head * size, heads, dim * size)
+            tensors += (cache.k, cache.v)
+            if ks_at is not None:
+                rows += (ks_at, ks_slot * 4, ks_head * 4, heads, 4, vs_at, vs_slot * 4, vs_head * 4, heads, 4)
+                tensors += (cache.k_scale, cache.v_scale)
         else:
             x = getattr(cache, "bounds", None)
             if x is None:

@@ -20,14 +20,14 @@ _INT = (torch.int32, torch.int64)
 
 
 def _check_requests(req_to_token, seq_lens):
-    t = req_to_token
-    if t.ndim != 2 or t.dtype != torch.int32 or t.shape[0] < 1 or t.shape[1] < 1 or (t.stride(1) != 1 and t.shape[1] > 1):
+    t, shape, dtype = req_to_token, req_to_token.shape, seq_lens.dtype
+    if len(shape) != 2 or t.dtype != torch.int32 or shape[0] < 1 or shape[1] < 1 or (t.stride(1) != 1 and shape[1] > 1):
         raise ValueError("req_to_token must be row-contiguous int32 [rows, L]")
     _distinct(t, "req_to_token")
-    if seq_lens.shape != (t.shape[0],) or seq_lens.dtype not in _INT or not seq_lens.is_contiguous():
+    if seq_lens.shape != shape[:1] or dtype not in _INT or not seq_lens.is_contiguous():
         raise ValueError("seq_lens must be a contiguous int32/int64 vector of the table's rows")
-    stride = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    return t.data_ptr(), t.shape[0], stride, t.shape[1], seq_lens.data_ptr(), int(seq_lens.dtype == torch.int64)
+    stride = t.stride(0) if shape[0] > 1 else shape[1]
+    return t.data_ptr(), shape[0], stride, shape[1], seq_lens.data_ptr(), int(dtype == torch.int64)
 
 
 def _check_shared(shared):
