@@ -137,10 +137,9 @@ __global__ __launch_bounds__(BI_THREADS) void k_index_blocks(IndexParams P) {
 // over 2 * dim elements of an index row as it lies in memory.  The matrix cores take 16 blocks as rows and 16 queries as
 // columns; a block's score is the largest of its columns'.
 // ---------------------------------------------------------------------------------------
-constexpr int SB_THREADS = 256, SB_WAVES = SB_THREADS / WAVE;
+constexpr int SB_WAVES = 4, SB_MANY = 8;  // waves of a workgroup, and where the queries take much LDS
 constexpr int SB_STAGE = 60;  // pieces of 16 queries' 32 elements (1 KB) in LDS at most
-constexpr int SB_STEP = SB_WAVES * 16;  // blocks of a step: 16 a wave (32, with fewer steps: 43 us for 41)
-constexpr int SB_STEPS = 8;             // steps of a workgroup at most
+constexpr int SB_STEPS = 8;   // steps of a workgroup at most, 16 blocks a wave each (32, with fewer steps: 43 us for 41)
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bhalf8 __attribute__((ext_vector_type(8)));
@@ -173,8 +172,9 @@ __device__ __forceinline__ void split_signs(uint32_t w, uint32_t& negative, uint
 // bounds in registers for all of the queries.  Bound by memory: 64 requests of 8k to 64k positions in blocks of 64, up to 17
 // nodes, 147 MB of bounds: 38 us, 3.9 TB/s (the next step's bounds loaded into a second set of registers first: 42 us for 41;
 // queries split by sign in LDS, twice the memory and half the workgroups a CU: 62 us).  One node over 32k: 4.8 us, latency.
-template <int IT, int NC, bool FULL>
-__global__ __launch_bounds__(SB_THREADS) void k_score_blocks(ScoreParams P) {
+template <int IT, int NC, bool FULL, int WAVES>
+__global__ __launch_bounds__(WAVES * WAVE) void k_score_blocks(ScoreParams P) {
+  constexpr int SB_STEP = WAVES * 16;  // blocks of a step
   const dsv_score_blocks_args& a = P.a;
   const dsv_block_index& x = a.index;
   const int dim = FULL ? NC * 32 : x.dim;
@@ -200,7 +200,7 @@ __global__ __launch_bounds__(SB_THREADS) void k_score_blocks(ScoreParams P) {
   float* const out = a.scores + (int64_t)bh * cols;
   const int32_t* const table = a.block_table + b * a.block_stride;
   const int64_t row0 = a.row_offsets ? load_index(a.row_offsets, a.row_offsets_i64, b) : (int64_t)b * a.T;
-  for (int64_t i = (end > first ? end : first) + tid; i < past; i += SB_THREADS) out[i] = -INFINITY;
+  for (int64_t i = (end > first ? end : first) + tid; i < past; i += WAVES * WAVE) out[i] = -INFINITY;
   if (end <= first) return;
   uint4 k[NC][2];
   bool there = false;
@@ -224,11 +224,11 @@ __global__ __launch_bounds__(SB_THREADS) void k_score_blocks(ScoreParams P) {
     const int here = tiles - t0 < P.staged ? tiles - t0 : P.staged;
     if (t0) __syncthreads();
     // (the first step's bounds are asked for behind the first queries)
-    for (int i0 = wave; i0 < here * NC || i0 == wave; i0 += SB_WAVES * AHEAD) {
+    for (int i0 = wave; i0 < here * NC || i0 == wave; i0 += WAVES * AHEAD) {
       uint4 w[AHEAD];
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
-        const int i = i0 + u * SB_WAVES, t = i / NC, c = i - t * NC;
+        const int i = i0 + u * WAVES, t = i / NC, c = i - t * NC;
         int r = (t0 + t) * 16 + m;
         r = r < rows ? r : rows - 1;  // (a row again: the largest stays the largest)
         const int node = (int)P.G.div((uint32_t)r), head = h * (int)P.G.d + r - node * (int)P.G.d;
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(SB_THREADS) void k_score_blocks(ScoreParams P) {
       if (i0 == wave) load(first + wave * 16);
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u)
-        if (i0 + u * SB_WAVES < here * NC) s_q[(i0 + u * SB_WAVES) * WAVE + lane] = w[u];
+        if (i0 + u * WAVES < here * NC) s_q[(i0 + u * WAVES) * WAVE + lane] = w[u];
     }
     __syncthreads();
     for (int step = 0; step < P.steps; ++step) {
@@ -544,25 +544,36 @@ extern "C" int dsv_score_blocks(const dsv_score_blocks_args* args, dsv_stream_t 
   P.a = a;
   P.G = fast_div((uint32_t)(a.q_heads / a.index.heads));
   P.shift = __builtin_ctz((unsigned)a.index.block_size);
-  const int64_t steps = (a.block_cols + SB_STEP - 1) / SB_STEP, bh = (int64_t)a.bs * a.index.heads;
-  const int64_t per = steps * bh / 4096;  // (half and twice as many workgroups: 44 and 42 us for 41)
+  const int64_t bh = (int64_t)a.bs * a.index.heads;
+  const int tiles = (a.T * (int)P.G.d + 15) / 16, pieces = a.index.dim <= 64 ? 2 : (a.index.dim <= 128 ? 4 : 8);
+  P.staged = tiles < SB_STAGE / pieces ? tiles : SB_STAGE / pieces;
+  // Waves of a workgroup: queries of 20 KB (68 rows of dim 128) 41.6 us with four and 43.9 with eight, of 40 KB (68 of dim 256) 22.8
+  // and 17.9: eight where LDS holds only a few workgroups.
+  const bool many = P.staged * pieces > 32;
+  const int step = (many ? SB_MANY : SB_WAVES) * 16;
+  const int64_t steps = (a.block_cols + step - 1) / step;
+  const int64_t per = steps * bh / (many ? 2048 : 4096);  // (half and twice as many workgroups: 44 and 42 us for 41)
   P.steps = (int)(per < 1 ? 1 : (per > SB_STEPS ? SB_STEPS : per));
   P.chunks = (int)((steps + P.steps - 1) / P.steps);
   if (bh * P.chunks > 0x7fffffffll) DSV_FAIL(DSV_ERR_INVALID, "dsv_score_blocks: too many blocks for one call");
-  const int tiles = (a.T * (int)P.G.d + 15) / 16;
-  auto launch = [&](auto kern, int pieces) {
-    P.staged = tiles < SB_STAGE / pieces ? tiles : SB_STAGE / pieces;
-    hipLaunchKernelGGL(kern, dim3((unsigned)(bh * P.chunks)), dim3(SB_THREADS), (unsigned)(P.staged * pieces) * 1024u, stream, P);
+  auto launch = [&](auto few, auto more) {
+    hipLaunchKernelGGL(many ? more : few, dim3((unsigned)(bh * P.chunks)), dim3((many ? SB_MANY : SB_WAVES) * WAVE),
+                       (unsigned)(P.staged * pieces) * 1024u, stream, P);
   };
   auto type = [&](auto it) {
     constexpr int IT = decltype(it)::value;
     const int D = a.index.dim;
+    auto width = [&](auto nc, auto full) {
+      constexpr int NC = decltype(nc)::value;
+      constexpr bool FULL = decltype(full)::value;
+      launch(k_score_blocks<IT, NC, FULL, SB_WAVES>, k_score_blocks<IT, NC, FULL, SB_MANY>);
+    };
     if (D <= 64)
-      D == 64 ? launch(k_score_blocks<IT, 2, true>, 2) : launch(k_score_blocks<IT, 2, false>, 2);
+      D == 64 ? width(Int<2>{}, Int<1>{}) : width(Int<2>{}, Int<0>{});
     else if (D <= 128)
-      D == 128 ? launch(k_score_blocks<IT, 4, true>, 4) : launch(k_score_blocks<IT, 4, false>, 4);
+      D == 128 ? width(Int<4>{}, Int<1>{}) : width(Int<4>{}, Int<0>{});
     else
-      D == 256 ? launch(k_score_blocks<IT, 8, true>, 8) : launch(k_score_blocks<IT, 8, false>, 8);
+      D == 256 ? width(Int<8>{}, Int<1>{}) : width(Int<8>{}, Int<0>{});
   };
   a.index.dtype == DSV_BF16 ? type(Int<DSV_BF16>{}) : type(Int<DSV_F16>{});
   DSV_CHECK_LAUNCH("k_score_blocks");
