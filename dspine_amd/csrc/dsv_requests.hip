@@ -32,10 +32,29 @@ struct TableParams {
   int64_t chunks;
 };
 
+// N indices at any places (`at(r)`; -1 where it is negative), and the clamped lengths of rows (0 for a row that is none): one test
+// of the width for all of them.
+template <int N, class At>
+__device__ __forceinline__ void load_indices(const void* p, int i64, At at, int64_t (&out)[N]) {
+  if (i64) {
+#pragma unroll
+    for (int r = 0; r < N; ++r) out[r] = at(r) < 0 ? -1 : reinterpret_cast<const int64_t*>(p)[at(r)];
+  } else {
+#pragma unroll
+    for (int r = 0; r < N; ++r) out[r] = at(r) < 0 ? -1 : (int64_t) reinterpret_cast<const int32_t*>(p)[at(r)];
+  }
+}
+template <int N>
+__device__ __forceinline__ void load_lens(const void* lens, int i64, const int64_t (&row)[N], int64_t cols, int64_t (&len)[N]) {
+  load_indices<N>(lens, i64, [&](int r) { return row[r]; }, len);
+#pragma unroll
+  for (int r = 0; r < N; ++r) len[r] = len[r] < 0 ? 0 : (len[r] > cols ? cols : len[r]);
+}
+
 // Samples of one prompt hold its slots at the same positions, so a thread takes its column's entries of RQ_ROWS rows and
 // counts equal ones together: what bounds a fork or a release of long prompts is the touch of a scattered count for each
 // slot (about 28 G/s; a plain read and write is as slow as the atomic, and neighbouring slots share their lines).  128 rows
-// of 20000 positions, two of each prompt, slots in random order: 60 us a fork and 55 a release, 96 each with an atomic
+// of 20000 positions, two of each prompt, slots in random order: 58 us a fork and 56 a release, 96 each with an atomic
 // an entry; without the counts a fork is 17.
 constexpr int RQ_ROWS = 8;
 __device__ __forceinline__ void add_holders(const TableParams& P, int32_t (&slot)[RQ_ROWS], int sign) {
@@ -59,30 +78,30 @@ __device__ __forceinline__ void add_holders(const TableParams& P, int32_t (&slot
 __global__ __launch_bounds__(RQ_THREADS) void k_fork(TableParams P, const void* children) {
   const int64_t group = blockIdx.x / P.chunks, chunk = blockIdx.x - group * P.chunks;
   const int64_t p = chunk * RQ_THREADS + threadIdx.x;
+  // (every load of a kind before the first of the next: a wait for each kind, not for each row)
   int32_t slot[RQ_ROWS];
-  int64_t child[RQ_ROWS];
-#pragma unroll
-  for (int r = 0; r < RQ_ROWS; ++r) {
-    const int64_t i = group * RQ_ROWS + r;
-    const int64_t parent = i < P.n ? load_index(P.at, P.rows_i64, i) : -1;
-    child[r] = i < P.n ? load_index(children, P.rows_i64, i) : -1;
-    if (parent < 0 || parent >= P.rows || child[r] < 0 || child[r] >= P.rows || child[r] == parent) child[r] = -1;
-    const int64_t len = child[r] < 0 ? 0 : held(P.lens, P.lens_i64, parent, P.cols);
-    if (p == 0 && child[r] >= 0) set_len(P.lens, P.lens_i64, child[r], len);
-    if (p >= len) child[r] = -1;
-    slot[r] = child[r] < 0 ? -1 : P.table[parent * P.stride + p];
-  }
+  int64_t parent[RQ_ROWS], child[RQ_ROWS], len[RQ_ROWS];
+  auto pair = [&](int r) { return group * RQ_ROWS + r < P.n ? group * RQ_ROWS + r : -1; };
+  load_indices<RQ_ROWS>(P.at, P.rows_i64, pair, parent);
+  load_indices<RQ_ROWS>(children, P.rows_i64, pair, child);
 #pragma unroll
   for (int r = 0; r < RQ_ROWS; ++r)
-    if (child[r] >= 0) P.table[child[r] * P.stride + p] = slot[r];
+    if (parent[r] >= P.rows || child[r] < 0 || child[r] >= P.rows || child[r] == parent[r]) parent[r] = -1;
+  load_lens<RQ_ROWS>(P.lens, P.lens_i64, parent, P.cols, len);
+#pragma unroll
+  for (int r = 0; r < RQ_ROWS; ++r) slot[r] = p < len[r] ? P.table[parent[r] * P.stride + p] : -1;
+#pragma unroll
+  for (int r = 0; r < RQ_ROWS; ++r) {
+    if (p == 0 && parent[r] >= 0) set_len(P.lens, P.lens_i64, child[r], len[r]);
+    if (p < len[r]) P.table[child[r] * P.stride + p] = slot[r];
+  }
   add_holders(P, slot, 1);
 }
 
 // The rows of a group that are named before, as bits (every thread of the workgroup).
 __device__ __forceinline__ uint32_t named_before(const TableParams& P, int64_t first, uint32_t* scratch) {
   int64_t row[RQ_ROWS];
-#pragma unroll
-  for (int r = 0; r < RQ_ROWS; ++r) row[r] = first + r < P.n ? load_index(P.at, P.rows_i64, first + r) : -1;
+  load_indices<RQ_ROWS>(P.at, P.rows_i64, [&](int r) { return first + r < P.n ? first + r : -1; }, row);
   uint32_t again = 0;
 #pragma unroll
   for (int r = 1; r < RQ_ROWS; ++r)
@@ -107,12 +126,14 @@ __device__ __forceinline__ uint32_t named_before(const TableParams& P, int64_t f
 // A column's entries of a group of rows, those named before left out.
 __device__ __forceinline__ void release_column(const TableParams& P, int64_t first, uint32_t again, int64_t p) {
   int32_t slot[RQ_ROWS];
+  int64_t row[RQ_ROWS], len[RQ_ROWS];
+  load_indices<RQ_ROWS>(P.at, P.rows_i64, [&](int r) { return first + r < P.n && !((again >> r) & 1) ? first + r : -1; }, row);
 #pragma unroll
-  for (int r = 0; r < RQ_ROWS; ++r) {
-    const int64_t row = first + r < P.n && !((again >> r) & 1) ? load_index(P.at, P.rows_i64, first + r) : -1;
-    const int64_t len = row < 0 || row >= P.rows ? 0 : held(P.lens, P.lens_i64, row, P.cols);
-    slot[r] = p < len ? P.table[row * P.stride + p] : -1;
-  }
+  for (int r = 0; r < RQ_ROWS; ++r)
+    if (row[r] >= P.rows) row[r] = -1;
+  load_lens<RQ_ROWS>(P.lens, P.lens_i64, row, P.cols, len);
+#pragma unroll
+  for (int r = 0; r < RQ_ROWS; ++r) slot[r] = p < len[r] ? P.table[row[r] * P.stride + p] : -1;
   add_holders(P, slot, -1);
 }
 
@@ -170,31 +191,67 @@ __global__ __launch_bounds__(RQ_THREADS) void k_emit_freed(TableParams P, const 
   }
 }
 
-// A few rows of a small pool, all of it in one workgroup (RQ_SMALL_ENTRIES columns of rows, RQ_SMALL_SLOTS slots at most): a
-// launch in place of three (5.8 us for 3.3 + 3.4 + 3.8 and their gaps, and two launches less of the host's).
+// Rows of a small pool, all of it in one workgroup: a launch in place of three (2 rows of 750 columns: 4.1 us for 3.3 + 3.4 + 3.8
+// and their gaps, and two launches less of the host's).  The rows and their lengths are read once, and the columns of all groups
+// of RQ_ROWS rows are dealt to the threads in one row, so that many short rows wait for memory no longer than a few.
 constexpr int RQ_WIDE = 1024, RQ_SMALL_ENTRIES = 8 * RQ_WIDE, RQ_SMALL_SLOTS = 16 * RQ_WIDE;
+struct SmallRows {
+  int64_t row[RQ_WIDE];
+  int32_t len[RQ_WIDE];
+};
+// What one workgroup takes: rows, columns of groups, entries (36000: 18 to 22 us, more than the three launches).
+static bool few_rows(int64_t n, int64_t cols) {
+  return n <= RQ_WIDE && (n + RQ_ROWS - 1) / RQ_ROWS * cols <= RQ_SMALL_ENTRIES && n * cols <= 3 * RQ_SMALL_ENTRIES;
+}
+__device__ __forceinline__ void read_rows(const TableParams& t, SmallRows& s) {
+  const int i = (int)threadIdx.x;
+  const int64_t row = i < t.n ? load_index(t.at, t.rows_i64, i) : -1;
+  s.row[i] = row;
+  s.len[i] = row < 0 || row >= t.rows ? 0 : (int32_t)held(t.lens, t.lens_i64, row, t.cols);
+  __syncthreads();
+}
+// The entries of a column of a group of rows; false where there is none left for this thread.
+__device__ __forceinline__ bool column_of(const TableParams& t, const SmallRows& s, uint32_t unit, int32_t (&slot)[RQ_ROWS]) {
+  const uint32_t group = unit / (uint32_t)t.cols, p = unit - group * (uint32_t)t.cols, first = group * RQ_ROWS;
+  if (first >= (uint32_t)t.n) return false;
+#pragma unroll
+  for (int r = 0; r < RQ_ROWS; ++r)
+    slot[r] = (int32_t)p < s.len[first + r] ? t.table[s.row[first + r] * t.stride + p] : -1;
+  return true;
+}
+// The holders that each slot loses are counted in LDS: one workgroup's atomics on memory were most of its time (75 rows of 490
+// columns: 33 us of 39).
 __global__ __launch_bounds__(RQ_WIDE) void k_free_small(TableParams P, int64_t* free_slots, int64_t capacity, int32_t* free_count) {
   __shared__ int s_red[RQ_WIDE / WAVE];
-  __shared__ uint32_t s_again;
-  for (int64_t first = 0; first < P.n; first += RQ_ROWS) {
-    const uint32_t again = named_before(P, first, &s_again);
-    for (int64_t p = threadIdx.x; p < P.cols; p += RQ_WIDE) release_column(P, first, again, p);
-  }
-  publish_wait();  // (the counts have reached what the loads below read)
+  __shared__ SmallRows s_rows;
+  __shared__ int32_t s_lost[RQ_SMALL_SLOTS];
+  const int tid = threadIdx.x;
+  for (int k = tid; k < P.num_slots; k += RQ_WIDE) s_lost[k] = 0;
+  read_rows(P, s_rows);
+  bool again = false;  // (a row that is named before counts once)
+  for (int k = 0; k < tid && tid < P.n; ++k) again |= s_rows.row[k] == s_rows.row[tid];
   __syncthreads();
-  for (int64_t k = threadIdx.x; k < P.n; k += RQ_WIDE) {
-    const int64_t row = load_index(P.at, P.rows_i64, k);
-    if (row >= 0 && row < P.rows) set_len(P.lens, P.lens_i64, row, 0);
-  }
-  const int per = (int)((P.num_slots + RQ_WIDE - 1) / RQ_WIDE), s0 = (int)threadIdx.x * per;
+  if (again) s_rows.len[tid] = 0;
+  __syncthreads();
+  int32_t slot[RQ_ROWS];
+  for (uint32_t unit = tid; column_of(P, s_rows, unit, slot); unit += RQ_WIDE)
+#pragma unroll
+    for (int r = 0; r < RQ_ROWS; ++r)
+      if (slot[r] >= 0 && slot[r] < P.num_slots) atomicAdd(&s_lost[slot[r]], 1);
+  __syncthreads();  // (and every length has been read)
+  if (tid < P.n && s_rows.row[tid] >= 0 && s_rows.row[tid] < P.rows) set_len(P.lens, P.lens_i64, s_rows.row[tid], 0);
+  const int per = (int)((P.num_slots + RQ_WIDE - 1) / RQ_WIDE), s0 = tid * per;
   uint32_t freed = 0;
-  for (int k = 0; k < per; ++k) freed |= (s0 + k < P.num_slots && ld_dev(P.shared + s0 + k) < 0 ? 1u : 0u) << k;
+  for (int k = 0; k < per && s0 + k < P.num_slots; ++k) {
+    const int32_t lost = s_lost[s0 + k], was = P.shared[s0 + k], now = was - lost;
+    if (now < 0) freed |= 1u << k;
+    if (now < 0 || lost) P.shared[s0 + k] = now < 0 ? 0 : now;
+  }
   int total;
   int64_t at = block_excl_scan<RQ_WIDE / WAVE>((int)__popc(freed), s_red, &total);
-  if (threadIdx.x == 0) *free_count = total;
+  if (tid == 0) *free_count = total;
   for (int k = 0; k < per; ++k) {
     if (!((freed >> k) & 1)) continue;
-    P.shared[s0 + k] = 0;
     if (at < capacity) free_slots[at] = s0 + k;
     ++at;
   }
@@ -280,27 +337,18 @@ __global__ __launch_bounds__(RQ_THREADS) void k_plan_moves(CompactParams P) {
 constexpr int RQ_BITS = 2 * 16 * RQ_WIDE;  // slots at most
 __global__ __launch_bounds__(RQ_WIDE) void k_plan_small(CompactParams P) {
   __shared__ uint32_t s_bits[RQ_BITS / 32];
+  __shared__ SmallRows s_rows;
   __shared__ int s_red[RQ_WIDE / WAVE];
   const TableParams& t = P.t;
   const int tid = threadIdx.x;
   static_assert(RQ_BITS / 32 == RQ_WIDE, "a word a thread");
-  s_bits[tid] = 0;
-  __syncthreads();
-  for (int64_t first = 0; first < t.n; first += RQ_ROWS) {
-    int64_t row[RQ_ROWS], len[RQ_ROWS];
+  s_bits[tid] = 0;  // (a barrier follows, where the rows are read)
+  read_rows(t, s_rows);
+  int32_t slot[RQ_ROWS];
+  for (uint32_t unit = tid; column_of(t, s_rows, unit, slot); unit += RQ_WIDE)
 #pragma unroll
-    for (int r = 0; r < RQ_ROWS; ++r) row[r] = first + r < t.n ? load_index(t.at, t.rows_i64, first + r) : -1;
-#pragma unroll
-    for (int r = 0; r < RQ_ROWS; ++r) len[r] = row[r] < 0 || row[r] >= t.rows ? 0 : held(t.lens, t.lens_i64, row[r], t.cols);
-    for (int64_t p = tid; p < t.cols; p += RQ_WIDE) {
-      int32_t slot[RQ_ROWS];
-#pragma unroll
-      for (int r = 0; r < RQ_ROWS; ++r) slot[r] = p < len[r] ? t.table[row[r] * t.stride + p] : -1;
-#pragma unroll
-      for (int r = 0; r < RQ_ROWS; ++r)
-        if (slot[r] >= 0 && slot[r] < t.num_slots) atomicOr(&s_bits[slot[r] / 32], 1u << (slot[r] % 32));
-    }
-  }
+    for (int r = 0; r < RQ_ROWS; ++r)
+      if (slot[r] >= 0 && slot[r] < t.num_slots) atomicOr(&s_bits[slot[r] / 32], 1u << (slot[r] % 32));
   __syncthreads();
   const uint32_t word = s_bits[tid];
   const int U = block_sum<RQ_WIDE / WAVE>((int)__popc(word), s_red);
@@ -541,7 +589,7 @@ extern "C" int dsv_free_requests(int32_t* req_to_token, int64_t rows, int64_t rt
   TableParams P{req_to_token, rows, rt_stride, rt_cols, seq_lens, seq_lens_i64, rows_i64, at, n, num_slots, shared,
                 (rt_cols + RQ_THREADS - 1) / RQ_THREADS};
   int32_t* counts = reinterpret_cast<int32_t*>(workspace);
-  if (num_slots <= RQ_SMALL_SLOTS && (n + RQ_ROWS - 1) / RQ_ROWS * rt_cols <= RQ_SMALL_ENTRIES) {
+  if (num_slots <= RQ_SMALL_SLOTS && few_rows(n, rt_cols)) {
     hipLaunchKernelGGL(k_free_small, dim3(1), dim3(RQ_WIDE), 0, stream, P, free_slots, capacity, free_count);
     DSV_CHECK_LAUNCH("k_free_small");
     return DSV_OK;
@@ -591,7 +639,7 @@ extern "C" int dsv_compact_requests(int32_t* req_to_token, int64_t rows, int64_t
   P.dst = dst;
   P.out = counts;
   P.pool = (int)pool;
-  if (num_slots <= RQ_BITS && (n + RQ_ROWS - 1) / RQ_ROWS * rt_cols <= RQ_SMALL_ENTRIES) {
+  if (num_slots <= RQ_BITS && few_rows(n, rt_cols)) {
     hipLaunchKernelGGL(k_plan_small, dim3(1), dim3(RQ_WIDE), 0, stream, P);
     DSV_CHECK_LAUNCH("k_plan_small");
   } else {
