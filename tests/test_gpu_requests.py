@@ -236,3 +236,33 @@ def test_a_round_of_samples(device):
         assert sorted(free_slots[:60].tolist()) == free_slots[:60].tolist() == sorted(perm[400:460].tolist())
         for a, b in zip(before, after):
             assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("rows, cols", [(40, 60), (75, 320), (75, 330), (1030, 7), (1, 8000), (9, 4096), (9, 4097)])
+def test_many_short_rows_and_few_long_ones(device, rows, cols):
+    """On both sides of what one workgroup takes: rows that share, rows named again in another group of eight, all of them
+    ended in two calls, and the rest compacted between."""
+    from dspine_amd.runtime.requests import compact_requests, free_requests
+
+    g = _gen(rows + cols)
+    lens = torch.randint(0, min(cols, 16000 // rows) + 1, (rows,), generator=g).tolist()
+    lend = [(i, i + 1, min(lens[i], lens[i + 1]) // 2) for i in range(0, rows - 1, 2)]
+    slots = max(1, min(16384, sum(lens) + 50))
+    table, full, shared = _pool(rows, rows=rows, cols=cols, slots=slots, lens=lens, lend=lend)
+    t, n, s = (x.to(device) for x in (table, full, shared))
+    dead = torch.randint(-1, rows + 1, (rows,), generator=g).tolist() + [0, 0]
+    for what in (dead, list(range(rows))):
+        got, count = free_requests(t, n, s, _ids(device, what, torch.int32))
+        want = B.free(table, full, shared, what)
+        assert got[: int(count)].tolist() == want
+        assert torch.equal(n.cpu(), full) and torch.equal(s.cpu(), shared)
+        cache = _cache_cpu(g, slots, 1, 16, BF, BF)
+        gpu = _to(cache, device)
+        live = list(range(rows - 1, -1, -1)) + [0]
+        moves, counts = compact_requests(t, n, _ids(device, live, torch.int64), gpu, shared=s)
+        src, dst, used = B.compact(table, full, live, slots, shared)
+        assert counts.tolist() == [used, len(src)] and moves[0, : len(src)].tolist() == src
+        assert torch.equal(t.cpu(), table) and torch.equal(s.cpu(), shared)
+        cache[0][dst] = cache[0][src]
+        assert torch.equal(gpu.k.cpu(), cache[0])
+    assert not bool(n.any())
