@@ -89,7 +89,8 @@ def index_blocks(index: BlockIndex, cache: KVCache, *, page_table: torch.Tensor,
                  from_lens: torch.Tensor, to_lens: torch.Tensor, longest: int | None = None) -> None:
     """The bounds of the blocks that each request finished as it grew from ``from_lens[b]`` to ``to_lens[b]``
     positions (int32 [bs]) whose keys are written: of each block j with from // block_size <= j < to // block_size into
-    index row ``block_table[b, j]`` (int32 [bs, L]), on the current stream.
+    index row ``block_table[b, j]`` (int32 [bs, L]), on the current stream.  ``page_table`` is that of these positions: after
+    a commit the request table's rows as the commit left them, not the window's of the attention before it.
 
     Keys are what ``read_kv`` gives, rounded once to the index's type (so a bound may lie half a step inside); a
     NaN makes both bounds of its element NaN.  Positions past ``page_table`` (int32 [bs, L]) and slots outside the cache
