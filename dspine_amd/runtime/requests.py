@@ -95,7 +95,9 @@ def compact_requests(req_to_token: torch.Tensor, seq_lens: torch.Tensor, rows: t
     The rows' entries, ``shared`` and every tensor of ``caches`` (a ``KVCache``, a ``BlockIndex`` for a block table, or
     a list of them: the model's layers) follow; what lies in a slot that was moved from stays there.  Returns ``(moves,
     counts)``: int64 [2, >= num_slots // 2], from and to, and int32 [2], U and the number of moves; entries past it are
-    left as they were.  Slots of drafts that no length counts yet are not held: call between rounds."""
+    left as they were.  A slot that none of ``rows`` holds is unused, and may be written over: slots that are kept outside the
+    table (padding's, a prefix cache's) need a row of their own among them.  Slots of drafts that no length counts yet are not
+    held: call between rounds."""
     table = _check_requests(req_to_token, seq_lens)
     i64 = _check_rows(rows, "rows")
     parts, tensors, slots = slot_rows(caches)

@@ -629,7 +629,8 @@ int64_t dsv_free_requests_workspace_bytes(int64_t num_slots);
 /* With U distinct slots in the rows at[i], i < n, which are all the rows that hold any: the used slots  */
 /* at or above U move, in ascending order, into the unused ones below U, in ascending order.  The rows' */
 /* entries, shared (may be NULL) and the tensors of slot_rows follow.  src, dst [capacity >= num_slots  */
-/* / 2]: the moves; counts [2]: U and the number of moves.                                             */
+/* / 2]: the moves; counts [2]: U and the number of moves.  What lies in a slot that none of the rows    */
+/* holds may be written over.                                                                         */
 int dsv_compact_requests(int32_t* req_to_token, int64_t rows, int64_t rt_stride, int64_t rt_cols,
                          const void* seq_lens, int32_t seq_lens_i64, int32_t* shared, int64_t num_slots,
                          const void* at, int32_t rows_i64, int64_t n, const dsv_slot_rows* slot_rows,

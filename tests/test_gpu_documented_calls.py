@@ -78,3 +78,31 @@ def test_a_long_contexts_round(device, rows, pool, lens_dtype):
             else:
                 assert not bool(row.any())
     assert done == 3 and req_to_token[pool[0], 62:65].tolist() == before[pool[0], [62, 64, 67]].tolist()
+
+
+def test_requests_that_share_slots(device):
+    """Forked, ended and compacted; a row of its own holds the slots that no request may be given, and they stay or move
+    with what lies in them."""
+    from dspine_amd.kernels.cache import KVCache
+
+    g = torch.Generator().manual_seed(5)
+    slots, cols, H, D = 300, 90, 2, 32
+    perm = 2 + torch.randperm(slots - 3, generator=g).to(torch.int32)
+    table = torch.zeros(8, cols, dtype=torch.int32)
+    lens = torch.tensor([40, 55, 0, 0, 0, 0, 0, 3], dtype=torch.int32)
+    table[0, :40], table[1, :55] = perm[:40], perm[40:95]
+    table[7, :3] = torch.tensor([0, 1, slots - 1])  # padding's slots and one that somebody outside reads
+    first = [torch.randn(slots, H, D, generator=g).to(BF).to(device) for _ in range(4)]
+    caches = [KVCache(first[0].clone(), first[1].clone()), KVCache(first[2].clone(), first[3].clone())]
+    state = dict(torch=torch, num_slots=slots, caches=caches, req_to_token=table.to(device), seq_lens=lens.to(device),
+                 parents=torch.tensor([0, 0, 1], device=device), children=torch.tensor([2, 3, 4], device=device),
+                 rows=torch.tensor([0, 1, 3], device=device), live_rows=torch.tensor([2, 4, 7], device=device))
+    exec(_example("fork_requests", "free_requests", "compact_requests"), state)
+    t = state["req_to_token"]
+    assert state["seq_lens"].tolist() == [0, 0, 40, 0, 55, 0, 0, 3] and int(state["free_count"]) == 0
+    assert state["counts"].tolist()[0] == 40 + 55 + 3 and not bool(state["shared"].any())
+    held = torch.cat((t[2, :40], t[4, :55], t[7, :3])).long()
+    assert sorted(held.tolist()) == list(range(98)) and t[7, :2].tolist() == [0, 1]
+    old = torch.cat((perm[:95], table[7, :3])).long().to(device)
+    for cache, (k, v) in zip(caches, (first[:2], first[2:])):
+        assert torch.equal(cache.k[held], k[old]) and torch.equal(cache.v[held], v[old])
