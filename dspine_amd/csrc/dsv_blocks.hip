@@ -193,13 +193,18 @@ __global__ __launch_bounds__(WAVES * WAVE) void k_score_blocks(ScoreParams P) {
   const int64_t full = pre < 0 ? 0 : pre >> P.shift;
   int n = a.verify_lens ? a.verify_lens[b] : a.T;
   n = n < 0 ? 0 : (n > a.T ? a.T : n);
+  int64_t row0 = a.row_offsets ? load_index(a.row_offsets, a.row_offsets_i64, b) : (int64_t)b * a.T;
+  // (nodes whose rows lie outside q are not there)
+  const int skip = row0 < 0 ? (row0 > -(int64_t)n ? (int)-row0 : n) : 0;
+  row0 += skip;
+  n -= skip;
+  if (n > 0 && a.rows - row0 < n) n = row0 < a.rows ? (int)(a.rows - row0) : 0;
   const int rows = n * (int)P.G.d, tiles = (rows + 15) / 16;
   const int64_t cols = a.block_cols, first = (int64_t)chunk * P.steps * SB_STEP;
   const int64_t past = first + P.steps * SB_STEP < cols ? first + P.steps * SB_STEP : cols;  // of the table
   const int64_t end = rows == 0 ? first : (past < full ? past : full);               // of the blocks that have a score
   float* const out = a.scores + (int64_t)bh * cols;
   const int32_t* const table = a.block_table + b * a.block_stride;
-  const int64_t row0 = a.row_offsets ? load_index(a.row_offsets, a.row_offsets_i64, b) : (int64_t)b * a.T;
   for (int64_t i = (end > first ? end : first) + tid; i < past; i += WAVES * WAVE) out[i] = -INFINITY;
   if (end <= first) return;
   uint4 k[NC][2];
@@ -232,11 +237,10 @@ __global__ __launch_bounds__(WAVES * WAVE) void k_score_blocks(ScoreParams P) {
         int r = (t0 + t) * 16 + m;
         r = r < rows ? r : rows - 1;  // (a row again: the largest stays the largest)
         const int node = (int)P.G.div((uint32_t)r), head = h * (int)P.G.d + r - node * (int)P.G.d;
-        const int64_t row = row0 + node;
         const int d = c * 32 + g * 8;
         w[u] = make_uint4(0, 0, 0, 0);
-        if (i < here * NC && row >= 0 && row < a.rows && (FULL || d < dim))
-          w[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + row * a.q_row_stride +
+        if (i < here * NC && (FULL || d < dim))
+          w[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(a.q) + (row0 + node) * a.q_row_stride +
                                                  head * a.q_head_stride + d);
       }
       if (i0 == wave) load(first + wave * 16);

@@ -120,8 +120,8 @@ def score_blocks(q: torch.Tensor, index: BlockIndex, *, T: int, block_table: tor
 
     q [rows, q_heads, dim] of the index's dtype, ``T``, ``prefix_lens``, ``verify_lens`` and ``row_offsets`` as in
     ``tree_attention``; 0 < ``scale``, default 1 / sqrt(dim).  Blocks from prefix_lens[b] // block_size on, rows outside the
-    index and requests without nodes get -inf; a NaN in a query or a bound, or an infinite bound beside a zero, gives NaN.
-    ``out``: a contiguous tensor to fill."""
+    index and requests without nodes (one whose row lies outside q is none) get -inf; a NaN in a query or a bound, or an
+    infinite bound beside a zero, gives NaN.  ``out``: a contiguous tensor to fill."""
     if q.ndim != 3 or q.dtype not in _ACT:
         raise ValueError("q must be bfloat16 or float16 [rows, q_heads, dim]")
     x = index_fields(index)
