@@ -37,6 +37,14 @@ __device__ __forceinline__ void join_bounds(float* lo, float* hi, int lane) {
   }
 }
 
+// A finite bound past the index type's range as its largest number: infinite, a block of finite keys would have scores of
+// no use, 0 * infinity among them.
+template <int IT>
+__device__ __forceinline__ float in_range(float v) {
+  constexpr float TOP = IT == DSV_F16 ? 65504.f : 0x1.fep127f;
+  return fabsf(v) < INFINITY ? fminf(fmaxf(v, -TOP), TOP) : v;
+}
+
 // Bounds of a finished block, a wave a (block, head): its lanes hold the block's slots, groups of G lanes take a position's
 // row, 16 bytes a lane, BI_ROWS rows in flight together.  NaN counts as the least and the largest.  Bound by memory: the
 // blocks of four prompts, 88 MB of e4m3 keys: 19.8 us, 4.5 TB/s (a workgroup a block and head, two rows in flight: 57 us).
@@ -121,7 +129,9 @@ __global__ __launch_bounds__(BI_THREADS) void k_index_blocks(IndexParams P) {
   uint16_t* out = reinterpret_cast<uint16_t*>(P.x.bounds) + ((int64_t)row * c.heads + h) * 2 * c.dim + d;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    const float* v = k ? hi : lo;
+    float* const v = k ? hi : lo;
+#pragma unroll
+    for (int e = 0; e < LEFT; ++e) v[e] = in_range<IT>(v[e]);
     if constexpr (LEFT >= 2) {
 #pragma unroll
       for (int e = 0; e < LEFT; e += 2)

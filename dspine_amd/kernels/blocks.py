@@ -92,11 +92,11 @@ def index_blocks(index: BlockIndex, cache: KVCache, *, page_table: torch.Tensor,
     index row ``block_table[b, j]`` (int32 [bs, L]), on the current stream.  ``page_table`` is that of these positions: after
     a commit the request table's rows as the commit left them, not the window's of the attention before it.
 
-    Keys are what ``read_kv`` gives, rounded once to the index's type (so a bound may lie half a step inside); a
-    NaN makes both bounds of its element NaN.  Positions past ``page_table`` (int32 [bs, L]) and slots outside the cache
-    do not count, a block of nothing else gets zeros.  Blocks past ``block_table`` and rows outside the index are
-    skipped; the rows of a call must be distinct.  ``longest``: the most positions that any request grew by
-    (default: the page table's width); a growth beyond it is not indexed."""
+    Keys are what ``read_kv`` gives in float32, rounded once to the index's type (so a bound may lie half a step inside), those
+    that are finite but past its range to its largest number; a NaN makes both bounds of its element NaN.  Positions
+    past ``page_table`` (int32 [bs, L]) and slots outside the cache do not count, a block of nothing else gets zeros.  Blocks
+    past ``block_table`` and rows outside the index are skipped; the rows of a call must be distinct.  ``longest``: the most
+    positions that any request grew by (default: the page table's width); a growth beyond it is not indexed."""
     x, c = index_fields(index), cache_fields(cache)
     if (x.heads, x.dim) != (c.heads, c.dim):
         raise ValueError("the index and the cache must have the same heads and dim")
