@@ -143,8 +143,8 @@ __global__ __launch_bounds__(BI_THREADS) void k_index_blocks(IndexParams P) {
 }
 
 // ---------------------------------------------------------------------------------------
-// Scores: with q+ and q- a query's positive and negative elements, sum_d max(q lo, q hi) = q- . lo + q+ . hi, a product
-// over 2 * dim elements of an index row as it lies in memory.  The matrix cores take 16 blocks as rows and 16 queries as
+// Scores: with q+ and q- a query's positive and negative elements, sum_d max(q lo, q hi) = q- . lo + q+ . hi where the bounds
+// are finite, a product over 2 * dim elements of an index row as it lies in memory.  The matrix cores take 16 blocks as rows and 16 queries as
 // columns; a block's score is the largest of its columns'.
 // ---------------------------------------------------------------------------------------
 constexpr int SB_WAVES = 4, SB_MANY = 8;  // waves of a workgroup, and where the queries take much LDS
@@ -178,12 +178,47 @@ __device__ __forceinline__ void split_signs(uint32_t w, uint32_t& negative, uint
   positive = w & ~sign;
 }
 
+// The largest sum by its definition, a row of queries at a time over the lanes' elements, for a block that the product gave
+// NaN: with an infinite bound beside an element of the other sign it adds a 0 * infinity that is no term of the sum.
+// NaN where no bound is infinite.
+template <int IT>
+__device__ __forceinline__ float defined_sum(const dsv_score_blocks_args& a, const FastDiv& G, int32_t block, int h, int64_t row0,
+                                             int rows, int lane) {
+  const dsv_block_index& x = a.index;
+  const uint16_t* from = reinterpret_cast<const uint16_t*>(x.bounds) + ((int64_t)block * x.heads + h) * 2 * x.dim;
+  const int d = lane * 4;  // (four elements a lane: up to 256)
+  const bool in = d < x.dim;
+  auto four = [&](const uint16_t* p, float (&f)[4]) {
+    const uint2 w = in ? *reinterpret_cast<const uint2*>(p + d) : make_uint2(0, 0);
+    f[0] = act_to_f32<IT>(w.x & 0xffffu), f[1] = act_to_f32<IT>(w.x >> 16);
+    f[2] = act_to_f32<IT>(w.y & 0xffffu), f[3] = act_to_f32<IT>(w.y >> 16);
+  };
+  float lo[4], hi[4];
+  four(from, lo);
+  four(from + x.dim, hi);
+  bool infinite = false;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) infinite |= fabsf(lo[e]) == INFINITY || fabsf(hi[e]) == INFINITY;
+  if (!__any(infinite)) return NAN;
+  float best = -INFINITY;
+  for (int r = 0; r < rows; ++r) {
+    const int node = (int)G.div((uint32_t)r), head = h * (int)G.d + r - node * (int)G.d;
+    float q[4], sum = 0.f;
+    four(reinterpret_cast<const uint16_t*>(a.q) + (row0 + node) * a.q_row_stride + head * a.q_head_stride, q);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sum += __builtin_elementwise_maximum(q[e] * lo[e], q[e] * hi[e]);
+    best = __builtin_elementwise_maximum(best, wave_sum(sum));
+  }
+  return best;
+}
+
 // A workgroup some steps of a (request, head)'s blocks, its queries as operands in LDS; a wave 16 blocks a step, their
 // bounds in registers for all of the queries.  Bound by memory: 64 requests of 8k to 64k positions in blocks of 64, up to 17
 // nodes, 147 MB of bounds: 38 us, 3.9 TB/s (the next step's bounds loaded into a second set of registers first: 42 us for 41;
 // queries split by sign in LDS, twice the memory and half the workgroups a CU: 62 us).  One node over 32k: 4.8 us, latency.
+// (Five waves a SIMD at dims 80 to 112: with the registers of four, 16 x 17 nodes of dim 96 take 19.0 us for 18.3.)
 template <int IT, int NC, bool FULL, int WAVES>
-__global__ __launch_bounds__(WAVES * WAVE) void k_score_blocks(ScoreParams P) {
+__global__ __launch_bounds__(WAVES * WAVE, NC == 4 && !FULL ? 5 : 1) void k_score_blocks(ScoreParams P) {
   constexpr int SB_STEP = WAVES * 16;  // blocks of a step
   const dsv_score_blocks_args& a = P.a;
   const dsv_block_index& x = a.index;
@@ -293,13 +328,19 @@ __global__ __launch_bounds__(WAVES * WAVE) void k_score_blocks(ScoreParams P) {
         mine = m == r ? v : mine;
       }
       const int64_t j = j0 + g * 4 + m;
-      if (m < 4 && j < end) {
-        const int at = (int)(j - first);
-        if (t0) mine = __builtin_elementwise_maximum(mine, s_best[at]);
-        if (t0 + here < tiles)
-          s_best[at] = mine;  // (read by the same lane)
-        else
+      const bool writes = m < 4 && j < end, final = t0 + here == tiles;
+      const int at = (int)(j - first);
+      if (writes && t0) mine = __builtin_elementwise_maximum(mine, s_best[at]);
+      for (uint64_t odd = __ballot(writes && final && has && mine != mine); odd; odd &= odd - 1) {
+        const int l = __ffsll((unsigned long long)odd) - 1;
+        const float v = defined_sum<IT>(a, P.G, table[j0 + (l >> 4) * 4 + (l & 15)], h, row0, rows, lane);
+        if (lane == l) mine = v;
+      }
+      if (writes) {
+        if (final)
           out[j] = has ? mine * a.scale : -INFINITY;
+        else
+          s_best[at] = mine;  // (read by the same lane)
       }
     }
   }

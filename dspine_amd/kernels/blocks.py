@@ -115,13 +115,14 @@ def score_blocks(q: torch.Tensor, index: BlockIndex, *, T: int, block_table: tor
                  verify_lens: torch.Tensor | None = None, row_offsets: torch.Tensor | None = None,
                  scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """float32 [bs, heads, L]: for each block j of ``block_table`` (int32 [bs, L]) the largest, over the request's nodes and
-    the query heads of a cache head, of scale * sum_d (min(q_d, 0) least_d + max(q_d, 0) largest_d), which no scaled score of
-    the block's keys exceeds (but for the bounds' rounding).
+    the query heads of a cache head, of scale * sum_d max(q_d least_d, q_d largest_d), which no scaled score of the block's
+    keys exceeds (but for the bounds' rounding).
 
     q [rows, q_heads, dim] of the index's dtype, ``T``, ``prefix_lens``, ``verify_lens`` and ``row_offsets`` as in
     ``tree_attention``; 0 < ``scale``, default 1 / sqrt(dim).  Blocks from prefix_lens[b] // block_size on, rows outside the
-    index and requests without nodes (one whose row lies outside q is none) get -inf; a NaN in a query or a bound, or an
-    infinite bound beside a zero, gives NaN.  ``out``: a contiguous tensor to fill."""
+    index and requests without nodes (one whose row lies outside q is none) get -inf.  A NaN among a block's terms makes its
+    score NaN, whichever node it is of: a query with a NaN, a NaN bound, an infinite one beside a query of zero, infinities of
+    both signs.  ``out``: a contiguous tensor to fill."""
     if q.ndim != 3 or q.dtype not in _ACT:
         raise ValueError("q must be bfloat16 or float16 [rows, q_heads, dim]")
     x = index_fields(index)

@@ -551,11 +551,11 @@ int dsv_index_blocks(const dsv_block_index* index, const dsv_kv_cache* cache, co
                      int64_t longest, dsv_stream_t stream);
 
 /* scores[b, h, j] (float32 [bs, heads, block_cols], contiguous): the largest, over request b's nodes   */
-/* and the query heads of cache head h, of scale * sum_d (min(q_d, 0) least_d + max(q_d, 0) largest_d), */
-/* which no scaled score of the block's keys exceeds but for rounding; float32 sums.  -inf for blocks   */
-/* that are not finished, rows outside the index and requests without nodes; NaN where a query, a bound */
-/* or their product is.  Nodes and rows as in dsv_tree_attention (one whose row lies outside q is not      */
-/* there); 0 < scale <= 2^100.                                                                        */
+/* and the query heads of cache head h, of scale * sum_d max(q_d least_d, q_d largest_d), which no      */
+/* scaled score of the block's keys exceeds but for rounding; float32 sums.  -inf for blocks that are   */
+/* not finished, rows outside the index and requests without nodes; NaN where any of the block's terms  */
+/* or sums is (a NaN query or bound, an infinite bound beside a query of zero).  Nodes and rows as in    */
+/* dsv_tree_attention (one whose row lies outside q is not there); 0 < scale <= 2^100.                  */
 typedef struct dsv_score_blocks_args {
   dsv_block_index index;
   const void* q;               /* [rows, q_heads, dim] of the index's type, 16-byte-aligned rows */

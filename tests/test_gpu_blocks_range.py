@@ -1,4 +1,4 @@
-"""Finite keys past the index type's range."""
+"""Finite keys past the index type's range, and bounds that are infinite."""
 
 import math
 
@@ -63,3 +63,52 @@ def test_finite_keys_past_the_types_range(device, D, size, act, dtype, unit):
     scores = score_blocks(q.to(act).to(device), index, T=1, block_table=table, prefix_lens=pre, scale=2.0 ** -10)
     assert bool(torch.isfinite(scores).all())
     assert select_blocks(scores, 1, prefix_lens=pre, block_size=size).flatten().tolist() == [2, 2]
+
+
+def _definition(q, bounds, size, *, T, block_table, prefix_lens, scale):
+    """(scores, tolerance): the largest over nodes and heads of sum_d max(q_d least_d, q_d largest_d), NaN where a term is."""
+    Hq, D = q.shape[1:]
+    H, (bs, L) = bounds.shape[1], block_table.shape
+    out = torch.full((bs, H, L), -math.inf, dtype=torch.float64)
+    tol = torch.zeros_like(out)
+    for b in range(bs):
+        x = q[b * T: (b + 1) * T].double().view(T, H, Hq // H, D)
+        for j in range(int(prefix_lens[b]) // size):
+            lo, hi = bounds[int(block_table[b, j])].double().view(1, H, 1, 2, D).unbind(3)
+            term = torch.maximum(x * lo, x * hi)
+            out[b, :, j] = term.sum(-1).amax((0, 2)) * scale
+            mag = term.abs().sum(-1)
+            tol[b, :, j] = (2 * D + 8) * R.U32 * torch.where(torch.isfinite(mag), mag, 0.0).amax((0, 2)) * scale
+    return out, tol
+
+
+@pytest.mark.parametrize("act", [BF, HF])
+@pytest.mark.parametrize("T, H, G, D, L", [(1, 1, 1, 16, 7), (5, 3, 2, 80, 40), (17, 2, 4, 128, 300), (64, 1, 32, 64, 33), (3, 2, 5, 256, 70)])
+def test_scores_of_infinite_bounds(device, T, H, G, D, L, act):
+    """An element's larger product, where the other one is that of an infinity; zero queries beside one, NaN bounds, and
+    infinities of both signs (whose sum is none)."""
+    from dspine_amd.kernels.blocks import BlockIndex, score_blocks
+
+    g = torch.Generator().manual_seed(D + L)
+    bs, size, scale = 2, 16, 0.25
+    q = torch.randn(bs * T, H * G, D, generator=g).to(act)
+    q[:, :, 3] = q[:, :, 3].abs() + 0.5
+    q[:, :, 4] = -q[:, :, 4].abs() - 0.5
+    q[T // 2, :, 5] = 0.0
+    low = torch.randn(bs * L + 2, H, D, generator=g)
+    high = low + torch.rand(low.shape, generator=g)
+    kinds = [  # of block i % 9 + ...: (element, least, largest)
+        [], [(3, -math.inf, 1.0)], [(3, 0.5, math.inf)], [(4, -1.0, math.inf)], [(4, -math.inf, 2.0)], [(6, -math.inf, math.inf)],
+        [(5, 0.0, math.inf)], [(3, -math.inf, -math.inf), (4, -math.inf, 0.0)], [(7, math.nan, math.nan), (3, -math.inf, 1.0)]]
+    for i in range(bs * L):
+        for d, l, h in kinds[i % len(kinds)]:
+            low[i, :, d], high[i, :, d] = l, h
+    low[5 % (bs * L), 0, :], high[5 % (bs * L), 0, :] = math.inf, math.inf
+    bounds = torch.stack((low, high), 2).to(act)
+    d = dict(T=T, block_table=torch.randperm(bs * L, generator=g).to(torch.int32).view(bs, L),
+             prefix_lens=torch.tensor([L * size + 3, (L - 1) * size], dtype=torch.int32), scale=scale)
+    want, tol = _definition(q, bounds, size, **d)
+    assert bool(torch.isfinite(want).any()) and bool((want == math.inf).any()) and bool(torch.isnan(want).any())
+    got = score_blocks(q.to(device), BlockIndex(bounds.to(device), size),
+                       **{k: (x.to(device) if isinstance(x, torch.Tensor) else x) for k, x in d.items()})
+    R.close(got, want, tol)
