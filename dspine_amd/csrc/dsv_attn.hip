@@ -23,7 +23,8 @@ constexpr int AJ_THREADS = 256, AJ_PARTS = 4;
 // lengths, then the parts: 4.9 us after one request's few parts, 7 to 8 us for most batches) and, for many rows, by the
 // sums' bytes (14.3 us for 16 requests of 512 rows a head).  A launch of its own: a last workgroup that joins would need
 // counters that somebody clears.
-template <int XT, int DP, bool BLOCKS>
+// AHEAD: the next few parts are on their way while these are added, which takes the registers of twice as many waves.
+template <int XT, int DP, bool BLOCKS, bool AHEAD>
 __global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
   const dsv_tree_attention_args& a = P.a;
   const dsv_kv_cache& c = a.cache;
@@ -47,7 +48,7 @@ __global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
     return ((int64_t)(2 * i + (i == i0 && plan.start(i) < before ? 1 : 0)) * c.heads + h) * rows + r;
   };
   float top = AT_LOW, ref = 0.f, lt = 0.f, sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  // (the references and the sums of a few parts are asked for at once, those of the next few while these are added)
+  // (the references and the sums of a few parts are asked for at once)
   float4 next_ml[AJ_PARTS];
   f32x4 next_x[AJ_PARTS][2];
   auto ask = [&](int i) {
@@ -59,13 +60,14 @@ __global__ __launch_bounds__(AJ_THREADS) void k_attn_join(AttnParams P) {
       next_x[j][1] = *reinterpret_cast<const f32x4*>(P.part_o + at * c.dim + d + 4);
     }
   };
-  ask(i0);
+  if (AHEAD) ask(i0);
   for (int i = i0; i <= i1; i += AJ_PARTS) {
+    if (!AHEAD) ask(i);
     float4 ml[AJ_PARTS];
     f32x4 x[AJ_PARTS][2];
 #pragma unroll
     for (int j = 0; j < AJ_PARTS; ++j) ml[j] = next_ml[j], x[j][0] = next_x[j][0], x[j][1] = next_x[j][1];
-    if (i + AJ_PARTS <= i1) ask(i + AJ_PARTS);
+    if (AHEAD && i + AJ_PARTS <= i1) ask(i + AJ_PARTS);
     const float old = top;
 #pragma unroll
     for (int j = 0; j < AJ_PARTS; ++j) top = fmaxf(top, ml[j].x);  // (the last part again, where there are fewer)
@@ -218,13 +220,20 @@ static int attention(const char* what, const dsv_tree_attention_args& a, const d
          : launch_attn<DSV_F16, DSV_F16, BLOCKS>(P, s, (unsigned)blocks, stream);
     DSV_CHECK_LAUNCH("k_attn");
     if (P.most > 1) {
-      auto join = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)joins), dim3(AJ_THREADS), 0, stream, P); };
-      if (wide == 64)
-        bf ? join(k_attn_join<DSV_BF16, 64, BLOCKS>) : join(k_attn_join<DSV_F16, 64, BLOCKS>);
-      else if (wide == 128)
-        bf ? join(k_attn_join<DSV_BF16, 128, BLOCKS>) : join(k_attn_join<DSV_F16, 128, BLOCKS>);
-      else
-        bf ? join(k_attn_join<DSV_BF16, 256, BLOCKS>) : join(k_attn_join<DSV_F16, 256, BLOCKS>);
+      auto launch = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)joins), dim3(AJ_THREADS), 0, stream, P); };
+      auto join = [&](auto ahead) {
+        constexpr bool AHEAD = decltype(ahead)::value;
+        if (wide == 64)
+          bf ? launch(k_attn_join<DSV_BF16, 64, BLOCKS, AHEAD>) : launch(k_attn_join<DSV_F16, 64, BLOCKS, AHEAD>);
+        else if (wide == 128)
+          bf ? launch(k_attn_join<DSV_BF16, 128, BLOCKS, AHEAD>) : launch(k_attn_join<DSV_F16, 128, BLOCKS, AHEAD>);
+        else
+          bf ? launch(k_attn_join<DSV_BF16, 256, BLOCKS, AHEAD>) : launch(k_attn_join<DSV_F16, 256, BLOCKS, AHEAD>);
+      };
+      // Ahead up to two workgroups a CU; with more of them the waves that its registers leave no room for gain more.  Ahead and
+      // not, us: 8 workgroups (1 x 1 node, 32k) 12.2 and 26.4, 160 6.2 and 8.3, 320 (8 x 17 nodes, group 4) 5.9 and 6.2, 512 (2 x 64,
+      // group 8) 9.0 and 9.0, 768 9.4 and 9.0, 1280 (32 x 17) 8.2 and 7.1, 4096 (16 x 64, group 8) 17.4 and 14.5.
+      joins <= 512 ? join(Int<1>{}) : join(Int<0>{});
       DSV_CHECK_LAUNCH("k_attn_join");
     }
     return DSV_OK;
