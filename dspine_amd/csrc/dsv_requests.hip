@@ -194,15 +194,22 @@ __global__ __launch_bounds__(RQ_THREADS) void k_emit_freed(TableParams P, const 
 // Rows of a small pool, all of it in one workgroup: a launch in place of three (2 rows of 750 columns: 4.1 us for 3.3 + 3.4 + 3.8
 // and their gaps, and two launches less of the host's).  The rows and their lengths are read once, and the columns of all groups
 // of RQ_ROWS rows are dealt to the threads in one row, so that many short rows wait for memory no longer than a few.
-constexpr int RQ_WIDE = 1024, RQ_SMALL_ENTRIES = 8 * RQ_WIDE, RQ_SMALL_SLOTS = 16 * RQ_WIDE;
+constexpr int RQ_WIDE = 1024, RQ_SMALL_SLOTS = 16 * RQ_WIDE;
 struct SmallRows {
   int64_t row[RQ_WIDE];
   int32_t len[RQ_WIDE];
 };
-// What one workgroup takes: rows, columns of groups, entries (36000: 18 to 22 us, more than the three launches).
-static bool few_rows(int64_t n, int64_t cols) {
-  return n <= RQ_WIDE && (n + RQ_ROWS - 1) / RQ_ROWS * cols <= RQ_SMALL_ENTRIES && n * cols <= 3 * RQ_SMALL_ENTRIES;
+// What one workgroup takes: rows, columns of groups of rows, entries.  Replayed, us, and those of the launches in its place (whose
+// host's time it saves):
+//   an end      2 x 750 13.5 and 14.5, 4 x 1000 17.7 and 15.4, 8 x 1000 18.5 and 19.1, 16 x 500 18.7 and 18.9; not taken:
+//               1 x 8000 23.1 and 15.0, 40 x 300 24.2 and 19.7, 75 x 320 29.1 and 20.0, 1000 x 8 40.7 and 17.4
+//   compaction  2 x 750 11.0 and 13.9, 8 x 1000 13.9 and 14.9, 8 x 2000 8.5 and 10.5, 75 x 320 14.3 and 14.0, 1000 x 8 14.2 and
+//               15.5, 1 x 8000 19.4 and 14.8
+static bool few_rows(int64_t n, int64_t cols, int64_t rows, int64_t columns, int64_t entries) {
+  return n <= rows && (n + RQ_ROWS - 1) / RQ_ROWS * cols <= columns && n * cols <= entries;
 }
+static bool few_to_free(int64_t n, int64_t cols) { return few_rows(n, cols, 64, 2 * RQ_WIDE, 8 * RQ_WIDE); }
+static bool few_to_plan(int64_t n, int64_t cols) { return few_rows(n, cols, RQ_WIDE, 8 * RQ_WIDE, 24 * RQ_WIDE); }
 __device__ __forceinline__ void read_rows(const TableParams& t, SmallRows& s) {
   const int i = (int)threadIdx.x;
   const int64_t row = i < t.n ? load_index(t.at, t.rows_i64, i) : -1;
@@ -219,8 +226,8 @@ __device__ __forceinline__ bool column_of(const TableParams& t, const SmallRows&
     slot[r] = (int32_t)p < s.len[first + r] ? t.table[s.row[first + r] * t.stride + p] : -1;
   return true;
 }
-// The holders that each slot loses are counted in LDS: one workgroup's atomics on memory were most of its time (75 rows of 490
-// columns: 33 us of 39).
+// The holders that each slot loses are counted in LDS: with one workgroup's atomics on memory 2 rows of 750 columns take 8.8 us
+// for 4.0, 8 of 1024 28.2 for 12.1.
 __global__ __launch_bounds__(RQ_WIDE) void k_free_small(TableParams P, int64_t* free_slots, int64_t capacity, int32_t* free_count) {
   __shared__ int s_red[RQ_WIDE / WAVE];
   __shared__ SmallRows s_rows;
@@ -589,7 +596,7 @@ extern "C" int dsv_free_requests(int32_t* req_to_token, int64_t rows, int64_t rt
   TableParams P{req_to_token, rows, rt_stride, rt_cols, seq_lens, seq_lens_i64, rows_i64, at, n, num_slots, shared,
                 (rt_cols + RQ_THREADS - 1) / RQ_THREADS};
   int32_t* counts = reinterpret_cast<int32_t*>(workspace);
-  if (num_slots <= RQ_SMALL_SLOTS && few_rows(n, rt_cols)) {
+  if (num_slots <= RQ_SMALL_SLOTS && few_to_free(n, rt_cols)) {
     hipLaunchKernelGGL(k_free_small, dim3(1), dim3(RQ_WIDE), 0, stream, P, free_slots, capacity, free_count);
     DSV_CHECK_LAUNCH("k_free_small");
     return DSV_OK;
@@ -639,7 +646,7 @@ extern "C" int dsv_compact_requests(int32_t* req_to_token, int64_t rows, int64_t
   P.dst = dst;
   P.out = counts;
   P.pool = (int)pool;
-  if (num_slots <= RQ_BITS && few_rows(n, rt_cols)) {
+  if (num_slots <= RQ_BITS && few_to_plan(n, rt_cols)) {
     hipLaunchKernelGGL(k_plan_small, dim3(1), dim3(RQ_WIDE), 0, stream, P);
     DSV_CHECK_LAUNCH("k_plan_small");
   } else {
