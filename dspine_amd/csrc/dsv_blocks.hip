@@ -602,9 +602,11 @@ extern "C" int dsv_score_blocks(const dsv_score_blocks_args* args, dsv_stream_t 
   const int64_t bh = (int64_t)a.bs * a.index.heads;
   const int tiles = (a.T * (int)P.G.d + 15) / 16, pieces = a.index.dim <= 64 ? 2 : (a.index.dim <= 128 ? 4 : 8);
   P.staged = tiles < SB_STAGE / pieces ? tiles : SB_STAGE / pieces;
-  // Waves of a workgroup: queries of 20 KB (68 rows of dim 128) 41.6 us with four and 43.9 with eight, of 40 KB (68 of dim 256) 22.8
-  // and 17.9: eight where LDS holds only a few workgroups.
-  const bool many = P.staged * pieces > 32;
+  // Waves of a workgroup, replayed, us, four and eight (16 requests, 32k positions at dim 128): queries of 16 KB (128 rows of dim 64,
+  // 32 of 256) 20.0 and 19.4, 15.6 and 17.4; 20 KB (68 of 128) 16.6 and 17.0; 24 KB (96 of 128, 48 of 256) 17.3 and 17.1, 16.6 and 16.9;
+  // 32 KB (256 of 64, 128 of 128, 64 of 256) 26.4 and 24.3, 18.6 and 17.8, 17.6 and 17.2; 56 to 60 KB (480, 240, 112) 44.0 and 32.9, 27.6
+  // and 22.1, 20.6 and 19.2: eight where LDS holds few workgroups.
+  const bool many = P.staged * pieces > 24;
   const int step = (many ? SB_MANY : SB_WAVES) * 16;
   const int64_t steps = (a.block_cols + step - 1) / step;
   const int64_t per = steps * bh / (many ? 2048 : 4096);  // (half and twice as many workgroups: 44 and 42 us for 41)
