@@ -21,22 +21,25 @@
 // Only the device knows the lengths: every wave computes the same plan from them.  A request within one range is
 // finished there; the parts of the others are left as sums and joined by k_attn_join.
 //
-// Measured, a call among others (8 cache heads, dim 128; the card copies at 4.8 TB/s and multiplies at 1.36 PF):
-//   64 requests, 17 nodes, 4 query heads a cache head, bf16, 1k to 8k positions   268 us   4.5 TB/s: memory
-//   8 requests, 1 node, int8, 16k to 64k positions                                175 us   3.9 TB/s: memory, and 8 to 16 bits
-//   16 requests, 64 nodes, 8 query heads a cache head, e4m3, 4k to 12k            430 us   0.62 PF: a wave's own chain of LDS
+// Measured in kernel traces of replayed graphs, the attention and the join, us, a few percent more than a call takes in a row of
+// eager ones (8 cache heads, dim 128; the card copies at 4.7 to 5.3 TB/s and multiplies at 1.37 PF):
+//   64 requests, 17 nodes, 4 query heads a cache head, bf16, 1k to 8k positions   270 + 7.6   4.4 TB/s: memory
+//   8 requests, 1 node, int8, 16k to 64k positions                                178 + 5.4   3.7 TB/s: memory, and 8 to 16 bits
+//   16 requests, 64 nodes, 8 query heads a cache head, e4m3, 4k to 12k            432 + 14.7  0.60 PF: a wave's own chain of LDS
 //       reads, products, exponentials and products (matrix pipe busy 25 % of the time, VALU 40 %)
-//   4 requests, 25 nodes, bf16, 1.5k to 4.7k                                       36 us   1.5 TB/s: latency (the plan, the
+//   4 requests, 25 nodes, bf16, 1.5k to 4.7k                                      28 + 6.0    1.6 TB/s: latency (the plan, the
 //       first loads, the outputs and the second launch take longer than a workgroup's six tiles)
-//   1 request, 1 node, bf16, 640                                                   17 us   latency (8.6 + 5.1 us in two launches)
+//   1 request, 1 node, bf16, 640                                                  9.0 + 4.0   latency
 //
 // BLOCKS: the same over a list of blocks for each (request, cache head).  The positions are numbered as they are read, so only
 // the way to a slot differs: a group of 16 positions lies in one block, and its list entry is asked for a step (a tile, where
 // tiles are staged) before its slots.
-//   64 requests, up to 17 nodes, 4 query heads a cache head, bf16, 64 blocks of 64  260 us   4.2 TB/s: memory, 256 bytes at a time
-//   16 requests, 1 node, 8192 positions in blocks of 16, 64, 128     bf16 130 to 135, int8 101 to 104: memory (int8: 282 MB, and a
-//       third more for scales whose neighbours are other heads'; heads as the caches' outer dimension: 123 and 95)
-//   1 request, 1 node, 32 blocks of 64                                              15 us   latency (9.4 + 5.3 in two launches)
+//   64 requests, up to 17 nodes, 4 query heads a cache head, bf16, 64 blocks of 64  275 + 7.8  (263 a call in a row of eager
+//       ones, 4.2 TB/s): memory, 256 bytes at a time
+//   1 request, 1 node, 32 blocks of 64                                              9.4 + 5.7  latency
+//   16 requests, 1 node, 8192 positions in blocks of 16, 64, 128, both launches: bf16 130 to 135, int8 101 to 104 (277 MB, 2.7 TB/s);
+//       with heads as the caches' outer dimension, where a slot's scales no longer lie beside other heads', 123 and 95.  What keeps
+//       the 8-bit ones from the rate of whole contexts is not known.
 #pragma once
 #include "dsv_cache.h"
 #include "dsv_common.h"
@@ -329,8 +332,9 @@ __global__ __launch_bounds__(WAVES * WAVE, OCC) void k_attn(AttnParams P) {
   // weight (times its value scale) is rounded to it once, by 2^-9 (bfloat16) or 2^-12 at most.  The errors are random: over n
   // positions of like weight they leave 1 / sqrt(n) of that.  Measured against float64, the output's own rounding included:
   // bfloat16 caches 1.7e-3 to 2.3e-3 (with float32 weights 1.7e-3), 8-bit ones 1.7e-3 (1.7e-3), float16 ones 2.5e-4
-  // (2.1e-4).  Keeping the low half would take a second product of every value.  Sums, references, partial outputs and the
-  // join are float32.
+  // (2.1e-4).  That is at most what the output's rounding to bfloat16 adds anyway.  Keeping the low half takes a second product of
+  // every value: 64 x 17 nodes of 4 heads 299 us for 277 (over selected blocks 300 for 293), 16 x 64 of 8 over blocks 423 for
+  // 336, single nodes 130 for 129.  Sums, references, partial outputs and the join are float32.
   constexpr int PT = CT == DSV_BF16 ? DSV_BF16 : DSV_F16;
   // float16 weights are held 2^11 higher, so that what their range loses lies below 2^-35 of the row's largest
   constexpr float SHIFT = PT == DSV_F16 ? 11.f : 0.f, LIM = PT == DSV_F16 ? 4.f : 8.f;
@@ -1130,8 +1134,11 @@ struct AttnShape {
   int form, R, WR, RB;
   int waves;  // of a workgroup
 };
-// Waves a SIMD that the registers are for: 256 of them each, 512 where the sums of a wide dim need more.  (Two row tiles of dim
-// 128 want more than 256: 8 to 10 are spilled for 8-bit caches, none for 16-bit ones; up to 24 where the dim is not known.)
+// Waves a SIMD that the registers are for: 256 of them each, 512 where the sums of a wide dim need more.  Vector registers that
+// are spilled, over whole contexts and over blocks: two row tiles of dim 128 none and 2 (16-bit caches), 8 to 10 and 14 to 16 (8-bit
+// ones), of dims 80 to 112 10 and 16, 16 to 24 and 24 to 27; the direct form of 16-bit caches 7 and 13 at dims 80 to 112, 3 and 5 at
+// 256, up to 14 and 17 at 144 to 240 (which also keeps up to 469 scalar ones in vector lanes); one row tile a wave none and 2 at
+// 80 to 112, 17 and 22 at 144 to 240 (8-bit caches up to 2 and 6).  No other form spills any.
 constexpr int attn_occupancy(int form, int R, int dim) {
   return dim > 128 && form != AT_ROWS ? 1 : 2;
 }

@@ -20,8 +20,8 @@ extern template void launch_attn<DSV_F16, DSV_I8, true>(const AttnParams&, const
 constexpr int AJ_THREADS = 256, AJ_PARTS = 4;
 
 // The parts of a request joined: 8 elements of a row a thread, the parts in their order.  Bound by latency (the plan's
-// lengths, then the parts: 4.9 us after one request's few parts, 7 to 8 us for most batches) and, for many rows, by the
-// sums' bytes (14.3 us for 16 requests of 512 rows a head).  A launch of its own: a last workgroup that joins would need
+// lengths, then the parts: 4.0 us after one request's few parts, 5 to 8 us for most batches) and, for many rows, by the
+// sums' bytes (14.7 us for 16 requests of 512 rows a head).  A launch of its own: a last workgroup that joins would need
 // counters that somebody clears.
 // AHEAD: the next few parts are on their way while these are added, which takes the registers of twice as many waves.
 template <int XT, int DP, bool BLOCKS, bool AHEAD>

@@ -47,8 +47,8 @@ __device__ __forceinline__ float in_range(float v) {
 
 // Bounds of a finished block, a wave a (block, head): its lanes hold the block's slots, groups of G lanes take a position's
 // row, 16 bytes a lane, BI_ROWS rows in flight together.  NaN counts as the least and the largest.  Bound by memory: the
-// blocks of four prompts, 88 MB of e4m3 keys: 19.8 us, 4.5 TB/s (a workgroup a block and head, two rows in flight: 57 us).
-// A round's few blocks: 5.3 us, latency.
+// blocks of four prompts, 88 MB of e4m3 keys: 19.8 us in a kernel trace, 4.5 TB/s (a workgroup a block and head, two rows in
+// flight: 57 us).  A round's few blocks: 5.1 us, latency.
 constexpr int BI_ROWS = 8;
 template <int CT, int IT, int G>
 __global__ __launch_bounds__(BI_THREADS) void k_index_blocks(IndexParams P) {
@@ -214,8 +214,10 @@ __device__ __forceinline__ float defined_sum(const dsv_score_blocks_args& a, con
 
 // A workgroup some steps of a (request, head)'s blocks, its queries as operands in LDS; a wave 16 blocks a step, their
 // bounds in registers for all of the queries.  Bound by memory: 64 requests of 8k to 64k positions in blocks of 64, up to 17
-// nodes, 147 MB of bounds: 38 us, 3.9 TB/s (the next step's bounds loaded into a second set of registers first: 42 us for 41;
-// queries split by sign in LDS, twice the memory and half the workgroups a CU: 62 us).  One node over 32k: 4.8 us, latency.
+// nodes, 154 MB read and written: 43.0 us in a kernel trace, 39.8 a call in a row of eager ones (3.6 and 3.9 TB/s).  Of 41 us in such
+// a row, the next step's bounds loaded into a second set of registers first take 42; queries split by sign in LDS, twice the
+// memory and half the workgroups a CU, 62.  Many rows are bound by operations, the split of the queries for each 16 blocks among
+// them, and measured at 68 rows these say nothing of those.  One node over 32k: 5.0 us, latency.
 // (Five waves a SIMD at dims 80 to 112: with the registers of four, 16 x 17 nodes of dim 96 take 19.0 us for 18.3.)
 template <int IT, int NC, bool FULL, int WAVES>
 __global__ __launch_bounds__(WAVES * WAVE, NC == 4 && !FULL ? 5 : 1) void k_score_blocks(ScoreParams P) {
@@ -360,7 +362,7 @@ struct SelectParams {
 // A workgroup a (request, head), its scores in registers as keys that order like them.  The `need`-th largest key is
 // found in 256 equal bins of the range that holds it, again within that bin until at most 64 keys are left, which one
 // wave ranks by counting; equal keys count by their index, the lowest first.  The chosen ones are written in order.  Bound by
-// latency: 8 heads of 500 blocks 6.6 us, 512 of up to 2000 7.8 us.
+// latency: 8 heads of 500 blocks 6.2 us, 512 of up to 2000 7.7 us.
 template <int NW, int PER>
 __global__ __launch_bounds__(NW * WAVE) void k_select_blocks(SelectParams P) {
   constexpr int NT = NW * WAVE;

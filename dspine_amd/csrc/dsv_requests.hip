@@ -54,8 +54,8 @@ __device__ __forceinline__ void load_lens(const void* lens, int i64, const int64
 // Samples of one prompt hold its slots at the same positions, so a thread takes its column's entries of RQ_ROWS rows and
 // counts equal ones together: what bounds a fork or a release of long prompts is the touch of a scattered count for each
 // slot (about 28 G/s; a plain read and write is as slow as the atomic, and neighbouring slots share their lines).  128 rows
-// of 20000 positions, two of each prompt, slots in random order: 58 us a fork and 56 a release, 96 each with an atomic
-// an entry; without the counts a fork is 17.
+// of 20000 positions, two of each prompt, slots in random order: 57 us a fork and 56 a release, 96 each with an atomic
+// an entry; without the counts a fork is 17.  (Entries sorted by ranges of slots first, each range counted in LDS, was not tried.)
 constexpr int RQ_ROWS = 8;
 __device__ __forceinline__ void add_holders(const TableParams& P, int32_t (&slot)[RQ_ROWS], int sign) {
   int times[RQ_ROWS];
@@ -144,7 +144,7 @@ __global__ __launch_bounds__(RQ_THREADS) void k_release(TableParams P) {
   release_column(P, group * RQ_ROWS, again, chunk * RQ_THREADS + threadIdx.x);
 }
 
-// Slots below zero in each chunk of the pool; the rows' lengths become zero.  (1.6 M slots: 5.8 us, and the list 7.3.)
+// Slots below zero in each chunk of the pool; the rows' lengths become zero.  (1.6 M slots: 5.8 us, and the list 7.1.)
 __global__ __launch_bounds__(RQ_THREADS) void k_count_freed(TableParams P, int32_t* counts) {
   __shared__ int s_red[RQ_THREADS / WAVE];
   const int64_t first = (int64_t)blockIdx.x * RQ_CHUNK;
@@ -191,7 +191,7 @@ __global__ __launch_bounds__(RQ_THREADS) void k_emit_freed(TableParams P, const 
   }
 }
 
-// Rows of a small pool, all of it in one workgroup: a launch in place of three (2 rows of 750 columns: 4.1 us for 3.3 + 3.4 + 3.8
+// Rows of a small pool, all of it in one workgroup: a launch in place of three (2 rows of 750 columns: 3.7 us for 3.3 + 3.4 + 3.8
 // and their gaps, and two launches less of the host's).  The rows and their lengths are read once, and the columns of all groups
 // of RQ_ROWS rows are dealt to the threads in one row, so that many short rows wait for memory no longer than a few.
 constexpr int RQ_WIDE = 1024, RQ_SMALL_SLOTS = 16 * RQ_WIDE;
@@ -340,7 +340,7 @@ __global__ __launch_bounds__(RQ_THREADS) void k_plan_moves(CompactParams P) {
 }
 
 // The same for a small pool and few rows, in one workgroup, the used slots as bits in its LDS: a launch in place of four
-// (7 rows of 2700 columns, 14000 slots: 10.7 us for 11 in all, and three launches less of the host's).
+// (7 rows of 2700 columns, 14000 slots: 11.2 us for 11 in all, and three launches less of the host's).
 constexpr int RQ_BITS = 2 * 16 * RQ_WIDE;  // slots at most
 __global__ __launch_bounds__(RQ_WIDE) void k_plan_small(CompactParams P) {
   __shared__ uint32_t s_bits[RQ_BITS / 32];
@@ -405,7 +405,7 @@ struct CopyParams {
 typedef uint32_t uint32x4 __attribute__((ext_vector_type(4)));
 
 // Groups of G lanes take CS_ROWS moves at once, all loaded before the first is stored.  Bound by memory: 45000 slots' rows of
-// four layers, 1.6 GB read and written: 286 us, 5.5 TB/s (314 with loads and stores that the caches keep).
+// four layers, 1.6 GB read and written: 293 us, 5.5 TB/s (314 with loads and stores that the caches keep).
 template <class V>
 __device__ __forceinline__ void copy_rows(const CopyParams& P, const CopyPart& part, int64_t n) {
   const int l = threadIdx.x & (part.G - 1), groups = RQ_THREADS / part.G;
