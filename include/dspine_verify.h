@@ -544,7 +544,8 @@ typedef struct dsv_block_index {
 /* dsv_kv_read gives them in float32, rounded once (finite ones to the type's largest number at most);  */
 /* a NaN makes both of its element's bounds NaN.  Positions that hold nothing (past page_cols, slots   */
 /* outside the cache) do not count, a block without any other has zeros.  Blocks past block_cols and    */
-/* rows outside the index are skipped.                                                                */
+/* rows outside the index are skipped.  The page table is that of the to_lens[b] positions: after a      */
+/* commit the request table's rows as it left them, not the window's.                                  */
 int dsv_index_blocks(const dsv_block_index* index, const dsv_kv_cache* cache, const int32_t* page_table,
                      int64_t page_stride, int64_t page_cols, const int32_t* block_table, int64_t block_stride,
                      int64_t block_cols, const int32_t* from_lens, const int32_t* to_lens, int32_t bs,
